@@ -319,6 +319,116 @@ ZTCP_API int ztcp_wire_ring_push(ztcp_wire_ring* ring, const uint8_t* blobs, siz
 ZTCP_API int ztcp_wire_ring_wait(ztcp_wire_ring* ring, int32_t slot, const uint8_t** host, size_t* nbytes);
 ZTCP_API int ztcp_wire_ring_destroy(ztcp_wire_ring* ring);
 
+/* Operators on hot pages (no counterpart in the reference): the steps of a
+ * serving engine that write the hot pages, read them, and choose which of them
+ * go cold.  Enqueued on `stream`; they synchronize nothing and allocate
+ * nothing, so they can be recorded into a HIP graph.  Every array is a DEVICE
+ * pointer.  Argument errors return ZTCP_EINVAL / ZTCP_EOVERLAP
+ * (ztcp_last_error says why); indexes that live on the device cannot be
+ * refused there and are bounded by the kernels as each entry says.
+ *
+ * A pool holds n_pages pages of [num_tokens, num_heads, head_dim] elements
+ * (ztcp_geometry; rope_dim is the append's), page p at k + p * k_stride and
+ * v + p * v_stride elements.  Pointers are 16-byte aligned and strides
+ * multiples of 8 elements. */
+typedef struct ztcp_page_pool {
+    void* k;
+    void* v;            /* NULL for single-buffer pages */
+    int64_t n_pages;
+    int64_t k_stride;   /* elements between pages */
+    int64_t v_stride;
+} ztcp_page_pool;
+
+/* A batch of sequences over a pool.  Row s of the table lists sequence s's
+ * pages in order: token j is in page table[s][j / num_tokens].  An entry
+ * outside [0, n_pages) is a page that is not there (cold): its tokens take no
+ * part.  Lengths are cut to 0 .. max_pages * num_tokens.  The new tokens of
+ * sequence s are rows q_starts[s] .. q_starts[s + 1] - 1 of q, the last ones
+ * of its kv_lens[s] tokens: the i-th of n sees tokens
+ * j <= kv_lens[s] - n + i.  Rows that no sequence has are left as they were. */
+typedef struct ztcp_paged_batch {
+    const int32_t* page_table;   /* [n_seqs, max_pages], rows table_stride apart */
+    int64_t table_stride;
+    int64_t max_pages;
+    const int32_t* kv_lens;      /* [n_seqs], the new tokens among them */
+    const int32_t* q_starts;     /* [n_seqs + 1], ascending */
+    int64_t n_seqs;
+    int64_t n_rows;              /* rows of q */
+    int64_t max_q_len;           /* most new tokens of a sequence; 0 = not known.  A
+                                    hint: too small a value costs time only */
+} ztcp_paged_batch;
+
+/* New tokens into their pages: norms of queries and keys for each head, position
+ * rotation, and the write, in one pass.
+ *   q [n, q_heads, head_dim] -> q_out (may be q itself), k [n, num_heads, head_dim]
+ *   -> pool K, v (NULL with pool->v for single-buffer pages) -> pool V; tokens are
+ *   *_stride elements apart, a token's heads contiguous.
+ *   Norm: x / sqrt(mean(x^2) + eps) * weight in fp32.  A weight of head_dim entries
+ *   norms the head vector, one of head_dim - rope_dim entries the columns behind the
+ *   rotated ones only, 0 entries (NULL) nothing.  Weights have the hot dtype.
+ *   Rotation of the leading rope_dim columns by the angles of row positions[i] of
+ *   rope, [max_position, rope_dim] fp32: cosines then sines of the rope_dim / 2
+ *   angles.  Pairs are (c, c + rope_dim / 2), or (2c, 2c + 1) when interleaved.  A
+ *   position outside the table has no angle: its rotated columns become NaN.
+ *   Slots: page * num_tokens + token of each new token.  One outside the pool
+ *   writes no page (rows of a padded batch).  Where a slot occurs twice, each head
+ *   vector is that of one of its tokens. */
+ZTCP_API int ztcp_append_tokens(const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride,
+                       const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                       int64_t n_tokens, int64_t q_heads, const ztcp_page_pool* pool,
+                       const ztcp_geometry* g, const int64_t* slots, const int32_t* positions,
+                       const float* rope, int64_t max_position, const void* q_weight,
+                       int64_t q_weight_len, const void* k_weight, int64_t k_weight_len, float eps,
+                       int32_t interleaved, void* stream);
+
+/* Attention of the batch's new tokens over its hot pages: softmax of scale * q . k
+ * over the tokens a row sees, times V, in one pass with fp32 statistics.
+ *   q [n_rows, q_heads, head_dim], tokens q_stride elements apart; query head h
+ *   reads KV head h / (q_heads / num_heads); head_dim at most 256.
+ *   out [n_rows, q_heads, head_dim] of the hot dtype.
+ *   lse [n_rows, q_heads] fp32 (may be NULL): the logarithm of each row's sum of
+ *   exponentials, as ztcp_attention_mass takes it.
+ * A row that sees no token gets zeros and -infinity.  What stands in pages behind
+ * a sequence's length or after a row's own token, NaN and infinities among it,
+ * does not reach the row.  workspace: ztcp_paged_attention_workspace(...) bytes
+ * (may be 0; (size_t)-1 for arguments that the call refuses), needed until the
+ * call's work is done, by one call at a time. */
+ZTCP_API size_t ztcp_paged_attention_workspace(const ztcp_paged_batch* batch, const ztcp_page_pool* pool,
+                                      const ztcp_geometry* g, int64_t q_heads);
+ZTCP_API int ztcp_paged_attention(const void* q, int64_t q_stride, void* out, float* lse, int64_t q_heads,
+                         const ztcp_page_pool* pool, const ztcp_paged_batch* batch,
+                         const ztcp_geometry* g, float scale, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* The attention weight that each page of the batch received from its new tokens,
+ * added to the accounts:
+ *   out[s, h, p] = decay * mass[s, h, p] + sum of exp(scale * q . k - lse) over the
+ *   rows of KV head h's query heads and the tokens of page p that they see.
+ * mass, out [n_seqs, num_heads, max_pages] fp32; out may be mass itself.  lse as
+ * ztcp_paged_attention gives it; a row with -infinity adds nothing.  The pool's v is
+ * not read and may be NULL.  Sums are in fp32, in an order that the call fixes. */
+ZTCP_API int ztcp_attention_mass(const void* q, int64_t q_stride, const float* lse, int64_t q_heads,
+                        const ztcp_page_pool* pool, const ztcp_paged_batch* batch,
+                        const ztcp_geometry* g, float scale, const float* mass, float decay,
+                        float* out, void* stream);
+
+/* Which pages a sequence gives up: of its n = ceil(kv_lens[s] / num_tokens) pages
+ * (at most max_pages), all but the first `sink` and the last `recent` (>= 1) may go,
+ * and those with the least mass go, until `budget` remain or none may go.  A page's
+ * mass is the sum of its num_heads accounts in 64 bits; of equal ones the
+ * first goes, NaN counts as more than every number.  Pages keep their order.
+ *   mass [n_seqs, num_heads, max_pages] fp32, table rows table_stride apart;
+ *   out_table [n_seqs, max_pages], out_mass, out_lens: what is kept, gaps closed,
+ *   -1 and 0 behind it (a page gone shortens the sequence by num_tokens);
+ *   evicted [n_seqs, max_pages]: the ids given up, in order, -1 behind them;
+ *   n_evicted [n_seqs].
+ * out_table, out_mass and out_lens may be the inputs themselves. */
+ZTCP_API int ztcp_evict_pages(const float* mass, const int32_t* page_table, int64_t table_stride,
+                     const int32_t* kv_lens, int64_t n_seqs, int64_t num_heads, int64_t max_pages,
+                     int64_t num_tokens, int64_t budget, int64_t sink, int64_t recent,
+                     int32_t* out_table, int64_t out_table_stride, float* out_mass, int32_t* out_lens,
+                     int32_t* evicted, int32_t* n_evicted, void* stream);
+
 /* Short description of a return code. */
 ZTCP_API const char* ztcp_strerror(int code);
 

@@ -8,6 +8,8 @@ Modules:
   keyring           session key ring, drop-in for EphemeralSessionKeyRing
                     (research/baseline_codec/fused_quant_crypto.py:99-659), native state
   pages             descriptor-based batch API for paged, multi-layer KV pools
+  attention         operators on hot pages: append with norms and rotation, paged
+                    attention, the weight each page received, eviction
   serving           PoisonShield hit bitmap from per-page verdicts, pinned host ring
                     for the egress wire step
   spec              wire constants, AAD record and payload sizing (cold_page_spec.py mirror)
@@ -15,7 +17,7 @@ Modules:
 """
 from . import spec  # noqa: F401
 
-__all__ = ["spec", "native_hip_codec", "codec", "keyring", "pages", "serving", "workloads", "load_native"]
+__all__ = ["spec", "native_hip_codec", "codec", "keyring", "pages", "attention", "serving", "workloads", "load_native"]
 
 
 def load_native():

@@ -29,7 +29,8 @@ EXPORTS = (
     "ztcp_chacha20_xor", "ztcp_siphash128",
     "ztcp_selftest", "ztcp_device_diag", "ztcp_debug_spin_limit", "ztcp_strerror",
     "ztcp_last_error", "ztcp_hit_bitmap", "ztcp_wire_ring_create", "ztcp_wire_ring_push",
-    "ztcp_wire_ring_wait", "ztcp_wire_ring_destroy",
+    "ztcp_wire_ring_wait", "ztcp_wire_ring_destroy", "ztcp_append_tokens",
+    "ztcp_paged_attention_workspace", "ztcp_paged_attention", "ztcp_attention_mass", "ztcp_evict_pages",
 )
 
 # Every symbol include/ztcp_keyring.h declares (host code, callable without a GPU).
@@ -69,6 +70,17 @@ class PageDesc(C.Structure):
                 ("token_hash", C.c_int64), ("sequence_nonce", C.c_uint64),
                 ("layer_id", C.c_uint16), ("head_group_id", C.c_uint16),
                 ("reserved", C.c_uint32)]
+
+
+class PagePool(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("n_pages", C.c_int64),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64)]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [("page_table", C.c_void_p), ("table_stride", C.c_int64), ("max_pages", C.c_int64),
+                ("kv_lens", C.c_void_p), ("q_starts", C.c_void_p), ("n_seqs", C.c_int64),
+                ("n_rows", C.c_int64), ("max_q_len", C.c_int64)]
 
 
 # The phase-timer build of the same sources (vlx-tee_amd/build.py): the same
@@ -146,6 +158,18 @@ def lib() -> C.CDLL:
     L.ztcp_wire_ring_wait.restype = i32
     L.ztcp_wire_ring_destroy.argtypes = [P]
     L.ztcp_wire_ring_destroy.restype = i32
+    PP, PB, f32 = C.POINTER(PagePool), C.POINTER(PagedBatch), C.c_float
+    L.ztcp_append_tokens.argtypes = [P, i64, P, i64, P, i64, P, i64, i64, i64, PP, G, P, P, P, i64, P, i64, P, i64,
+                                     f32, i32, P]
+    L.ztcp_append_tokens.restype = i32
+    L.ztcp_paged_attention_workspace.argtypes = [PB, PP, G, i64]
+    L.ztcp_paged_attention_workspace.restype = C.c_size_t
+    L.ztcp_paged_attention.argtypes = [P, i64, P, P, i64, PP, PB, G, f32, P, C.c_size_t, P]
+    L.ztcp_paged_attention.restype = i32
+    L.ztcp_attention_mass.argtypes = [P, i64, P, i64, PP, PB, G, f32, P, f32, P, P]
+    L.ztcp_attention_mass.restype = i32
+    L.ztcp_evict_pages.argtypes = [P, P, i64, P, i64, i64, i64, i64, i64, i64, i64, P, i64, P, P, P, P, P]
+    L.ztcp_evict_pages.restype = i32
     _bind_keyring(L)
     _lib = L
     return L

@@ -52,6 +52,14 @@ int fail_arg(int rc, const char* why) {
     return rc;
 }
 
+}  // namespace
+
+namespace ztcp {
+int arg_result(int rc, const char* why) { return fail_arg(rc, why); }
+}  // namespace ztcp
+
+namespace {
+
 // Per-device library state, created on the first call on that device.
 int device_ctx(DeviceCtx** out) {
     int dev = 0;

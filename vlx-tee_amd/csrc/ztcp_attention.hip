@@ -1,0 +1,783 @@
+// ztcp_attention.hip -- attention of new tokens over hot pages.
+//
+//   s_ij = scale * q_i . k_j  for the tokens j that row i sees,
+//   o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i),  lse_i = m_i + log(sum_j ...)
+//
+// in one pass over the keys with a running maximum m and sum.  A KV head's
+// queries are the rows of its products: row r is new token r / group, query
+// head r % group of the KV head's group.  Scores are made transposed (K rows
+// times Q columns): a row of the softmax is then one column of the result, one
+// lane's registers and its partners', and these registers are, as they stand,
+// the operand of the second product (V columns times P columns), whose depth,
+// the keys, is in the same order on both sides.
+#include <type_traits>
+
+#include "ztcp_hot.h"
+
+using namespace ztcp;
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct AttendParams {
+    PagedView batch;
+    const uint8_t* q;
+    uint8_t* out;
+    float* lse;                      // or nullptr
+    int64_t q_stride;                // elements between tokens
+    const uint8_t* k_pool;
+    const uint8_t* v_pool;
+    int64_t k_page, v_page;          // elements between pages
+    int32_t kv_heads, group, head_dim;
+    float scale_log2;                // scale * log2(e): exponentials are powers of two
+    int32_t few_rows;                // sequences of at most so many rows are the few kernel's, others the many kernel's
+    int32_t splits, split_tokens;    // pieces of a sequence's tokens, and tokens of a piece
+    float* partial;                  // [row, query head, partial_splits, head_dim + 2]: sums, maximum, total
+    int32_t partial_splits;
+};
+
+__device__ __forceinline__ float* partial_of(const AttendParams& p, int row, int q_head, int split) {
+    return p.partial + (((int64_t)row * p.kv_heads * p.group + q_head) * p.partial_splits + split) * (p.head_dim + 2);
+}
+
+// Pieces of a sequence that have tokens (one at least: it answers for a sequence without tokens).
+__device__ __forceinline__ int live_splits(const AttendParams& p, int len) {
+    return len > 0 ? (len - 1) / p.split_tokens + 1 : 1;
+}
+
+// What a row does not see must not reach it, but 0 * NaN is NaN: in a tile
+// whose keys some rows see and others do not, V numbers that are no finite
+// numbers leave the product (set to 0) and are added afterwards to the rows
+// that see them.  An infinity or a NaN needs no weight for that.
+template <int DT>
+__device__ __forceinline__ bool not_finite16(uint32_t h) {
+    constexpr uint32_t e = DT == kHotBf16 ? 0x7F80u : 0x7C00u;
+    return (h & e) == e;
+}
+template <int DT>
+__device__ __forceinline__ bool drop_not_finite(uint4& x) {
+    uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (not_finite16<DT>(w[i])) w[i] &= 0xFFFF0000u, any = true;
+        if (not_finite16<DT>(w[i] >> 16)) w[i] &= 0x0000FFFFu, any = true;
+    }
+    if (any) x = make_uint4(w[0], w[1], w[2], w[3]);
+    return any;
+}
+// Four numbers of a V row from column d on: those that are not finite, 0 for the others.
+template <int DT>
+__device__ __forceinline__ f32x4 only_not_finite(const AttendParams& p, const Place& at, int head, int d) {
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    if (at.page < 0 || d >= p.head_dim) return y;
+    const uint8_t* src = p.v_pool + 2 * ((int64_t)at.page * p.v_page + ((int64_t)at.row * p.kv_heads + head) * p.head_dim + d);
+    const uint2 w = *reinterpret_cast<const uint2*>(src);
+    const float x[4] = {hot_lo<DT>(w.x), hot_hi<DT>(w.x), hot_lo<DT>(w.y), hot_hi<DT>(w.y)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (!(__builtin_fabsf(x[i]) < INFINITY)) y[i] = x[i];
+    return y;
+}
+
+// ---- few rows -----------------------------------------------------------------
+// Decoding: reading K and V is the work.  A workgroup of four waves takes one
+// KV head of one piece of one sequence; each wave takes every fourth tile of 32
+// keys and has its loads of the next tile in flight while it works on this one:
+// K as the products want it (lane = key, 16 bytes of its row), V by whole rows,
+// through 32 rows of LDS of the wave's own that the transposing reads take.
+// Waves join their maxima, totals and sums at the end.
+
+template <int DT, int DP, int NT>
+__global__ __launch_bounds__(256) void few_kernel(AttendParams p) {
+    constexpr int kSteps = DP / 32, kChunks = DP / 8;         // products of depth 32; 16-byte pieces of a row
+    constexpr int kVLoads = 32 * kChunks / 64;                // V loads of a lane for a tile
+    constexpr int kVRows = 64 / kChunks;                      // rows a load covers
+    constexpr int kJoinRow = DP + 4;
+    constexpr int kWaveBytes = 32 * DP * 2;
+    constexpr int kBytes = 4 * kWaveBytes > 4 * 16 * kJoinRow * 4 ? 4 * kWaveBytes : 4 * 16 * kJoinRow * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kBytes];
+    __shared__ float join_m[4][16], join_l[4][16];
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int col = lane & 15, quad = lane >> 4;
+    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads);
+    const uint32_t rest = blockIdx.x / (uint32_t)p.kv_heads;
+    const int split = (int)(rest % (uint32_t)p.splits), s = (int)(rest / (uint32_t)p.splits);
+    const Seq seq = seq_of(p.batch, s);
+    const int rows = seq.n_new * p.group;
+    if (rows == 0 || rows > p.few_rows || split >= live_splits(p, seq.len)) return;
+    const int key0 = split * p.split_tokens;
+    const int key1 = key0 + min(seq.len - key0, p.split_tokens);
+    uint8_t* vt = lds + wave * kWaveBytes;
+    // 16-byte pieces of V rows are permuted within the row so that the rows a
+    // transposing read takes lie in different banks
+    auto swizzle = [](int row, int chunk) {
+        if constexpr (DP == 64) return chunk ^ (((row >> 1) & 3) << 1);
+        else return chunk ^ ((row & 7) << 1);
+    };
+    const int v_row = lane / kChunks, v_chunk = lane % kChunks;
+    const bool v_has = v_chunk * 8 < p.head_dim;
+
+    for (int r0 = 0; r0 < rows; r0 += 16 * NT) {
+        int limit[NT];                                        // tokens that the lane's rows see
+        uint4 qf[NT][kSteps];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int r = r0 + 16 * t + col;
+            const int token = r / p.group, h = r - token * p.group;
+            limit[t] = r < rows ? max(0, seq.len - seq.n_new + token + 1) : 0;
+            const uint8_t* src = p.q + 2 * ((int64_t)(seq.row0 + token) * p.q_stride + (int64_t)(head * p.group + h) * p.head_dim);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const int d = 32 * i + 8 * quad;
+                qf[t][i] = r < rows && d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
+            }
+        }
+        const int last = min(rows, r0 + 16 * NT) - 1;
+        const int stop = min(key1, max(0, seq.len - seq.n_new + last / p.group + 1));
+        float m[NT], l[NT];
+        f32x4 o[NT][DP / 16];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            m[t] = -INFINITY;
+            l[t] = 0.f;
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        uint4 kf[2][kSteps], vf[kVLoads];
+        Place at;                                             // of key (lane % 32) of the tile to be loaded
+        uint32_t valid = 0, v_valid = 0;                      // keys of the loaded tile that are there; this lane's V rows of them
+        auto load = [&](const Place& at) {
+            const bool has = at.page >= 0;
+            valid = (uint32_t)__ballot(has);
+            const int page = has ? at.page : 0, row = has ? at.row : 0;
+            v_valid = 0;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int from = 16 * t + col;
+                const int64_t pg = __shfl(page, from), rw = __shfl(row, from);
+                const uint8_t* src = p.k_pool + 2 * (pg * p.k_page + (rw * p.kv_heads + head) * p.head_dim);
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    const int d = 32 * i + 8 * quad;
+                    kf[t][i] = d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kVLoads; ++i) {
+                const int from = i * kVRows + v_row;
+                const int64_t pg = __shfl(page, from), rw = __shfl(row, from);
+                const uint8_t* src = p.v_pool + 2 * (pg * p.v_page + (rw * p.kv_heads + head) * p.head_dim);
+                vf[i] = v_has ? ldg16(src + 16 * v_chunk) : make_uint4(0, 0, 0, 0);
+                v_valid |= ((valid >> from) & 1u) << i;
+            }
+        };
+        const int first_sees = max(0, seq.len - seq.n_new + r0 / p.group + 1);   // the row that sees least
+        int kb = key0 + 32 * wave;
+        if (kb < stop) {
+            load(place_of(p.batch, seq, kb + (lane & 31), stop));
+            at = place_of(p.batch, seq, kb + 128 + (lane & 31), stop);
+        }
+        for (; kb < stop; kb += 128) {
+            const uint32_t here = valid;
+            f32x4 sc[NT][2];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    sc[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < kSteps; ++i) sc[t][u] = mfma16<DT>(kf[u][i], qf[t][i], sc[t][u]);
+                }
+            uint32_t apart = 0;                               // keys with numbers to be added apart
+            if (kb + 32 > first_sees && first_sees < stop) {
+#pragma unroll
+                for (int i = 0; i < kVLoads; ++i)
+                    if (drop_not_finite<DT>(vf[i])) apart |= 1u << (i * kVRows + v_row);
+                if (__any(apart != 0))
+                    for (int k = 1; k < 64; k <<= 1) apart |= __shfl_xor(apart, k);
+                apart &= here;
+            }
+#pragma unroll
+            for (int i = 0; i < kVLoads; ++i) {
+                const int row = i * kVRows + v_row;
+                const uint4 x = (v_valid >> i) & 1u ? vf[i] : make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(vt + row * DP * 2 + swizzle(row, v_chunk) * 16) = x;
+            }
+            if (kb + 128 < stop) {
+                load(at);
+                at = place_of(p.batch, seq, kb + 256 + (lane & 31), stop);
+            }
+            uint4 pf[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float x[8];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = 16 * u + 4 * quad + i;
+                        const bool seen = ((here >> key) & 1u) && kb + key < limit[t];
+                        x[4 * u + i] = seen ? sc[t][u][i] * p.scale_log2 : -INFINITY;
+                    }
+                float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float m_new = fmaxf(m[t], top);
+                const float base = m_new == -INFINITY ? 0.f : m_new;   // no key seen yet: every power is 0
+                if (__any(m_new != m[t])) {
+                    const float fade = __builtin_amdgcn_exp2f(m[t] - base);
+                    l[t] *= fade;
+#pragma unroll
+                    for (int i = 0; i < DP / 16; ++i) o[t][i] *= fade;
+                }
+                m[t] = m_new;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x[i] = __builtin_amdgcn_exp2f(x[i] - base);
+                    l[t] += x[i];
+                }
+                // probabilities are rounded to the hot dtype for the product with V (their total is not):
+                // relative to the result that costs about what its own final rounding does
+                pf[t] = make_uint4(pack_hot<DT>(x[0], x[1]), pack_hot<DT>(x[2], x[3]), pack_hot<DT>(x[4], x[5]),
+                                   pack_hot<DT>(x[6], x[7]));
+            }
+#pragma unroll
+            for (int n = 0; n < DP / 16; ++n) {
+                uint2 v[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int row = 16 * u + 4 * quad + col / 4, chunk = 2 * n + (col & 3) / 2;
+                    v[u] = lds_read_transposed(vt + row * DP * 2 + swizzle(row, chunk) * 16 + (col & 1) * 8);
+                }
+                const uint4 a = make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) o[t][n] = mfma16<DT>(a, pf[t], o[t][n]);
+            }
+            for (apart = __builtin_amdgcn_readfirstlane(apart); apart; apart &= apart - 1) {
+                const int key = kb + __ffs((int)apart) - 1;
+                const Place where = place_of(p.batch, seq, key, stop);
+#pragma unroll
+                for (int n = 0; n < DP / 16; ++n) {
+                    const f32x4 x = only_not_finite<DT>(p, where, head, 16 * n + 4 * quad);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+                        if (key < limit[t]) o[t][n] += x;
+                }
+            }
+        }
+        // join the four waves
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            l[t] += __shfl_xor(l[t], 16);
+            l[t] += __shfl_xor(l[t], 32);
+            __syncthreads();   // the waves' V rows, or the previous rows' sums, have been read
+            float* join = reinterpret_cast<float*>(lds);
+#pragma unroll
+            for (int n = 0; n < DP / 16; ++n)
+                *reinterpret_cast<f32x4*>(join + (wave * 16 + col) * kJoinRow + 16 * n + 4 * quad) = o[t][n];
+            if (quad == 0) {
+                join_m[wave][col] = m[t];
+                join_l[wave][col] = l[t];
+            }
+            __syncthreads();
+            const int row = (int)threadIdx.x / 16, part = (int)threadIdx.x % 16;
+            const int r = r0 + 16 * t + row;
+            if (r < rows) {
+                float top = -INFINITY, total = 0.f, w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, join_m[i][row]);
+                const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[i] = __builtin_amdgcn_exp2f(join_m[i][row] - base);
+                    total += w[i] * join_l[i][row];
+                }
+                const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
+                float* part_out = p.partial ? partial_of(p, seq.row0 + token, q_head, split) : nullptr;
+                const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+                uint8_t* dst = p.out + 2 * ((int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head) * p.head_dim;
+                for (int d = 8 * part; d < p.head_dim; d += 128) {
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        y[e] = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y[e] = __builtin_fmaf(w[i], join[(i * 16 + row) * kJoinRow + d + e], y[e]);
+                    }
+                    if (part_out) {
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) *reinterpret_cast<float2*>(part_out + d + e) = make_float2(y[e], y[e + 1]);
+                    } else {
+                        stg16(dst + 2 * d, 0, make_uint4(pack_hot<DT>(y[0] * inv, y[1] * inv), pack_hot<DT>(y[2] * inv, y[3] * inv),
+                                                         pack_hot<DT>(y[4] * inv, y[5] * inv), pack_hot<DT>(y[6] * inv, y[7] * inv)));
+                    }
+                }
+                if (part == 0) {
+                    if (part_out) {
+                        part_out[p.head_dim] = top;
+                        part_out[p.head_dim + 1] = total;
+                    } else if (p.lse) {
+                        p.lse[(int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head] =
+                            total == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(total)) * kLn2;
+                    }
+                }
+            }
+        }
+    }
+}
+
+// ---- many rows ----------------------------------------------------------------
+// Chunks of prompts: the products are the work.  A workgroup of four waves
+// takes 128 rows, 32 a wave, of one KV head; tiles of 64 keys pass through LDS,
+// read by all four, the next one on its way in registers meanwhile.
+
+constexpr int kManyRows = 128;
+
+// The unit-th block of kManyRows rows of the batch's sequences of more than
+// p.few_rows rows; false if there are fewer.
+__device__ __forceinline__ bool find_unit(const AttendParams& p, int unit, int& s, int& block) {
+    const int lane = (int)threadIdx.x & 63;
+    for (int base = 0; base < p.batch.n_seqs; base += 64) {
+        int n = 0;
+        if (base + lane < p.batch.n_seqs) {
+            const int rows = seq_of(p.batch, base + lane).n_new * p.group;
+            n = rows > p.few_rows ? (rows + kManyRows - 1) / kManyRows : 0;
+        }
+        int upto = n;
+        for (int m = 1; m < 64; m <<= 1) {
+            const int y = __shfl_up(upto, m);
+            upto += lane >= m ? y : 0;
+        }
+        const uint64_t past = __ballot(upto > unit);
+        if (past) {
+            const int at = __ffsll((unsigned long long)past) - 1;
+            s = base + at;
+            const int n_at = __shfl(n, at);
+            block = n_at - 1 - (unit - (__shfl(upto, at) - n_at));   // the last rows, which see most, first
+            return true;
+        }
+        unit -= __shfl(upto, 63);
+    }
+    return false;
+}
+
+template <int DT, int DP>
+__global__ __launch_bounds__(256) void many_kernel(AttendParams p) {
+    constexpr int kSteps = DP / 16, kChunks = DP / 8;
+    constexpr int kLoads = 64 * kChunks / 256;                // 16-byte pieces of K, and of V, a thread loads of a tile
+    constexpr int kRowsPerLoad = 256 / kChunks;               // rows the workgroup's one load covers
+    __shared__ __attribute__((aligned(16))) uint8_t kt[64 * DP * 2], vt[64 * DP * 2];
+    __shared__ uint32_t apart_lds[2];                         // keys of the tile with V numbers to be added apart
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int col = lane & 31, half = lane >> 5;
+    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads);
+    const uint32_t rest = blockIdx.x / (uint32_t)p.kv_heads;
+    const int split = (int)(rest % (uint32_t)p.splits);
+    int s, block;
+    if (!find_unit(p, (int)(rest / (uint32_t)p.splits), s, block)) return;
+    const Seq seq = seq_of(p.batch, s);
+    const int rows = seq.n_new * p.group;
+    if (split >= live_splits(p, seq.len)) return;
+    const int key0 = split * p.split_tokens, key1 = key0 + min(seq.len - key0, p.split_tokens);
+    const int r0 = block * kManyRows + wave * 32, r = r0 + col;
+    const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
+    const int limit = r < rows ? max(0, seq.len - seq.n_new + token + 1) : 0;
+    auto sees = [&](int row) { return max(0, seq.len - seq.n_new + row / p.group + 1); };
+    const int stop = min(key1, sees(min(rows, (block + 1) * kManyRows) - 1));            // of the workgroup
+    const int wave_stop = r0 < rows ? min(key1, sees(min(rows, r0 + 32) - 1)) : 0;       // of this wave
+    const int first_sees = sees(block * kManyRows);                                      // the row that sees least
+    const int wave_full = r0 + 32 <= rows ? sees(r0) : 0;                                // keys that all its rows see
+    auto k_swizzle = [](int row, int chunk) { return chunk ^ (row & (kChunks < 16 ? kChunks - 1 : 15)); };
+    auto v_swizzle = [](int row, int chunk) {
+        if constexpr (DP == 64) return chunk ^ (((row >> 1) & 1) << 2);
+        else return chunk ^ ((row & 3) << 2);
+    };
+    const int my_row = (int)threadIdx.x / kChunks, my_chunk = (int)threadIdx.x % kChunks;
+    const bool my_has = my_chunk * 8 < p.head_dim;
+
+    uint4 qf[kSteps];
+    {
+        const uint8_t* src = p.q + 2 * ((int64_t)(seq.row0 + token) * p.q_stride + (int64_t)q_head * p.head_dim);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const int d = 16 * i + 8 * half;
+            qf[i] = r < rows && d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    float m = -INFINITY, l = 0.f;
+    f32x16 o[DP / 32];
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
+    uint4 kr[kLoads], vr[kLoads];
+    uint64_t valid = 0;
+    auto load = [&](const Place& at) {
+        const bool has = at.page >= 0;
+        valid = __ballot(has);
+        const int page = has ? at.page : 0, row = has ? at.row : 0;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int from = i * kRowsPerLoad + my_row;
+            const int64_t pg = __shfl(page, from), at_row = (int64_t)__shfl(row, from) * p.kv_heads + head;
+            const bool ok = my_has && ((valid >> from) & 1u);
+            kr[i] = ok ? ldg16(p.k_pool + 2 * (pg * p.k_page + at_row * p.head_dim) + 16 * my_chunk) : make_uint4(0, 0, 0, 0);
+            vr[i] = ok ? ldg16(p.v_pool + 2 * (pg * p.v_page + at_row * p.head_dim) + 16 * my_chunk) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    Place next{-1, 0};
+    if (key0 < stop) {
+        load(place_of(p.batch, seq, key0 + lane, stop));
+        next = place_of(p.batch, seq, key0 + 64 + lane, stop);
+    }
+    for (int kb = key0; kb < stop; kb += 64) {
+        __syncthreads();   // the previous tile has been read
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int row = i * kRowsPerLoad + my_row;
+            *reinterpret_cast<uint4*>(kt + row * DP * 2 + k_swizzle(row, my_chunk) * 16) = kr[i];
+            *reinterpret_cast<uint4*>(vt + row * DP * 2 + v_swizzle(row, my_chunk) * 16) = vr[i];
+        }
+        const uint64_t here = valid;
+        __syncthreads();
+        if (kb + 64 < stop) {
+            load(next);
+            next = place_of(p.batch, seq, kb + 128 + lane, stop);
+        }
+        uint64_t apart = 0;
+        if (kb + 64 > first_sees && first_sees < stop) {
+            if (threadIdx.x < 2) apart_lds[threadIdx.x] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int row = i * kRowsPerLoad + my_row;
+                uint4* at = reinterpret_cast<uint4*>(vt + row * DP * 2 + v_swizzle(row, my_chunk) * 16);
+                uint4 x = *at;
+                if (drop_not_finite<DT>(x)) {
+                    *at = x;
+                    atomicOr(&apart_lds[row / 32], 1u << (row % 32));
+                }
+            }
+            __syncthreads();
+            apart = (uint64_t)__builtin_amdgcn_readfirstlane(apart_lds[0]) |
+                    (uint64_t)__builtin_amdgcn_readfirstlane(apart_lds[1]) << 32;
+        }
+        if (kb >= wave_stop) continue;
+        f32x16 sc[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[u][i] = 0.f;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const int row = 32 * u + col;
+                const uint4 a = *reinterpret_cast<const uint4*>(kt + row * DP * 2 + k_swizzle(row, 2 * i + half) * 16);
+                sc[u] = mfma32<DT>(a, qf[i], sc[u]);
+            }
+        }
+        if (kb + 64 > wave_full || here != ~0ull) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = 32 * u + 8 * (i / 4) + 4 * half + i % 4;
+                    if (!((here >> key) & 1u) || kb + key >= limit) sc[u][i] = -INFINITY;
+                }
+        }
+        float top = sc[0][0];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[u][i]);
+        top = fmaxf(top, __shfl_xor(top, 32)) * p.scale_log2;
+        const float m_new = fmaxf(m, top);
+        const float base = m_new == -INFINITY ? 0.f : m_new;
+        if (__any(m_new != m)) {
+            const float fade = __builtin_amdgcn_exp2f(m - base);
+            l *= fade;
+#pragma unroll
+            for (int n = 0; n < DP / 32; ++n) o[n] *= fade;
+        }
+        m = m_new;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                sc[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i], p.scale_log2, -base));
+                l += sc[u][i];
+            }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = pack_hot<DT>(sc[u / 2][8 * (u & 1) + 2 * i], sc[u / 2][8 * (u & 1) + 2 * i + 1]);
+            const uint4 pf = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+            for (int n = 0; n < DP / 32; ++n) {
+                uint2 v[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int row = 16 * u + 8 * j + 4 * half + (lane & 15) / 4;
+                    const int chunk = 4 * n + 2 * ((lane >> 4) & 1) + (lane & 3) / 2;
+                    v[j] = lds_read_transposed(vt + row * DP * 2 + v_swizzle(row, chunk) * 16 + (lane & 1) * 8);
+                }
+                o[n] = mfma32<DT>(make_uint4(v[0].x, v[0].y, v[1].x, v[1].y), pf, o[n]);
+            }
+        }
+        for (; apart; apart &= apart - 1) {
+            const int key = kb + __ffsll((unsigned long long)apart) - 1;
+            const Place where = place_of(p.batch, seq, key, stop);
+#pragma unroll
+            for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 x = only_not_finite<DT>(p, where, head, 32 * n + 8 * i + 4 * half);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (key < limit) o[n][4 * i + e] += x[e];
+                }
+        }
+    }
+    l += __shfl_xor(l, 32);
+    if (r >= rows) return;
+    const int64_t row_head = (int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head;
+    const float base = m == -INFINITY ? 0.f : m;
+    if (p.partial) {
+        float* dst = partial_of(p, seq.row0 + token, q_head, split);
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d = 32 * n + 8 * i + 4 * half;
+                if (d < p.head_dim) {
+                    *reinterpret_cast<float2*>(dst + d) = make_float2(o[n][4 * i], o[n][4 * i + 1]);
+                    *reinterpret_cast<float2*>(dst + d + 2) = make_float2(o[n][4 * i + 2], o[n][4 * i + 3]);
+                }
+            }
+        if (half == 0) {
+            dst[p.head_dim] = m;
+            dst[p.head_dim + 1] = l;
+        }
+        return;
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    uint8_t* dst = p.out + 2 * row_head * p.head_dim;
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = 32 * n + 8 * i + 4 * half;
+            if (d < p.head_dim)
+                *reinterpret_cast<uint2*>(dst + 2 * d) = make_uint2(pack_hot<DT>(o[n][4 * i] * inv, o[n][4 * i + 1] * inv),
+                                                                    pack_hot<DT>(o[n][4 * i + 2] * inv, o[n][4 * i + 3] * inv));
+        }
+    if (half == 0 && p.lse) p.lse[row_head] = l == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// ---- pieces joined --------------------------------------------------------------
+// One wave per row and query head: the pieces' sums under one maximum.
+
+template <int DT>
+__global__ __launch_bounds__(256) void join_kernel(AttendParams p, bool many) {
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads);
+    const uint32_t rest = blockIdx.x / (uint32_t)p.kv_heads;
+    int s, block = 0;
+    if (!many) s = (int)rest;
+    else if (!find_unit(p, (int)rest, s, block)) return;
+    const Seq seq = seq_of(p.batch, s);
+    const int rows = seq.n_new * p.group;
+    if (!many && rows > p.few_rows) return;
+    const int n = live_splits(p, seq.len);
+    const int end = many ? min(rows, (block + 1) * kManyRows) : rows;
+    for (int r = block * kManyRows + wave; r < end; r += 4) {
+        const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
+        const float* src = partial_of(p, seq.row0 + token, q_head, 0);
+        const int64_t step = p.head_dim + 2;
+        float top = -INFINITY;
+        for (int i = lane; i < n; i += 64) top = fmaxf(top, src[i * step + p.head_dim]);
+        for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
+        const float base = top == -INFINITY ? 0.f : top;
+        float total = 0.f;
+        for (int i = lane; i < n; i += 64)
+            total += __builtin_amdgcn_exp2f(src[i * step + p.head_dim] - base) * src[i * step + p.head_dim + 1];
+        total = xor_sum(total, 64);
+        const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+        const int64_t row_head = (int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head;
+        for (int d = 2 * lane; d < p.head_dim; d += 128) {
+            float a = 0.f, b = 0.f;
+            for (int i = 0; i < n; ++i) {
+                const float w = __builtin_amdgcn_exp2f(src[i * step + p.head_dim] - base);
+                const float2 x = *reinterpret_cast<const float2*>(src + i * step + d);
+                a = __builtin_fmaf(w, x.x, a);
+                b = __builtin_fmaf(w, x.y, b);
+            }
+            *reinterpret_cast<uint32_t*>(p.out + 2 * (row_head * p.head_dim + d)) = pack_hot<DT>(a * inv, b * inv);
+        }
+        if (lane == 0 && p.lse) p.lse[row_head] = total == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(total)) * kLn2;
+    }
+}
+
+// ---- host -------------------------------------------------------------------------
+
+// How a call is cut: what the few and the many kernel take, and into how many pieces.
+struct Plan {
+    int nt;                         // 16-row tiles of the few kernel
+    int few_rows;                   // 0: no few kernel
+    bool many;
+    int64_t many_units;             // blocks of kManyRows rows at most
+    int few_splits, few_tokens, many_splits, many_tokens;
+    int partial_splits;             // 0: no pieces
+};
+
+int pieces(int64_t groups, int64_t max_tokens, int64_t wanted, int least, int& tokens) {
+    int64_t n = groups > 0 ? (wanted + groups - 1) / groups : 1;
+    const int64_t most = (max_tokens + least - 1) / least;
+    if (n > most) n = most;
+    if (n < 1) n = 1;
+    if (n > 64) n = 64;
+    int64_t t = (max_tokens + n - 1) / n;
+    t = (t + 127) / 128 * 128;
+    tokens = (int)t;
+    return (int)((max_tokens + t - 1) / t);
+}
+
+Plan plan_call(const ztcp_paged_batch* b, const ztcp_geometry* g, int64_t q_heads, int cus) {
+    Plan plan{};
+    const int64_t group = q_heads / g->num_heads;
+    const int64_t most_q = b->max_q_len > 0 && b->max_q_len < b->n_rows ? b->max_q_len : b->n_rows;
+    const int64_t most_rows = most_q * group, max_tokens = b->max_pages * g->num_tokens;
+    plan.nt = 1;
+    if (most_rows <= 64) {
+        plan.nt = most_rows <= 16 ? 1 : most_rows <= 32 ? 2 : 4;
+        plan.few_rows = 0x7FFFFFFF;
+    } else {
+        plan.nt = group <= 16 ? 1 : group <= 32 ? 2 : 4;
+        plan.few_rows = b->n_seqs > 1 && group <= 64 ? 16 * plan.nt : 0;
+        plan.many = true;
+        plan.many_units = (b->n_rows * group + kManyRows - 1) / kManyRows + b->n_seqs;
+    }
+    plan.few_splits = plan.many_splits = 1;
+    if (plan.few_rows) plan.few_splits = pieces(b->n_seqs * g->num_heads, max_tokens, (int64_t)cus * 12, 256, plan.few_tokens);
+    if (plan.many) plan.many_splits = pieces(plan.many_units * g->num_heads, max_tokens, (int64_t)cus * 2, 512, plan.many_tokens);
+    const int splits = plan.few_splits > plan.many_splits ? plan.few_splits : plan.many_splits;
+    plan.partial_splits = splits > 1 ? splits : 0;
+    return plan;
+}
+
+int cu_count(int& cus) {
+    int dev = 0;
+    return hipGetDevice(&dev) == hipSuccess &&
+                   hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && cus > 0
+               ? ZTCP_OK
+               : ZTCP_EHIP;
+}
+
+template <int DT, int DP>
+void launch(const AttendParams& base, const Plan& plan, float* workspace, hipStream_t stream) {
+    AttendParams p = base;
+    p.partial_splits = plan.partial_splits;
+    p.few_rows = plan.few_rows;
+    if (plan.few_rows) {
+        p.splits = plan.few_splits;
+        p.split_tokens = plan.few_splits > 1 ? plan.few_tokens : p.batch.max_tokens;
+        p.partial = plan.few_splits > 1 ? workspace : nullptr;
+        const uint32_t seq_heads = (uint32_t)p.batch.n_seqs * (uint32_t)p.kv_heads;
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(seq_heads * (uint32_t)p.splits), dim3(256), 0, stream, p);
+        };
+        if (plan.nt == 1) go(few_kernel<DT, DP, 1>);
+        else if (plan.nt == 2) go(few_kernel<DT, DP, 2>);
+        else go(few_kernel<DT, DP, 4>);
+        if (p.partial) hipLaunchKernelGGL(join_kernel<DT>, dim3(seq_heads), dim3(256), 0, stream, p, false);
+    }
+    if (plan.many) {
+        p.splits = plan.many_splits;
+        p.split_tokens = plan.many_splits > 1 ? plan.many_tokens : p.batch.max_tokens;
+        p.partial = plan.many_splits > 1 ? workspace : nullptr;
+        const uint32_t unit_heads = (uint32_t)(plan.many_units * p.kv_heads);
+        hipLaunchKernelGGL((many_kernel<DT, DP>), dim3(unit_heads * (uint32_t)p.splits), dim3(256), 0, stream, p);
+        if (p.partial) hipLaunchKernelGGL(join_kernel<DT>, dim3(unit_heads), dim3(256), 0, stream, p, true);
+    }
+}
+
+const char* check_all(const ztcp_paged_batch* b, const ztcp_page_pool* pool, const ztcp_geometry* g, int64_t q_heads,
+                      PagedView& view) {
+    if (const char* why = check_pool(pool, g, 256)) return why;
+    return check_batch(b, pool, g, q_heads, view);
+}
+
+}  // namespace
+
+extern "C" size_t ztcp_paged_attention_workspace(const ztcp_paged_batch* batch, const ztcp_page_pool* pool,
+                                                 const ztcp_geometry* g, int64_t q_heads) {
+    arg_result(ZTCP_OK, "");
+    PagedView view;
+    if (const char* why = check_all(batch, pool, g, q_heads, view)) {
+        arg_result(ZTCP_EINVAL, why);
+        return (size_t)-1;
+    }
+    int cus = 0;
+    if (cu_count(cus) != ZTCP_OK) return (size_t)-1;
+    const Plan plan = plan_call(batch, g, q_heads, cus);
+    return (size_t)batch->n_rows * q_heads * plan.partial_splits * (g->head_dim + 2) * sizeof(float);
+}
+
+extern "C" int ztcp_paged_attention(const void* q, int64_t q_stride, void* out, float* lse, int64_t q_heads,
+                                    const ztcp_page_pool* pool, const ztcp_paged_batch* batch, const ztcp_geometry* g,
+                                    float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    arg_result(ZTCP_OK, "");
+    AttendParams p{};
+    if (const char* why = check_all(batch, pool, g, q_heads, p.batch)) return arg_result(ZTCP_EINVAL, why);
+    if (!pool->v) return arg_result(ZTCP_EINVAL, "attention needs K and V pages (single-buffer pages have none)");
+    if (!(scale > 0.f) || isinf(scale)) return arg_result(ZTCP_EINVAL, "scale must be a positive finite number");
+    if (batch->n_seqs == 0 || batch->n_rows == 0) return ZTCP_OK;
+    if (!q || !out) return arg_result(ZTCP_EINVAL, "q and out must not be NULL");
+    if (!hot_aligned(q) || !hot_aligned(out) || q_stride % 8 != 0)
+        return arg_result(ZTCP_EINVAL, "q and out must be 16-byte aligned");
+    const int64_t d = g->head_dim, row = q_heads * d, page = 2 * g->num_tokens * g->num_heads * d;
+    if (batch->n_rows > 1 && q_stride < row) return arg_result(ZTCP_EINVAL, "q_stride must cover a token's heads");
+    const int64_t q_bytes = 2 * ((batch->n_rows - 1) * q_stride + row);
+    auto misses = [&](const void* x, int64_t bytes) {
+        return !bytes_overlap(x, bytes, q, q_bytes) &&
+               !rows_overlap(x, 1, bytes, bytes, pool->k, pool->n_pages, page, 2 * pool->k_stride) &&
+               !rows_overlap(x, 1, bytes, bytes, pool->v, pool->n_pages, page, 2 * pool->v_stride);
+    };
+    const int64_t out_bytes = 2 * batch->n_rows * row, lse_bytes = lse ? 4 * batch->n_rows * q_heads : 0;
+    int cus = 0;
+    if (cu_count(cus) != ZTCP_OK) return ZTCP_EHIP;
+    const Plan plan = plan_call(batch, g, q_heads, cus);
+    const int64_t need = batch->n_rows * q_heads * plan.partial_splits * (d + 2) * (int64_t)sizeof(float);
+    if (need > 0 && (!workspace || (int64_t)workspace_bytes < need || !hot_aligned(workspace)))
+        return arg_result(ZTCP_EINVAL, "workspace must hold ztcp_paged_attention_workspace bytes, 16-byte aligned");
+    if (!misses(out, out_bytes) || !misses(lse, lse_bytes) || !misses(need ? workspace : nullptr, need) ||
+        bytes_overlap(out, out_bytes, lse, lse_bytes) || bytes_overlap(workspace, need, out, out_bytes) ||
+        bytes_overlap(workspace, need, lse, lse_bytes))
+        return arg_result(ZTCP_EOVERLAP, "out, lse and workspace must not overlap q, the pages or each other");
+    const int64_t blocks = g->num_heads * (plan.many_units * plan.many_splits + batch->n_seqs * plan.few_splits);
+    if (blocks >= (int64_t)1 << 31) return arg_result(ZTCP_EINVAL, "too many sequences and heads in one call");
+    p.q = (const uint8_t*)q;
+    p.out = (uint8_t*)out;
+    p.lse = lse;
+    p.q_stride = q_stride;
+    p.k_pool = (const uint8_t*)pool->k;
+    p.v_pool = (const uint8_t*)pool->v;
+    p.k_page = pool->k_stride;
+    p.v_page = pool->v_stride;
+    p.kv_heads = (int32_t)g->num_heads;
+    p.group = (int32_t)(q_heads / g->num_heads);
+    p.head_dim = (int32_t)d;
+    p.scale_log2 = scale * kLog2e;
+    auto go = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (d <= 64) launch<DT, 64>(p, plan, (float*)workspace, (hipStream_t)stream);
+        else if (d <= 128) launch<DT, 128>(p, plan, (float*)workspace, (hipStream_t)stream);
+        else launch<DT, 256>(p, plan, (float*)workspace, (hipStream_t)stream);
+    };
+    if (g->hot_dtype == ZTCP_HOT_BF16) go(std::integral_constant<int, kHotBf16>{});
+    else go(std::integral_constant<int, kHotFp16>{});
+    return hipGetLastError() == hipSuccess ? ZTCP_OK : ZTCP_EHIP;
+}

@@ -1,0 +1,185 @@
+// ztcp_hot.h -- what the operators on hot pages share (append, attention,
+// page weights, eviction): argument checks on the host, page addressing and
+// wave reductions on the device.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/ztcp.h"
+#include "ztcp_device.h"
+#include "ztcp_layout.h"
+
+namespace ztcp {
+
+// Sets the message ztcp_last_error returns (ztcp_abi.hip) and returns rc.
+int arg_result(int rc, const char* why);
+
+// ---- host ------------------------------------------------------------------
+
+inline bool hot_aligned(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+// Whether two arrays of rows share a byte.  a: an rows of ab bytes, as_ bytes
+// apart; b likewise.  Rows of one stride are compared modulo it, so that
+// views side by side in one buffer do not count; otherwise by their extents.
+inline bool rows_overlap(const void* a, int64_t an, int64_t ab, int64_t as_, const void* b, int64_t bn, int64_t bb,
+                         int64_t bs) {
+    if (!a || !b || an <= 0 || bn <= 0 || ab <= 0 || bb <= 0) return false;
+    const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+    const uintptr_t ae = a0 + (uintptr_t)((an - 1) * as_ + ab), be = b0 + (uintptr_t)((bn - 1) * bs + bb);
+    if (!(a0 < be && b0 < ae)) return false;
+    if (as_ != bs || as_ < ab || bs < bb) return true;
+    const uint64_t d = b0 >= a0 ? (uint64_t)(b0 - a0) % (uint64_t)as_
+                                : ((uint64_t)as_ - (uint64_t)(a0 - b0) % (uint64_t)as_) % (uint64_t)as_;
+    return d < (uint64_t)ab || (uint64_t)as_ - d < (uint64_t)bb;
+}
+
+inline bool bytes_overlap(const void* a, int64_t an, const void* b, int64_t bn) {
+    return rows_overlap(a, 1, an, an, b, 1, bn, bn);
+}
+
+// Division of 0 <= x < 2^31 by a page's tokens (1 <= d < 2^31):
+// floor(x / d) = (x * mul) >> shift with mul = floor(2^shift / d) + 1,
+// shift = 31 + ceil(log2 d): the product's excess over x * 2^shift / d is below
+// x * d / d <= 2^31 <= 2^shift / d, too little to reach the next whole number.
+struct DivBy {
+    uint32_t mul;
+    uint32_t shift;
+};
+inline DivBy div_by(uint32_t d) {
+    uint32_t s = 0;
+    while (((uint64_t)1 << s) < d) ++s;
+    return DivBy{(uint32_t)(((uint64_t)1 << (31 + s)) / d + 1), 31 + s};
+}
+
+// What is wrong with a pool and its geometry, or nullptr.
+inline const char* check_pool(const ztcp_page_pool* pool, const ztcp_geometry* g, int64_t max_head_dim) {
+    if (!pool || !g) return "pool and geometry must not be NULL";
+    if (!(g->num_tokens > 0 && g->num_heads > 0 && g->head_dim >= 16 && g->head_dim % 16 == 0))
+        return "num_tokens, num_heads must be positive, head_dim a positive multiple of 16";
+    if (g->head_dim > max_head_dim) return max_head_dim > 256 ? "head_dim must be at most 1024" : "head_dim must be at most 256";
+    if (!(g->rope_dim >= 0 && g->rope_dim <= g->head_dim && g->rope_dim % 16 == 0)) return "Invalid rope_dim";
+    if (g->hot_dtype != ZTCP_HOT_FP16 && g->hot_dtype != ZTCP_HOT_BF16)
+        return "hot_dtype must be ZTCP_HOT_FP16 or ZTCP_HOT_BF16";
+    const int64_t limit = (int64_t)1 << 30;
+    if (g->num_tokens >= limit || g->num_heads >= limit || g->num_tokens * g->num_heads >= limit ||
+        g->num_tokens * g->num_heads * g->head_dim >= limit)
+        return "page too large (num_tokens * num_heads * head_dim must be below 2^30)";
+    const int64_t page = g->num_tokens * g->num_heads * g->head_dim;
+    if (pool->n_pages < 1 || pool->n_pages > (int64_t)0x7FFFFFFF) return "n_pages must be 1 .. 2^31 - 1";
+    if (!pool->k) return "the pool's k must not be NULL";
+    if (pool->n_pages > 1 && (pool->k_stride < page || (pool->v && pool->v_stride < page)))
+        return "page strides must cover a page";
+    if (!hot_aligned(pool->k) || !hot_aligned(pool->v) || (pool->k_stride | pool->v_stride) % 8 != 0)
+        return "pages must be 16-byte aligned";
+    return nullptr;
+}
+
+// A batch of sequences over a pool, as the kernels take it.
+struct PagedView {
+    const int32_t* table;
+    const int32_t* lens;
+    const int32_t* starts;
+    int64_t table_stride;
+    int32_t n_seqs, n_rows, n_pages;
+    int32_t max_tokens;          // max_pages * page tokens
+    int32_t page_tokens;
+    DivBy page_div;
+};
+
+// What is wrong with a batch, or nullptr; fills `view`.
+inline const char* check_batch(const ztcp_paged_batch* b, const ztcp_page_pool* pool, const ztcp_geometry* g,
+                               int64_t q_heads, PagedView& view) {
+    if (!b) return "batch must not be NULL";
+    const int64_t most = (int64_t)1 << 31;
+    if (b->n_seqs < 0 || b->n_seqs >= (int64_t)1 << 24 || b->n_rows < 0 || b->n_rows >= most || b->max_q_len < 0)
+        return "n_seqs must be 0 .. 2^24 - 1, n_rows 0 .. 2^31 - 1, max_q_len not negative";
+    if (q_heads < 1 || q_heads > 65536 || q_heads % g->num_heads != 0)
+        return "q_heads must be a positive multiple of num_heads, at most 65536";
+    if (b->max_pages < 1 || b->max_pages > (most - 1024) / g->num_tokens)
+        return "max_pages must be positive, max_pages * num_tokens below 2^31 - 1024";
+    if (b->n_rows * q_heads >= most) return "too many query heads in one call (n_rows * q_heads must be below 2^31)";
+    if (b->n_seqs > 0 && (!b->page_table || !b->kv_lens || !b->q_starts))
+        return "page_table, kv_lens and q_starts must not be NULL";
+    if (b->n_seqs > 1 && b->table_stride < b->max_pages) return "table_stride must cover max_pages";
+    view = PagedView{b->page_table, b->kv_lens, b->q_starts, b->table_stride, (int32_t)b->n_seqs, (int32_t)b->n_rows,
+                     (int32_t)pool->n_pages, (int32_t)(b->max_pages * g->num_tokens), (int32_t)g->num_tokens,
+                     div_by((uint32_t)g->num_tokens)};
+    return nullptr;
+}
+
+// ---- device ----------------------------------------------------------------
+
+__device__ __forceinline__ int div_page(int x, DivBy d) { return (int)(((uint64_t)(uint32_t)x * d.mul) >> d.shift); }
+
+// A sequence of the batch; whatever the arrays hold, its rows are rows of q and
+// its tokens have table entries.
+struct Seq {
+    int row0, n_new, len;
+    const int32_t* table;
+};
+__device__ __forceinline__ Seq seq_of(const PagedView& v, int s) {
+    const int a = v.starts[s], b = v.starts[s + 1], len = v.lens[s];
+    Seq q;
+    q.row0 = min(max(a, 0), v.n_rows);
+    q.n_new = min(max(b, q.row0), v.n_rows) - q.row0;
+    q.len = min(max(len, 0), v.max_tokens);
+    q.table = v.table + s * v.table_stride;
+    return q;
+}
+
+// Where token `key` (below `stop`) is: its page, -1 if there is none, and its row in the page.
+struct Place {
+    int page, row;
+};
+__device__ __forceinline__ Place place_of(const PagedView& v, const Seq& q, int key, int stop) {
+    Place p{-1, 0};
+    if (key < stop) {
+        const int at = div_page(key, v.page_div);
+        const int id = q.table[at];
+        if (id >= 0 && id < v.n_pages) p.page = id;
+        p.row = key - at * v.page_tokens;
+    }
+    return p;
+}
+
+// MFMA operands and results.
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// Products of 16-bit operands in fp32.  Lane l holds eight numbers of row (A)
+// or column (B) l % 16 (32), at depths (l / 16) * 8 + 0..7 ((l / 32) * 8 + 0..7);
+// the result has column l % 16 (32) and rows (l / 16) * 4 + i
+// (8 * (i / 4) + 4 * (l / 32) + i % 4).
+template <int DT>
+__device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
+    if constexpr (DT == kHotBf16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <int DT>
+__device__ __forceinline__ f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
+    if constexpr (DT == kHotBf16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Transposing LDS read of 16-bit numbers: the 16 lanes of a group give the
+// addresses of four rows of 16 numbers (lane i: row i / 4, numbers (i % 4) * 4
+// + 0..3), and lane i receives number i of the four rows.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint2 lds_read_transposed(const uint8_t* p) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+}
+
+__device__ __forceinline__ float xor_sum(float x, int width) {  // over aligned groups of `width` lanes
+    for (int m = 1; m < width; m <<= 1) x += __shfl_xor(x, m);
+    return x;
+}
+
+}  // namespace ztcp
