@@ -91,7 +91,7 @@ __device__ __forceinline__ f32x4 only_not_finite(const AttendParams& p, const Pl
 // Waves join their maxima, totals and sums at the end.
 
 template <int DT, int DP, int NT>
-__global__ __launch_bounds__(256) void few_kernel(AttendParams p) {
+__global__ __launch_bounds__(256, NT == 1 && DP <= 128 ? 2 : 1) void few_kernel(AttendParams p) {
     constexpr int kSteps = DP / 32, kChunks = DP / 8;         // products of depth 32; 16-byte pieces of a row
     constexpr int kVLoads = 32 * kChunks / 64;                // V loads of a lane for a tile
     constexpr int kVRows = 64 / kChunks;                      // rows a load covers
@@ -175,6 +175,7 @@ __global__ __launch_bounds__(256) void few_kernel(AttendParams p) {
             }
         };
         const int first_sees = max(0, seq.len - seq.n_new + r0 / p.group + 1);   // the row that sees least
+        bool apart = false;                                   // V numbers have to be added apart
         int kb = key0 + 32 * wave;
         if (kb < stop) {
             load(place_of(p.batch, seq, kb + (lane & 31), stop));
@@ -191,14 +192,9 @@ __global__ __launch_bounds__(256) void few_kernel(AttendParams p) {
 #pragma unroll
                     for (int i = 0; i < kSteps; ++i) sc[t][u] = mfma16<DT>(kf[u][i], qf[t][i], sc[t][u]);
                 }
-            uint32_t apart = 0;                               // keys with numbers to be added apart
             if (kb + 32 > first_sees && first_sees < stop) {
 #pragma unroll
-                for (int i = 0; i < kVLoads; ++i)
-                    if (drop_not_finite<DT>(vf[i])) apart |= 1u << (i * kVRows + v_row);
-                if (__any(apart != 0))
-                    for (int k = 1; k < 64; k <<= 1) apart |= __shfl_xor(apart, k);
-                apart &= here;
+                for (int i = 0; i < kVLoads; ++i) apart |= drop_not_finite<DT>(vf[i]);
             }
 #pragma unroll
             for (int i = 0; i < kVLoads; ++i) {
@@ -256,18 +252,20 @@ __global__ __launch_bounds__(256) void few_kernel(AttendParams p) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t) o[t][n] = mfma16<DT>(a, pf[t], o[t][n]);
             }
-            for (apart = __builtin_amdgcn_readfirstlane(apart); apart; apart &= apart - 1) {
-                const int key = kb + __ffs((int)apart) - 1;
+        }
+        if (__any(apart))                                     // of this wave's tiles
+            for (int key = max(key0, first_sees); key < stop; ++key) {
+                if ((key - key0) / 32 % 4 != wave) continue;
                 const Place where = place_of(p.batch, seq, key, stop);
 #pragma unroll
                 for (int n = 0; n < DP / 16; ++n) {
                     const f32x4 x = only_not_finite<DT>(p, where, head, 16 * n + 4 * quad);
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
-                        if (key < limit[t]) o[t][n] += x;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[t][n][e] += key < limit[t] ? x[e] : 0.f;
                 }
             }
-        }
         // join the four waves
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -364,20 +362,35 @@ __device__ __forceinline__ bool find_unit(const AttendParams& p, int unit, int& 
     return false;
 }
 
+// Zeros that the tile loads read in the place of tokens that are not there: a row of 256 elements.
+__device__ __attribute__((aligned(16))) uint32_t g_zeros[128];
+
+// One wave's 64 pieces of 16 bytes from global memory to LDS, piece i at lds + 16 i,
+// without passing through registers; done once vmcnt says so.  Written in asm
+// because the compiler, which cannot tell the two buffers apart, would wait for
+// the next tile's loads before this tile's reads.  It has no output register,
+// and nothing else here uses m0.
+__device__ __forceinline__ void load_lds16(const uint8_t* src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
+}
+
 template <int DT, int DP>
-__global__ __launch_bounds__(256) void many_kernel(AttendParams p) {
-    constexpr int kSteps = DP / 16, kChunks = DP / 8;
-    constexpr int kLoads = 64 * kChunks / 256;                // 16-byte pieces of K, and of V, a thread loads of a tile
-    constexpr int kRowsPerLoad = 256 / kChunks;               // rows the workgroup's one load covers
-    __shared__ __attribute__((aligned(16))) uint8_t kt[64 * DP * 2], vt[64 * DP * 2];
-    __shared__ uint32_t apart_lds[2];                         // keys of the tile with V numbers to be added apart
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void many_kernel(AttendParams p) {
+    constexpr int kTile = DP <= 128 ? 64 : 32;                // keys of a tile
+    constexpr int kSub = kTile / 32;
+    constexpr int kSteps = DP / 16, kChunks = DP / 8, kRowBytes = DP * 2, kTileBytes = kTile * kRowBytes;
+    constexpr int kLoadRows = 64 / kChunks;                   // rows of a wave's load
+    constexpr int kLoads = kTile / kLoadRows / 4;             // loads of a wave for a tile's K, and V
+    __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2][kTileBytes];   // [buffer][K, V]
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads);
     const uint32_t rest = blockIdx.x / (uint32_t)p.kv_heads;
     const int split = (int)(rest % (uint32_t)p.splits);
     int s, block;
     if (!find_unit(p, (int)(rest / (uint32_t)p.splits), s, block)) return;
+    s = __builtin_amdgcn_readfirstlane(s);
+    block = __builtin_amdgcn_readfirstlane(block);
     const Seq seq = seq_of(p.batch, s);
     const int rows = seq.n_new * p.group;
     if (split >= live_splits(p, seq.len)) return;
@@ -390,13 +403,13 @@ __global__ __launch_bounds__(256) void many_kernel(AttendParams p) {
     const int wave_stop = r0 < rows ? min(key1, sees(min(rows, r0 + 32) - 1)) : 0;       // of this wave
     const int first_sees = sees(block * kManyRows);                                      // the row that sees least
     const int wave_full = r0 + 32 <= rows ? sees(r0) : 0;                                // keys that all its rows see
+    // 16-byte pieces are permuted within a row so that the rows of one read lie in different banks
     auto k_swizzle = [](int row, int chunk) { return chunk ^ (row & (kChunks < 16 ? kChunks - 1 : 15)); };
     auto v_swizzle = [](int row, int chunk) {
         if constexpr (DP == 64) return chunk ^ (((row >> 1) & 1) << 2);
         else return chunk ^ ((row & 3) << 2);
     };
-    const int my_row = (int)threadIdx.x / kChunks, my_chunk = (int)threadIdx.x % kChunks;
-    const bool my_has = my_chunk * 8 < p.head_dim;
+    const int load_row = lane / kChunks, load_chunk = lane % kChunks;
 
     uint4 qf[kSteps];
     {
@@ -413,104 +426,118 @@ __global__ __launch_bounds__(256) void many_kernel(AttendParams p) {
     for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
-    uint4 kr[kLoads], vr[kLoads];
-    uint64_t valid = 0;
-    auto load = [&](const Place& at) {
-        const bool has = at.page >= 0;
-        valid = __ballot(has);
-        const int page = has ? at.page : 0, row = has ? at.row : 0;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int from = i * kRowsPerLoad + my_row;
-            const int64_t pg = __shfl(page, from), at_row = (int64_t)__shfl(row, from) * p.kv_heads + head;
-            const bool ok = my_has && ((valid >> from) & 1u);
-            kr[i] = ok ? ldg16(p.k_pool + 2 * (pg * p.k_page + at_row * p.head_dim) + 16 * my_chunk) : make_uint4(0, 0, 0, 0);
-            vr[i] = ok ? ldg16(p.v_pool + 2 * (pg * p.v_page + at_row * p.head_dim) + 16 * my_chunk) : make_uint4(0, 0, 0, 0);
-        }
+    // The page of lane's key of the tile at kb, not looked at before the tile's loads: a wait for it would be
+    // one for all loads before it
+    auto look_up = [&](int kb) {
+        const int key = kb + (lane & (kTile - 1));
+        return key < stop ? seq.table[div_page(key, p.batch.page_div)] : -1;
     };
-    Place next{-1, 0};
-    if (key0 < stop) {
-        load(place_of(p.batch, seq, key0 + lane, stop));
-        next = place_of(p.batch, seq, key0 + 64 + lane, stop);
-    }
-    for (int kb = key0; kb < stop; kb += 64) {
-        __syncthreads();   // the previous tile has been read
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)&tiles[0][0][0];
+    auto load = [&](int kb, int id, int buffer) {             // returns which keys are there
+        const int key = kb + (lane & (kTile - 1));
+        const int row = key - div_page(key, p.batch.page_div) * p.batch.page_tokens;
+        const bool has = id >= 0 && id < p.batch.n_pages;
+        const int64_t in_page = (int64_t)(row * p.kv_heads + head) * p.head_dim;
+        const uint8_t* zeros = reinterpret_cast<const uint8_t*>(g_zeros);
+        const uint64_t k = (uint64_t)(has ? p.k_pool + 2 * (id * p.k_page + in_page) : zeros);
+        const uint64_t v = (uint64_t)(has ? p.v_pool + 2 * (id * p.v_page + in_page) : zeros);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int row = i * kRowsPerLoad + my_row;
-            *reinterpret_cast<uint4*>(kt + row * DP * 2 + k_swizzle(row, my_chunk) * 16) = kr[i];
-            *reinterpret_cast<uint4*>(vt + row * DP * 2 + v_swizzle(row, my_chunk) * 16) = vr[i];
+            const int first = (wave * kLoads + i) * kLoadRows, from = first + load_row;
+            const int kc = k_swizzle(from, load_chunk), vc = v_swizzle(from, load_chunk);
+            const uint8_t* ka = (const uint8_t*)__shfl(k, from) + 16 * kc;
+            const uint8_t* va = (const uint8_t*)__shfl(v, from) + 16 * vc;
+            if (p.head_dim < DP) {                            // columns behind head_dim are zeros
+                ka = kc * 8 < p.head_dim ? ka : zeros;
+                va = vc * 8 < p.head_dim ? va : zeros;
+            }
+            const uint32_t to = lds0 + (uint32_t)(2 * buffer * kTileBytes + first * kRowBytes);
+            load_lds16(ka, to);
+            load_lds16(va, to + kTileBytes);
         }
+        return __ballot(has);
+    };
+    bool apart = false;                                       // V numbers have to be added apart
+    uint64_t valid = 0;
+    int next = -1;
+    if (key0 < stop) {
+        const int id = look_up(key0);
+        next = look_up(key0 + kTile);
+        valid = load(key0, id, 0);
+    }
+    int buffer = 0;
+    for (int kb = key0; kb < stop; kb += kTile, buffer ^= 1) {
+        __builtin_amdgcn_s_waitcnt(0);                        // this wave's share of the tile
+        __syncthreads();                                      // everyone's; and the other buffer has been read
         const uint64_t here = valid;
-        __syncthreads();
-        if (kb + 64 < stop) {
-            load(next);
-            next = place_of(p.batch, seq, kb + 128 + lane, stop);
+        if (kb + kTile < stop) {
+            const int id = next;
+            next = look_up(kb + 2 * kTile);
+            valid = load(kb + kTile, id, buffer ^ 1);
         }
-        uint64_t apart = 0;
-        if (kb + 64 > first_sees && first_sees < stop) {
-            if (threadIdx.x < 2) apart_lds[threadIdx.x] = 0;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const int row = i * kRowsPerLoad + my_row;
-                uint4* at = reinterpret_cast<uint4*>(vt + row * DP * 2 + v_swizzle(row, my_chunk) * 16);
+        const uint8_t* kt = tiles[buffer][0];
+        uint8_t* vt = tiles[buffer][1];
+        if (kb + kTile > first_sees && first_sees < stop) {
+            bool dropped = false;
+            for (int i = (int)threadIdx.x; i < kTileBytes / 16; i += 256) {
+                uint4* at = reinterpret_cast<uint4*>(vt) + i;
                 uint4 x = *at;
                 if (drop_not_finite<DT>(x)) {
                     *at = x;
-                    atomicOr(&apart_lds[row / 32], 1u << (row % 32));
+                    dropped = true;
                 }
             }
-            __syncthreads();
-            apart = (uint64_t)__builtin_amdgcn_readfirstlane(apart_lds[0]) |
-                    (uint64_t)__builtin_amdgcn_readfirstlane(apart_lds[1]) << 32;
+            apart |= __syncthreads_or(dropped) != 0;
         }
         if (kb >= wave_stop) continue;
-        f32x16 sc[2];
+        f32x16 sc[kSub];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < kSub; ++u) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[u][i] = 0.f;
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 const int row = 32 * u + col;
-                const uint4 a = *reinterpret_cast<const uint4*>(kt + row * DP * 2 + k_swizzle(row, 2 * i + half) * 16);
+                const uint4 a = *reinterpret_cast<const uint4*>(kt + row * kRowBytes + k_swizzle(row, 2 * i + half) * 16);
                 sc[u] = mfma32<DT>(a, qf[i], sc[u]);
             }
         }
-        if (kb + 64 > wave_full || here != ~0ull) {
+        if (kb + kTile > wave_full || here != ~0ull) {
+            const int before = limit - kb - 4 * half;         // keys 32 u + 8 (i / 4) + i % 4 of this lane that its row sees
+            const uint64_t seen = (here >> (4 * half)) & (before >= 64 ? ~0ull : before > 0 ? (1ull << before) - 1 : 0ull);
+            const uint32_t bits[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < kSub; ++u)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int key = 32 * u + 8 * (i / 4) + 4 * half + i % 4;
-                    if (!((here >> key) & 1u) || kb + key >= limit) sc[u][i] = -INFINITY;
-                }
+                for (int i = 0; i < 16; ++i)
+                    if (!(bits[u] & (1u << (8 * (i / 4) + i % 4)))) sc[u][i] = -INFINITY;
         }
         float top = sc[0][0];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < kSub; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[u][i]);
         top = fmaxf(top, __shfl_xor(top, 32)) * p.scale_log2;
-        const float m_new = fmaxf(m, top);
-        const float base = m_new == -INFINITY ? 0.f : m_new;
-        if (__any(m_new != m)) {
-            const float fade = __builtin_amdgcn_exp2f(m - base);
+        // The reference of the exponentials follows the maximum only when that has
+        // grown by 2^8: weights up to 256 lose nothing in fp32 sums and 16-bit operands.
+        if (__any(top > m + 8.f)) {
+            const float m_new = fmaxf(m, top);
+            const float fade = m_new == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+            m = m_new;
             l *= fade;
 #pragma unroll
             for (int n = 0; n < DP / 32; ++n) o[n] *= fade;
         }
-        m = m_new;
+        const float base = m == -INFINITY ? 0.f : m;          // no key seen yet: every power is 0
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < kSub; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 sc[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i], p.scale_log2, -base));
                 l += sc[u][i];
             }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < 2 * kSub; ++u) {
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = pack_hot<DT>(sc[u / 2][8 * (u & 1) + 2 * i], sc[u / 2][8 * (u & 1) + 2 * i + 1]);
@@ -522,13 +549,14 @@ __global__ __launch_bounds__(256) void many_kernel(AttendParams p) {
                 for (int j = 0; j < 2; ++j) {
                     const int row = 16 * u + 8 * j + 4 * half + (lane & 15) / 4;
                     const int chunk = 4 * n + 2 * ((lane >> 4) & 1) + (lane & 3) / 2;
-                    v[j] = lds_read_transposed(vt + row * DP * 2 + v_swizzle(row, chunk) * 16 + (lane & 1) * 8);
+                    v[j] = lds_read_transposed(vt + row * kRowBytes + v_swizzle(row, chunk) * 16 + (lane & 1) * 8);
                 }
                 o[n] = mfma32<DT>(make_uint4(v[0].x, v[0].y, v[1].x, v[1].y), pf, o[n]);
             }
         }
-        for (; apart; apart &= apart - 1) {
-            const int key = kb + __ffsll((unsigned long long)apart) - 1;
+    }
+    if (apart)
+        for (int key = max(key0, first_sees); key < stop; ++key) {
             const Place where = place_of(p.batch, seq, key, stop);
 #pragma unroll
             for (int n = 0; n < DP / 32; ++n)
@@ -536,11 +564,9 @@ __global__ __launch_bounds__(256) void many_kernel(AttendParams p) {
                 for (int i = 0; i < 4; ++i) {
                     const f32x4 x = only_not_finite<DT>(p, where, head, 32 * n + 8 * i + 4 * half);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (key < limit) o[n][4 * i + e] += x[e];
+                    for (int e = 0; e < 4; ++e) o[n][4 * i + e] += key < limit ? x[e] : 0.f;
                 }
         }
-    }
     l += __shfl_xor(l, 32);
     if (r >= rows) return;
     const int64_t row_head = (int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head;
