@@ -333,6 +333,7 @@ __global__ __launch_bounds__(256, NT == 1 && DP <= 128 ? 2 : 1) void few_kernel(
 // read by all four, the next one on its way in registers meanwhile.
 
 constexpr int kManyRows = 128;
+constexpr int many_tile(int dp) { return dp <= 128 ? 64 : 32; }
 
 // The unit-th block of kManyRows rows of the batch's sequences of more than
 // p.few_rows rows; false if there are fewer.
@@ -373,25 +374,33 @@ __device__ __attribute__((aligned(16))) uint32_t g_zeros[128];
 __device__ __forceinline__ void load_lds16(const uint8_t* src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
 }
+// The same from a wave's own base and each lane's offset.
+__device__ __forceinline__ void load_lds16(const uint8_t* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
 
-template <int DT, int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void many_kernel(AttendParams p) {
-    constexpr int kTile = DP <= 128 ? 64 : 32;                // keys of a tile
+// EVEN: a wave's quarter of a tile never crosses a page and rows fill DP, so that the quarter's address is
+// one scalar; otherwise every lane has its own.
+template <int DT, int DP, bool EVEN>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1, DP <= 128 ? 2 : 1)))
+void many_kernel(AttendParams p) {
+    constexpr int kTile = many_tile(DP);                      // keys of a tile
+    constexpr int kShare = kTile / 4;                         // of which a wave loads so many
     constexpr int kSub = kTile / 32;
     constexpr int kSteps = DP / 16, kChunks = DP / 8, kRowBytes = DP * 2, kTileBytes = kTile * kRowBytes;
     constexpr int kLoadRows = 64 / kChunks;                   // rows of a wave's load
-    constexpr int kLoads = kTile / kLoadRows / 4;             // loads of a wave for a tile's K, and V
+    constexpr int kLoads = kShare / kLoadRows;                // loads of a wave for a tile's K, and V
     __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2][kTileBytes];   // [buffer][K, V]
-    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int lane = (int)threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads);
     const uint32_t rest = blockIdx.x / (uint32_t)p.kv_heads;
     const int split = (int)(rest % (uint32_t)p.splits);
     int s, block;
     if (!find_unit(p, (int)(rest / (uint32_t)p.splits), s, block)) return;
-    s = __builtin_amdgcn_readfirstlane(s);
-    block = __builtin_amdgcn_readfirstlane(block);
-    const Seq seq = seq_of(p.batch, s);
+    s = uniform(s);
+    block = uniform(block);
+    const Seq seq = uniform(seq_of(p.batch, s));
     const int rows = seq.n_new * p.group;
     if (split >= live_splits(p, seq.len)) return;
     const int key0 = split * p.split_tokens, key1 = key0 + min(seq.len - key0, p.split_tokens);
@@ -420,91 +429,178 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void many_kernel(AttendPara
             qf[i] = r < rows && d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
         }
     }
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l[2] = {0.f, 0.f};
     f32x16 o[DP / 32];
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
-    // The page of lane's key of the tile at kb, not looked at before the tile's loads: a wait for it would be
-    // one for all loads before it
-    auto look_up = [&](int kb) {
+
+    // Where a tile's keys are, lane = key: table entries as they were read, looked at a tile later.  What is not
+    // there is loaded from the pool's page 0 and taken out of the V tile afterwards.
+    struct Where {
+        int page, row;                                        // EVEN: of this wave's quarter; else of the lane's key
+        uint64_t here;                                        // which keys are there
+    };
+    auto fetch = [&](int kb) {
         const int key = kb + (lane & (kTile - 1));
         return key < stop ? seq.table[div_page(key, p.batch.page_div)] : -1;
     };
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)&tiles[0][0][0];
-    auto load = [&](int kb, int id, int buffer) {             // returns which keys are there
+    auto where = [&](int entry, int kb) {
         const int key = kb + (lane & (kTile - 1));
-        const int row = key - div_page(key, p.batch.page_div) * p.batch.page_tokens;
-        const bool has = id >= 0 && id < p.batch.n_pages;
-        const int64_t in_page = (int64_t)(row * p.kv_heads + head) * p.head_dim;
-        const uint8_t* zeros = reinterpret_cast<const uint8_t*>(g_zeros);
-        const uint64_t k = (uint64_t)(has ? p.k_pool + 2 * (id * p.k_page + in_page) : zeros);
-        const uint64_t v = (uint64_t)(has ? p.v_pool + 2 * (id * p.v_page + in_page) : zeros);
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int first = (wave * kLoads + i) * kLoadRows, from = first + load_row;
-            const int kc = k_swizzle(from, load_chunk), vc = v_swizzle(from, load_chunk);
-            const uint8_t* ka = (const uint8_t*)__shfl(k, from) + 16 * kc;
-            const uint8_t* va = (const uint8_t*)__shfl(v, from) + 16 * vc;
-            if (p.head_dim < DP) {                            // columns behind head_dim are zeros
-                ka = kc * 8 < p.head_dim ? ka : zeros;
-                va = vc * 8 < p.head_dim ? va : zeros;
-            }
-            const uint32_t to = lds0 + (uint32_t)(2 * buffer * kTileBytes + first * kRowBytes);
-            load_lds16(ka, to);
-            load_lds16(va, to + kTileBytes);
-        }
-        return __ballot(has);
+        const bool present = (uint32_t)entry < (uint32_t)p.batch.n_pages;
+        const int page = present ? entry : 0, row = key - div_page(key, p.batch.page_div) * p.batch.page_tokens;
+        const uint64_t here = __ballot(present);
+        if constexpr (EVEN)
+            return Where{__builtin_amdgcn_readlane(page, wave * kShare), __builtin_amdgcn_readlane(row, wave * kShare), here};
+        else return Where{page, row, here};
     };
-    bool apart = false;                                       // V numbers have to be added apart
-    uint64_t valid = 0;
-    int next = -1;
-    if (key0 < stop) {
-        const int id = look_up(key0);
-        next = look_up(key0 + kTile);
-        valid = load(key0, id, 0);
-    }
-    int buffer = 0;
-    for (int kb = key0; kb < stop; kb += kTile, buffer ^= 1) {
-        __builtin_amdgcn_s_waitcnt(0);                        // this wave's share of the tile
-        __syncthreads();                                      // everyone's; and the other buffer has been read
-        const uint64_t here = valid;
-        if (kb + kTile < stop) {
-            const int id = next;
-            next = look_up(kb + 2 * kTile);
-            valid = load(kb + kTile, id, buffer ^ 1);
-        }
-        const uint8_t* kt = tiles[buffer][0];
-        uint8_t* vt = tiles[buffer][1];
-        if (kb + kTile > first_sees && first_sees < stop) {
-            bool dropped = false;
-            for (int i = (int)threadIdx.x; i < kTileBytes / 16; i += 256) {
-                uint4* at = reinterpret_cast<uint4*>(vt) + i;
-                uint4 x = *at;
-                if (drop_not_finite<DT>(x)) {
-                    *at = x;
-                    dropped = true;
-                }
+    constexpr uint64_t kAll = ~0ull;                          // (tiles of 32 keys: both halves of the lanes)
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)&tiles[0][0][0];
+    const uint32_t row_bytes = 2u * (uint32_t)p.kv_heads * (uint32_t)p.head_dim;         // from a token to the next
+    // This wave's quarter of a tile of K (which = 0) or V (1) into a buffer
+    auto load = [&](const Where& at, int buffer, auto which) {
+        constexpr bool is_v = decltype(which)::value != 0;
+        const uint8_t* pool = is_v ? p.v_pool : p.k_pool;
+        const int64_t page_step = is_v ? p.v_page : p.k_page;
+        auto swizzle = [&](int row, int chunk) { return is_v ? v_swizzle(row, chunk) : k_swizzle(row, chunk); };
+        const uint32_t to = lds0 + (uint32_t)((2 * buffer + (is_v ? 1 : 0)) * kTileBytes + wave * kShare * kRowBytes);
+        if constexpr (EVEN) {
+            const uint8_t* src = pool + 2 * (at.page * page_step + (int64_t)(at.row * p.kv_heads + head) * DP);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                load_lds16(src + (uint64_t)(i * kLoadRows) * row_bytes,
+                           load_row * row_bytes + 16 * swizzle(wave * kShare + i * kLoadRows + load_row, load_chunk),
+                           to + i * kLoadRows * kRowBytes);
+        } else {
+            const uint64_t mine = (uint64_t)(pool + 2 * (at.page * page_step + (int64_t)(at.row * p.kv_heads + head) * p.head_dim));
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int from = wave * kShare + i * kLoadRows + load_row, chunk = swizzle(from, load_chunk);
+                const uint8_t* src = (const uint8_t*)__shfl(mine, from) + 16 * chunk;
+                if (chunk * 8 >= p.head_dim) src = reinterpret_cast<const uint8_t*>(g_zeros);   // columns behind head_dim
+                load_lds16(src, to + i * kLoadRows * kRowBytes);
             }
-            apart |= __syncthreads_or(dropped) != 0;
         }
-        if (kb >= wave_stop) continue;
+    };
+    using IsK = std::integral_constant<int, 0>;
+    using IsV = std::integral_constant<int, 1>;
+
+    // What a tile's products read of LDS: addresses that differ by constants only
+    uint32_t k_at[kSteps], v_at[DP / 32];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) k_at[i] = (uint32_t)(col * kRowBytes + k_swizzle(col, 2 * i + half) * 16);
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) {
+        const int row = 4 * half + (lane & 15) / 4;
+        v_at[n] = (uint32_t)(row * kRowBytes + v_swizzle(row, 4 * n + 2 * ((lane >> 4) & 1) + (lane & 3) / 2) * 16 + (lane & 1) * 8);
+    }
+    bool apart = false;                                       // V numbers have to be added apart
+    int entry = -1;                                           // of the next tile
+    uint64_t before = 0;                                      // keys of the previous tile
+    uint32_t pw[8 * kSub];                                    // the previous tile's weights, two a word
+    Where at{};                                               // of this tile
+    auto weigh = [&](const f32x16 (&sc)[kSub], float base, int w) {
+        float x[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[w / 8][2 * (w % 8) + e], p.scale_log2, -base));
+            l[e] += x[e];
+        }
+        pw[w] = pack_hot<DT>(x[0], x[1]);
+        asm volatile("" : "+v"(pw[w]), "+v"(l[0]), "+v"(l[1]));              // here, not where the next tile uses it
+    };
+    constexpr int kProducts = 2 * kSub * (DP / 32), kAhead = 4;
+    // Products with V of the tile whose weights pw are made, and (WEIGH) this tile's weights from its scores sc:
+    // a 16-key group's weights take the place of the previous tile's once their products have been issued, so
+    // that the wave has products and vector work at the same time.  LDS reads run four products ahead; the
+    // barriers keep the compiler from putting each read right before its product.
+    auto products = [&](int v_buffer, f32x16 (&sc)[kSub], float base, auto weigh_c) {
+        constexpr bool kWeigh = decltype(weigh_c)::value;
+        const uint8_t* vt = tiles[v_buffer][1];
+        uint4 vf[kAhead + 1];
+        auto read_v = [&](int k) {
+            const uint8_t* src = vt + v_at[k % (DP / 32)] + 16 * (k / (DP / 32)) * kRowBytes;
+            const uint2 x = lds_read_transposed(src), y = lds_read_transposed(src + 8 * kRowBytes);
+            vf[k % (kAhead + 1)] = make_uint4(x.x, x.y, y.x, y.y);
+        };
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) read_v(k);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < kProducts + DP / 32; ++k) {
+            const int u = k / (DP / 32), n = k % (DP / 32);
+            if (k + kAhead < kProducts) read_v(k + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+            if (k < kProducts)
+                o[n] = mfma32<DT>(vf[k % (kAhead + 1)], make_uint4(pw[4 * u], pw[4 * u + 1], pw[4 * u + 2], pw[4 * u + 3]), o[n]);
+            if (kWeigh && u > 0)
+#pragma unroll
+                for (int w = 4 * (u - 1); w < 4 * u; ++w)
+                    if ((w - 4 * (u - 1)) * (DP / 32) / 4 == n) weigh(sc, base, w);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // Takes out of a V tile what must not reach its products
+    auto mend = [&](int kb, int v_buffer, uint64_t there) {
+        if (there == kAll && !(kb + kTile > first_sees && first_sees < stop)) return;
+        bool dropped = false;
+        for (int i = (int)threadIdx.x; i < kTileBytes / 16; i += 256) {
+            uint4* piece = reinterpret_cast<uint4*>(tiles[v_buffer][1]) + i;
+            uint4 x = *piece;
+            if (!((there >> (i / kChunks)) & 1u)) *piece = make_uint4(0, 0, 0, 0);
+            else if (first_sees < stop && drop_not_finite<DT>(x)) {
+                *piece = x;
+                dropped = true;
+            }
+        }
+        apart |= __syncthreads_or(dropped) != 0;
+    };
+    // One tile: its scores, the previous tile's products and its own weights.
+    auto step = [&](int kb, auto buffer_c, auto first_c) {
+        constexpr int buffer = decltype(buffer_c)::value;
+        constexpr bool kFirst = decltype(first_c)::value;
+        __builtin_amdgcn_s_waitcnt(0);                        // this wave's share of this tile's K and the last one's V
+        __syncthreads();                                      // everyone's; and what is loaded over has been read
+        const Where next = where(entry, kb + kTile);
+        entry = fetch(kb + 2 * kTile);
+        if (kb + kTile < stop) load(next, buffer ^ 1, IsK{});
+        load(at, buffer, IsV{});
+        if (!kFirst) mend(kb - kTile, buffer ^ 1, before);
+        before = at.here;
+        at = next;
         f32x16 sc[kSub];
+        if (kb >= wave_stop) {
+            if (!kFirst && kb - kTile < wave_stop) products(buffer ^ 1, sc, 0.f, std::false_type{});
+            return;
+        }
+        {
+            const uint8_t* kt = tiles[buffer][0];
+            uint4 kf[3][kSub];
+            auto read_k = [&](int i) {
 #pragma unroll
-        for (int u = 0; u < kSub; ++u) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sc[u][i] = 0.f;
+                for (int u = 0; u < kSub; ++u) kf[i % 3][u] = *reinterpret_cast<const uint4*>(kt + k_at[i] + 32 * u * kRowBytes);
+            };
+            read_k(0);
+            read_k(1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
-                const int row = 32 * u + col;
-                const uint4 a = *reinterpret_cast<const uint4*>(kt + row * kRowBytes + k_swizzle(row, 2 * i + half) * 16);
-                sc[u] = mfma32<DT>(a, qf[i], sc[u]);
+                if (i + 2 < kSteps) read_k(i + 2);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < kSub; ++u) {
+                    if (i == 0)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
+                    sc[u] = mfma32<DT>(kf[i % 3][u], qf[i], sc[u]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (kb + kTile > wave_full || here != ~0ull) {
-            const int before = limit - kb - 4 * half;         // keys 32 u + 8 (i / 4) + i % 4 of this lane that its row sees
-            const uint64_t seen = (here >> (4 * half)) & (before >= 64 ? ~0ull : before > 0 ? (1ull << before) - 1 : 0ull);
+        if (kb + kTile > wave_full || before != kAll) {       // (before: this tile's keys by now)
+            const int most = limit - kb - 4 * half;           // keys 32 u + 8 (i / 4) + i % 4 of this lane that its row sees
+            const uint64_t seen = (before >> (4 * half)) & (most >= 64 ? ~0ull : most > 0 ? (1ull << most) - 1 : 0ull);
             const uint32_t bits[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
 #pragma unroll
             for (int u = 0; u < kSub; ++u)
@@ -512,62 +608,72 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void many_kernel(AttendPara
                 for (int i = 0; i < 16; ++i)
                     if (!(bits[u] & (1u << (8 * (i / 4) + i % 4)))) sc[u][i] = -INFINITY;
         }
-        float top = sc[0][0];
+        float tops[4];                                        // four chains, not one of 16 dependent steps
 #pragma unroll
-        for (int u = 0; u < kSub; ++u)
+        for (int e = 0; e < 4; ++e) {
+            tops[e] = sc[0][e];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[u][i]);
-        top = fmaxf(top, __shfl_xor(top, 32)) * p.scale_log2;
+            for (int i = e; i < 16 * kSub; i += 4) tops[e] = fmaxf(tops[e], sc[i / 16][i % 16]);
+        }
+        const float top = max_halves(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))) * p.scale_log2;
         // The reference of the exponentials follows the maximum only when that has
         // grown by 2^8: weights up to 256 lose nothing in fp32 sums and 16-bit operands.
-        if (__any(top > m + 8.f)) {
+        const bool grown = __any(top > m + 8.f);
+        float fade = 1.f;
+        if (grown) {
             const float m_new = fmaxf(m, top);
-            const float fade = m_new == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+            fade = m_new == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
             m = m_new;
-            l *= fade;
-#pragma unroll
-            for (int n = 0; n < DP / 32; ++n) o[n] *= fade;
+            l[0] *= fade;
+            l[1] *= fade;
         }
         const float base = m == -INFINITY ? 0.f : m;          // no key seen yet: every power is 0
+        if constexpr (kFirst) {
 #pragma unroll
-        for (int u = 0; u < kSub; ++u)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                sc[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i], p.scale_log2, -base));
-                l += sc[u][i];
-            }
-#pragma unroll
-        for (int u = 0; u < 2 * kSub; ++u) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = pack_hot<DT>(sc[u / 2][8 * (u & 1) + 2 * i], sc[u / 2][8 * (u & 1) + 2 * i + 1]);
-            const uint4 pf = make_uint4(w[0], w[1], w[2], w[3]);
-#pragma unroll
-            for (int n = 0; n < DP / 32; ++n) {
-                uint2 v[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int row = 16 * u + 8 * j + 4 * half + (lane & 15) / 4;
-                    const int chunk = 4 * n + 2 * ((lane >> 4) & 1) + (lane & 3) / 2;
-                    v[j] = lds_read_transposed(vt + row * kRowBytes + v_swizzle(row, chunk) * 16 + (lane & 1) * 8);
-                }
-                o[n] = mfma32<DT>(make_uint4(v[0].x, v[0].y, v[1].x, v[1].y), pf, o[n]);
-            }
+            for (int w = 0; w < 8 * kSub; ++w) weigh(sc, base, w);
+        } else {
+            products(buffer ^ 1, sc, base, std::true_type{});
         }
+        if (grown)                                            // the sums are relative to the old reference up to here
+#pragma unroll
+            for (int n = 0; n < DP / 32; ++n) o[n] *= fade;
+    };
+    if (key0 < stop) {
+        at = where(fetch(key0), key0);
+        entry = fetch(key0 + kTile);
+        load(at, 0, IsK{});
+        using B0 = std::integral_constant<int, 0>;
+        using B1 = std::integral_constant<int, 1>;
+        int kb = key0, last = 0;
+        step(kb, B0{}, std::true_type{});
+        for (kb += kTile; kb < stop; kb += kTile) {
+            step(kb, B1{}, std::false_type{});
+            last = 1;
+            if ((kb += kTile) >= stop) break;
+            step(kb, B0{}, std::false_type{});
+            last = 0;
+        }
+        // the last tile's products
+        const int end = key0 + (stop - 1 - key0) / kTile * kTile;
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        mend(end, last, before);
+        f32x16 none[kSub];
+        if (end < wave_stop) products(last, none, 0.f, std::false_type{});
     }
     if (apart)
         for (int key = max(key0, first_sees); key < stop; ++key) {
-            const Place where = place_of(p.batch, seq, key, stop);
+            const Place from = place_of(p.batch, seq, key, stop);
 #pragma unroll
             for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const f32x4 x = only_not_finite<DT>(p, where, head, 32 * n + 8 * i + 4 * half);
+                    const f32x4 x = only_not_finite<DT>(p, from, head, 32 * n + 8 * i + 4 * half);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[n][4 * i + e] += key < limit ? x[e] : 0.f;
                 }
         }
-    l += __shfl_xor(l, 32);
+    const float total = sum_halves(l[0] + l[1]);
     if (r >= rows) return;
     const int64_t row_head = (int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head;
     const float base = m == -INFINITY ? 0.f : m;
@@ -585,11 +691,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void many_kernel(AttendPara
             }
         if (half == 0) {
             dst[p.head_dim] = m;
-            dst[p.head_dim + 1] = l;
+            dst[p.head_dim + 1] = total;
         }
         return;
     }
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
     uint8_t* dst = p.out + 2 * row_head * p.head_dim;
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n)
@@ -600,7 +706,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void many_kernel(AttendPara
                 *reinterpret_cast<uint2*>(dst + 2 * d) = make_uint2(pack_hot<DT>(o[n][4 * i] * inv, o[n][4 * i + 1] * inv),
                                                                     pack_hot<DT>(o[n][4 * i + 2] * inv, o[n][4 * i + 3] * inv));
         }
-    if (half == 0 && p.lse) p.lse[row_head] = l == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(l)) * kLn2;
+    if (half == 0 && p.lse) p.lse[row_head] = total == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
 // ---- pieces joined --------------------------------------------------------------
@@ -725,7 +831,11 @@ void launch(const AttendParams& base, const Plan& plan, float* workspace, hipStr
         p.split_tokens = plan.many_splits > 1 ? plan.many_tokens : p.batch.max_tokens;
         p.partial = plan.many_splits > 1 ? workspace : nullptr;
         const uint32_t unit_heads = (uint32_t)(plan.many_units * p.kv_heads);
-        hipLaunchKernelGGL((many_kernel<DT, DP>), dim3(unit_heads * (uint32_t)p.splits), dim3(256), 0, stream, p);
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(unit_heads * (uint32_t)p.splits), dim3(256), 0, stream, p);
+        };
+        if (p.batch.page_tokens % (many_tile(DP) / 4) == 0 && p.head_dim == DP) go(many_kernel<DT, DP, true>);
+        else go(many_kernel<DT, DP, false>);
         if (p.partial) hipLaunchKernelGGL(join_kernel<DT>, dim3(unit_heads), dim3(256), 0, stream, p, true);
     }
 }

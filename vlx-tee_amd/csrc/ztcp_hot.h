@@ -119,6 +119,16 @@ struct Seq {
     int row0, n_new, len;
     const int32_t* table;
 };
+// A value that every lane of the wave has, in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+template <class T>
+__device__ __forceinline__ T* uniform(T* p) {
+    const uint64_t x = (uint64_t)p;
+    return (T*)((uint64_t)(uint32_t)uniform((int)(uint32_t)x) | (uint64_t)(uint32_t)uniform((int)(uint32_t)(x >> 32)) << 32);
+}
+__device__ __forceinline__ Seq uniform(Seq q) {
+    return Seq{uniform(q.row0), uniform(q.n_new), uniform(q.len), uniform(q.table)};
+}
 __device__ __forceinline__ Seq seq_of(const PagedView& v, int s) {
     const int a = v.starts[s], b = v.starts[s + 1], len = v.lens[s];
     Seq q;
@@ -175,6 +185,17 @@ __device__ __forceinline__ f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint2 lds_read_transposed(const uint8_t* p) {
     return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+}
+
+// The larger, and the sum, of a lane's number and that of the lane 32 further on.
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float max_halves(float x) {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r.x) + __uint_as_float(r.y);
 }
 
 __device__ __forceinline__ float xor_sum(float x, int width) {  // over aligned groups of `width` lanes
