@@ -33,13 +33,13 @@ struct AttendParams {
     int32_t kv_heads, group, head_dim;
     float scale_log2;                // scale * log2(e): exponentials are powers of two
     int32_t few_rows;                // sequences of at most so many rows are the few kernel's, others the many kernel's
-    int32_t splits, split_tokens;    // pieces of a sequence's tokens, and tokens of a piece
-    float* partial;                  // [row, query head, partial_splits, head_dim + 2]: sums, maximum, total
-    int32_t partial_splits;
+    int32_t few_groups;              // few kernel: workgroups of a KV head
+    int32_t splits, split_tokens;    // many kernel: pieces of a sequence's tokens, and tokens of a piece
+    float* partial;                  // results of pieces: sums [head_dim], maximum, total
 };
 
-__device__ __forceinline__ float* partial_of(const AttendParams& p, int row, int q_head, int split) {
-    return p.partial + (((int64_t)row * p.kv_heads * p.group + q_head) * p.partial_splits + split) * (p.head_dim + 2);
+__device__ __forceinline__ float* many_partial(const AttendParams& p, int row, int q_head, int split) {
+    return p.partial + (((int64_t)row * p.kv_heads * p.group + q_head) * p.splits + split) * (p.head_dim + 2);
 }
 
 // Pieces of a sequence that have tokens (one at least: it answers for a sequence without tokens).
@@ -83,33 +83,93 @@ __device__ __forceinline__ f32x4 only_not_finite(const AttendParams& p, const Pl
 }
 
 // ---- few rows -----------------------------------------------------------------
-// Decoding: reading K and V is the work.  A workgroup of four waves takes one
-// KV head of one piece of one sequence; each wave takes every fourth tile of 32
-// keys and has its loads of the next tile in flight while it works on this one:
-// K as the products want it (lane = key, 16 bytes of its row), V by whole rows,
-// through 32 rows of LDS of the wave's own that the transposing reads take.
-// Waves join their maxima, totals and sums at the end.
+// Decoding: reading K and V is the work.  The tokens of all sequences of few
+// rows lie one behind the other in tiles of 128, and every workgroup of a KV
+// head takes an equal number of tiles, so that all end together whatever the
+// sequences' lengths are; where it ends inside a sequence it leaves a partial
+// result.  Of a tile each of its four waves takes 32 keys, with its loads of
+// the next tile in flight while it works on this one: K as the products want
+// it (lane = key, 16 bytes of its row), V by whole rows, through 32 rows of LDS
+// of the wave's own that the transposing reads take.  Waves join their maxima,
+// totals and sums at the end of a sequence.
+
+constexpr int kFewTile = 128;
+
+__device__ __forceinline__ int few_tiles(const AttendParams& p, const Seq& q, int most_rows) {
+    const int64_t rows = (int64_t)q.n_new * p.group;
+    if (rows == 0 || rows > p.few_rows) return 0;
+    if (rows > most_rows) return 1;                           // more than the caller said: one workgroup does them all
+    return max(1, (q.len + kFewTile - 1) / kFewTile);
+}
+
+// All tiles, and those of the sequences before s.
+__device__ __forceinline__ int count_tiles(const AttendParams& p, int most_rows, int s, int& before) {
+    const int lane = (int)threadIdx.x & 63;
+    int total = 0;
+    before = 0;
+    for (int base = 0; base < p.batch.n_seqs; base += 64) {
+        int n = base + lane < p.batch.n_seqs ? few_tiles(p, seq_of(p.batch, base + lane), most_rows) : 0;
+        int first = base + lane < s ? n : 0;
+        for (int m = 1; m < 64; m <<= 1) {
+            n += __shfl_xor(n, m);
+            first += __shfl_xor(first, m);
+        }
+        total += n;
+        before += first;
+    }
+    return total;
+}
+
+// The sequence that has tile `tile`, which becomes the number of the tile in it.
+__device__ __forceinline__ int find_tile(const AttendParams& p, int most_rows, int& tile) {
+    const int lane = (int)threadIdx.x & 63;
+    for (int base = 0; base < p.batch.n_seqs; base += 64) {
+        const int n = base + lane < p.batch.n_seqs ? few_tiles(p, seq_of(p.batch, base + lane), most_rows) : 0;
+        int upto = n;
+        for (int m = 1; m < 64; m <<= 1) {
+            const int y = __shfl_up(upto, m);
+            upto += lane >= m ? y : 0;
+        }
+        const uint64_t past = __ballot(upto > tile);
+        if (past) {
+            const int at = __ffsll((unsigned long long)past) - 1;
+            tile -= __shfl(upto, at) - __shfl(n, at);
+            return base + at;
+        }
+        tile -= __shfl(upto, 63);
+    }
+    return p.batch.n_seqs;
+}
+
+// The partial result of workgroup `group` (of a KV head) for a row of sequence s: the workgroups' pieces in order are
+// one further either in the workgroup or in the sequence.
+__device__ __forceinline__ float* few_partial(const AttendParams& p, int most_rows, int group, int s, int head, int row) {
+    return p.partial + ((((int64_t)group + s) * p.kv_heads + head) * most_rows + row) * (p.head_dim + 2);
+}
 
 template <int DT, int DP, int NT>
-__global__ __launch_bounds__(256, NT == 1 && DP <= 128 ? 2 : 1) void few_kernel(AttendParams p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 128 && NT == 1 ? 2 : 1)))
+void few_kernel(AttendParams p) {
     constexpr int kSteps = DP / 32, kChunks = DP / 8;         // products of depth 32; 16-byte pieces of a row
     constexpr int kVLoads = 32 * kChunks / 64;                // V loads of a lane for a tile
     constexpr int kVRows = 64 / kChunks;                      // rows a load covers
     constexpr int kJoinRow = DP + 4;
     constexpr int kWaveBytes = 32 * DP * 2;
     constexpr int kBytes = 4 * kWaveBytes > 4 * 16 * kJoinRow * 4 ? 4 * kWaveBytes : 4 * 16 * kJoinRow * 4;
+    constexpr int kMostRows = 16 * NT;
     __shared__ __attribute__((aligned(16))) uint8_t lds[kBytes];
     __shared__ float join_m[4][16], join_l[4][16];
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int lane = (int)threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, quad = lane >> 4;
-    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads);
-    const uint32_t rest = blockIdx.x / (uint32_t)p.kv_heads;
-    const int split = (int)(rest % (uint32_t)p.splits), s = (int)(rest / (uint32_t)p.splits);
-    const Seq seq = seq_of(p.batch, s);
-    const int rows = seq.n_new * p.group;
-    if (rows == 0 || rows > p.few_rows || split >= live_splits(p, seq.len)) return;
-    const int key0 = split * p.split_tokens;
-    const int key1 = key0 + min(seq.len - key0, p.split_tokens);
+    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads), group = (int)(blockIdx.x / (uint32_t)p.kv_heads);
+    int none;
+    const int total = uniform(count_tiles(p, kMostRows, 0, none));
+    const int quota = (total + p.few_groups - 1) / p.few_groups;
+    if ((int64_t)group * quota >= total) return;
+    int tile = group * quota;
+    int left = min(quota, total - tile);
+    int s = uniform(find_tile(p, kMostRows, tile));
+    tile = uniform(tile);
     uint8_t* vt = lds + wave * kWaveBytes;
     // 16-byte pieces of V rows are permuted within the row so that the rows a
     // transposing read takes lie in different banks
@@ -120,210 +180,220 @@ __global__ __launch_bounds__(256, NT == 1 && DP <= 128 ? 2 : 1) void few_kernel(
     const int v_row = lane / kChunks, v_chunk = lane % kChunks;
     const bool v_has = v_chunk * 8 < p.head_dim;
 
-    for (int r0 = 0; r0 < rows; r0 += 16 * NT) {
-        int limit[NT];                                        // tokens that the lane's rows see
-        uint4 qf[NT][kSteps];
+    for (; left > 0 && s < p.batch.n_seqs; ++s, tile = 0) {
+        const Seq seq = uniform(seq_of(p.batch, s));
+        const int rows = seq.n_new * p.group, n_tiles = few_tiles(p, seq, kMostRows);
+        const int take = min(n_tiles - tile, left);
+        if (n_tiles == 0) continue;
+        left -= take;
+        const bool whole = take == n_tiles;
+        const int key0 = tile * kFewTile, key1 = whole ? seq.len : min(seq.len, key0 + take * kFewTile);
+        for (int r0 = 0; r0 < rows; r0 += 16 * NT) {
+            int limit[NT];                                        // tokens that the lane's rows see
+            uint4 qf[NT][kSteps];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int r = r0 + 16 * t + col;
-            const int token = r / p.group, h = r - token * p.group;
-            limit[t] = r < rows ? max(0, seq.len - seq.n_new + token + 1) : 0;
-            const uint8_t* src = p.q + 2 * ((int64_t)(seq.row0 + token) * p.q_stride + (int64_t)(head * p.group + h) * p.head_dim);
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                const int d = 32 * i + 8 * quad;
-                qf[t][i] = r < rows && d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
-            }
-        }
-        const int last = min(rows, r0 + 16 * NT) - 1;
-        const int stop = min(key1, max(0, seq.len - seq.n_new + last / p.group + 1));
-        float m[NT], l[NT];
-        f32x4 o[NT][DP / 16];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            m[t] = -INFINITY;
-            l[t] = 0.f;
-#pragma unroll
-            for (int i = 0; i < DP / 16; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        uint4 kf[2][kSteps], vf[kVLoads];
-        Place at;                                             // of key (lane % 32) of the tile to be loaded
-        uint32_t valid = 0, v_valid = 0;                      // keys of the loaded tile that are there; this lane's V rows of them
-        auto load = [&](const Place& at) {
-            const bool has = at.page >= 0;
-            valid = (uint32_t)__ballot(has);
-            const int page = has ? at.page : 0, row = has ? at.row : 0;
-            v_valid = 0;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int from = 16 * t + col;
-                const int64_t pg = __shfl(page, from), rw = __shfl(row, from);
-                const uint8_t* src = p.k_pool + 2 * (pg * p.k_page + (rw * p.kv_heads + head) * p.head_dim);
+            for (int t = 0; t < NT; ++t) {
+                const int r = r0 + 16 * t + col;
+                const int token = r / p.group, h = r - token * p.group;
+                limit[t] = r < rows ? max(0, seq.len - seq.n_new + token + 1) : 0;
+                const uint8_t* src = p.q + 2 * ((int64_t)(seq.row0 + token) * p.q_stride + (int64_t)(head * p.group + h) * p.head_dim);
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i) {
                     const int d = 32 * i + 8 * quad;
-                    kf[t][i] = d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
+                    qf[t][i] = r < rows && d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < kVLoads; ++i) {
-                const int from = i * kVRows + v_row;
-                const int64_t pg = __shfl(page, from), rw = __shfl(row, from);
-                const uint8_t* src = p.v_pool + 2 * (pg * p.v_page + (rw * p.kv_heads + head) * p.head_dim);
-                vf[i] = v_has ? ldg16(src + 16 * v_chunk) : make_uint4(0, 0, 0, 0);
-                v_valid |= ((valid >> from) & 1u) << i;
-            }
-        };
-        const int first_sees = max(0, seq.len - seq.n_new + r0 / p.group + 1);   // the row that sees least
-        bool apart = false;                                   // V numbers have to be added apart
-        int kb = key0 + 32 * wave;
-        if (kb < stop) {
-            load(place_of(p.batch, seq, kb + (lane & 31), stop));
-            at = place_of(p.batch, seq, kb + 128 + (lane & 31), stop);
-        }
-        for (; kb < stop; kb += 128) {
-            const uint32_t here = valid;
-            f32x4 sc[NT][2];
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    sc[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int i = 0; i < kSteps; ++i) sc[t][u] = mfma16<DT>(kf[u][i], qf[t][i], sc[t][u]);
-                }
-            if (kb + 32 > first_sees && first_sees < stop) {
-#pragma unroll
-                for (int i = 0; i < kVLoads; ++i) apart |= drop_not_finite<DT>(vf[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < kVLoads; ++i) {
-                const int row = i * kVRows + v_row;
-                const uint4 x = (v_valid >> i) & 1u ? vf[i] : make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4*>(vt + row * DP * 2 + swizzle(row, v_chunk) * 16) = x;
-            }
-            if (kb + 128 < stop) {
-                load(at);
-                at = place_of(p.batch, seq, kb + 256 + (lane & 31), stop);
-            }
-            uint4 pf[NT];
+            const int last = min(rows, r0 + 16 * NT) - 1;
+            const int stop = min(key1, max(0, seq.len - seq.n_new + last / p.group + 1));
+            float m[NT], l[NT];
+            f32x4 o[NT][DP / 16];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                float x[8];
+                m[t] = -INFINITY;
+                l[t] = 0.f;
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int i = 0; i < DP / 16; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+            uint4 kf[2][kSteps], vf[kVLoads];
+            Place at;                                             // of key (lane % 32) of the tile to be loaded
+            uint32_t valid = 0, v_valid = 0;                      // keys of the loaded tile that are there; this lane's V rows of them
+            auto load = [&](const Place& at) {
+                const bool has = at.page >= 0;
+                valid = (uint32_t)__ballot(has);
+                const int page = has ? at.page : 0, row = has ? at.row : 0;
+                v_valid = 0;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int key = 16 * u + 4 * quad + i;
-                        const bool seen = ((here >> key) & 1u) && kb + key < limit[t];
-                        x[4 * u + i] = seen ? sc[t][u][i] * p.scale_log2 : -INFINITY;
+                for (int t = 0; t < 2; ++t) {
+                    const int from = 16 * t + col;
+                    const int64_t pg = __shfl(page, from), rw = __shfl(row, from);
+                    const uint8_t* src = p.k_pool + 2 * (pg * p.k_page + (rw * p.kv_heads + head) * p.head_dim);
+#pragma unroll
+                    for (int i = 0; i < kSteps; ++i) {
+                        const int d = 32 * i + 8 * quad;
+                        kf[t][i] = d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
                     }
-                float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float m_new = fmaxf(m[t], top);
-                const float base = m_new == -INFINITY ? 0.f : m_new;   // no key seen yet: every power is 0
-                if (__any(m_new != m[t])) {
-                    const float fade = __builtin_amdgcn_exp2f(m[t] - base);
-                    l[t] *= fade;
-#pragma unroll
-                    for (int i = 0; i < DP / 16; ++i) o[t][i] *= fade;
                 }
-                m[t] = m_new;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    x[i] = __builtin_amdgcn_exp2f(x[i] - base);
-                    l[t] += x[i];
+                for (int i = 0; i < kVLoads; ++i) {
+                    const int from = i * kVRows + v_row;
+                    const int64_t pg = __shfl(page, from), rw = __shfl(row, from);
+                    const uint8_t* src = p.v_pool + 2 * (pg * p.v_page + (rw * p.kv_heads + head) * p.head_dim);
+                    vf[i] = v_has ? ldg16(src + 16 * v_chunk) : make_uint4(0, 0, 0, 0);
+                    v_valid |= ((valid >> from) & 1u) << i;
                 }
-                // probabilities are rounded to the hot dtype for the product with V (their total is not):
-                // relative to the result that costs about what its own final rounding does
-                pf[t] = make_uint4(pack_hot<DT>(x[0], x[1]), pack_hot<DT>(x[2], x[3]), pack_hot<DT>(x[4], x[5]),
-                                   pack_hot<DT>(x[6], x[7]));
+            };
+            const int first_sees = max(0, seq.len - seq.n_new + r0 / p.group + 1);   // the row that sees least
+            bool apart = false;                                   // V numbers have to be added apart
+            int kb = key0 + 32 * wave;
+            if (kb < stop) {
+                load(place_of(p.batch, seq, kb + (lane & 31), stop));
+                at = place_of(p.batch, seq, kb + 128 + (lane & 31), stop);
             }
+            for (; kb < stop; kb += 128) {
+                const uint32_t here = valid;
+                f32x4 sc[NT][2];
 #pragma unroll
-            for (int n = 0; n < DP / 16; ++n) {
-                uint2 v[2];
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int row = 16 * u + 4 * quad + col / 4, chunk = 2 * n + (col & 3) / 2;
-                    v[u] = lds_read_transposed(vt + row * DP * 2 + swizzle(row, chunk) * 16 + (col & 1) * 8);
+                    for (int u = 0; u < 2; ++u) {
+                        sc[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int i = 0; i < kSteps; ++i) sc[t][u] = mfma16<DT>(kf[u][i], qf[t][i], sc[t][u]);
+                    }
+                if (kb + 32 > first_sees && first_sees < stop) {
+#pragma unroll
+                    for (int i = 0; i < kVLoads; ++i) apart |= drop_not_finite<DT>(vf[i]);
                 }
-                const uint4 a = make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
 #pragma unroll
-                for (int t = 0; t < NT; ++t) o[t][n] = mfma16<DT>(a, pf[t], o[t][n]);
-            }
-        }
-        if (__any(apart))                                     // of this wave's tiles
-            for (int key = max(key0, first_sees); key < stop; ++key) {
-                if ((key - key0) / 32 % 4 != wave) continue;
-                const Place where = place_of(p.batch, seq, key, stop);
+                for (int i = 0; i < kVLoads; ++i) {
+                    const int row = i * kVRows + v_row;
+                    const uint4 x = (v_valid >> i) & 1u ? vf[i] : make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(vt + row * DP * 2 + swizzle(row, v_chunk) * 16) = x;
+                }
+                if (kb + 128 < stop) {
+                    load(at);
+                    at = place_of(p.batch, seq, kb + 256 + (lane & 31), stop);
+                }
+                uint4 pf[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    float x[8];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int key = 16 * u + 4 * quad + i;
+                            const bool seen = ((here >> key) & 1u) && kb + key < limit[t];
+                            x[4 * u + i] = seen ? sc[t][u][i] * p.scale_log2 : -INFINITY;
+                        }
+                    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const float m_new = fmaxf(m[t], top);
+                    const float base = m_new == -INFINITY ? 0.f : m_new;   // no key seen yet: every power is 0
+                    if (__any(m_new != m[t])) {
+                        const float fade = __builtin_amdgcn_exp2f(m[t] - base);
+                        l[t] *= fade;
+#pragma unroll
+                        for (int i = 0; i < DP / 16; ++i) o[t][i] *= fade;
+                    }
+                    m[t] = m_new;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        x[i] = __builtin_amdgcn_exp2f(x[i] - base);
+                        l[t] += x[i];
+                    }
+                    // probabilities are rounded to the hot dtype for the product with V (their total is not):
+                    // relative to the result that costs about what its own final rounding does
+                    pf[t] = make_uint4(pack_hot<DT>(x[0], x[1]), pack_hot<DT>(x[2], x[3]), pack_hot<DT>(x[4], x[5]),
+                                       pack_hot<DT>(x[6], x[7]));
+                }
 #pragma unroll
                 for (int n = 0; n < DP / 16; ++n) {
-                    const f32x4 x = only_not_finite<DT>(p, where, head, 16 * n + 4 * quad);
+                    uint2 v[2];
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
+                    for (int u = 0; u < 2; ++u) {
+                        const int row = 16 * u + 4 * quad + col / 4, chunk = 2 * n + (col & 3) / 2;
+                        v[u] = lds_read_transposed(vt + row * DP * 2 + swizzle(row, chunk) * 16 + (col & 1) * 8);
+                    }
+                    const uint4 a = make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[t][n][e] += key < limit[t] ? x[e] : 0.f;
+                    for (int t = 0; t < NT; ++t) o[t][n] = mfma16<DT>(a, pf[t], o[t][n]);
                 }
             }
-        // join the four waves
+            if (__any(apart))                                     // of this wave's tiles
+                for (int key = max(key0, first_sees); key < stop; ++key) {
+                    if ((key - key0) / 32 % 4 != wave) continue;
+                    const Place where = place_of(p.batch, seq, key, stop);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            l[t] += __shfl_xor(l[t], 16);
-            l[t] += __shfl_xor(l[t], 32);
-            __syncthreads();   // the waves' V rows, or the previous rows' sums, have been read
-            float* join = reinterpret_cast<float*>(lds);
+                    for (int n = 0; n < DP / 16; ++n) {
+                        const f32x4 x = only_not_finite<DT>(p, where, head, 16 * n + 4 * quad);
 #pragma unroll
-            for (int n = 0; n < DP / 16; ++n)
-                *reinterpret_cast<f32x4*>(join + (wave * 16 + col) * kJoinRow + 16 * n + 4 * quad) = o[t][n];
-            if (quad == 0) {
-                join_m[wave][col] = m[t];
-                join_l[wave][col] = l[t];
-            }
-            __syncthreads();
-            const int row = (int)threadIdx.x / 16, part = (int)threadIdx.x % 16;
-            const int r = r0 + 16 * t + row;
-            if (r < rows) {
-                float top = -INFINITY, total = 0.f, w[4];
+                        for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, join_m[i][row]);
-                const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    w[i] = __builtin_amdgcn_exp2f(join_m[i][row] - base);
-                    total += w[i] * join_l[i][row];
-                }
-                const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
-                float* part_out = p.partial ? partial_of(p, seq.row0 + token, q_head, split) : nullptr;
-                const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
-                uint8_t* dst = p.out + 2 * ((int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head) * p.head_dim;
-                for (int d = 8 * part; d < p.head_dim; d += 128) {
-                    float y[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        y[e] = 0.f;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) y[e] = __builtin_fmaf(w[i], join[(i * 16 + row) * kJoinRow + d + e], y[e]);
-                    }
-                    if (part_out) {
-#pragma unroll
-                        for (int e = 0; e < 8; e += 2) *reinterpret_cast<float2*>(part_out + d + e) = make_float2(y[e], y[e + 1]);
-                    } else {
-                        stg16(dst + 2 * d, 0, make_uint4(pack_hot<DT>(y[0] * inv, y[1] * inv), pack_hot<DT>(y[2] * inv, y[3] * inv),
-                                                         pack_hot<DT>(y[4] * inv, y[5] * inv), pack_hot<DT>(y[6] * inv, y[7] * inv)));
+                            for (int e = 0; e < 4; ++e) o[t][n][e] += key < limit[t] ? x[e] : 0.f;
                     }
                 }
-                if (part == 0) {
-                    if (part_out) {
-                        part_out[p.head_dim] = top;
-                        part_out[p.head_dim + 1] = total;
-                    } else if (p.lse) {
-                        p.lse[(int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head] =
-                            total == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(total)) * kLn2;
+            // join the four waves
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                l[t] += __shfl_xor(l[t], 16);
+                l[t] += __shfl_xor(l[t], 32);
+                __syncthreads();   // the waves' V rows, or the previous rows' sums, have been read
+                float* join = reinterpret_cast<float*>(lds);
+#pragma unroll
+                for (int n = 0; n < DP / 16; ++n)
+                    *reinterpret_cast<f32x4*>(join + (wave * 16 + col) * kJoinRow + 16 * n + 4 * quad) = o[t][n];
+                if (quad == 0) {
+                    join_m[wave][col] = m[t];
+                    join_l[wave][col] = l[t];
+                }
+                __syncthreads();
+                const int row = (int)threadIdx.x / 16, part = (int)threadIdx.x % 16;
+                const int r = r0 + 16 * t + row;
+                if (r < rows) {
+                    float top = -INFINITY, total = 0.f, w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, join_m[i][row]);
+                    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        w[i] = __builtin_amdgcn_exp2f(join_m[i][row] - base);
+                        total += w[i] * join_l[i][row];
+                    }
+                    const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
+                    float* part_out = whole ? nullptr : few_partial(p, kMostRows, group, s, head, r);
+                    const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+                    uint8_t* dst = p.out + 2 * ((int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head) * p.head_dim;
+                    for (int d = 8 * part; d < p.head_dim; d += 128) {
+                        float y[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            y[e] = 0.f;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) y[e] = __builtin_fmaf(w[i], join[(i * 16 + row) * kJoinRow + d + e], y[e]);
+                        }
+                        if (part_out) {
+#pragma unroll
+                            for (int e = 0; e < 8; e += 2) *reinterpret_cast<float2*>(part_out + d + e) = make_float2(y[e], y[e + 1]);
+                        } else {
+                            stg16(dst + 2 * d, 0, make_uint4(pack_hot<DT>(y[0] * inv, y[1] * inv), pack_hot<DT>(y[2] * inv, y[3] * inv),
+                                                             pack_hot<DT>(y[4] * inv, y[5] * inv), pack_hot<DT>(y[6] * inv, y[7] * inv)));
+                        }
+                    }
+                    if (part == 0) {
+                        if (part_out) {
+                            part_out[p.head_dim] = top;
+                            part_out[p.head_dim + 1] = total;
+                        } else if (p.lse) {
+                            p.lse[(int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head] =
+                                total == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(total)) * kLn2;
+                        }
                     }
                 }
             }
         }
+        __syncthreads();   // the sums have been read
     }
 }
 
@@ -677,8 +747,8 @@ void many_kernel(AttendParams p) {
     if (r >= rows) return;
     const int64_t row_head = (int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head;
     const float base = m == -INFINITY ? 0.f : m;
-    if (p.partial) {
-        float* dst = partial_of(p, seq.row0 + token, q_head, split);
+    if (p.splits > 1) {
+        float* dst = many_partial(p, seq.row0 + token, q_head, split);
 #pragma unroll
         for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
@@ -713,43 +783,63 @@ void many_kernel(AttendParams p) {
 // One wave per row and query head: the pieces' sums under one maximum.
 
 template <int DT>
-__global__ __launch_bounds__(256) void join_kernel(AttendParams p, bool many) {
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads);
-    const uint32_t rest = blockIdx.x / (uint32_t)p.kv_heads;
-    int s, block = 0;
-    if (!many) s = (int)rest;
-    else if (!find_unit(p, (int)rest, s, block)) return;
-    const Seq seq = seq_of(p.batch, s);
-    const int rows = seq.n_new * p.group;
-    if (!many && rows > p.few_rows) return;
-    const int n = live_splits(p, seq.len);
-    const int end = many ? min(rows, (block + 1) * kManyRows) : rows;
-    for (int r = block * kManyRows + wave; r < end; r += 4) {
-        const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
-        const float* src = partial_of(p, seq.row0 + token, q_head, 0);
-        const int64_t step = p.head_dim + 2;
-        float top = -INFINITY;
-        for (int i = lane; i < n; i += 64) top = fmaxf(top, src[i * step + p.head_dim]);
-        for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
-        const float base = top == -INFINITY ? 0.f : top;
-        float total = 0.f;
-        for (int i = lane; i < n; i += 64)
-            total += __builtin_amdgcn_exp2f(src[i * step + p.head_dim] - base) * src[i * step + p.head_dim + 1];
-        total = xor_sum(total, 64);
-        const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
-        const int64_t row_head = (int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head;
-        for (int d = 2 * lane; d < p.head_dim; d += 128) {
-            float a = 0.f, b = 0.f;
-            for (int i = 0; i < n; ++i) {
-                const float w = __builtin_amdgcn_exp2f(src[i * step + p.head_dim] - base);
-                const float2 x = *reinterpret_cast<const float2*>(src + i * step + d);
-                a = __builtin_fmaf(w, x.x, a);
-                b = __builtin_fmaf(w, x.y, b);
-            }
-            *reinterpret_cast<uint32_t*>(p.out + 2 * (row_head * p.head_dim + d)) = pack_hot<DT>(a * inv, b * inv);
+__device__ __forceinline__ void join_row(const AttendParams& p, const float* src, int64_t step, int n, int64_t row_head) {
+    const int lane = (int)threadIdx.x & 63;
+    float top = -INFINITY;
+    for (int i = lane; i < n; i += 64) top = fmaxf(top, src[i * step + p.head_dim]);
+    for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
+    const float base = top == -INFINITY ? 0.f : top;
+    float total = 0.f;
+    for (int i = lane; i < n; i += 64)
+        total += __builtin_amdgcn_exp2f(src[i * step + p.head_dim] - base) * src[i * step + p.head_dim + 1];
+    total = xor_sum(total, 64);
+    const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+    for (int d = 2 * lane; d < p.head_dim; d += 128) {
+        float a = 0.f, b = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float w = __builtin_amdgcn_exp2f(src[i * step + p.head_dim] - base);
+            const float2 x = *reinterpret_cast<const float2*>(src + i * step + d);
+            a = __builtin_fmaf(w, x.x, a);
+            b = __builtin_fmaf(w, x.y, b);
         }
-        if (lane == 0 && p.lse) p.lse[row_head] = total == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(total)) * kLn2;
+        *reinterpret_cast<uint32_t*>(p.out + 2 * (row_head * p.head_dim + d)) = pack_hot<DT>(a * inv, b * inv);
+    }
+    if (lane == 0 && p.lse) p.lse[row_head] = total == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(total)) * kLn2;
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void join_few_kernel(AttendParams p, int most_rows) {
+    const int wave = (int)threadIdx.x >> 6;
+    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads), s = (int)(blockIdx.x / (uint32_t)p.kv_heads);
+    const Seq seq = seq_of(p.batch, s);
+    const int tiles = few_tiles(p, seq, most_rows);
+    if (tiles == 0) return;
+    int first;
+    const int total = count_tiles(p, most_rows, s, first), quota = (total + p.few_groups - 1) / p.few_groups;
+    const int group0 = first / quota, group1 = (first + tiles - 1) / quota;
+    if (group0 == group1) return;                             // one workgroup had the sequence whole
+    const int rows = seq.n_new * p.group;
+    const int64_t step = (int64_t)p.kv_heads * most_rows * (p.head_dim + 2);
+    for (int r = wave; r < rows; r += 4) {
+        const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
+        join_row<DT>(p, few_partial(p, most_rows, group0, s, head, r), step, group1 - group0 + 1,
+                     (int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head);
+    }
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void join_many_kernel(AttendParams p) {
+    const int wave = (int)threadIdx.x >> 6;
+    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads);
+    int s, block;
+    if (!find_unit(p, (int)(blockIdx.x / (uint32_t)p.kv_heads), s, block)) return;
+    const Seq seq = seq_of(p.batch, s);
+    const int rows = seq.n_new * p.group, n = live_splits(p, seq.len);
+    for (int r = block * kManyRows + wave; r < min(rows, (block + 1) * kManyRows); r += 4) {
+        const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
+        join_row<DT>(p, many_partial(p, seq.row0 + token, q_head, 0), p.head_dim + 2, n,
+                     (int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head);
     }
 }
 
@@ -757,46 +847,53 @@ __global__ __launch_bounds__(256) void join_kernel(AttendParams p, bool many) {
 
 // How a call is cut: what the few and the many kernel take, and into how many pieces.
 struct Plan {
-    int nt;                         // 16-row tiles of the few kernel
-    int few_rows;                   // 0: no few kernel
+    int nt;                         // 16-row tiles of the few kernel, 0: no few kernel
+    int few_rows;                   // most rows of its sequences
+    int few_groups;                 // its workgroups of a KV head
     bool many;
     int64_t many_units;             // blocks of kManyRows rows at most
-    int few_splits, few_tokens, many_splits, many_tokens;
-    int partial_splits;             // 0: no pieces
+    int splits, split_tokens;       // of the many kernel
+    int64_t workspace;              // floats
 };
-
-int pieces(int64_t groups, int64_t max_tokens, int64_t wanted, int least, int& tokens) {
-    int64_t n = groups > 0 ? (wanted + groups - 1) / groups : 1;
-    const int64_t most = (max_tokens + least - 1) / least;
-    if (n > most) n = most;
-    if (n < 1) n = 1;
-    if (n > 64) n = 64;
-    int64_t t = (max_tokens + n - 1) / n;
-    t = (t + 127) / 128 * 128;
-    tokens = (int)t;
-    return (int)((max_tokens + t - 1) / t);
-}
 
 Plan plan_call(const ztcp_paged_batch* b, const ztcp_geometry* g, int64_t q_heads, int cus) {
     Plan plan{};
-    const int64_t group = q_heads / g->num_heads;
+    const int64_t heads = g->num_heads, group = q_heads / heads, piece = g->head_dim + 2;
     const int64_t most_q = b->max_q_len > 0 && b->max_q_len < b->n_rows ? b->max_q_len : b->n_rows;
     const int64_t most_rows = most_q * group, max_tokens = b->max_pages * g->num_tokens;
-    plan.nt = 1;
-    if (most_rows <= 64) {
-        plan.nt = most_rows <= 16 ? 1 : most_rows <= 32 ? 2 : 4;
+    const int most_nt = g->head_dim <= 128 ? 2 : 1;
+    if (most_rows <= 16 * most_nt) {
+        plan.nt = most_rows <= 16 ? 1 : 2;
         plan.few_rows = 0x7FFFFFFF;
     } else {
-        plan.nt = group <= 16 ? 1 : group <= 32 ? 2 : 4;
-        plan.few_rows = b->n_seqs > 1 && group <= 64 ? 16 * plan.nt : 0;
+        plan.nt = b->n_seqs > 1 && group <= 16 * most_nt ? (group <= 16 ? 1 : 2) : 0;
+        plan.few_rows = 16 * plan.nt;
         plan.many = true;
         plan.many_units = (b->n_rows * group + kManyRows - 1) / kManyRows + b->n_seqs;
     }
-    plan.few_splits = plan.many_splits = 1;
-    if (plan.few_rows) plan.few_splits = pieces(b->n_seqs * g->num_heads, max_tokens, (int64_t)cus * 12, 256, plan.few_tokens);
-    if (plan.many) plan.many_splits = pieces(plan.many_units * g->num_heads, max_tokens, (int64_t)cus * 2, 512, plan.many_tokens);
-    const int splits = plan.few_splits > plan.many_splits ? plan.few_splits : plan.many_splits;
-    plan.partial_splits = splits > 1 ? splits : 0;
+    if (plan.nt) {
+        // as many as the card holds at once, and no more than tiles
+        const int64_t resident = (int64_t)cus * (g->head_dim <= 64 ? 3 : g->head_dim <= 128 ? 2 : 1);
+        const int64_t tiles = b->n_seqs * ((max_tokens + kFewTile - 1) / kFewTile);
+        int64_t n = (resident + heads - 1) / heads;
+        n = n < tiles ? n : tiles;
+        plan.few_groups = (int)(n > 1 ? n : 1);
+        if (plan.few_groups > 1) plan.workspace = (plan.few_groups + b->n_seqs) * heads * 16 * plan.nt * piece;
+    }
+    plan.splits = 1;
+    plan.split_tokens = (int)max_tokens;
+    if (plan.many) {
+        const int64_t groups = plan.many_units * heads, most = (max_tokens + 511) / 512;
+        int64_t n = ((int64_t)cus * 2 + groups - 1) / groups;
+        n = n < most ? n : most;
+        n = n < 64 ? n : 64;
+        if (n > 1) {
+            plan.split_tokens = (int)(((max_tokens + n - 1) / n + 127) / 128 * 128);
+            plan.splits = (int)((max_tokens + plan.split_tokens - 1) / plan.split_tokens);
+        }
+        const int64_t need = plan.splits > 1 ? b->n_rows * q_heads * plan.splits * piece : 0;
+        plan.workspace = need > plan.workspace ? need : plan.workspace;
+    }
     return plan;
 }
 
@@ -811,32 +908,27 @@ int cu_count(int& cus) {
 template <int DT, int DP>
 void launch(const AttendParams& base, const Plan& plan, float* workspace, hipStream_t stream) {
     AttendParams p = base;
-    p.partial_splits = plan.partial_splits;
+    p.partial = workspace;
     p.few_rows = plan.few_rows;
-    if (plan.few_rows) {
-        p.splits = plan.few_splits;
-        p.split_tokens = plan.few_splits > 1 ? plan.few_tokens : p.batch.max_tokens;
-        p.partial = plan.few_splits > 1 ? workspace : nullptr;
-        const uint32_t seq_heads = (uint32_t)p.batch.n_seqs * (uint32_t)p.kv_heads;
-        auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(seq_heads * (uint32_t)p.splits), dim3(256), 0, stream, p);
-        };
-        if (plan.nt == 1) go(few_kernel<DT, DP, 1>);
-        else if (plan.nt == 2) go(few_kernel<DT, DP, 2>);
-        else go(few_kernel<DT, DP, 4>);
-        if (p.partial) hipLaunchKernelGGL(join_kernel<DT>, dim3(seq_heads), dim3(256), 0, stream, p, false);
+    p.few_groups = plan.few_groups;
+    p.splits = plan.splits;
+    p.split_tokens = plan.split_tokens;
+    const uint32_t heads = (uint32_t)p.kv_heads;
+    if (plan.nt) {
+        const dim3 grid(heads * (uint32_t)plan.few_groups);
+        if constexpr (DP <= 128) {
+            if (plan.nt == 2) hipLaunchKernelGGL((few_kernel<DT, DP, 2>), grid, dim3(256), 0, stream, p);
+        }
+        if (plan.nt == 1) hipLaunchKernelGGL((few_kernel<DT, DP, 1>), grid, dim3(256), 0, stream, p);
+        if (plan.few_groups > 1)
+            hipLaunchKernelGGL(join_few_kernel<DT>, dim3(heads * (uint32_t)p.batch.n_seqs), dim3(256), 0, stream, p, 16 * plan.nt);
     }
     if (plan.many) {
-        p.splits = plan.many_splits;
-        p.split_tokens = plan.many_splits > 1 ? plan.many_tokens : p.batch.max_tokens;
-        p.partial = plan.many_splits > 1 ? workspace : nullptr;
-        const uint32_t unit_heads = (uint32_t)(plan.many_units * p.kv_heads);
-        auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(unit_heads * (uint32_t)p.splits), dim3(256), 0, stream, p);
-        };
+        const uint32_t units = (uint32_t)plan.many_units * heads;
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(units * (uint32_t)p.splits), dim3(256), 0, stream, p); };
         if (p.batch.page_tokens % (many_tile(DP) / 4) == 0 && p.head_dim == DP) go(many_kernel<DT, DP, true>);
         else go(many_kernel<DT, DP, false>);
-        if (p.partial) hipLaunchKernelGGL(join_kernel<DT>, dim3(unit_heads), dim3(256), 0, stream, p, true);
+        if (p.splits > 1) hipLaunchKernelGGL(join_many_kernel<DT>, dim3(units), dim3(256), 0, stream, p);
     }
 }
 
@@ -859,7 +951,7 @@ extern "C" size_t ztcp_paged_attention_workspace(const ztcp_paged_batch* batch, 
     int cus = 0;
     if (cu_count(cus) != ZTCP_OK) return (size_t)-1;
     const Plan plan = plan_call(batch, g, q_heads, cus);
-    return (size_t)batch->n_rows * q_heads * plan.partial_splits * (g->head_dim + 2) * sizeof(float);
+    return (size_t)plan.workspace * sizeof(float);
 }
 
 extern "C" int ztcp_paged_attention(const void* q, int64_t q_stride, void* out, float* lse, int64_t q_heads,
@@ -886,15 +978,16 @@ extern "C" int ztcp_paged_attention(const void* q, int64_t q_stride, void* out, 
     int cus = 0;
     if (cu_count(cus) != ZTCP_OK) return ZTCP_EHIP;
     const Plan plan = plan_call(batch, g, q_heads, cus);
-    const int64_t need = batch->n_rows * q_heads * plan.partial_splits * (d + 2) * (int64_t)sizeof(float);
+    const int64_t need = plan.workspace * (int64_t)sizeof(float);
     if (need > 0 && (!workspace || (int64_t)workspace_bytes < need || !hot_aligned(workspace)))
         return arg_result(ZTCP_EINVAL, "workspace must hold ztcp_paged_attention_workspace bytes, 16-byte aligned");
     if (!misses(out, out_bytes) || !misses(lse, lse_bytes) || !misses(need ? workspace : nullptr, need) ||
         bytes_overlap(out, out_bytes, lse, lse_bytes) || bytes_overlap(workspace, need, out, out_bytes) ||
         bytes_overlap(workspace, need, lse, lse_bytes))
         return arg_result(ZTCP_EOVERLAP, "out, lse and workspace must not overlap q, the pages or each other");
-    const int64_t blocks = g->num_heads * (plan.many_units * plan.many_splits + batch->n_seqs * plan.few_splits);
-    if (blocks >= (int64_t)1 << 31) return arg_result(ZTCP_EINVAL, "too many sequences and heads in one call");
+    const int64_t most = (int64_t)1 << 31, tiles = batch->n_seqs * (p.batch.max_tokens / kFewTile + 1);
+    if (g->num_heads * plan.many_units * plan.splits >= most || g->num_heads * batch->n_seqs >= most || tiles >= most)
+        return arg_result(ZTCP_EINVAL, "too many sequences and heads in one call");
     p.q = (const uint8_t*)q;
     p.out = (uint8_t*)out;
     p.lse = lse;
