@@ -179,6 +179,10 @@ def test_python_checks(N):
         A.paged_attention(x, pages, None, i32[None], i32[:1], i32)
     with pytest.raises(ValueError, match="mass must be a HIP tensor"):
         A.evict_pages(torch.zeros((1, 2, 2)), i32[None], i32[:1], page_tokens=16, budget=1)
+    with pytest.raises(ValueError, match="k_pages requires a gradient"):
+        A.paged_attention(x, pages.clone().requires_grad_(), pages, i32[None], i32[:1], i32)
+    with pytest.raises(ValueError, match="q must be a tensor"):
+        A.paged_attention(None, pages, pages, i32[None], i32[:1], i32)
     with pytest.raises(ValueError, match="even"):
         A.rope_table(4, 3, device="cpu")
     t = A.rope_table(9, 4, base=100.0, device="cpu")

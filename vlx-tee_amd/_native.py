@@ -175,6 +175,16 @@ def lib() -> C.CDLL:
     return L
 
 
+def torch_binding():
+    """The torch binding of the operators on hot pages (raises if it has not been built)."""
+    lib()
+    try:
+        from . import _ztcp_torch
+    except ImportError as e:
+        raise RuntimeError(f"torch binding missing or unusable ({e}); build it with python vlx-tee_amd/build.py") from e
+    return _ztcp_torch
+
+
 def _bind_keyring(L: C.CDLL) -> None:
     P, S, B, SZ = C.c_void_p, C.c_char_p, C.c_char_p, C.c_size_t
     u64, u32, u16, i32 = C.c_uint64, C.c_uint32, C.c_uint16, C.c_int

@@ -13,6 +13,9 @@ counts (start-up, waits of each wave role, end) into a device buffer that
 ``ztcp_phase_timers_read`` returns.  Only ``bench.py --phase-timers`` loads
 it; the product library carries no timer code.
 
+``_ztcp_torch.so`` (binding/ztcp_torch.cpp, host code) takes torch tensors to
+the operators on hot pages for ``attention.py``.
+
 Flags: ``-ffp-contract=off`` and no fast-math (the quantizer's fp32 rounding
 order must match the reference's), packed-FP32 instructions disabled.
 """
@@ -28,6 +31,8 @@ HERE = Path(__file__).resolve().parent
 LIB = HERE / "libztcp_hip.so"
 EXAMPLE_SRC = HERE / "example" / "ztcp_capi_example.cpp"
 EXAMPLE = HERE / "ztcp_capi_example"   # a C++ caller of include/ztcp.h, linked against LIB
+BINDING_SRC = HERE / "binding" / "ztcp_torch.cpp"
+BINDING = HERE / "_ztcp_torch.so"      # Python module, linked against LIB and torch
 LIB_TIMERS = HERE / "libztcp_hip_timers.so"
 OBJ = HERE / "_build"
 ARCH = os.environ.get("ZTCP_OFFLOAD_ARCH", "gfx950")
@@ -90,7 +95,26 @@ def build(verbose: bool = False, timers: bool = True) -> Path:
                 f.result()
             _link(hipcc, objs, out, verbose)
     _build_example(hipcc, verbose)
+    _build_binding(verbose)
     return LIB
+
+
+def _build_binding(verbose: bool) -> None:
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", str(root / "include"), "-isystem", "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"],
+           str(BINDING_SRC), "-o", str(tmp), f"-L{HERE}", "-lztcp_hip", f"-L{root / 'lib'}", "-lc10", "-lc10_hip",
+           "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, BINDING)
 
 
 def _build_example(hipcc: str, verbose: bool) -> None:
