@@ -102,45 +102,6 @@ __device__ __forceinline__ int few_tiles(const AttendParams& p, const Seq& q, in
     return max(1, (q.len + kFewTile - 1) / kFewTile);
 }
 
-// All tiles, and those of the sequences before s.
-__device__ __forceinline__ int count_tiles(const AttendParams& p, int most_rows, int s, int& before) {
-    const int lane = (int)threadIdx.x & 63;
-    int total = 0;
-    before = 0;
-    for (int base = 0; base < p.batch.n_seqs; base += 64) {
-        int n = base + lane < p.batch.n_seqs ? few_tiles(p, seq_of(p.batch, base + lane), most_rows) : 0;
-        int first = base + lane < s ? n : 0;
-        for (int m = 1; m < 64; m <<= 1) {
-            n += __shfl_xor(n, m);
-            first += __shfl_xor(first, m);
-        }
-        total += n;
-        before += first;
-    }
-    return total;
-}
-
-// The sequence that has tile `tile`, which becomes the number of the tile in it.
-__device__ __forceinline__ int find_tile(const AttendParams& p, int most_rows, int& tile) {
-    const int lane = (int)threadIdx.x & 63;
-    for (int base = 0; base < p.batch.n_seqs; base += 64) {
-        const int n = base + lane < p.batch.n_seqs ? few_tiles(p, seq_of(p.batch, base + lane), most_rows) : 0;
-        int upto = n;
-        for (int m = 1; m < 64; m <<= 1) {
-            const int y = __shfl_up(upto, m);
-            upto += lane >= m ? y : 0;
-        }
-        const uint64_t past = __ballot(upto > tile);
-        if (past) {
-            const int at = __ffsll((unsigned long long)past) - 1;
-            tile -= __shfl(upto, at) - __shfl(n, at);
-            return base + at;
-        }
-        tile -= __shfl(upto, 63);
-    }
-    return p.batch.n_seqs;
-}
-
 // The partial result of workgroup `group` (of a KV head) for a row of sequence s: the workgroups' pieces in order are
 // one further either in the workgroup or in the sequence.
 __device__ __forceinline__ float* few_partial(const AttendParams& p, int most_rows, int group, int s, int head, int row) {
@@ -163,12 +124,13 @@ void few_kernel(AttendParams p) {
     const int col = lane & 15, quad = lane >> 4;
     const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads), group = (int)(blockIdx.x / (uint32_t)p.kv_heads);
     int none;
-    const int total = uniform(count_tiles(p, kMostRows, 0, none));
+    auto tiles_of = [&](const Seq& q) { return few_tiles(p, q, kMostRows); };
+    const int total = uniform(count_tiles(p.batch, 0, none, tiles_of));
     const int quota = (total + p.few_groups - 1) / p.few_groups;
     if ((int64_t)group * quota >= total) return;
     int tile = group * quota;
     int left = min(quota, total - tile);
-    int s = uniform(find_tile(p, kMostRows, tile));
+    int s = uniform(find_tile(p.batch, tile, tiles_of));
     tile = uniform(tile);
     uint8_t* vt = lds + wave * kWaveBytes;
     // 16-byte pieces of V rows are permuted within the row so that the rows a
@@ -408,46 +370,18 @@ constexpr int many_tile(int dp) { return dp <= 128 ? 64 : 32; }
 // The unit-th block of kManyRows rows of the batch's sequences of more than
 // p.few_rows rows; false if there are fewer.
 __device__ __forceinline__ bool find_unit(const AttendParams& p, int unit, int& s, int& block) {
-    const int lane = (int)threadIdx.x & 63;
-    for (int base = 0; base < p.batch.n_seqs; base += 64) {
-        int n = 0;
-        if (base + lane < p.batch.n_seqs) {
-            const int rows = seq_of(p.batch, base + lane).n_new * p.group;
-            n = rows > p.few_rows ? (rows + kManyRows - 1) / kManyRows : 0;
-        }
-        int upto = n;
-        for (int m = 1; m < 64; m <<= 1) {
-            const int y = __shfl_up(upto, m);
-            upto += lane >= m ? y : 0;
-        }
-        const uint64_t past = __ballot(upto > unit);
-        if (past) {
-            const int at = __ffsll((unsigned long long)past) - 1;
-            s = base + at;
-            const int n_at = __shfl(n, at);
-            block = n_at - 1 - (unit - (__shfl(upto, at) - n_at));   // the last rows, which see most, first
-            return true;
-        }
-        unit -= __shfl(upto, 63);
-    }
-    return false;
+    auto blocks = [&](const Seq& q) {
+        const int rows = q.n_new * p.group;
+        return rows > p.few_rows ? (rows + kManyRows - 1) / kManyRows : 0;
+    };
+    s = find_tile(p.batch, unit, blocks);
+    if (s >= p.batch.n_seqs) return false;
+    block = blocks(seq_of(p.batch, s)) - 1 - unit;            // the last rows, which see most, first
+    return true;
 }
 
 // Zeros that the tile loads read in the place of tokens that are not there: a row of 256 elements.
 __device__ __attribute__((aligned(16))) uint32_t g_zeros[128];
-
-// One wave's 64 pieces of 16 bytes from global memory to LDS, piece i at lds + 16 i,
-// without passing through registers; done once vmcnt says so.  Written in asm
-// because the compiler, which cannot tell the two buffers apart, would wait for
-// the next tile's loads before this tile's reads.  It has no output register,
-// and nothing else here uses m0.
-__device__ __forceinline__ void load_lds16(const uint8_t* src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
-}
-// The same from a wave's own base and each lane's offset.
-__device__ __forceinline__ void load_lds16(const uint8_t* base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
-}
 
 // EVEN: a wave's quarter of a tile never crosses a page and rows fill DP, so that the quarter's address is
 // one scalar; otherwise every lane has its own.
@@ -526,10 +460,10 @@ void many_kernel(AttendParams p) {
         else return Where{page, row, here};
     };
     constexpr uint64_t kAll = ~0ull;                          // (tiles of 32 keys: both halves of the lanes)
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)&tiles[0][0][0];
+    const uint32_t lds0 = lds_address(&tiles[0][0][0]);
     const uint32_t row_bytes = 2u * (uint32_t)p.kv_heads * (uint32_t)p.head_dim;         // from a token to the next
     // This wave's quarter of a tile of K (which = 0) or V (1) into a buffer
-    auto load = [&](const Where& at, int buffer, auto which) {
+    auto load = [&](const Where& at, int buffer, auto which) __attribute__((always_inline)) {
         constexpr bool is_v = decltype(which)::value != 0;
         const uint8_t* pool = is_v ? p.v_pool : p.k_pool;
         const int64_t page_step = is_v ? p.v_page : p.k_page;
@@ -585,7 +519,7 @@ void many_kernel(AttendParams p) {
     // a 16-key group's weights take the place of the previous tile's once their products have been issued, so
     // that the wave has products and vector work at the same time.  LDS reads run four products ahead; the
     // barriers keep the compiler from putting each read right before its product.
-    auto products = [&](int v_buffer, f32x16 (&sc)[kSub], float base, auto weigh_c) {
+    auto products = [&](int v_buffer, f32x16 (&sc)[kSub], float base, auto weigh_c) __attribute__((always_inline)) {
         constexpr bool kWeigh = decltype(weigh_c)::value;
         const uint8_t* vt = tiles[v_buffer][1];
         uint4 vf[kAhead + 1];
@@ -627,7 +561,7 @@ void many_kernel(AttendParams p) {
         apart |= __syncthreads_or(dropped) != 0;
     };
     // One tile: its scores, the previous tile's products and its own weights.
-    auto step = [&](int kb, auto buffer_c, auto first_c) {
+    auto step = [&](int kb, auto buffer_c, auto first_c) __attribute__((always_inline)) {
         constexpr int buffer = decltype(buffer_c)::value;
         constexpr bool kFirst = decltype(first_c)::value;
         __builtin_amdgcn_s_waitcnt(0);                        // this wave's share of this tile's K and the last one's V
@@ -816,7 +750,8 @@ __global__ __launch_bounds__(256) void join_few_kernel(AttendParams p, int most_
     const int tiles = few_tiles(p, seq, most_rows);
     if (tiles == 0) return;
     int first;
-    const int total = count_tiles(p, most_rows, s, first), quota = (total + p.few_groups - 1) / p.few_groups;
+    const int total = count_tiles(p.batch, s, first, [&](const Seq& q) { return few_tiles(p, q, most_rows); });
+    const int quota = (total + p.few_groups - 1) / p.few_groups;
     const int group0 = first / quota, group1 = (first + tiles - 1) / quota;
     if (group0 == group1) return;                             // one workgroup had the sequence whole
     const int rows = seq.n_new * p.group;
@@ -895,14 +830,6 @@ Plan plan_call(const ztcp_paged_batch* b, const ztcp_geometry* g, int64_t q_head
         plan.workspace = need > plan.workspace ? need : plan.workspace;
     }
     return plan;
-}
-
-int cu_count(int& cus) {
-    int dev = 0;
-    return hipGetDevice(&dev) == hipSuccess &&
-                   hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && cus > 0
-               ? ZTCP_OK
-               : ZTCP_EHIP;
 }
 
 template <int DT, int DP>

@@ -53,6 +53,15 @@ inline DivBy div_by(uint32_t d) {
     return DivBy{(uint32_t)(((uint64_t)1 << (31 + s)) / d + 1), 31 + s};
 }
 
+// Compute units of the current device.
+inline int cu_count(int& cus) {
+    int dev = 0;
+    return hipGetDevice(&dev) == hipSuccess &&
+                   hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && cus > 0
+               ? ZTCP_OK
+               : ZTCP_EHIP;
+}
+
 // What is wrong with a pool and its geometry, or nullptr.
 inline const char* check_pool(const ztcp_page_pool* pool, const ztcp_geometry* g, int64_t max_head_dim) {
     if (!pool || !g) return "pool and geometry must not be NULL";
@@ -111,6 +120,14 @@ inline const char* check_batch(const ztcp_paged_batch* b, const ztcp_page_pool* 
 
 // ---- device ----------------------------------------------------------------
 
+// A value that every lane of the wave has, in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+template <class T>
+__device__ __forceinline__ T* uniform(T* p) {
+    const uint64_t x = (uint64_t)p;
+    return (T*)((uint64_t)(uint32_t)uniform((int)(uint32_t)x) | (uint64_t)(uint32_t)uniform((int)(uint32_t)(x >> 32)) << 32);
+}
+
 __device__ __forceinline__ int div_page(int x, DivBy d) { return (int)(((uint64_t)(uint32_t)x * d.mul) >> d.shift); }
 
 // A sequence of the batch; whatever the arrays hold, its rows are rows of q and
@@ -119,13 +136,6 @@ struct Seq {
     int row0, n_new, len;
     const int32_t* table;
 };
-// A value that every lane of the wave has, in a scalar register.
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-template <class T>
-__device__ __forceinline__ T* uniform(T* p) {
-    const uint64_t x = (uint64_t)p;
-    return (T*)((uint64_t)(uint32_t)uniform((int)(uint32_t)x) | (uint64_t)(uint32_t)uniform((int)(uint32_t)(x >> 32)) << 32);
-}
 __device__ __forceinline__ Seq uniform(Seq q) {
     return Seq{uniform(q.row0), uniform(q.n_new), uniform(q.len), uniform(q.table)};
 }
@@ -137,6 +147,48 @@ __device__ __forceinline__ Seq seq_of(const PagedView& v, int s) {
     q.len = min(max(len, 0), v.max_tokens);
     q.table = v.table + s * v.table_stride;
     return q;
+}
+
+// Work laid out sequence behind sequence, tiles(q) units of each: all of it, and
+// what lies before sequence s.  Every lane of the wave takes part and gets the answer.
+template <class F>
+__device__ __forceinline__ int count_tiles(const PagedView& v, int s, int& before, F&& tiles) {
+    const int lane = (int)threadIdx.x & 63;
+    int total = 0;
+    before = 0;
+    for (int base = 0; base < v.n_seqs; base += 64) {
+        int n = base + lane < v.n_seqs ? tiles(seq_of(v, base + lane)) : 0;
+        int first = base + lane < s ? n : 0;
+        for (int m = 1; m < 64; m <<= 1) {
+            n += __shfl_xor(n, m);
+            first += __shfl_xor(first, m);
+        }
+        total += n;
+        before += first;
+    }
+    return total;
+}
+
+// The sequence that has unit `tile`, which becomes its number there; v.n_seqs if there are fewer units.
+template <class F>
+__device__ __forceinline__ int find_tile(const PagedView& v, int& tile, F&& tiles) {
+    const int lane = (int)threadIdx.x & 63;
+    for (int base = 0; base < v.n_seqs; base += 64) {
+        const int n = base + lane < v.n_seqs ? tiles(seq_of(v, base + lane)) : 0;
+        int upto = n;
+        for (int m = 1; m < 64; m <<= 1) {
+            const int y = __shfl_up(upto, m);
+            upto += lane >= m ? y : 0;
+        }
+        const uint64_t past = __ballot(upto > tile);
+        if (past) {
+            const int at = __ffsll((unsigned long long)past) - 1;
+            tile -= __shfl(upto, at) - __shfl(n, at);
+            return base + at;
+        }
+        tile -= __shfl(upto, 63);
+    }
+    return v.n_seqs;
 }
 
 // Where token `key` (below `stop`) is: its page, -1 if there is none, and its row in the page.
@@ -152,6 +204,20 @@ __device__ __forceinline__ Place place_of(const PagedView& v, const Seq& q, int 
         p.row = key - at * v.page_tokens;
     }
     return p;
+}
+
+// 64 pieces of 16 bytes from global memory to LDS, a wave's piece i to lds + 16 i, without passing through registers;
+// done once vmcnt says so.  Written in asm because the compiler, which cannot tell two buffers apart, would wait for
+// the next tile's loads before this tile's reads.  It has no output register, and nothing else in these kernels uses
+// m0.  The second form takes a base of the wave and each lane's offset.
+__device__ __forceinline__ void load_lds16(const uint8_t* src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(uniform((int)lds)), "v"(src) : "memory");
+}
+__device__ __forceinline__ void load_lds16(const uint8_t* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(uniform((int)lds)), "v"(offset), "s"(uniform(base)) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 
 // MFMA operands and results.

@@ -11,7 +11,7 @@ using namespace ztcp;
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kBlockKeys = 256;
+constexpr int kFewKeys = 128, kManyKeys = 64;   // keys that a workgroup of either kernel has in registers, 32 a wave
 
 struct MassParams {
     PagedView batch;
@@ -23,102 +23,421 @@ struct MassParams {
     const uint8_t* k_pool;
     int64_t k_page;
     int32_t kv_heads, group, head_dim, max_pages;
-    int32_t group_pages;             // pages of a workgroup
+    int32_t few_rows;                // sequences of at most so many rows are the few kernel's
+    int32_t few_groups;              // its workgroups of a KV head
+    int32_t group_pages;             // pages of a tile: as many as the kernel's keys hold, one at least
+    DivBy group_div;
     float scale_log2, decay;
 };
 
-// A workgroup owns whole pages of one KV head, 64 of up to 256 keys a wave: K
-// stays in registers while the rows pass by, each key's sum over the rows in
-// fp32 registers, so every page's account has one writer and one order of
-// additions.
-template <int DT, int DP>
-__global__ __launch_bounds__(256) void mass_kernel(MassParams p) {
-    constexpr int kSteps = DP / 32;
-    __shared__ float key_sum[kBlockKeys];
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    const int col = lane & 15, quad = lane >> 4;
-    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads);
-    const uint32_t rest = blockIdx.x / (uint32_t)p.kv_heads;
-    const int groups = (p.max_pages + p.group_pages - 1) / p.group_pages;
-    const int page0 = (int)(rest % (uint32_t)groups) * p.group_pages, s = (int)(rest / (uint32_t)groups);
-    const Seq seq = seq_of(p.batch, s);
-    const int rows = seq.n_new * p.group;
-    const int pages = min(p.group_pages, p.max_pages - page0);
+__device__ __forceinline__ int mass_tiles(const MassParams& p, const Seq& q) {
+    const int keys = p.group_pages * p.batch.page_tokens;
+    return (q.len + keys - 1) / keys;
+}
+
+__device__ __forceinline__ int pages_of(const MassParams& p, const Seq& q) {
+    return (q.len + p.batch.page_tokens - 1) / p.batch.page_tokens;
+}
+
+// A tile of pages is summed key by key into LDS, in blocks of KEYS keys (kb) from its first (key0) on: thread i adds up
+// its page's keys, block by block.
+template <int KEYS>
+__device__ __forceinline__ float page_sum(const MassParams& p, const float* key_sum, int kb, int key0, float sum) {
     const int T = p.batch.page_tokens;
-    const int key0 = page0 * T, key1 = min(seq.len, key0 + pages * T);
-    const float* account = p.mass + ((int64_t)s * p.kv_heads + head) * p.max_pages + page0;
-    float* out = p.out + ((int64_t)s * p.kv_heads + head) * p.max_pages + page0;
-    float sum = 0.f;                                          // thread i: of page page0 + i
-    for (int kb = key0; kb < key1 && rows > 0; kb += kBlockKeys) {
-        const int wb = kb + 64 * wave;
-        uint64_t here = 0;
-        float acc[4][4] = {};
-        if (wb < key1) {
-            const Place at = place_of(p.batch, seq, wb + lane, key1);
-            here = __ballot(at.page >= 0);
-            const int page = max(at.page, 0), row = at.page >= 0 ? at.row : 0;
-            uint4 kf[4][kSteps];
+    if ((int)threadIdx.x < p.group_pages) {
+        const int from = max(kb, key0 + (int)threadIdx.x * T), to = min(kb + KEYS, key0 + ((int)threadIdx.x + 1) * T);
+#pragma unroll 4
+        for (int k = from; k < to; ++k) sum += key_sum[k - kb];
+    }
+    return sum;
+}
+
+__device__ __forceinline__ void store_account(const MassParams& p, const Seq& q, int s, int head, int page0, float sum) {
+    if ((int)threadIdx.x < p.group_pages && page0 + (int)threadIdx.x < pages_of(p, q)) {
+        const int64_t at = ((int64_t)s * p.kv_heads + head) * p.max_pages + page0 + threadIdx.x;
+        p.out[at] = __builtin_fmaf(p.decay, p.mass[at], sum);
+    }
+}
+
+// Accounts of a sequence that receive nothing: of pages behind its tokens, all of them if it has no rows.
+__device__ __forceinline__ void rest_of(const MassParams& p, int s, int head) {
+    if (p.out == p.mass && p.decay == 1.f) return;
+    const Seq seq = seq_of(p.batch, s);
+    const int from = seq.n_new > 0 ? pages_of(p, seq) : 0;
+    const int64_t at = ((int64_t)s * p.kv_heads + head) * p.max_pages;
+    for (int i = from + (int)threadIdx.x; i < p.max_pages; i += 256) p.out[at + i] = p.decay * p.mass[at + i];
+}
+
+// ---- few rows -------------------------------------------------------------------
+// Decoding: reading K is the work.  The tiles of all sequences lie one behind the
+// other and every workgroup of a KV head takes an equal number of them; a wave has
+// 32 keys of a block and its loads of the next block in flight while it works on
+// this one.  The rows stay in registers for a whole sequence.
+
+template <int DT, int DP, int NT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 128 && NT == 1 ? 3 : 2)))
+void mass_few_kernel(MassParams p) {
+    constexpr int kSteps = DP / 32;
+    __shared__ float key_sum[2][kFewKeys];
+    const int lane = (int)threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+    const int col = lane & 15, quad = lane >> 4;
+    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads), group = (int)(blockIdx.x / (uint32_t)p.kv_heads);
+    auto tiles_of = [&](const Seq& q) {
+        const int64_t rows = (int64_t)q.n_new * p.group;
+        return rows == 0 || rows > p.few_rows ? 0 : mass_tiles(p, q);
+    };
+    for (int i = group; i < p.batch.n_seqs; i += p.few_groups) rest_of(p, i, head);
+    int none;
+    const int total = uniform(count_tiles(p.batch, 0, none, tiles_of)), quota = (total + p.few_groups - 1) / p.few_groups;
+    if ((int64_t)group * quota >= total) return;
+    int tile = group * quota, left = min(quota, total - tile), flip = 0;
+    int s = uniform(find_tile(p.batch, tile, tiles_of));
+    tile = uniform(tile);
+    const int tile_keys = p.group_pages * p.batch.page_tokens;
+    for (; left > 0 && s < p.batch.n_seqs; ++s, tile = 0) {
+        const Seq seq = uniform(seq_of(p.batch, s));
+        const int rows = seq.n_new * p.group, n_tiles = tiles_of(seq);
+        if (n_tiles == 0) continue;
+        const int end = tile + min(n_tiles - tile, left);
+        left -= end - tile;
+        const int key_end = min(seq.len, end * tile_keys);
+        int limit[NT];                                        // tokens that the lane's row sees
+        float base[NT];
+        uint4 qf[NT][kSteps];
+        auto load_q = [&](int r0) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int64_t pg = __shfl(page, 16 * u + col), rw = __shfl(row, 16 * u + col);
-                const uint8_t* src = p.k_pool + 2 * (pg * p.k_page + (rw * p.kv_heads + head) * p.head_dim);
+            for (int t = 0; t < NT; ++t) {
+                const int r = r0 + 16 * t + col, token = r / p.group, q_head = head * p.group + (r - token * p.group);
+                const uint8_t* src = p.q + 2 * ((int64_t)(seq.row0 + token) * p.q_stride + (int64_t)q_head * p.head_dim);
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    const int d = 32 * i + 8 * quad;
+                    qf[t][i] = r < rows && d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
+                }
+                const float lse = r < rows ? p.lse[(int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head] : -INFINITY;
+                limit[t] = lse == -INFINITY ? 0 : seq.len - seq.n_new + token + 1;   // -infinity: the row saw nothing
+                base[t] = lse == -INFINITY ? 0.f : lse * kLog2e;
+            }
+        };
+        load_q(0);
+        uint4 kf[2][kSteps];
+        uint32_t valid = 0;
+        int entry = -1;                                       // of key lane % 32 of the wave's share of the block to be loaded
+        auto look_up = [&](int kb) {
+            const int key = kb + 32 * wave + (lane & 31);
+            return key < key_end ? seq.table[div_page(key, p.batch.page_div)] : -1;
+        };
+        auto load = [&](int kb) {
+            const int key = kb + 32 * wave + (lane & 31);
+            const bool has = (uint32_t)entry < (uint32_t)p.batch.n_pages;
+            valid = (uint32_t)__ballot(has);
+            const int row = key - div_page(key, p.batch.page_div) * p.batch.page_tokens;
+            const uint64_t mine =
+                (uint64_t)(p.k_pool + (has ? 2 * (entry * p.k_page + (int64_t)(row * p.kv_heads + head) * p.head_dim) : 0));
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint8_t* src = (const uint8_t*)__shfl(mine, 16 * u + col);
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i) {
                     const int d = 32 * i + 8 * quad;
                     kf[u][i] = d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
                 }
             }
-            // rows that see the wave's first key
-            const int t0 = max(0, wb - (seq.len - seq.n_new));
-            for (int r0 = t0 < seq.n_new ? t0 * p.group / 16 * 16 : rows; r0 < rows; r0 += 16) {
-                const int r = r0 + col;
-                const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
-                int limit = r < rows ? seq.len - seq.n_new + token + 1 : 0;
-                const uint8_t* src = p.q + 2 * ((int64_t)(seq.row0 + token) * p.q_stride + (int64_t)q_head * p.head_dim);
-                uint4 qf[kSteps];
+        };
+        // blocks of a tile: one, or several of a page of more than kFewKeys tokens
+        auto next_block = [&](int kb, int key0) { return kb + kFewKeys < key0 + tile_keys ? kb + kFewKeys : key0 + tile_keys; };
+        int key0 = tile * tile_keys, kb = key0;
+        entry = look_up(kb);
+        load(kb);
+        entry = look_up(next_block(kb, key0));
+        float sum = 0.f;
+        while (kb < key_end) {
+            const uint32_t here = valid;
+            const int next = next_block(kb, key0), most = min(kb + kFewKeys, min(next, key_end)) - (kb + 32 * wave);
+            float x[8] = {};
+            auto weigh = [&]() {
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
-                    const int d = 32 * i + 8 * quad;
-                    qf[i] = r < rows && d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
-                }
-                const float lse = r < rows ? p.lse[(int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head] : 0.f;
-                if (lse == -INFINITY) limit = 0;             // the row saw nothing
-                const float base = lse == -INFINITY ? 0.f : lse * kLog2e;
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+                    for (int u = 0; u < 2; ++u) {
+                        f32x4 sc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int i = 0; i < kSteps; ++i) sc = mfma16<DT>(kf[u][i], qf[i], sc);
+                        for (int i = 0; i < kSteps; ++i) sc = mfma16<DT>(kf[u][i], qf[t][i], sc);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], p.scale_log2, -base));
-                        acc[u][i] += wb + 16 * u + 4 * quad + i < limit ? w : 0.f;
+                        for (int i = 0; i < 4; ++i) {
+                            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], p.scale_log2, -base[t]));
+                            x[4 * u + i] += kb + 32 * wave + 16 * u + 4 * quad + i < limit[t] ? w : 0.f;
+                        }
                     }
+            };
+            weigh();
+            if (rows > 16 * NT) {                             // more rows than the caller said: they come again for every block
+                for (int r0 = 16 * NT; r0 < rows; r0 += 16 * NT) {
+                    load_q(r0);
+                    weigh();
                 }
+                load_q(0);
+            }
+            if (next < key_end) {
+                load(next);
+                entry = look_up(next_block(next, next < key0 + tile_keys ? key0 : next));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int key = 16 * (i / 4) + 4 * quad + i % 4;
+                const float y = xor_sum(x[i], 16);
+                if (col == 0) key_sum[flip][32 * wave + key] = ((here >> key) & 1u) && key < most ? y : 0.f;
+            }
+            __syncthreads();
+            sum = page_sum<kFewKeys>(p, key_sum[flip], kb, key0, sum);
+            flip ^= 1;
+            kb = next;
+            if (next == key0 + tile_keys) {
+                store_account(p, seq, s, head, tile * p.group_pages, sum);
+                sum = 0.f;
+                ++tile;
+                key0 = next;
             }
         }
+        if (key0 < key_end) store_account(p, seq, s, head, tile * p.group_pages, sum);   // the last page's blocks behind the end
+    }
+}
+
+// ---- many rows ------------------------------------------------------------------
+// Chunks of prompts: the products and exponentials are the work.  A workgroup
+// owns a tile of pages of one KV head: K stays in registers, 32 of a block's keys
+// a wave, while the rows, 128 (64) at a time, pass through LDS, the next ones on their
+// way meanwhile.  Two waves have the same keys and each half of the rows, so that
+// tiles are small and many: early ones, which more rows see, start first, and
+// the card ends evenly.  Every page's account has one writer and one order of additions.
+
+template <int DT, int DP>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1)))
+void mass_many_kernel(MassParams p) {
+    constexpr int kSub = DP <= 128 ? 2 : 1;                   // 32-row tiles that a wave works on at a time
+    constexpr int kRowTile = 64 * kSub, kScores = 16 * kSub;
+    constexpr int kSteps = DP / 16, kChunks = DP / 8, kRowBytes = DP * 2, kTileBytes = kRowTile * kRowBytes;
+    constexpr int kLoadRows = 64 / kChunks, kLoads = kRowTile / kLoadRows / 4;
+    __shared__ __attribute__((aligned(16))) uint8_t tiles[2][kTileBytes];
+    __shared__ float key_sum[2][kManyKeys];
+    const int lane = (int)threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const int row_half = wave >> 1;
+    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads);
+    const uint32_t rest = blockIdx.x / (uint32_t)p.kv_heads;
+    const int s = (int)(rest % (uint32_t)p.batch.n_seqs), tile = (int)(rest / (uint32_t)p.batch.n_seqs);   // early keys, which most rows see, first
+    const Seq seq = uniform(seq_of(p.batch, s));
+    const int rows = seq.n_new * p.group;
+    if (!p.few_groups && tile == 0) rest_of(p, s, head);
+    if (rows <= p.few_rows || tile >= mass_tiles(p, seq)) return;
+    const int tile_keys = p.group_pages * p.batch.page_tokens, key0 = tile * tile_keys, key_end = min(seq.len, key0 + tile_keys);
+    const int before = seq.len - seq.n_new;                   // tokens that every row sees
+    const uint32_t lds0 = lds_address(&tiles[0][0]);
+    const int load_row = lane / kChunks, load_chunk = lane % kChunks;
+    auto swizzle = [](int row, int chunk) { return chunk ^ (row & (kChunks < 16 ? kChunks - 1 : 15)); };
+    // This wave's quarter of the rows from r0 on.  Where the group is a power of two that divides the rows, the loads
+    // of every step lie alike: a scalar says where the rows begin, eight more how far behind that a load does, and a
+    // lane's offset in its load is always the same.  Otherwise, and for the last rows, every lane has its own address
+    // (rows behind the last one are the last one's numbers; columns behind head_dim are not written).
+    const bool even = p.head_dim == DP && (p.group & (p.group - 1)) == 0 && p.group <= kRowTile &&
+                      kRowTile * p.q_stride < ((int64_t)1 << 30);
+    const int lane_token = p.group < kLoadRows ? load_row / p.group : 0;
+    const uint32_t lane_offset = even ? (uint32_t)(2 * (lane_token * p.q_stride + (load_row - lane_token * p.group) * p.head_dim)) : 0;
+    int load_offset[kLoads];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+    for (int i = 0; i < kLoads; ++i) {
+        const int first = (wave * kLoads + i) * kLoadRows, token = div_page(first, p.group_div);
+        load_offset[i] = even ? (int)(2 * (token * p.q_stride + (first - token * p.group) * DP)) : 0;
+    }
+    auto load_rows = [&](int r0, int buffer) __attribute__((always_inline)) {
+        if (even && r0 + kRowTile <= rows) {
+            const uint8_t* base = p.q + 2 * ((int64_t)(seq.row0 + div_page(r0, p.group_div)) * p.q_stride + (int64_t)head * p.group * DP);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = 16 * u + 4 * quad + i;
-                const float x = xor_sum(acc[u][i], 16);
-                if (col == 0) key_sum[64 * wave + key] = (here >> key) & 1u ? x : 0.f;
+            for (int i = 0; i < kLoads; ++i) {
+                const int first = (wave * kLoads + i) * kLoadRows;
+                load_lds16(base + load_offset[i], lane_offset + 16 * swizzle(first + load_row, load_chunk),
+                           lds0 + (uint32_t)(buffer * kTileBytes + first * kRowBytes));
             }
-        __syncthreads();
-        if ((int)threadIdx.x < pages) {
-            const int from = max(kb, key0 + (int)threadIdx.x * T), to = min(kb + kBlockKeys, key0 + ((int)threadIdx.x + 1) * T);
-            for (int k = from; k < to; ++k) sum += key_sum[k - kb];
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int first = (wave * kLoads + i) * kLoadRows, row = first + load_row, r = min(r0 + row, rows - 1);
+                const int token = div_page(r, p.group_div), chunk = swizzle(row, load_chunk);
+                const uint8_t* src = p.q + 2 * ((int64_t)(seq.row0 + token) * p.q_stride +
+                                                (int64_t)(head * p.group + (r - token * p.group)) * p.head_dim);
+                if (chunk * 8 < p.head_dim) load_lds16(src + 16 * chunk, lds0 + (uint32_t)(buffer * kTileBytes + first * kRowBytes));
+            }
         }
+    };
+    if (p.head_dim < DP) {
+        for (int i = (int)threadIdx.x; i < 2 * kTileBytes / 16; i += 256)
+            reinterpret_cast<uint4*>(&tiles[0][0])[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
     }
-    if ((int)threadIdx.x < pages) out[threadIdx.x] = __builtin_fmaf(p.decay, account[threadIdx.x], sum);
+    uint32_t q_at[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) q_at[i] = (uint32_t)((32 * kSub * row_half + col) * kRowBytes + swizzle(col, 2 * i + half) * 16);
+
+    float sum = 0.f;
+    for (int kb = key0; kb < key_end; kb += kManyKeys) {
+        const int wb = kb + 32 * (wave & 1);                        // this wave's first key
+        const int most = min(kb + kManyKeys, key_end) - wb;
+        uint4 kf[kSteps];
+        uint32_t here;
+        {
+            const Place at = place_of(p.batch, seq, wb + col, min(kb + kManyKeys, key_end));
+            here = (uint32_t)__ballot(at.page >= 0);
+            const uint8_t* src = p.k_pool + (at.page >= 0 ? 2 * (at.page * p.k_page + (int64_t)(at.row * p.kv_heads + head) * p.head_dim) : 0);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const int d = 16 * i + 8 * half;
+                kf[i] = d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
+            }
+        }
+        // from the first row that sees the block's first key
+        const int first_token = max(0, kb - before);
+        const int row0 = first_token < seq.n_new ? first_token * p.group / kRowTile * kRowTile : rows;
+        float acc[16] = {};
+        // a row's lse, and the tokens that it sees, one tile ahead
+        float lse[kSub];
+        int sees[kSub];
+        auto load_lse = [&](int r0) {
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+                const int r = r0 + 32 * kSub * row_half + 32 * u + col, at = min(r, rows - 1), token = div_page(at, p.group_div);
+                sees[u] = r < rows ? before + token + 1 : 0;
+                lse[u] = p.lse[(int64_t)(seq.row0 + token) * p.kv_heads * p.group + head * p.group + (at - token * p.group)];
+            }
+        };
+        if (row0 < rows) {
+            load_lse(row0);
+            load_rows(row0, 0);
+        }
+        // The weights of 64 rows whose scores are made are taken beside the next rows' products, so that the wave has
+        // products and vector work at the same time; LDS reads run two steps ahead, and the barriers keep the compiler
+        // from putting each right before its product.
+        float base[kSub] = {};
+        int limit[kSub] = {};
+        auto hide = [&](f32x16 (&sc)[kSub]) {                    // what the scores' rows do not see
+            if (__all(min(limit[0], limit[kSub - 1]) >= wb + 32)) return;
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+                const int seen = limit[u] - wb - 4 * half;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (8 * (i / 4) + i % 4 >= seen) sc[u][i] = -INFINITY;
+            }
+        };
+        auto weigh = [&](const f32x16 (&sc)[kSub], int w) {
+            acc[w % 16] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[w / 16][w % 16], p.scale_log2, -base[w / 16]));
+            asm volatile("" : "+v"(acc[w % 16]));
+        };
+        auto step = [&](int r0, auto buffer_c, f32x16 (&sc)[kSub], f32x16 (&next)[kSub]) __attribute__((always_inline)) {
+            constexpr int buffer = decltype(buffer_c)::value;
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            float z[kSub];
+            int z_sees[kSub];
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+                z[u] = lse[u];
+                z_sees[u] = sees[u];
+            }
+            if (r0 + kRowTile < rows) {
+                load_lse(r0 + kRowTile);
+                load_rows(r0 + kRowTile, buffer ^ 1);
+            }
+            hide(sc);
+            uint4 qf[3][kSub];
+            auto read_q = [&](int i) {
+#pragma unroll
+                for (int u = 0; u < kSub; ++u)
+                    qf[i % 3][u] = *reinterpret_cast<const uint4*>(tiles[buffer] + q_at[i] + 32 * u * kRowBytes);
+            };
+            read_q(0);
+            read_q(1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                if (i + 2 < kSteps) read_q(i + 2);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < kSub; ++u) {
+                    if (i == 0)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) next[u][e] = 0.f;
+                    next[u] = mfma32<DT>(kf[i], qf[i % 3][u], next[u]);
+#pragma unroll
+                    for (int w = 0; w < kScores; ++w)
+                        if (w * kSub * kSteps / kScores == kSub * i + u) weigh(sc, w);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+                base[u] = z[u] == -INFINITY ? 0.f : z[u] * kLog2e;
+                limit[u] = z[u] == -INFINITY ? 0 : z_sees[u];   // -infinity: the row saw nothing
+            }
+        };
+        if (row0 < rows) {
+            f32x16 a[kSub], b[kSub];
+#pragma unroll
+            for (int i = 0; i < kScores; ++i) a[i / 16][i % 16] = -INFINITY;   // no rows yet
+            auto finish = [&](f32x16 (&sc)[kSub]) {
+                hide(sc);
+#pragma unroll
+                for (int w = 0; w < kScores; ++w) weigh(sc, w);
+            };
+            for (int r0 = uniform(row0);;) {
+                step(r0, std::integral_constant<int, 0>{}, a, b);
+                if ((r0 += kRowTile) >= rows) {
+                    finish(b);
+                    break;
+                }
+                step(r0, std::integral_constant<int, 1>{}, b, a);
+                if ((r0 += kRowTile) >= rows) {
+                    finish(a);
+                    break;
+                }
+            }
+        }
+        __syncthreads();                                      // the last rows, and the previous block's sums, have been read
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int key = 8 * (i / 4) + 4 * half + i % 4;
+            const float x = xor_sum(acc[i], 32);
+            if (col == 0) key_sum[row_half][32 * (wave & 1) + key] = ((here >> key) & 1u) && key < most ? x : 0.f;
+        }
+        __syncthreads();
+        if (threadIdx.x < kManyKeys) key_sum[0][threadIdx.x] += key_sum[1][threadIdx.x];
+        __syncthreads();
+        sum = page_sum<kManyKeys>(p, key_sum[0], kb, key0, sum);
+    }
+    store_account(p, seq, s, head, tile * p.group_pages, sum);
 }
 
 template <int DT, int DP>
-void launch(const MassParams& p, hipStream_t stream) {
-    const int64_t groups = (p.max_pages + p.group_pages - 1) / p.group_pages;
-    hipLaunchKernelGGL((mass_kernel<DT, DP>), dim3((uint32_t)(p.batch.n_seqs * groups * p.kv_heads)), dim3(256), 0, stream, p);
+void launch(MassParams p, int64_t most_rows, int cus, hipStream_t stream) {
+    const int64_t heads = p.kv_heads;
+    auto tiles_of = [&](int keys) {                           // of a table row
+        p.group_pages = p.batch.page_tokens >= keys ? 1 : keys / p.batch.page_tokens;
+        return (int64_t)(p.max_pages + p.group_pages - 1) / p.group_pages;
+    };
+    // rows of a decoding sequence fit 16 or 32; where none can have more the few kernel does all
+    const int nt = most_rows <= 16 ? 1 : most_rows <= 32 ? 2 : p.group <= 16 ? 1 : p.group <= 32 ? 2 : 0;
+    const bool many = most_rows > 32 || nt == 0;
+    p.few_rows = many ? 16 * nt : 0x7FFFFFFF;
+    if (nt) {
+        const int64_t resident = ((int64_t)cus * (DP <= 128 && nt == 1 ? 3 : 2) + heads - 1) / heads, tiles = p.batch.n_seqs * tiles_of(kFewKeys);
+        p.few_groups = (int32_t)(resident < tiles ? resident : tiles);
+        const dim3 grid((uint32_t)(p.few_groups * heads));
+        if (nt == 1) hipLaunchKernelGGL((mass_few_kernel<DT, DP, 1>), grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL((mass_few_kernel<DT, DP, 2>), grid, dim3(256), 0, stream, p);
+    }
+    if (many) {
+        const int64_t tiles = p.batch.n_seqs * tiles_of(kManyKeys);
+        hipLaunchKernelGGL((mass_many_kernel<DT, DP>), dim3((uint32_t)(tiles * heads)), dim3(256), 0, stream, p);
+    }
 }
 
 }  // namespace
@@ -153,19 +472,22 @@ extern "C" int ztcp_attention_mass(const void* q, int64_t q_stride, const float*
     p.k_page = pool->k_stride;
     p.kv_heads = (int32_t)g->num_heads;
     p.group = (int32_t)(q_heads / g->num_heads);
+    p.group_div = div_by((uint32_t)p.group);
     p.head_dim = (int32_t)d;
     p.max_pages = (int32_t)batch->max_pages;
-    p.group_pages = (int32_t)(g->num_tokens >= kBlockKeys ? 1 : kBlockKeys / g->num_tokens);
     p.scale_log2 = scale * kLog2e;
     p.decay = decay;
-    const int64_t groups = (p.max_pages + p.group_pages - 1) / p.group_pages;
-    if (batch->n_seqs * groups * g->num_heads >= (int64_t)1 << 31)
+    const int64_t most_q = batch->max_q_len > 0 && batch->max_q_len < batch->n_rows ? batch->max_q_len : batch->n_rows;
+    const int64_t most_rows = most_q * p.group;
+    int cus = 0;
+    if (cu_count(cus) != ZTCP_OK) return ZTCP_EHIP;
+    if (batch->n_seqs * batch->max_pages * g->num_heads >= (int64_t)1 << 31)
         return arg_result(ZTCP_EINVAL, "too many sequences, pages and heads in one call");
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        if (d <= 64) launch<DT, 64>(p, (hipStream_t)stream);
-        else if (d <= 128) launch<DT, 128>(p, (hipStream_t)stream);
-        else launch<DT, 256>(p, (hipStream_t)stream);
+        if (d <= 64) launch<DT, 64>(p, most_rows, cus, (hipStream_t)stream);
+        else if (d <= 128) launch<DT, 128>(p, most_rows, cus, (hipStream_t)stream);
+        else launch<DT, 256>(p, most_rows, cus, (hipStream_t)stream);
     };
     if (g->hot_dtype == ZTCP_HOT_BF16) go(std::integral_constant<int, kHotBf16>{});
     else go(std::integral_constant<int, kHotFp16>{});
