@@ -22,7 +22,8 @@ struct AppendParams {
     const uint8_t* q_weight;
     const uint8_t* k_weight;
     int32_t q_weight_len, k_weight_len;
-    uint32_t vecs, vecs_per_token;                        // head vectors of the call, of a token
+    uint32_t n_tokens, parts;                             // a token's vectors are shared by `parts` waves,
+    int32_t vecs, part_vecs;                              // part_vecs of its vecs each
     int32_t q_heads, kv_heads, head_dim, rope_dim, page_tokens;
     int32_t interleaved;
     float eps;
@@ -34,8 +35,7 @@ struct Chunk {
 };
 
 template <int DT>
-__device__ __forceinline__ Chunk load_chunk(const uint8_t* p) {
-    const uint4 w = ldg16(p);
+__device__ __forceinline__ Chunk unpack(uint4 w) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
     Chunk c;
 #pragma unroll
@@ -52,127 +52,170 @@ __device__ __forceinline__ uint4 pack_chunk(const Chunk& c) {
                       pack_hot<DT>(c.x[6], c.x[7]));
 }
 
-// One head vector per group of LANES lanes (a power of two, eight elements a
-// lane and chunk; CHUNKS > 1 only for the vectors of more than 512 elements).
-// The pass reads and writes every element once and is bound by that; the sum
-// of squares is a butterfly over the group, and the partner of a rotated pair
-// sits rope_dim / 16 lanes away (or in the same lane when interleaved), so a
-// vector never leaves registers.
-template <int DT, int LANES, int CHUNKS>
+// A group of LANES lanes (a power of two, eight elements a lane and chunk; CHUNKS > 1 only for vectors of more than
+// 512 elements) has a head vector; a wave has a token's vectors, or a part of them, in turns of 64 / LANES.  The pass
+// reads and writes every element once and is bound by that: the angles and weights are loaded once for a wave's
+// vectors, the next turns' loads are in flight during a turn, the sum of squares is a butterfly over the group, and
+// the partner of a rotated pair sits rope_dim / 16 lanes away (or in the same lane when interleaved), so a vector
+// never leaves registers.  Prompt of 16,384 tokens of 32 + 8 + 8 vectors of 128: a wave for every four vectors, with
+// angles and weights of its own, took 147 us.
+template <int DT, int LANES, int CHUNKS, int AHEAD>
 __global__ __launch_bounds__(256) void append_kernel(AppendParams p) {
-    const int lane = (int)threadIdx.x % LANES;
-    const uint32_t vec = blockIdx.x * (256u / LANES) + threadIdx.x / LANES;
-    const bool live = vec < p.vecs;
-    const uint32_t token = live ? vec / p.vecs_per_token : 0u;
-    const int h = live ? (int)(vec - token * p.vecs_per_token) : 0;
-    const bool is_q = h < p.q_heads, is_k = !is_q && h < p.q_heads + p.kv_heads;
-    const int head = is_q ? h : is_k ? h - p.q_heads : h - p.q_heads - p.kv_heads;
-    const int64_t stride = is_q ? p.q_stride : is_k ? p.k_stride : p.v_stride;
-    const uint8_t* src = (is_q ? p.q : is_k ? p.k : p.v) + 2 * ((int64_t)token * stride + (int64_t)head * p.head_dim);
-    const int n_chunks = live ? p.head_dim / 8 : 0;
-    Chunk c[CHUNKS];
+    constexpr int kTurn = 64 / LANES;                         // vectors of a turn
+    constexpr int kAhead = AHEAD;                             // turns in flight
+    const int lane = (int)threadIdx.x % LANES, group = ((int)threadIdx.x & 63) / LANES;
+    const uint32_t unit = (uint32_t)uniform((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    const uint32_t token = unit / p.parts, part = unit - token * p.parts;
+    if (token >= p.n_tokens) return;
+    const int first = (int)part * p.part_vecs, end = min(first + p.part_vecs, p.vecs);
+    const int n_chunks = p.head_dim / 8;
+    const uint8_t* q = p.q + 2 * (int64_t)token * p.q_stride;
+    const uint8_t* k = p.k + 2 * (int64_t)token * p.k_stride;
+    const uint8_t* v = p.v + 2 * (int64_t)token * p.v_stride;
+    uint8_t* q_out = p.q_out + 2 * (int64_t)token * p.q_out_stride;
+    const int64_t slot = p.slots[token];
+    const int32_t position = p.rope_dim > 0 ? p.positions[token] : 0;
+
+    // where the token's K and V go
+    uint8_t* k_out = nullptr;
+    uint8_t* v_out = nullptr;
+    if (slot >= 0 && slot < p.n_slots) {
+        const int64_t page = slot / p.page_tokens, row = slot - page * p.page_tokens;
+        const int64_t in_page = row * p.kv_heads * p.head_dim;
+        k_out = p.k_pool + 2 * (page * p.k_page + in_page);
+        v_out = p.v_pool + 2 * (page * p.v_page + in_page);
+    }
+    // Cosines and sines of this lane's elements, (1, 0) for those that do not turn; of a pair's second half the sine
+    // that its first has, negated, so that both are x cos - partner sin.  All rotated columns are in a lane's chunk 0
+    // (rope_dim <= 512).
+    const int half = p.rope_dim / 16;                         // chunks of half the rotated columns
+    const bool turned = lane < 2 * half;
+    float cs[8], sn[8];
+    {
+        const bool known = position >= 0 && position < p.max_position;
+        const float* row = p.rope + (int64_t)(known ? position : 0) * p.rope_dim;
+        const int a0 = p.interleaved ? 4 * lane : 8 * (lane < half ? lane : lane - half);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            cs[e] = 1.f;
+            sn[e] = 0.f;
+            if (turned && (!p.interleaved || e < 4)) {
+                cs[e] = known ? row[a0 + e] : __builtin_nanf("");
+                sn[e] = known ? row[8 * half + a0 + e] : __builtin_nanf("");
+                if (!p.interleaved && lane >= half) sn[e] = -sn[e];
+            }
+        }
+    }
+    const int partner = ((int)threadIdx.x & 63) + (!turned ? 0 : lane < half ? half : -half);
+    // Weights of this lane's elements
+    uint4 wq[CHUNKS], wk[CHUNKS];
+    const int q_first = (p.head_dim - p.q_weight_len) / 8, k_first = (p.head_dim - p.k_weight_len) / 8;   // first normed chunk
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
         const int at = lane + i * LANES;
-        if (at < n_chunks) c[i] = load_chunk<DT>(src + 16 * at);
-        else
-#pragma unroll
-            for (int e = 0; e < 8; ++e) c[i].x[e] = 0.f;
+        wq[i] = at >= q_first && at < n_chunks ? ldg16(p.q_weight + 16 * (at - q_first)) : make_uint4(0, 0, 0, 0);
+        wk[i] = at >= k_first && at < n_chunks ? ldg16(p.k_weight + 16 * (at - k_first)) : make_uint4(0, 0, 0, 0);
     }
-    // where the vector goes
-    uint8_t* dst = nullptr;
-    if (live) {
-        if (is_q) {
-            dst = p.q_out + 2 * ((int64_t)token * p.q_out_stride + (int64_t)head * p.head_dim);
-        } else {
-            const int64_t slot = p.slots[token];
-            if (slot >= 0 && slot < p.n_slots) {
-                const int64_t page = slot / p.page_tokens, row = slot - page * p.page_tokens;
-                dst = (is_k ? p.k_pool + 2 * page * p.k_page : p.v_pool + 2 * page * p.v_page) +
-                      2 * (row * p.kv_heads + head) * p.head_dim;
-            }
-        }
-    }
-    // norm of the last weight_len columns
-    const int weight_len = is_q ? p.q_weight_len : is_k ? p.k_weight_len : 0;
-    const int first = (p.head_dim - weight_len) / 8;   // first normed chunk
-    float ss = 0.f;
+
+    // (no lambdas: what they choose between by lane they would choose by address, in scratch memory)
+    uint4 c[kAhead][CHUNKS];
+    for (int h1 = first - kAhead * kTurn; h1 < end; h1 += kAhead * kTurn) {
 #pragma unroll
-    for (int i = 0; i < CHUNKS; ++i)
-        if (lane + i * LANES >= first)
+        for (int i = 0; i < kAhead; ++i) {
+            if (h1 >= first) {
+                const int h0 = h1 + i * kTurn, h = h0 + group;
+                const bool is_q = h < p.q_heads, is_k = !is_q && h < p.q_heads + p.kv_heads;
+                Chunk x[CHUNKS];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(c[i].x[e], c[i].x[e], ss);
-    ss = xor_sum(ss, LANES);
-    if (weight_len > 0) {
-        const float inv = rsqrtf(ss / (float)weight_len + p.eps);
-        const uint8_t* weight = is_q ? p.q_weight : p.k_weight;
+                for (int j = 0; j < CHUNKS; ++j) x[j] = unpack<DT>(c[i][j]);
+                if (h0 < p.q_heads + p.kv_heads) {                    // not V alone
+                    const int normed = is_q ? q_first : is_k ? k_first : n_chunks;
+                    float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < CHUNKS; ++i) {
-            const int at = lane + i * LANES;
-            if (at >= first && at < n_chunks) {
-                const Chunk w = load_chunk<DT>(weight + 16 * (at - first));
+                    for (int j = 0; j < CHUNKS; ++j)
+                        if (lane + j * LANES >= normed)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) c[i].x[e] = c[i].x[e] * inv * w.x[e];
-            }
-        }
-    }
-    // rotation; all rotated columns are in chunk 0 of a lane (rope_dim <= 512)
-    const int half = p.rope_dim / 16;   // chunks of half the rotated columns
-    if (half > 0) {
-        const bool turned = lane < 2 * half && live && (is_q || is_k);
-        const int32_t pos = turned ? p.positions[token] : 0;
-        const bool known = pos >= 0 && pos < p.max_position;
-        const float* row = p.rope + (int64_t)(known ? pos : 0) * p.rope_dim;
-        float cs[8], sn[8];
-        const int a0 = p.interleaved ? 4 * lane : 8 * (lane < half ? lane : lane - half);
-        const int n = p.interleaved ? 4 : 8;
+                            for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(x[j].x[e], x[j].x[e], ss);
+                    ss = xor_sum(ss, LANES);
+                    const int len = p.head_dim - 8 * normed;
+                    const float inv = len > 0 ? rsqrtf(ss / (float)len + p.eps) : 1.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const bool has = turned && e < n;
-            cs[e] = has ? (known ? row[a0 + e] : __builtin_nanf("")) : 1.f;
-            sn[e] = has ? (known ? row[8 * half + a0 + e] : __builtin_nanf("")) : 0.f;
-        }
-        if (p.interleaved) {
-            if (turned)
+                    for (int j = 0; j < CHUNKS; ++j) {
+                        const Chunk w = unpack<DT>(make_uint4(is_q ? wq[j].x : wk[j].x, is_q ? wq[j].y : wk[j].y,
+                                                              is_q ? wq[j].z : wk[j].z, is_q ? wq[j].w : wk[j].w));
+                        if (lane + j * LANES >= normed)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float a = c[0].x[2 * e], b = c[0].x[2 * e + 1];
-                    c[0].x[2 * e] = __builtin_fmaf(a, cs[e], -(b * sn[e]));
-                    c[0].x[2 * e + 1] = __builtin_fmaf(b, cs[e], a * sn[e]);
+                            for (int e = 0; e < 8; ++e) x[j].x[e] = x[j].x[e] * inv * w.x[e];
+                    }
+                    if (half > 0) {
+                        const bool turns = turned && (is_q || is_k);
+                        if (p.interleaved) {
+                            if (turns)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const float a = x[0].x[2 * e], b = x[0].x[2 * e + 1];
+                                    x[0].x[2 * e] = __builtin_fmaf(a, cs[e], -(b * sn[e]));
+                                    x[0].x[2 * e + 1] = __builtin_fmaf(b, cs[e], a * sn[e]);
+                                }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float o = __shfl(x[0].x[e], partner);
+                                if (turns) x[0].x[e] = __builtin_fmaf(x[0].x[e], cs[e], -(o * sn[e]));
+                            }
+                        }
+                    }
                 }
-        } else {
-            const int partner = (int)(threadIdx.x & 63u) + (lane < half ? half : -half);
+                uint8_t* dst = is_q ? q_out + 2 * (int64_t)(h * p.head_dim)
+                                    : is_k ? k_out + 2 * (int64_t)((h - p.q_heads) * p.head_dim)
+                                           : v_out + 2 * (int64_t)((h - p.q_heads - p.kv_heads) * p.head_dim);
+                if (h < end && (is_q || k_out))
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float o = __shfl(c[0].x[e], partner & 63);
-                if (turned)
-                    c[0].x[e] = lane < half ? __builtin_fmaf(c[0].x[e], cs[e], -(o * sn[e]))
-                                            : __builtin_fmaf(c[0].x[e], cs[e], o * sn[e]);
+                    for (int j = 0; j < CHUNKS; ++j) {
+                        const int at = lane + j * LANES;
+                        if (at < n_chunks) stg16(dst, at, pack_chunk<DT>(x[j]));
+                    }
+            }
+            const int h = h1 + (i + kAhead) * kTurn + group;  // the turn after the next ones
+            const bool is_q = h < p.q_heads, is_k = !is_q && h < p.q_heads + p.kv_heads;
+            const uint8_t* src = is_q ? q + 2 * (int64_t)(h * p.head_dim)
+                                      : is_k ? k + 2 * (int64_t)((h - p.q_heads) * p.head_dim)
+                                             : v + 2 * (int64_t)((h - p.q_heads - p.kv_heads) * p.head_dim);
+#pragma unroll
+            for (int j = 0; j < CHUNKS; ++j) {
+                const int at = lane + j * LANES;
+                c[i][j] = h < end && at < n_chunks ? ldg16(src + 16 * at) : make_uint4(0, 0, 0, 0);
             }
         }
     }
-    if (dst)
-#pragma unroll
-        for (int i = 0; i < CHUNKS; ++i) {
-            const int at = lane + i * LANES;
-            if (at < n_chunks) stg16(dst, at, pack_chunk<DT>(c[i]));
-        }
 }
 
 template <int DT>
-void launch(const AppendParams& p, hipStream_t stream) {
+void launch(AppendParams p, int cus, hipStream_t stream) {
     const int chunks = p.head_dim / 8;
-    auto go = [&](auto kernel, uint32_t lanes) {
-        const uint32_t per_block = 256 / lanes;
-        hipLaunchKernelGGL(kernel, dim3((p.vecs + per_block - 1) / per_block), dim3(256), 0, stream, p);
+    auto go = [&](auto kernel1, auto kernel4, int lanes) {
+        // A wave has all of a token's vectors where that leaves 16 waves to a SIMD's queue, fewer where tokens are
+        // few: a decoding step's 32 tokens of 48 vectors are 384 waves of one turn, 4.6 us (7.3 with four in flight).
+        const int turn = 64 / lanes, turns = (p.vecs + turn - 1) / turn;
+        int64_t parts = ((int64_t)cus * 64 + p.n_tokens - 1) / p.n_tokens;
+        parts = parts < turns ? parts : turns;
+        const int per_part = (int)((turns + parts - 1) / parts);
+        p.part_vecs = per_part * turn;
+        p.parts = (uint32_t)((turns + per_part - 1) / per_part);
+        const uint64_t units = (uint64_t)p.n_tokens * p.parts;
+        const dim3 grid((uint32_t)((units + 3) / 4));
+        if (per_part < 4) hipLaunchKernelGGL(kernel1, grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL(kernel4, grid, dim3(256), 0, stream, p);
     };
-    if (chunks <= 2) go(append_kernel<DT, 2, 1>, 2);
-    else if (chunks <= 4) go(append_kernel<DT, 4, 1>, 4);
-    else if (chunks <= 8) go(append_kernel<DT, 8, 1>, 8);
-    else if (chunks <= 16) go(append_kernel<DT, 16, 1>, 16);
-    else if (chunks <= 32) go(append_kernel<DT, 32, 1>, 32);
-    else if (chunks <= 64) go(append_kernel<DT, 64, 1>, 64);
-    else go(append_kernel<DT, 64, 2>, 64);
+#define ZT_GO(lanes, chunks) go(append_kernel<DT, lanes, chunks, 1>, append_kernel<DT, lanes, chunks, 4>, lanes)
+    if (chunks <= 2) ZT_GO(2, 1);
+    else if (chunks <= 4) ZT_GO(4, 1);
+    else if (chunks <= 8) ZT_GO(8, 1);
+    else if (chunks <= 16) ZT_GO(16, 1);
+    else if (chunks <= 32) ZT_GO(32, 1);
+    else if (chunks <= 64) ZT_GO(64, 1);
+    else ZT_GO(64, 2);
+#undef ZT_GO
 }
 
 }  // namespace
@@ -255,8 +298,8 @@ extern "C" int ztcp_append_tokens(const void* q, int64_t q_stride, void* q_out, 
     p.k_weight = (const uint8_t*)k_weight;
     p.q_weight_len = (int32_t)q_weight_len;
     p.k_weight_len = (int32_t)k_weight_len;
-    p.vecs = (uint32_t)(n_tokens * per_token);
-    p.vecs_per_token = (uint32_t)per_token;
+    p.n_tokens = (uint32_t)n_tokens;
+    p.vecs = (int32_t)per_token;
     p.q_heads = (int32_t)q_heads;
     p.kv_heads = (int32_t)g->num_heads;
     p.head_dim = (int32_t)d;
@@ -264,7 +307,9 @@ extern "C" int ztcp_append_tokens(const void* q, int64_t q_stride, void* q_out, 
     p.page_tokens = (int32_t)g->num_tokens;
     p.interleaved = interleaved;
     p.eps = eps;
-    if (g->hot_dtype == ZTCP_HOT_BF16) launch<kHotBf16>(p, (hipStream_t)stream);
-    else launch<kHotFp16>(p, (hipStream_t)stream);
+    int cus = 0;
+    if (cu_count(cus) != ZTCP_OK) return ZTCP_EHIP;
+    if (g->hot_dtype == ZTCP_HOT_BF16) launch<kHotBf16>(p, cus, (hipStream_t)stream);
+    else launch<kHotFp16>(p, cus, (hipStream_t)stream);
     return hipGetLastError() == hipSuccess ? ZTCP_OK : ZTCP_EHIP;
 }
