@@ -6,8 +6,6 @@ using namespace ztcp;
 
 namespace {
 
-constexpr int kEvictThreads = 1024;
-constexpr int kEvictWaves = kEvictThreads / 64;
 constexpr int kDigitBits = 11;
 constexpr int kBins = 1 << kDigitBits;
 constexpr int kKeysInLds = 16384;   // 128 KiB of keys; longer tables sum their accounts again on every pass
@@ -35,7 +33,21 @@ __device__ __forceinline__ uint64_t order_of(double x) {
     return (b >> 63) ? ~b : b | (1ull << 63);
 }
 
+// A page's key: its accounts added up in the order of the heads, in 64 bits.
+__device__ __forceinline__ uint64_t key_from_accounts(const EvictParams& p, const float* mass, int page) {
+    double t = 0.0;
+    for (int h0 = 0; h0 < p.heads; h0 += 8) {   // eight loads in flight
+        float m[8];
+#pragma unroll
+        for (int h = 0; h < 8; ++h) m[h] = h0 + h < p.heads ? mass[(int64_t)(h0 + h) * p.max_pages + page] : 0.f;
+#pragma unroll
+        for (int h = 0; h < 8; ++h) t += (double)m[h];
+    }
+    return order_of(t);
+}
+
 // Sum over the block's waves of each wave's value, and the sum before this wave.
+template <int WAVES>
 __device__ __forceinline__ int block_before(int of_wave, int* lds, int& total) {
     const int wave = (int)threadIdx.x / 64;
     __syncthreads();
@@ -44,7 +56,7 @@ __device__ __forceinline__ int block_before(int of_wave, int* lds, int& total) {
     int before = 0;
     total = 0;
 #pragma unroll
-    for (int i = 0; i < kEvictWaves; ++i) {
+    for (int i = 0; i < WAVES; ++i) {
         const int x = lds[i];
         before += i < wave ? x : 0;
         total += x;
@@ -53,16 +65,19 @@ __device__ __forceinline__ int block_before(int of_wave, int* lds, int& total) {
 }
 
 // One workgroup per sequence.  The page that the count-th smallest key belongs
-// to is found digit by digit from the top (11 bits of the 64: a histogram of
-// the keys that share the digits found so far, then the bin in which the count
-// runs out); pages below it go, and of the pages equal to it the first ones.
-// Then one walk in page order closes the gaps: a page moves down by the number
-// of pages gone before it, so that a chunk that has been read whole may be
-// written over itself.
-__global__ __launch_bounds__(kEvictThreads) void evict_kernel(EvictParams p) {
+// to is found digit by digit from the highest bit in which the keys differ (11
+// bits at a time: a histogram of the keys that share the digits found so far,
+// then the bin in which the count runs out); pages below it go, and of the pages
+// equal to it the first ones.  Then one walk in page order closes the gaps: a
+// page moves down by the number of pages gone before it, so that a chunk that
+// has been read whole may be written over itself.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void evict_kernel(EvictParams p) {
+    constexpr int kWaves = THREADS / 64, kOwn = kBins / THREADS;
     extern __shared__ uint64_t keys[];
     __shared__ int bins[kBins];
-    __shared__ int scan[kEvictWaves];
+    __shared__ int scan[kWaves];
+    __shared__ uint64_t same[2][kWaves];
     __shared__ int found[3];
     const int64_t s = blockIdx.x;
     const int tid = (int)threadIdx.x, lane = tid & 63;
@@ -77,42 +92,54 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(EvictParams p) {
     const int64_t over = (int64_t)n - p.budget;
     const int count = (int)(over < 0 ? 0 : over < last - first ? over : last - first);
     const bool in_lds = p.max_pages <= kKeysInLds;
-    auto sum_key = [&](int page) {
-        double t = 0.0;
-        for (int h = 0; h < p.heads; ++h) t += (double)mass[(int64_t)h * p.max_pages + page];
-        return order_of(t);
-    };
-    auto key_of = [&](int page) { return in_lds ? keys[page] : sum_key(page); };
+    auto key_of = [&](int page) { return in_lds ? keys[page] : key_from_accounts(p, mass, page); };
 
     uint64_t bound = 0;   // the count-th smallest key's digits found so far
     int shift = 64, left = count, ties = 0;
     if (count > 0) {
-        if (in_lds)
-            for (int i = first + tid; i < last; i += kEvictThreads) keys[i] = sum_key(i);
+        uint64_t all = ~0ull, any = 0;
+#pragma unroll 4
+        for (int i = first + tid; i < last; i += THREADS) {
+            const uint64_t k = key_from_accounts(p, mass, i);
+            if (in_lds) keys[i] = k;
+            all &= k, any |= k;
+        }
+        for (int m = 1; m < 64; m <<= 1) {
+            all &= (uint64_t)__shfl_xor((unsigned long long)all, m);
+            any |= (uint64_t)__shfl_xor((unsigned long long)any, m);
+        }
+        if (lane == 0) same[0][tid / 64] = all, same[1][tid / 64] = any;
+        __syncthreads();
+        for (int w = 0; w < kWaves; ++w) all &= same[0][w], any |= same[1][w];
+        shift = all == any ? 0 : 64 - __clzll((long long)(all ^ any));
+        bound = shift < 64 ? all >> shift << shift : 0;
+        ties = last - first;   // what is left of the keys if they are all equal
         while (shift > 0) {
             const int bits = shift < kDigitBits ? shift : kDigitBits;
             const int next = shift - bits;
-            for (int i = tid; i < kBins; i += kEvictThreads) bins[i] = 0;
+            for (int i = tid; i < kBins; i += THREADS) bins[i] = 0;
             __syncthreads();
-            for (int i = first + tid; i < last; i += kEvictThreads) {
+            for (int i = first + tid; i < last; i += THREADS) {
                 const uint64_t k = key_of(i);
-                if (shift == 64 || (k >> shift) == (bound >> shift))
+                if (shift == 64 || ((k ^ bound) >> shift) == 0)
                     atomicAdd(&bins[(int)((k >> next) & ((1u << bits) - 1u))], 1);
             }
             __syncthreads();
-            // two bins a thread: the bin where the count runs out
-            const int b0 = bins[2 * tid], b1 = bins[2 * tid + 1];
-            int x = b0 + b1;
+            // the bin where the count runs out
+            int of[kOwn], own = 0;
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) own += of[j] = bins[kOwn * tid + j];
+            int x = own;
             for (int m = 1; m < 64; m <<= 1) {
                 const int y = __shfl_up(x, m);
                 x += lane >= m ? y : 0;
             }
             int total;
-            const int before = block_before(__shfl(x, 63), scan, total) + x - (b0 + b1);
-            if (before < left && left <= before + b0) {
-                found[0] = 2 * tid, found[1] = before, found[2] = b0;
-            } else if (before + b0 < left && left <= before + b0 + b1) {
-                found[0] = 2 * tid + 1, found[1] = before + b0, found[2] = b1;
+            int before = block_before<kWaves>(__shfl(x, 63), scan, total) + x - own;
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) {
+                if (before < left && left <= before + of[j]) found[0] = kOwn * tid + j, found[1] = before, found[2] = of[j];
+                before += of[j];
             }
             __syncthreads();
             bound |= (uint64_t)(uint32_t)found[0] << next;
@@ -128,7 +155,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(EvictParams p) {
     int32_t* evicted = p.evicted + s * p.max_pages;
     // a page goes if its digits are below the bound's, or equal and it is among the first `left` of those
     int ties_before = 0, gone_before = 0;
-    for (int base = 0; base < p.max_pages; base += kEvictThreads) {
+    for (int base = 0; base < p.max_pages; base += THREADS) {
         const int i = base + tid;
         const bool may = count > 0 && i >= first && i < last;
         const uint64_t k = may ? key_of(i) >> shift : ~0ull;
@@ -136,19 +163,20 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(EvictParams p) {
         const uint64_t lower = (1ull << lane) - 1ull;
         const uint64_t tm = __ballot(tie);
         int t_total, g_total;
-        const int t_at = ties_before + block_before(__popcll(tm), scan, t_total) + __popcll(tm & lower);
+        const int t_at = ties_before + block_before<kWaves>(__popcll(tm), scan, t_total) + __popcll(tm & lower);
         const bool gone = below || (tie && t_at < left);
         const uint64_t gm = __ballot(gone);
-        const int g_at = gone_before + block_before(__popcll(gm), scan, g_total) + __popcll(gm & lower);
+        const int g_at = gone_before + block_before<kWaves>(__popcll(gm), scan, g_total) + __popcll(gm & lower);
         const int32_t id = i < n ? table[i] : -1;
         const bool kept = i < n && !gone;
         const int to = i - g_at;
-        // everything of this chunk is read before any of it is written
+        // every wave has read its part of this chunk before any of it is written; a barrier alone does not wait for loads
         for (int h0 = 0; h0 < p.heads; h0 += 8) {
             float m[8];
 #pragma unroll
             for (int h = 0; h < 8; ++h)
                 m[h] = kept && h0 + h < p.heads ? mass[(int64_t)(h0 + h) * p.max_pages + i] : 0.f;
+            __builtin_amdgcn_s_waitcnt(0);
             __syncthreads();
 #pragma unroll
             for (int h = 0; h < 8; ++h)
@@ -160,7 +188,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(EvictParams p) {
         gone_before += g_total;
     }
     __syncthreads();
-    for (int i = tid; i < p.max_pages; i += kEvictThreads) {
+    for (int i = tid; i < p.max_pages; i += THREADS) {
         if (i >= count) evicted[i] = -1;
         if (i >= n - count) {
             out_table[i] = -1;
@@ -228,11 +256,14 @@ extern "C" int ztcp_evict_pages(const float* mass, const int32_t* page_table, in
     p.evicted = evicted;
     p.n_evicted = n_evicted;
     const size_t lds = max_pages <= kKeysInLds ? (size_t)max_pages * sizeof(uint64_t) : 0;
-    // over 64 KiB of dynamic LDS has to be asked for
-    if (lds > (size_t)48 * 1024 &&
-        hipFuncSetAttribute((const void*)evict_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                            kKeysInLds * (int)sizeof(uint64_t)) != hipSuccess)
-        return ZTCP_EHIP;
-    hipLaunchKernelGGL(evict_kernel, dim3((uint32_t)n_seqs), dim3(kEvictThreads), lds, (hipStream_t)stream, p);
-    return hipGetLastError() == hipSuccess ? ZTCP_OK : ZTCP_EHIP;
+    auto go = [&](auto kernel, uint32_t threads) {
+        // over 64 KiB of dynamic LDS has to be asked for
+        if (lds > (size_t)48 * 1024 &&
+            hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                kKeysInLds * (int)sizeof(uint64_t)) != hipSuccess)
+            return ZTCP_EHIP;
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)n_seqs), dim3(threads), lds, (hipStream_t)stream, p);
+        return hipGetLastError() == hipSuccess ? ZTCP_OK : ZTCP_EHIP;
+    };
+    return max_pages <= 1024 ? go(evict_kernel<256>, 256u) : go(evict_kernel<1024>, 1024u);
 }
