@@ -155,7 +155,8 @@ def _evict(N, **kw):
 
 
 def test_evict_arguments(N):
-    for kw in (dict(s=-1), dict(heads=0), dict(mp=0), dict(t=0), dict(mp=1 << 27), dict(budget=-1), dict(sink=-1),
+    for kw in (dict(s=-1), dict(heads=0), dict(mp=0), dict(t=0), dict(mp=1 << 27), dict(mp=(1 << 31) - 4095, t=1),
+               dict(budget=-1), dict(sink=-1),
                dict(recent=0), dict(stride=7), dict(ots=7), dict(mass=None), dict(table=None), dict(lens=None),
                dict(ot=None), dict(om=None), dict(ol=None), dict(ev=None), dict(ne=None)):
         assert _evict(N, **kw) == N.EINVAL, kw

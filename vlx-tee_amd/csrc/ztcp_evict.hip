@@ -8,6 +8,7 @@ namespace {
 
 constexpr int kDigitBits = 11;
 constexpr int kBins = 1 << kDigitBits;
+constexpr int kFew = 256;           // so many keys are ranked by counting
 constexpr int kKeysInLds = 16384;   // 128 KiB of keys; longer tables sum their accounts again on every pass
 
 struct EvictParams {
@@ -64,128 +65,189 @@ __device__ __forceinline__ int block_before(int of_wave, int* lds, int& total) {
     return before;
 }
 
-// One workgroup per sequence.  The page that the count-th smallest key belongs
-// to is found digit by digit from the highest bit in which the keys differ (11
-// bits at a time: a histogram of the keys that share the digits found so far,
-// then the bin in which the count runs out); pages below it go, and of the pages
-// equal to it the first ones.  Then one walk in page order closes the gaps: a
-// page moves down by the number of pages gone before it, so that a chunk that
-// has been read whole may be written over itself.
-template <int THREADS>
+__device__ __forceinline__ int pages_of(const EvictParams& p, int32_t len) {
+    const int64_t want = ((int64_t)(len < 0 ? 0 : len) + p.page_tokens - 1) / p.page_tokens;
+    return (int)(want < p.max_pages ? want : p.max_pages);
+}
+
+// One workgroup per sequence.  What goes is found by closing in: of the keys
+// from low to high, which hold the count-th smallest, the least and the greatest
+// are found (equal ones are done), their span is cut into 2048 bins, and low and
+// high become the bin's in which the count runs out; the last 256 keys are
+// ranked by counting.  Sums of 32-bit accounts seldom need more than two rounds,
+// also where a third of the pages has none.  Below low all go, and of those from
+// low to high the first ones.  Then one walk in page order closes the gaps: a
+// page moves down by the number of pages gone before it, so that a part that has
+// been read whole may be written over itself.
+//
+// It is bound by latencies: what one compute unit has in flight brings about 16
+// bytes a nanosecond.  8 sequences of 256 pages and 8 heads: 9.2 us by 256
+// threads (13.4 by 1024, whose barriers and redundant scans cost more).  128
+// sequences of up to 8,192 pages: 47.6 us, of which the keys take 16, finding
+// what goes 9, the walk 20 with two pages a thread (51 with one; four spill); as
+// three kernels, with keys and accounts moved by all compute units, 50.5.
+template <int THREADS, bool IN_LDS>
 __global__ __launch_bounds__(THREADS) void evict_kernel(EvictParams p) {
-    constexpr int kWaves = THREADS / 64, kOwn = kBins / THREADS;
+    constexpr int kWaves = THREADS / 64, kOwn = kBins / THREADS, kOwnPages = THREADS == 1024 ? 2 : 1;
     extern __shared__ uint64_t keys[];
     __shared__ int bins[kBins];
     __shared__ int scan[kWaves];
-    __shared__ uint64_t same[2][kWaves];
-    __shared__ int found[3];
+    __shared__ uint64_t ends[2][kWaves];
+    __shared__ uint64_t few[kFew];
+    __shared__ int found[3], n_few;
     const int64_t s = blockIdx.x;
     const int tid = (int)threadIdx.x, lane = tid & 63;
     const float* mass = p.mass + s * p.heads * p.max_pages;
     const int32_t* table = p.table + s * p.table_stride;
     const int32_t raw_len = p.lens[s];
-    const int32_t len = raw_len < 0 ? 0 : raw_len;
-    const int64_t want = ((int64_t)len + p.page_tokens - 1) / p.page_tokens;
-    const int n = (int)(want < p.max_pages ? want : p.max_pages);
+    const int n = pages_of(p, raw_len);
     const int first = (int)(p.sink < n ? p.sink : n);
     const int last = (int)(n - p.recent > first ? n - p.recent : first);   // candidates are first .. last - 1
     const int64_t over = (int64_t)n - p.budget;
     const int count = (int)(over < 0 ? 0 : over < last - first ? over : last - first);
-    const bool in_lds = p.max_pages <= kKeysInLds;
-    auto key_of = [&](int page) { return in_lds ? keys[page] : key_from_accounts(p, mass, page); };
+    auto key_of = [&](int page) {
+        if constexpr (IN_LDS) return keys[page];
+        else return key_from_accounts(p, mass, page);
+    };
 
-    uint64_t bound = 0;   // the count-th smallest key's digits found so far
-    int shift = 64, left = count, ties = 0;
-    if (count > 0) {
-        uint64_t all = ~0ull, any = 0;
-#pragma unroll 4
-        for (int i = first + tid; i < last; i += THREADS) {
-            const uint64_t k = key_from_accounts(p, mass, i);
-            if (in_lds) keys[i] = k;
-            all &= k, any |= k;
-        }
-        for (int m = 1; m < 64; m <<= 1) {
-            all &= (uint64_t)__shfl_xor((unsigned long long)all, m);
-            any |= (uint64_t)__shfl_xor((unsigned long long)any, m);
-        }
-        if (lane == 0) same[0][tid / 64] = all, same[1][tid / 64] = any;
-        __syncthreads();
-        for (int w = 0; w < kWaves; ++w) all &= same[0][w], any |= same[1][w];
-        shift = all == any ? 0 : 64 - __clzll((long long)(all ^ any));
-        bound = shift < 64 ? all >> shift << shift : 0;
-        ties = last - first;   // what is left of the keys if they are all equal
-        while (shift > 0) {
-            const int bits = shift < kDigitBits ? shift : kDigitBits;
-            const int next = shift - bits;
-            for (int i = tid; i < kBins; i += THREADS) bins[i] = 0;
-            __syncthreads();
+    uint64_t low = 0, high = ~0ull;   // the keys below low go, and the first `left` of those from low to high
+    int left = count, inside = last - first;
+    for (bool summed = false; left > 0; summed = true) {
+        if (summed && inside <= kFew) {   // a thread for each, which counts those below it
             for (int i = first + tid; i < last; i += THREADS) {
                 const uint64_t k = key_of(i);
-                if (shift == 64 || ((k ^ bound) >> shift) == 0)
-                    atomicAdd(&bins[(int)((k >> next) & ((1u << bits) - 1u))], 1);
+                if (k >= low && k <= high) few[atomicAdd(&n_few, 1)] = k;
             }
             __syncthreads();
-            // the bin where the count runs out
-            int of[kOwn], own = 0;
-#pragma unroll
-            for (int j = 0; j < kOwn; ++j) own += of[j] = bins[kOwn * tid + j];
-            int x = own;
-            for (int m = 1; m < 64; m <<= 1) {
-                const int y = __shfl_up(x, m);
-                x += lane >= m ? y : 0;
-            }
-            int total;
-            int before = block_before<kWaves>(__shfl(x, 63), scan, total) + x - own;
-#pragma unroll
-            for (int j = 0; j < kOwn; ++j) {
-                if (before < left && left <= before + of[j]) found[0] = kOwn * tid + j, found[1] = before, found[2] = of[j];
-                before += of[j];
+            if (tid < inside) {
+                const uint64_t mine = few[tid];
+                int less = 0, same = 0;
+#pragma unroll 8
+                for (int j = 0; j < inside; ++j) less += few[j] < mine, same += few[j] == mine;
+                if (less < left && left <= less + same) ends[0][0] = mine, found[0] = less;
             }
             __syncthreads();
-            bound |= (uint64_t)(uint32_t)found[0] << next;
-            left -= found[1];
-            ties = found[2];
-            shift = next;
-            __syncthreads();
-            if (left == ties) break;   // every key with these digits goes
+            low = high = ends[0][0];
+            left -= found[0];
+            break;
         }
+        uint64_t least = ~0ull, most = 0;
+#pragma unroll 1
+        for (int i = first + tid; i < last; i += THREADS) {
+            const uint64_t k = summed ? key_of(i) : key_from_accounts(p, mass, i);
+            if (IN_LDS && !summed) keys[i] = k;
+            if (k >= low && k <= high) least = k < least ? k : least, most = k > most ? k : most;
+        }
+        for (int m = 1; m < 64; m <<= 1) {
+            const uint64_t a = (uint64_t)__shfl_xor((unsigned long long)least, m);
+            const uint64_t b = (uint64_t)__shfl_xor((unsigned long long)most, m);
+            least = a < least ? a : least, most = b > most ? b : most;
+        }
+        if (lane == 0) ends[0][tid / 64] = least, ends[1][tid / 64] = most;
+        for (int i = tid; i < kBins; i += THREADS) bins[i] = 0;
+        if (tid == 0) n_few = 0;
+        __syncthreads();
+        low = ends[0][0], high = ends[1][0];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) {
+            low = ends[0][w] < low ? ends[0][w] : low;
+            high = ends[1][w] > high ? ends[1][w] : high;
+        }
+        if (low == high) break;
+        const int bits = 64 - __clzll((long long)(high - low)), shift = bits > kDigitBits ? bits - kDigitBits : 0;
+#pragma unroll 4
+        for (int i = first + tid; i < last; i += THREADS) {
+            const uint64_t k = key_of(i);
+            if (k >= low && k <= high) atomicAdd(&bins[(int)((k - low) >> shift)], 1);
+        }
+        __syncthreads();
+        // the bin where the count runs out
+        int of[kOwn], own = 0, total;
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) own += of[j] = bins[kOwn * tid + j];
+        int x = own;
+        for (int m = 1; m < 64; m <<= 1) {
+            const int y = __shfl_up(x, m);
+            x += lane >= m ? y : 0;
+        }
+        int before = block_before<kWaves>(__shfl(x, 63), scan, total) + x - own;
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) {
+            if (before < left && left <= before + of[j]) found[0] = kOwn * tid + j, found[1] = before, found[2] = of[j];
+            before += of[j];
+        }
+        __syncthreads();
+        low += (uint64_t)(uint32_t)found[0] << shift;
+        const uint64_t width = ((uint64_t)1 << shift) - 1;
+        if (high - low > width) high = low + width;
+        left -= found[1];
+        inside = found[2];
+        if (left == inside) break;   // all of them go
     }
     int32_t* out_table = p.out_table + s * p.out_table_stride;
     float* out_mass = p.out_mass + s * p.heads * p.max_pages;
     int32_t* evicted = p.evicted + s * p.max_pages;
-    // a page goes if its digits are below the bound's, or equal and it is among the first `left` of those
+    // a wave has kOwnPages times 64 pages in a row, so that a part of the walk needs two sums over the waves
     int ties_before = 0, gone_before = 0;
-    for (int base = 0; base < p.max_pages; base += THREADS) {
-        const int i = base + tid;
-        const bool may = count > 0 && i >= first && i < last;
-        const uint64_t k = may ? key_of(i) >> shift : ~0ull;
-        const bool below = may && k < (bound >> shift), tie = may && k == (bound >> shift);
-        const uint64_t lower = (1ull << lane) - 1ull;
-        const uint64_t tm = __ballot(tie);
-        int t_total, g_total;
-        const int t_at = ties_before + block_before<kWaves>(__popcll(tm), scan, t_total) + __popcll(tm & lower);
-        const bool gone = below || (tie && t_at < left);
-        const uint64_t gm = __ballot(gone);
-        const int g_at = gone_before + block_before<kWaves>(__popcll(gm), scan, g_total) + __popcll(gm & lower);
-        const int32_t id = i < n ? table[i] : -1;
-        const bool kept = i < n && !gone;
-        const int to = i - g_at;
-        // every wave has read its part of this chunk before any of it is written; a barrier alone does not wait for loads
-        for (int h0 = 0; h0 < p.heads; h0 += 8) {
-            float m[8];
+    const uint64_t lower = (1ull << lane) - 1ull;
+    for (int base = 0; base < p.max_pages; base += THREADS * kOwnPages) {
+        const int at = base + tid / 64 * (64 * kOwnPages) + lane;
+        int32_t id[kOwnPages];
+        uint64_t below[kOwnPages], tie[kOwnPages];
+        int of_wave = 0, total;
 #pragma unroll
-            for (int h = 0; h < 8; ++h)
-                m[h] = kept && h0 + h < p.heads ? mass[(int64_t)(h0 + h) * p.max_pages + i] : 0.f;
+        for (int j = 0; j < kOwnPages; ++j) {
+            const int i = at + j * 64;
+            id[j] = i < n ? table[i] : -1;
+            const bool may = count > 0 && i >= first && i < last;
+            const uint64_t k = may ? key_of(i) : ~0ull;
+            below[j] = __ballot(may && k < low);
+            tie[j] = __ballot(may && k >= low && k <= high);
+            of_wave += __popcll(tie[j]);
+        }
+        int rank = ties_before + block_before<kWaves>(of_wave, scan, total);
+        ties_before += total;
+        of_wave = 0;
+#pragma unroll
+        for (int j = 0; j < kOwnPages; ++j) {
+            const bool goes = (tie[j] >> lane & 1) && rank + __popcll(tie[j] & lower) < left;
+            rank += __popcll(tie[j]);
+            below[j] |= __ballot(goes);   // all that go
+            of_wave += __popcll(below[j]);
+        }
+        rank = gone_before + block_before<kWaves>(of_wave, scan, total);
+        gone_before += total;
+        int to[kOwnPages];   // where a page that stays moves, or -1 - where the id of one that goes is listed
+#pragma unroll
+        for (int j = 0; j < kOwnPages; ++j) {
+            const int g = rank + __popcll(below[j] & lower);
+            to[j] = (below[j] >> lane & 1) ? -1 - g : at + j * 64 - g;
+            rank += __popcll(below[j]);
+        }
+        // every wave has read its share of this part before any of it is written; a barrier alone does not wait for loads
+        for (int h = 0; h < p.heads; h += 8) {
+            float m[8][kOwnPages];
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+#pragma unroll
+                for (int j = 0; j < kOwnPages; ++j)
+                    m[c][j] = h + c < p.heads && at + j * 64 < n ? mass[(int64_t)(h + c) * p.max_pages + at + j * 64] : 0.f;
             __builtin_amdgcn_s_waitcnt(0);
             __syncthreads();
 #pragma unroll
-            for (int h = 0; h < 8; ++h)
-                if (kept && h0 + h < p.heads) out_mass[(int64_t)(h0 + h) * p.max_pages + to] = m[h];
+            for (int c = 0; c < 8; ++c)
+#pragma unroll
+                for (int j = 0; j < kOwnPages; ++j)
+                    if (h + c < p.heads && at + j * 64 < n && to[j] >= 0)
+                        out_mass[(int64_t)(h + c) * p.max_pages + to[j]] = m[c][j];
         }
-        if (kept) out_table[to] = id;
-        if (gone) evicted[g_at] = id;
-        ties_before += t_total;
-        gone_before += g_total;
+#pragma unroll
+        for (int j = 0; j < kOwnPages; ++j) {
+            const int i = at + j * 64;
+            if (i >= n) continue;
+            if (to[j] >= 0) out_table[to[j]] = id[j];
+            else evicted[-1 - to[j]] = id[j];
+        }
     }
     __syncthreads();
     for (int i = tid; i < p.max_pages; i += THREADS) {
@@ -211,8 +273,9 @@ extern "C" int ztcp_evict_pages(const float* mass, const int32_t* page_table, in
     arg_result(ZTCP_OK, "");
     const int64_t most = (int64_t)1 << 31;
     if (n_seqs < 0 || num_heads < 1 || max_pages < 1 || num_tokens < 1 || n_seqs >= most || num_heads >= most ||
-        max_pages >= most || num_tokens >= most || max_pages > (most - 1) / num_tokens)
-        return arg_result(ZTCP_EINVAL, "num_heads, max_pages, num_tokens must be positive, max_pages * num_tokens below 2^31");
+        max_pages > most - 4096 || num_tokens >= most || max_pages > (most - 1) / num_tokens)
+        return arg_result(ZTCP_EINVAL, "num_heads, max_pages, num_tokens must be positive, max_pages * num_tokens below 2^31, "
+                                       "max_pages at most 2^31 - 4096");
     if (budget < 0 || sink < 0 || recent < 1)
         return arg_result(ZTCP_EINVAL, "budget and sink must not be negative, recent at least 1");
     if (n_seqs == 0) return ZTCP_OK;
@@ -265,5 +328,6 @@ extern "C" int ztcp_evict_pages(const float* mass, const int32_t* page_table, in
         hipLaunchKernelGGL(kernel, dim3((uint32_t)n_seqs), dim3(threads), lds, (hipStream_t)stream, p);
         return hipGetLastError() == hipSuccess ? ZTCP_OK : ZTCP_EHIP;
     };
-    return max_pages <= 1024 ? go(evict_kernel<256>, 256u) : go(evict_kernel<1024>, 1024u);
+    if (max_pages <= 1024) return go(evict_kernel<256, true>, 256u);
+    return lds ? go(evict_kernel<1024, true>, 1024u) : go(evict_kernel<1024, false>, 1024u);
 }
