@@ -360,8 +360,8 @@ void few_kernel(AttendParams p) {
                     }
                 }
             }
+            __syncthreads();   // the sums have been read
         }
-        __syncthreads();   // the sums have been read
     }
 }
 
