@@ -420,7 +420,8 @@ ZTCP_API int ztcp_attention_mass(const void* q, int64_t q_stride, const float* l
  *   mass [n_seqs, num_heads, max_pages] fp32, table rows table_stride apart;
  *   out_table [n_seqs, max_pages], out_mass, out_lens: what is kept, gaps closed,
  *   -1 and 0 behind it (a page gone shortens the sequence by num_tokens);
- *   evicted [n_seqs, max_pages]: the ids given up, in order, -1 behind them;
+ *   evicted [n_seqs, max_pages]: the table entries given up, in order (one that was no
+ *   page of the pool among them, as it stood), -1 behind them;
  *   n_evicted [n_seqs].
  * out_table, out_mass and out_lens may be the inputs themselves. */
 ZTCP_API int ztcp_evict_pages(const float* mass, const int32_t* page_table, int64_t table_stride,

@@ -184,6 +184,8 @@ def test_python_checks(N):
         A.paged_attention(x, pages.clone().requires_grad_(), pages, i32[None], i32[:1], i32)
     with pytest.raises(ValueError, match="q must be a tensor"):
         A.paged_attention(None, pages, pages, i32[None], i32[:1], i32)
+    with pytest.raises(ValueError, match="return_lse must be true or false"):
+        A.paged_attention(x, pages, pages, i32[None], i32[:1], i32, return_lse=torch.ones(2))
     with pytest.raises(ValueError, match="even"):
         A.rope_table(4, 3, device="cpu")
     t = A.rope_table(9, 4, base=100.0, device="cpu")

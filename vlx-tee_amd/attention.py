@@ -19,8 +19,9 @@ of ``q``.
 Every call is enqueued on the current stream of its tensors' device,
 synchronizes nothing, and can be recorded into a graph.  No operator has a
 gradient (they serve, as the codec does): a tensor that requires one is
-refused outside ``torch.no_grad()``.  Wrong arguments raise ``ValueError``; indexes on the device are bounded by the kernels as
-include/ztcp.h says (ztcp_append_tokens and the entries after it).
+refused outside ``torch.no_grad()``.  Wrong arguments raise ``ValueError``;
+indexes on the device are bounded by the kernels as include/ztcp.h says
+(ztcp_append_tokens and the entries after it).
 """
 from __future__ import annotations
 
@@ -120,6 +121,9 @@ def evict_pages(mass: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Ten
     left or none may go.  ``in_place`` updates ``mass``, ``page_table`` and
     ``kv_lens`` themselves.
 
-    ``descriptors[result.evicted[s, :n]]`` are then the descriptors of those
-    pages (``pages.build_descriptors`` of the whole pool) for ``pages.egress``."""
+    Of the ids given up, ``gone = result.evicted[s, :n]``, those inside the pool
+    select their descriptors (``pages.build_descriptors`` of the whole pool) for
+    ``pages.egress``: ``descriptors[gone[gone >= 0].long()]``.  An entry that was
+    cold already (a page that is not there) has its account and its turn like
+    any other, and is listed as the table had it."""
     return Eviction._make(_call().evict_pages(mass, page_table, kv_lens, page_tokens, budget, sink, recent, in_place))

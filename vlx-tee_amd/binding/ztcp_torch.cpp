@@ -65,6 +65,15 @@ double number(PyObject* o, const char* name) {
     return x;
 }
 
+bool truth(PyObject* o, const char* name) {
+    const int x = PyObject_IsTrue(o);
+    if (x < 0) {
+        PyErr_Clear();
+        throw Refused(std::string(name) + " must be true or false");
+    }
+    return x != 0;
+}
+
 void* stream_of(const at::Device& d) { return (void*)c10::hip::getCurrentHIPStream(d.index()).stream(); }
 
 at::Tensor make(at::IntArrayRef shape, at::ScalarType type, const at::Device& d) {
@@ -168,7 +177,7 @@ PyObject* append_tokens(PyObject* const* a) {
     const c10::DeviceGuard guard(d);
     done(ztcp_append_tokens(q->data_ptr(), qs, out.data_ptr(), os, k->data_ptr(), ks, v ? v->data_ptr() : nullptr, vs, n,
                             q->size(1), &p.pool, &p.g, (const int64_t*)slot_ptr, (const int32_t*)pos_ptr,
-                            (const float*)rope_ptr, rope->size(0), w[0], wl[0], w[1], wl[1], eps, PyObject_IsTrue(a[11]),
+                            (const float*)rope_ptr, rope->size(0), w[0], wl[0], w[1], wl[1], eps, truth(a[11], "interleaved"),
                             stream_of(d)),
          "append_tokens");
     return THPVariable_Wrap(out);
@@ -182,7 +191,7 @@ PyObject* paged_attention(PyObject* const* a) {
     need(a[2] != Py_None, "paged_attention needs K and V pages (single-buffer pages have none)");
     const at::Tensor *q = tensor(a[0], "q"), *k_pages = tensor(a[1], "k_pages"), *v_pages = tensor(a[2], "v_pages");
     const at::Tensor *table = tensor(a[3], "page_table"), *lens = tensor(a[4], "kv_lens"), *starts = tensor(a[5], "q_starts");
-    const bool want_lse = PyObject_IsTrue(a[8]);
+    const bool want_lse = truth(a[8], "return_lse");
     const at::Tensor* given = tensor_or_none(a[9], "out");
     const Pool p(k_pages, v_pages, 0);
     const at::Device d = p.device();
@@ -238,7 +247,7 @@ PyObject* evict_pages(PyObject* const* a) {
     const int64_t stride = Pool::table(*table, d), s = table->size(0), mp = table->size(1), heads = mass->size(1);
     const void* mass_ptr = Pool::plain(*mass, "mass", at::kFloat, {s, heads, mp}, d);
     const void* lens_ptr = Pool::plain(*lens, "kv_lens", at::kInt, {s}, d);
-    const bool in_place = PyObject_IsTrue(a[7]);
+    const bool in_place = truth(a[7], "in_place");
     at::Tensor out[5];
     out[0] = in_place ? *table : make({s, mp}, at::kInt, d);
     out[1] = in_place ? *mass : make({s, heads, mp}, at::kFloat, d);
