@@ -338,6 +338,16 @@ def test_wrong_arrays_stay_in_bounds(A):
     torch.cuda.synchronize()
 
 
+def test_a_chunk_in_a_wide_table(A):
+    """Pieces are cut by the sequences' lengths, not by the table's width: decoding sequences, one of them longer than
+    the chunk's, beside two chunks; and the same chunk alone, whose pieces are others."""
+    _say("wide table")
+    for lens in ([(1, 40), (300, 3001), (1, 5000), (0, 7), (130, 131)], [(300, 3001)], [(40, 600), (33, 33)]):
+        b = _batch(lens, 4, 2, 128, 16, BF, seed=11, extra_cols=3000)
+        _, lse = _check_attend(A, b, lens)
+        _check_mass(A, b, lse, lens)
+
+
 @pytest.mark.parametrize("d", [64, 256])
 def test_a_hint_too_small_by_many_rows(A, d):
     """Sequences whose rows come in many turns of a kernel made for 16: each turn begins with the last one's numbers

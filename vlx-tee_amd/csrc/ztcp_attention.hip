@@ -34,18 +34,17 @@ struct AttendParams {
     float scale_log2;                // scale * log2(e): exponentials are powers of two
     int32_t few_rows;                // sequences of at most so many rows are the few kernel's, others the many kernel's
     int32_t few_groups;              // few kernel: workgroups of a KV head
-    int32_t splits, split_tokens;    // many kernel: pieces of a sequence's tokens, and tokens of a piece
+    int32_t splits, resident;        // many kernel: most pieces of a sequence's tokens; workgroups the card holds at once
     float* partial;                  // results of pieces: sums [head_dim], maximum, total
+    int32_t* cut;                    // what the many kernel's first workgroup leaves its join: pieces, tokens of a piece
 };
 
 __device__ __forceinline__ float* many_partial(const AttendParams& p, int row, int q_head, int split) {
     return p.partial + (((int64_t)row * p.kv_heads * p.group + q_head) * p.splits + split) * (p.head_dim + 2);
 }
 
-// Pieces of a sequence that have tokens (one at least: it answers for a sequence without tokens).
-__device__ __forceinline__ int live_splits(const AttendParams& p, int len) {
-    return len > 0 ? (len - 1) / p.split_tokens + 1 : 1;
-}
+// Pieces of `tokens` that a sequence has (one at least: it answers for a sequence without tokens).
+__device__ __forceinline__ int pieces_of(int len, int tokens) { return len > 0 ? (len - 1) / tokens + 1 : 1; }
 
 // What a row does not see must not reach it, but 0 * NaN is NaN: in a tile
 // whose keys some rows see and others do not, V numbers that are no finite
@@ -396,6 +395,35 @@ __device__ __forceinline__ bool find_unit(const AttendParams& p, int unit, int& 
     return true;
 }
 
+// Into how many pieces the tokens of the many kernel's sequences are cut, and how
+// long these are: as many as the card holds at once, of 512 tokens at least.  The
+// lengths are the device's, so it is decided there, alike by every wave.  Eleven
+// decoding sequences beside a chunk of 700 tokens, 5 KV heads: 68 us a call when
+// the host cut by the most blocks and tokens that there could be, 56 now.
+struct Cut {
+    int n, tokens;
+};
+__device__ __forceinline__ Cut cut_of(const AttendParams& p) {
+    if (p.splits == 1) return Cut{1, p.batch.max_tokens};
+    const int lane = (int)threadIdx.x & 63;
+    int units = 0, longest = 1;
+    for (int base = 0; base < p.batch.n_seqs; base += 64) {
+        if (base + lane >= p.batch.n_seqs) continue;
+        const Seq q = seq_of(p.batch, base + lane);
+        const int rows = q.n_new * p.group;
+        if (rows <= p.few_rows) continue;
+        units += (rows + kManyRows - 1) / kManyRows;
+        longest = max(longest, q.len);
+    }
+    for (int m = 1; m < 64 && m < p.batch.n_seqs; m <<= 1) {  // (lane 0's are used)
+        units += __shfl_xor(units, m);
+        longest = max(longest, __shfl_xor(longest, m));
+    }
+    longest = uniform(longest);
+    const int n = max(1, min(min(p.splits, (longest + 511) / 512), p.resident / max(1, uniform(units) * p.kv_heads)));
+    return Cut{n, ((longest + n - 1) / n + 127) / 128 * 128};
+}
+
 // Zeros that the tile loads read in the place of tokens that are not there: a row of 256 elements.
 __device__ __attribute__((aligned(16))) uint32_t g_zeros[128];
 
@@ -415,15 +443,17 @@ void many_kernel(AttendParams p) {
     const int col = lane & 31, half = lane >> 5;
     const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads);
     const uint32_t rest = blockIdx.x / (uint32_t)p.kv_heads;
-    const int split = (int)(rest % (uint32_t)p.splits);
+    const Cut cut = cut_of(p);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && p.splits > 1) p.cut[0] = cut.n, p.cut[1] = cut.tokens;
+    const int split = (int)(rest % (uint32_t)cut.n);
     int s, block;
-    if (!find_unit(p, (int)(rest / (uint32_t)p.splits), s, block)) return;
+    if (!find_unit(p, (int)(rest / (uint32_t)cut.n), s, block)) return;
     s = uniform(s);
     block = uniform(block);
     const Seq seq = uniform(seq_of(p.batch, s));
     const int rows = seq.n_new * p.group;
-    if (split >= live_splits(p, seq.len)) return;
-    const int key0 = split * p.split_tokens, key1 = key0 + min(seq.len - key0, p.split_tokens);
+    if (split >= pieces_of(seq.len, cut.tokens)) return;
+    const int key0 = split * cut.tokens, key1 = key0 + min(seq.len - key0, cut.tokens);
     const int r0 = block * kManyRows + wave * 32, r = r0 + col;
     const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
     const int limit = r < rows ? max(0, seq.len - seq.n_new + token + 1) : 0;
@@ -697,7 +727,7 @@ void many_kernel(AttendParams p) {
     if (r >= rows) return;
     const int64_t row_head = (int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head;
     const float base = m == -INFINITY ? 0.f : m;
-    if (p.splits > 1) {
+    if (cut.n > 1) {
         float* dst = many_partial(p, seq.row0 + token, q_head, split);
 #pragma unroll
         for (int n = 0; n < DP / 32; ++n)
@@ -788,10 +818,11 @@ __global__ __launch_bounds__(256) void join_many_kernel(AttendParams p) {
     const int wave = (int)threadIdx.x >> 6;
     const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads);
     const uint32_t rest = blockIdx.x / (uint32_t)p.kv_heads;
+    const Cut cut{p.cut[0], p.cut[1]};
     int s, block;
-    if (!find_unit(p, (int)(rest / (kManyRows / kJoinRows)), s, block)) return;
+    if (cut.n == 1 || !find_unit(p, (int)(rest / (kManyRows / kJoinRows)), s, block)) return;
     const Seq seq = seq_of(p.batch, s);
-    const int rows = seq.n_new * p.group, n = live_splits(p, seq.len);
+    const int rows = seq.n_new * p.group, n = pieces_of(seq.len, cut.tokens);
     const int r0 = block * kManyRows + (int)(rest % (kManyRows / kJoinRows)) * kJoinRows;
     for (int r = r0 + wave; r < min(rows, r0 + kJoinRows); r += 4) {
         const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
@@ -802,6 +833,8 @@ __global__ __launch_bounds__(256) void join_many_kernel(AttendParams p) {
 
 // ---- host -------------------------------------------------------------------------
 
+constexpr int64_t kCutFloats = 4;   // in front of the many kernel's pieces
+
 // How a call is cut: what the few and the many kernel take, and into how many pieces.
 struct Plan {
     int nt;                         // 16-row tiles of the few kernel, 0: no few kernel
@@ -809,7 +842,8 @@ struct Plan {
     int few_groups;                 // its workgroups of a KV head
     bool many;
     int64_t many_units;             // blocks of kManyRows rows at most
-    int splits, split_tokens;       // of the many kernel
+    int splits, resident;           // of the many kernel
+    int64_t many_groups;            // its workgroups
     int64_t workspace;              // floats
 };
 
@@ -838,17 +872,18 @@ Plan plan_call(const ztcp_paged_batch* b, const ztcp_geometry* g, int64_t q_head
         if (plan.few_groups > 1) plan.workspace = (plan.few_groups + b->n_seqs) * heads * 16 * plan.nt * piece;
     }
     plan.splits = 1;
-    plan.split_tokens = (int)max_tokens;
+    plan.resident = cus * (g->head_dim <= 128 ? 2 : 1);
     if (plan.many) {
-        const int64_t groups = plan.many_units * heads, most = (max_tokens + 511) / 512;
-        int64_t n = ((int64_t)cus * 2 + groups - 1) / groups;
+        // blocks there are at least if all rows are chunks', and pieces of 512 tokens at least
+        const int64_t blocks = (b->n_rows * group + kManyRows - 1) / kManyRows * heads, most = (max_tokens + 511) / 512;
+        int64_t n = plan.resident / blocks;
         n = n < most ? n : most;
         n = n < 64 ? n : 64;
-        if (n > 1) {
-            plan.split_tokens = (int)(((max_tokens + n - 1) / n + 127) / 128 * 128);
-            plan.splits = (int)((max_tokens + plan.split_tokens - 1) / plan.split_tokens);
-        }
-        const int64_t need = plan.splits > 1 ? b->n_rows * q_heads * plan.splits * piece : 0;
+        plan.splits = (int)(n > 1 ? n : 1);
+        plan.many_groups = plan.many_units * heads;
+        const int64_t pieces = (plan.resident + heads - 1) / heads * heads;
+        if (plan.splits > 1 && plan.many_groups < pieces) plan.many_groups = pieces;
+        const int64_t need = plan.splits > 1 ? b->n_rows * q_heads * plan.splits * piece + kCutFloats : 0;
         plan.workspace = need > plan.workspace ? need : plan.workspace;
     }
     return plan;
@@ -861,7 +896,7 @@ void launch(const AttendParams& base, const Plan& plan, float* workspace, hipStr
     p.few_rows = plan.few_rows;
     p.few_groups = plan.few_groups;
     p.splits = plan.splits;
-    p.split_tokens = plan.split_tokens;
+    p.resident = plan.resident;
     const uint32_t heads = (uint32_t)p.kv_heads;
     if (plan.nt) {
         const dim3 grid(heads * (uint32_t)plan.few_groups);
@@ -873,8 +908,12 @@ void launch(const AttendParams& base, const Plan& plan, float* workspace, hipStr
             hipLaunchKernelGGL(join_few_kernel<DT>, dim3(heads * (uint32_t)p.batch.n_seqs), dim3(256), 0, stream, p, 16 * plan.nt);
     }
     if (plan.many) {
+        if (plan.splits > 1) {
+            p.cut = (int32_t*)workspace;
+            p.partial = workspace + kCutFloats;
+        }
         const uint32_t units = (uint32_t)plan.many_units * heads;
-        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(units * (uint32_t)p.splits), dim3(256), 0, stream, p); };
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((uint32_t)plan.many_groups), dim3(256), 0, stream, p); };
         if (p.batch.page_tokens % (many_tile(DP) / 4) == 0 && p.head_dim == DP) go(many_kernel<DT, DP, true>);
         else go(many_kernel<DT, DP, false>);
         if (p.splits > 1) hipLaunchKernelGGL(join_many_kernel<DT>, dim3(units * (kManyRows / kJoinRows)), dim3(256), 0, stream, p);
@@ -935,7 +974,7 @@ extern "C" int ztcp_paged_attention(const void* q, int64_t q_stride, void* out, 
         bytes_overlap(workspace, need, lse, lse_bytes))
         return arg_result(ZTCP_EOVERLAP, "out, lse and workspace must not overlap q, the pages or each other");
     const int64_t most = (int64_t)1 << 31, tiles = batch->n_seqs * (p.batch.max_tokens / kFewTile + 1);
-    if (g->num_heads * plan.many_units * (plan.splits > 16 ? plan.splits : 16) >= most ||
+    if (g->num_heads * plan.many_units * (kManyRows / kJoinRows) >= most ||
         g->num_heads * batch->n_seqs >= most || tiles >= most)
         return arg_result(ZTCP_EINVAL, "too many sequences and heads in one call");
     p.q = (const uint8_t*)q;
