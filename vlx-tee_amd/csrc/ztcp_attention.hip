@@ -87,16 +87,18 @@ __device__ __forceinline__ f32x4 only_not_finite(const AttendParams& p, const Pl
 // head takes an equal number of tiles, so that all end together whatever the
 // sequences' lengths are; where it ends inside a sequence it leaves a partial
 // result.  Of a tile each of its four waves takes 32 keys, with its loads of
-// the next tile in flight while it works on this one: K as the products want
-// it (lane = key, 16 bytes of its row), V by whole rows, through 32 rows of LDS
-// of the wave's own that the transposing reads take.  Waves join their maxima,
-// totals and sums at the end of a sequence.
+// the next tile in flight while it works on this one: K and V by whole rows,
+// through LDS of the wave's own to the products (K of vectors of more than 128
+// elements, for which there is no room, as the products want it: lane = key,
+// 16 bytes of its row).  Waves join their maxima, totals and sums at the end of a
+// sequence.
 //
 // 64 sequences of 500 to 16,384 tokens, 4 query heads to each of 8 KV heads of
-// 128, pages of 16 (1.16 GB): 231 to 238 us, 5.0 TB/s where a kernel that only
-// reads has 6.35; cut by sequence instead of in equal shares 281 us.  What is
-// left is what the loads in flight bring, a tile of K and V for each of two
-// workgroups on a compute unit: the registers they wait in allow no third.
+// 128, pages of 16 (1.16 GB): 202 us, 5.7 TB/s where a kernel that only reads has
+// 6.35.  Loads of whole rows that leave no trace in the caches made it that: with
+// K in 64-byte parts of rows and ordinary loads it took 237 (V's alone without
+// trace: 222; K's parts too: 234, each line fetched twice), and cut by sequence
+// instead of in equal shares 281.
 
 constexpr int kFewTile = 128;
 
@@ -121,7 +123,9 @@ void few_kernel(AttendParams p) {
     constexpr int kVRows = 64 / kChunks;                      // rows a load covers
     constexpr int kJoinRow = DP + 4;
     constexpr int kWaveBytes = 32 * DP * 2;
-    constexpr int kBytes = 4 * kWaveBytes > 4 * 16 * kJoinRow * 4 ? 4 * kWaveBytes : 4 * 16 * kJoinRow * 4;
+    constexpr bool kKInLds = DP <= 128;
+    constexpr int kVBytes = 4 * kWaveBytes > 4 * 16 * kJoinRow * 4 ? 4 * kWaveBytes : 4 * 16 * kJoinRow * 4;
+    constexpr int kBytes = kVBytes + (kKInLds ? 4 * kWaveBytes : 0);
     constexpr int kMostRows = 16 * NT;
     __shared__ __attribute__((aligned(16))) uint8_t lds[kBytes];
     __shared__ float join_m[4][16], join_l[4][16];
@@ -138,6 +142,8 @@ void few_kernel(AttendParams p) {
     int s = uniform(find_tile(p.batch, tile, tiles_of));
     tile = uniform(tile);
     uint8_t* vt = lds + wave * kWaveBytes;
+    uint8_t* kt = lds + kVBytes + wave * kWaveBytes;
+    auto k_swizzle = [](int row, int chunk) { return chunk ^ (row & (kChunks < 16 ? kChunks - 1 : 15)); };
     // 16-byte pieces of V rows are permuted within the row so that the rows a
     // transposing read takes lie in different banks
     auto swizzle = [](int row, int chunk) {
@@ -181,7 +187,7 @@ void few_kernel(AttendParams p) {
 #pragma unroll
                 for (int i = 0; i < DP / 16; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
-            uint4 kf[2][kSteps], vf[kVLoads];
+            uint4 kf[2][kSteps], vf[kVLoads];                     // (K in LDS: loads by whole rows as V's, in order)
             Place at;                                             // of key (lane % 32) of the tile to be loaded
             uint32_t valid = 0, v_valid = 0;                      // keys of the loaded tile that are there; this lane's V rows of them
             auto load = [&](const Place& at) {
@@ -189,23 +195,29 @@ void few_kernel(AttendParams p) {
                 valid = (uint32_t)__ballot(has);
                 const int page = has ? at.page : 0, row = has ? at.row : 0;
                 v_valid = 0;
+                if constexpr (!kKInLds) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int from = 16 * t + col;
-                    const int64_t pg = __shfl(page, from), rw = __shfl(row, from);
-                    const uint8_t* src = p.k_pool + 2 * (pg * p.k_page + (rw * p.kv_heads + head) * p.head_dim);
+                    for (int t = 0; t < 2; ++t) {
+                        const int from = 16 * t + col;
+                        const int64_t pg = __shfl(page, from), rw = __shfl(row, from);
+                        const uint8_t* src = p.k_pool + 2 * (pg * p.k_page + (rw * p.kv_heads + head) * p.head_dim);
 #pragma unroll
-                    for (int i = 0; i < kSteps; ++i) {
-                        const int d = 32 * i + 8 * quad;
-                        kf[t][i] = d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
+                        for (int i = 0; i < kSteps; ++i) {
+                            const int d = 32 * i + 8 * quad;
+                            kf[t][i] = d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
+                        }
                     }
                 }
 #pragma unroll
                 for (int i = 0; i < kVLoads; ++i) {
                     const int from = i * kVRows + v_row;
                     const int64_t pg = __shfl(page, from), rw = __shfl(row, from);
-                    const uint8_t* src = p.v_pool + 2 * (pg * p.v_page + (rw * p.kv_heads + head) * p.head_dim);
-                    vf[i] = v_has ? ldg16(src + 16 * v_chunk) : make_uint4(0, 0, 0, 0);
+                    const int64_t in_page = (rw * p.kv_heads + head) * p.head_dim;
+                    if constexpr (kKInLds)
+                        kf[i / kSteps][i % kSteps] = v_has ? ldg16_once(p.k_pool + 2 * (pg * p.k_page + in_page) + 16 * v_chunk)
+                                                           : make_uint4(0, 0, 0, 0);
+                    const uint8_t* src = p.v_pool + 2 * (pg * p.v_page + in_page);
+                    vf[i] = v_has ? ldg16_once(src + 16 * v_chunk) : make_uint4(0, 0, 0, 0);
                     v_valid |= ((valid >> from) & 1u) << i;
                 }
             };
@@ -218,6 +230,18 @@ void few_kernel(AttendParams p) {
             }
             for (; kb < stop; kb += 128) {
                 const uint32_t here = valid;
+                if constexpr (kKInLds) {
+#pragma unroll
+                    for (int i = 0; i < kVLoads; ++i) {
+                        const int row = i * kVRows + v_row;
+                        *reinterpret_cast<uint4*>(kt + row * DP * 2 + k_swizzle(row, v_chunk) * 16) = kf[i / kSteps][i % kSteps];
+                    }
+                }
+                auto k_part = [&](int u, int i) {
+                    if constexpr (kKInLds)
+                        return *reinterpret_cast<const uint4*>(kt + (16 * u + col) * DP * 2 + k_swizzle(col, 4 * i + quad) * 16);
+                    else return kf[u][i];
+                };
                 f32x4 sc[NT][2];
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
@@ -225,7 +249,7 @@ void few_kernel(AttendParams p) {
                     for (int u = 0; u < 2; ++u) {
                         sc[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int i = 0; i < kSteps; ++i) sc[t][u] = mfma16<DT>(kf[u][i], qf[t][i], sc[t][u]);
+                        for (int i = 0; i < kSteps; ++i) sc[t][u] = mfma16<DT>(k_part(u, i), qf[t][i], sc[t][u]);
                     }
                 if (kb + 32 > first_sees && first_sees < stop) {
 #pragma unroll
