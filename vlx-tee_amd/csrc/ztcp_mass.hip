@@ -75,13 +75,20 @@ __device__ __forceinline__ void rest_of(const MassParams& p, int s, int head) {
 // this one.  The rows stay in registers for a whole sequence.
 //
 // 64 sequences of 500 to 16,384 tokens, 8 KV heads of 128, pages of 16 (583 MB):
-// 127 to 133 us, 4.5 TB/s where a kernel that only reads has 6.35; cut by
-// sequence 198.  Bound by the loads in flight, as the attention beside it.
+// 120 us, 4.9 TB/s where a kernel that only reads has 6.35.  K comes by whole
+// rows with loads that leave no trace in the caches, and through LDS of the
+// wave's own to the products; taken as the products want it, 64 bytes of a row
+// a load, 133, and cut by sequence 198.  Bound by the loads in flight.
+
+// Waves of a SIMD, and so workgroups of a compute unit, that the registers allow without scratch memory.
+constexpr int few_waves(int dp, int nt) { return dp <= 128 && nt == 1 ? 3 : dp <= 128 || nt == 1 ? 2 : 1; }
 
 template <int DT, int DP, int NT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 128 && NT == 1 ? 3 : 2)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves(DP, NT))))
 void mass_few_kernel(MassParams p) {
-    constexpr int kSteps = DP / 32;
+    constexpr int kSteps = DP / 32, kChunks = DP / 8, kRowBytes = DP * 2;
+    constexpr int kLoads = 2 * kSteps, kLoadRows = 64 / kChunks;   // of a wave for its 32 keys; rows of a load
+    __shared__ __attribute__((aligned(16))) uint8_t tiles[4][32 * kRowBytes];
     __shared__ float key_sum[2][kFewKeys];
     const int lane = (int)threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, quad = lane >> 4;
@@ -98,6 +105,10 @@ void mass_few_kernel(MassParams p) {
     int s = uniform(find_tile(p.batch, tile, tiles_of));
     tile = uniform(tile);
     const int tile_keys = p.group_pages * p.batch.page_tokens;
+    // 16-byte pieces are permuted within a row so that the rows of one read lie in different banks
+    uint8_t* kt = tiles[wave];
+    const int load_row = lane / kChunks, load_chunk = lane % kChunks;
+    auto swizzle = [](int row, int chunk) { return chunk ^ (row & (kChunks < 16 ? kChunks - 1 : 15)); };
     for (; left > 0 && s < p.batch.n_seqs; ++s, tile = 0) {
         const Seq seq = uniform(seq_of(p.batch, s));
         const int rows = seq.n_new * p.group, n_tiles = tiles_of(seq);
@@ -124,7 +135,7 @@ void mass_few_kernel(MassParams p) {
             }
         };
         load_q(0);
-        uint4 kf[2][kSteps];
+        uint4 kf[kLoads];
         uint32_t valid = 0;
         int entry = -1;                                       // of key lane % 32 of the wave's share of the block to be loaded
         auto look_up = [&](int kb) {
@@ -139,13 +150,9 @@ void mass_few_kernel(MassParams p) {
             const uint64_t mine =
                 (uint64_t)(p.k_pool + (has ? 2 * (entry * p.k_page + (int64_t)(row * p.kv_heads + head) * p.head_dim) : 0));
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint8_t* src = (const uint8_t*)__shfl(mine, 16 * u + col);
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
-                    const int d = 32 * i + 8 * quad;
-                    kf[u][i] = d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
-                }
+            for (int i = 0; i < kLoads; ++i) {
+                const uint8_t* src = (const uint8_t*)__shfl(mine, i * kLoadRows + load_row);
+                kf[i] = load_chunk * 8 < p.head_dim ? ldg16_once(src + 16 * load_chunk) : make_uint4(0, 0, 0, 0);
             }
         };
         // blocks of a tile: one, or several of a page of more than kFewKeys tokens
@@ -159,14 +166,26 @@ void mass_few_kernel(MassParams p) {
             const uint32_t here = valid;
             const int next = next_block(kb, key0), most = min(kb + kFewKeys, min(next, key_end)) - (kb + 32 * wave);
             float x[8] = {};
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int row = i * kLoadRows + load_row;
+                *reinterpret_cast<uint4*>(kt + row * kRowBytes + swizzle(row, load_chunk) * 16) = kf[i];
+            }
+            if (next < key_end) {
+                load(next);
+                entry = look_up(next_block(next, next < key0 + tile_keys ? key0 : next));
+            }
             auto weigh = [&]() {
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+                        __builtin_amdgcn_sched_barrier(0);    // no more of K in registers at once
 #pragma unroll
-                        for (int i = 0; i < kSteps; ++i) sc = mfma16<DT>(kf[u][i], qf[t][i], sc);
+                        for (int i = 0; i < kSteps; ++i)
+                            sc = mfma16<DT>(*reinterpret_cast<const uint4*>(kt + (16 * u + col) * kRowBytes +
+                                                                            swizzle(col, 4 * i + quad) * 16), qf[t][i], sc);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], p.scale_log2, -base[t]));
@@ -181,10 +200,6 @@ void mass_few_kernel(MassParams p) {
                     weigh();
                 }
                 load_q(0);
-            }
-            if (next < key_end) {
-                load(next);
-                entry = look_up(next_block(next, next < key0 + tile_keys ? key0 : next));
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -440,7 +455,7 @@ void launch(MassParams p, int64_t most_rows, int cus, hipStream_t stream) {
     const bool many = most_rows > 32 || nt == 0;
     p.few_rows = many ? 16 * nt : 0x7FFFFFFF;
     if (nt) {
-        const int64_t resident = ((int64_t)cus * (DP <= 128 && nt == 1 ? 3 : 2) + heads - 1) / heads;
+        const int64_t resident = ((int64_t)cus * few_waves(DP, nt) + heads - 1) / heads;
         const int64_t tiles = p.batch.n_seqs * tiles_of(kFewKeys);
         p.few_groups = (int32_t)(resident < tiles ? resident : tiles);
         const dim3 grid((uint32_t)(p.few_groups * heads));
