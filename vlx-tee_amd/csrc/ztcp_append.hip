@@ -57,8 +57,9 @@ __device__ __forceinline__ uint4 pack_chunk(const Chunk& c) {
 // reads and writes every element once and is bound by that: the angles and weights are loaded once for a wave's
 // vectors, the next turns' loads are in flight during a turn, the sum of squares is a butterfly over the group, and
 // the partner of a rotated pair sits rope_dim / 16 lanes away (or in the same lane when interleaved), so a vector
-// never leaves registers.  Prompt of 16,384 tokens of 32 + 8 + 8 vectors of 128 (407 MB): 95 to 100 us, 4.1 to 4.3 TB/s
-// where a large copy has 5.0; a wave for every four vectors, with angles and weights of its own, took 147 us.
+// never leaves registers.  Prompt of 16,384 tokens of 32 + 8 + 8 vectors of 128 (407 MB): 88 us, 4.6 TB/s where a
+// large copy has 5.0; with loads that leave a trace in the caches 99 us, and a wave for every four vectors, with
+// angles and weights of its own, 147 us.
 template <int DT, int LANES, int CHUNKS, int AHEAD>
 __global__ __launch_bounds__(256) void append_kernel(AppendParams p) {
     constexpr int kTurn = 64 / LANES;                         // vectors of a turn
@@ -184,7 +185,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendParams p) {
 #pragma unroll
             for (int j = 0; j < CHUNKS; ++j) {
                 const int at = lane + j * LANES;
-                c[i][j] = h < end && at < n_chunks ? ldg16(src + 16 * at) : make_uint4(0, 0, 0, 0);
+                c[i][j] = h < end && at < n_chunks ? ldg16_once(src + 16 * at) : make_uint4(0, 0, 0, 0);
             }
         }
     }
