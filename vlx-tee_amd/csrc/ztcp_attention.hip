@@ -94,7 +94,7 @@ __device__ __forceinline__ f32x4 only_not_finite(const AttendParams& p, const Pl
 // sequence.
 //
 // 64 sequences of 500 to 16,384 tokens, 4 query heads to each of 8 KV heads of
-// 128, pages of 16 (1.16 GB): 202 us, 5.7 TB/s where a kernel that only reads has
+// 128, pages of 16 (1.16 GB): 198 to 203 us, 5.8 TB/s where a kernel that only reads has
 // 6.35.  Loads of whole rows that leave no trace in the caches made it that: with
 // K in 64-byte parts of rows and ordinary loads it took 237 (V's alone without
 // trace: 222; K's parts too: 234, each line fetched twice), and cut by sequence

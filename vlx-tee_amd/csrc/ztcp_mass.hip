@@ -75,7 +75,7 @@ __device__ __forceinline__ void rest_of(const MassParams& p, int s, int head) {
 // this one.  The rows stay in registers for a whole sequence.
 //
 // 64 sequences of 500 to 16,384 tokens, 8 KV heads of 128, pages of 16 (583 MB):
-// 120 us, 4.9 TB/s where a kernel that only reads has 6.35.  K comes by whole
+// 114 to 120 us, 5.0 TB/s where a kernel that only reads has 6.35.  K comes by whole
 // rows with loads that leave no trace in the caches, and through LDS of the
 // wave's own to the products; taken as the products want it, 64 bytes of a row
 // a load, 133, and cut by sequence 198.  Bound by the loads in flight.
