@@ -30,13 +30,13 @@ struct MassParams {
     float scale_log2, decay;
 };
 
+// (a page may have so many tokens that a length and a page's tokens together pass 2^31)
 __device__ __forceinline__ int mass_tiles(const MassParams& p, const Seq& q) {
-    const int keys = p.group_pages * p.batch.page_tokens;
-    return (q.len + keys - 1) / keys;
+    return q.len > 0 ? (q.len - 1) / (p.group_pages * p.batch.page_tokens) + 1 : 0;
 }
 
 __device__ __forceinline__ int pages_of(const MassParams& p, const Seq& q) {
-    return (q.len + p.batch.page_tokens - 1) / p.batch.page_tokens;
+    return q.len > 0 ? (q.len - 1) / p.batch.page_tokens + 1 : 0;
 }
 
 // A tile of pages is summed key by key into LDS, in blocks of KEYS keys (kb) from its first (key0) on: thread i adds up
