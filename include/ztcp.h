@@ -353,7 +353,7 @@ typedef struct ztcp_paged_batch {
     const int32_t* kv_lens;      /* [n_seqs], the new tokens among them */
     const int32_t* q_starts;     /* [n_seqs + 1], ascending */
     int64_t n_seqs;
-    int64_t n_rows;              /* rows of q */
+    int64_t n_rows;              /* rows of q; times q_heads at most 2^31 - 1024 */
     int64_t max_q_len;           /* most new tokens of a sequence; 0 = not known.  A
                                     hint: too small a value costs time only */
 } ztcp_paged_batch;

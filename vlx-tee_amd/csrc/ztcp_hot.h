@@ -108,7 +108,8 @@ inline const char* check_batch(const ztcp_paged_batch* b, const ztcp_page_pool* 
         return "q_heads must be a positive multiple of num_heads, at most 65536";
     if (b->max_pages < 1 || b->max_pages > (most - 1024) / g->num_tokens)
         return "max_pages must be positive, max_pages * num_tokens below 2^31 - 1024";
-    if (b->n_rows * q_heads >= most) return "too many query heads in one call (n_rows * q_heads must be below 2^31)";
+    if (b->n_rows * q_heads > most - 1024)   // blocks of up to 128 rows are counted beyond the last one
+        return "too many query heads in one call (n_rows * q_heads must be at most 2^31 - 1024)";
     if (b->n_seqs > 0 && (!b->page_table || !b->kv_lens || !b->q_starts))
         return "page_table, kv_lens and q_starts must not be NULL";
     if (b->n_seqs > 1 && b->table_stride < b->max_pages) return "table_stride must cover max_pages";
