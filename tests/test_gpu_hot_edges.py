@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import hot_reference as R
-from test_gpu_hot_ops import A, BF, _close, _say  # noqa: F401  (A: the module's fixture)
+from test_gpu_hot_ops import A, BF, FP, _batch, _check_attend, _close, _say  # noqa: F401  (A: the module's fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,37 @@ def test_accounts_of_a_length_a_page_short_of_2_31(A, new):
     _close(torch.stack([out[0, :, -1:], out[1, :, :1]]), want, tol, new)
     assert torch.equal(out[0, :, :-1], 0.5 * mass[0, :, :-1]) and torch.equal(out[1, :, 1:], 0.5 * mass[1, :, 1:])
     assert bool((guard[:mass.numel()] == 7).all())
+
+
+def _spoil(b, bad, t, tile):
+    """``bad`` in V's last head at tokens around the first new one of every sequence of several, each in a column of its
+    own: new tokens, the ones before them in the same tile of ``tile`` keys, others, and one beside a cold page."""
+    new = (b["starts"][1:] - b["starts"][:-1]).tolist()
+    for s, length in enumerate(b["lens"].tolist()):
+        if new[s] == 0:
+            continue
+        sees = length - new[s] + 1                             # tokens that the first row sees
+        tiles = [sees // w * w for w in (tile, 32, 64)]
+        at = [sees - 1, sees, length - 1, length - 2, sees - 2, sees - 7, 0, 5, *tiles, *(x - 1 for x in tiles),
+              *(x + 3 for x in tiles), length // 2]
+        if length > 200:
+            b["table"][s, 16 // t] = -1                        # the pages of tokens 16 to 31 are cold
+        for c, token in enumerate(dict.fromkeys(at)):
+            page = int(b["table"][s, token // t]) if 0 <= token < length else -1
+            if page >= 0:
+                b["vp"][page, token % t, -1, c] = bad
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("lens", [[(3, 40)], [(2, 33), (1, 70), (4, 300)], [(150, 150)], [(150, 333), (1, 64)], [(5, 5001)],
+                                  [(150, 3500)]])
+def test_numbers_that_rows_see_reach_them(A, lens, d, bad):
+    """An infinity or a NaN in V reaches every row that sees its token, wherever in a tile the token is, and no other row,
+    column or head: sequences of few and of many rows, whole and in pieces, with cold pages."""
+    _say("seen", lens, d, bad)
+    for dtype, t, group in ((BF, 16, 2), (FP, 8, 3)):
+        b = _batch(lens, group, 2, d, t, dtype, seed=d)
+        _spoil(b, bad, t, 64 if d <= 128 else 32)
+        for hint in (True, False):
+            _check_attend(A, b, (lens, d, bad, dtype, hint), hint)

@@ -46,10 +46,12 @@ __device__ __forceinline__ float* many_partial(const AttendParams& p, int row, i
 // Pieces of `tokens` that a sequence has (one at least: it answers for a sequence without tokens).
 __device__ __forceinline__ int pieces_of(int len, int tokens) { return len > 0 ? (len - 1) / tokens + 1 : 1; }
 
-// What a row does not see must not reach it, but 0 * NaN is NaN: in a tile
-// whose keys some rows see and others do not, V numbers that are no finite
-// numbers leave the product (set to 0) and are added afterwards to the rows
-// that see them.  An infinity or a NaN needs no weight for that.
+// What a row does not see must not reach it, but 0 * NaN is NaN: of the keys
+// that some rows of a workgroup see and others do not, those from `first_sees`
+// on, V numbers that are no finite numbers leave the product (set to 0) and are
+// added afterwards to the rows that see them.  An infinity or a NaN needs no
+// weight for that.  Keys in front of first_sees every row sees: they stay in
+// the product.
 template <int DT>
 __device__ __forceinline__ bool not_finite16(uint32_t h) {
     constexpr uint32_t e = DT == kHotBf16 ? 0x7F80u : 0x7C00u;
@@ -253,7 +255,8 @@ void few_kernel(AttendParams p) {
                     }
                 if (kb + 32 > first_sees && first_sees < stop) {
 #pragma unroll
-                    for (int i = 0; i < kVLoads; ++i) apart |= drop_not_finite<DT>(vf[i]);
+                    for (int i = 0; i < kVLoads; ++i)
+                        if (kb + i * kVRows + v_row >= first_sees) apart |= drop_not_finite<DT>(vf[i]);
                 }
 #pragma unroll
                 for (int i = 0; i < kVLoads; ++i) {
@@ -623,7 +626,7 @@ void many_kernel(AttendParams p) {
             uint4* piece = reinterpret_cast<uint4*>(tiles[v_buffer][1]) + i;
             uint4 x = *piece;
             if (!((there >> (i / kChunks)) & 1u)) *piece = make_uint4(0, 0, 0, 0);
-            else if (first_sees < stop && drop_not_finite<DT>(x)) {
+            else if (kb + i / kChunks >= first_sees && drop_not_finite<DT>(x)) {
                 *piece = x;
                 dropped = true;
             }
