@@ -73,3 +73,79 @@ def test_numbers_that_rows_see_reach_them(A, lens, d, bad):
         _spoil(b, bad, t, 64 if d <= 128 else 32)
         for hint in (True, False):
             _check_attend(A, b, (lens, d, bad, dtype, hint), hint)
+
+
+# A launch has fewer than 2^32 threads, 2^24 workgroups of 256: calls of more.
+
+def test_an_append_of_more_tokens_than_a_launch_has_threads_for(A):
+    _say("append of 2^26 tokens")
+    n, d = 2 ** 26 + 5, 16
+    k = torch.arange(n, dtype=torch.int32, device="cuda").view(n, 1, 1).repeat(1, 1, 8).view(BF).view(n, 1, d)
+    pages = torch.zeros((n, 1, 1, d), dtype=BF, device="cuda")
+    empty = torch.zeros((n, 0, d), dtype=BF, device="cuda")
+    slots = torch.arange(n - 1, -1, -1, device="cuda")
+    A.append_tokens(empty, k, None, pages, None, slots, torch.zeros(n, dtype=torch.int32, device="cuda"), A.rope_table(1, 0))
+    # numbers pass through fp32, which turns a NaN whose first mantissa bit is 0 into one where it is 1; all else is exact
+    got, want = pages[:, 0], k.flip(0)
+    nan = torch.isnan(want)
+    assert torch.equal(torch.isnan(got), nan)
+    assert bool(((got.view(torch.int16) == want.view(torch.int16)) | nan).all())
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_of_more_sequences_and_heads_than_a_launch_has(A, new):
+    """The joins of the pieces: workgroups for every sequence and head (few rows), and for eight rows of these (many).
+    All sequences but three have no new tokens, among them the last one, which is in pieces."""
+    _say("joins of 2^24 workgroups", new)
+    heads, t, d, seqs = 256, 16, 16, 65537 if new == 1 else 4097
+    gen = torch.Generator(device="cuda").manual_seed(new)
+    mp, some = 64, [3, seqs // 2, seqs - 1]
+    kp = torch.randn((3 * mp, t, heads, d), generator=gen, device="cuda").to(BF)
+    vp = torch.randn((3 * mp, t, heads, d), generator=gen, device="cuda").to(BF)
+    table = torch.full((seqs, mp), -1, dtype=torch.int32, device="cuda")
+    table[some] = torch.randperm(3 * mp, generator=gen, device="cuda").int().view(3, mp)
+    lens, count = torch.zeros(seqs, dtype=torch.int32, device="cuda"), torch.zeros(seqs, dtype=torch.int32, device="cuda")
+    lens[some] = torch.tensor([60, 700, mp * t - 5], dtype=torch.int32, device="cuda")
+    count[some] = torch.tensor([1, 1, new], dtype=torch.int32, device="cuda")
+    starts = torch.cat([count.new_zeros(1), count.cumsum(0).int()])
+    q = torch.randn((2 + new, heads, d), generator=gen, device="cuda").to(BF)
+    out, lse = A.paged_attention(q, kp, vp, table, lens, starts, max_q_len=new, return_lse=True)
+    few = torch.cat([starts[[s]] for s in some] + [starts[-1:]])
+    want, wl, tol, ltol = R.attention(q, kp, vp, table[some], lens[some], few, d ** -0.5)
+    _close(out, want, tol, "out")
+    _close(lse, wl, ltol, "lse")
+
+
+def test_accounts_of_more_tiles_than_a_launch_has(A):
+    """A chunk at the end of a wide table beside thousands of sequences without new tokens, all accounts in place."""
+    _say("accounts of 2^24 workgroups")
+    heads, t, d, seqs, mp, new = 2, 64, 64, 4097, 2049, 40
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    kp = torch.randn((4, t, heads, d), generator=gen, device="cuda").to(BF)
+    table = torch.full((seqs, mp), -1, dtype=torch.int32, device="cuda")
+    table[-1, [0, 1000, mp - 2, mp - 1]] = torch.tensor([2, 0, 3, 1], dtype=torch.int32, device="cuda")
+    lens = torch.full((seqs,), 500, dtype=torch.int32, device="cuda")
+    lens[-1] = mp * t - 3
+    starts = torch.zeros(seqs + 1, dtype=torch.int32, device="cuda")
+    starts[-1] = new
+    q = torch.randn((new, heads, d), generator=gen, device="cuda").to(BF)
+    _, lse, _, _ = R.attention(q, kp, kp, table[-1:], lens[-1:], starts[-2:], d ** -0.5)
+    lse = lse.float().cuda()
+    mass = torch.rand((seqs, heads, mp), generator=gen, device="cuda")
+    before = mass.clone()
+    A.attention_mass(q, lse, kp, table, lens, starts, mass, out=mass)
+    want, tol = R.attention(q, kp, None, table[-1:], lens[-1:], starts[-2:], d ** -0.5, (lse, before[-1:], 1.0))
+    _close(mass[-1:], want, tol, "accounts")
+    assert torch.equal(mass[:-1], before[:-1])
+
+
+def test_an_eviction_of_more_sequences_than_a_launch_has(A):
+    _say("eviction of 2^24 sequences")
+    seqs = 2 ** 24 + 3
+    table = torch.arange(2 * seqs, dtype=torch.int32, device="cuda").view(seqs, 2)
+    mass = torch.rand((seqs, 1, 2), device="cuda")
+    lens = torch.full((seqs,), 20, dtype=torch.int32, device="cuda")
+    e = A.evict_pages(mass, table, lens, page_tokens=16, budget=1, sink=0)
+    assert bool((e.n_evicted == 1).all()) and bool((e.kv_lens == 4).all())
+    assert torch.equal(e.evicted[:, 0], table[:, 0]) and torch.equal(e.page_table[:, 0], table[:, 1])
+    assert torch.equal(e.mass[:, 0, 0], mass[:, 0, 1]) and bool((e.page_table[:, 1] == -1).all())

@@ -27,6 +27,7 @@ struct AppendParams {
     int32_t q_heads, kv_heads, head_dim, rope_dim, page_tokens;
     int32_t interleaved;
     float eps;
+    uint32_t first_block;                                 // of this launch
 };
 
 // Eight elements of a head vector in fp32.
@@ -65,7 +66,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendParams p) {
     constexpr int kTurn = 64 / LANES;                         // vectors of a turn
     constexpr int kAhead = AHEAD;                             // turns in flight
     const int lane = (int)threadIdx.x % LANES, group = ((int)threadIdx.x & 63) / LANES;
-    const uint32_t unit = (uint32_t)uniform((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    const uint32_t unit = (uint32_t)uniform((int)((p.first_block + blockIdx.x) * 4 + (threadIdx.x >> 6)));
     const uint32_t token = unit / p.parts, part = unit - token * p.parts;
     if (token >= p.n_tokens) return;
     const int first = (int)part * p.part_vecs, end = min(first + p.part_vecs, p.vecs);
@@ -204,9 +205,7 @@ void launch(AppendParams p, int cus, hipStream_t stream) {
         p.part_vecs = per_part * turn;
         p.parts = (uint32_t)((turns + per_part - 1) / per_part);
         const uint64_t units = (uint64_t)p.n_tokens * p.parts;
-        const dim3 grid((uint32_t)((units + 3) / 4));
-        if (per_part < 4) hipLaunchKernelGGL(kernel1, grid, dim3(256), 0, stream, p);
-        else hipLaunchKernelGGL(kernel4, grid, dim3(256), 0, stream, p);
+        launch_blocks(per_part < 4 ? kernel1 : kernel4, (units + 3) / 4, 256, 0, stream, p);
     };
 #define ZT_GO(lanes, chunks) go(append_kernel<DT, lanes, chunks, 1>, append_kernel<DT, lanes, chunks, 4>, lanes)
     if (chunks <= 2) ZT_GO(2, 1);

@@ -37,6 +37,7 @@ struct AttendParams {
     int32_t splits, resident;        // many kernel: most pieces of a sequence's tokens; workgroups the card holds at once
     float* partial;                  // results of pieces: sums [head_dim], maximum, total
     int32_t* cut;                    // what the many kernel's first workgroup leaves its join: pieces, tokens of a piece
+    uint32_t first_block;            // of this launch
 };
 
 __device__ __forceinline__ float* many_partial(const AttendParams& p, int row, int q_head, int split) {
@@ -468,10 +469,11 @@ void many_kernel(AttendParams p) {
     __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2][kTileBytes];   // [buffer][K, V]
     const int lane = (int)threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
-    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads);
-    const uint32_t rest = blockIdx.x / (uint32_t)p.kv_heads;
+    const uint32_t unit = p.first_block + blockIdx.x;
+    const int head = (int)(unit % (uint32_t)p.kv_heads);
+    const uint32_t rest = unit / (uint32_t)p.kv_heads;
     const Cut cut = cut_of(p);
-    if (blockIdx.x == 0 && threadIdx.x == 0 && p.splits > 1) p.cut[0] = cut.n, p.cut[1] = cut.tokens;
+    if (unit == 0 && threadIdx.x == 0 && p.splits > 1) p.cut[0] = cut.n, p.cut[1] = cut.tokens;
     const int split = (int)(rest % (uint32_t)cut.n);
     int s, block;
     if (!find_unit(p, (int)(rest / (uint32_t)cut.n), s, block)) return;
@@ -818,7 +820,8 @@ __device__ __forceinline__ void join_row(const AttendParams& p, const float* src
 template <int DT>
 __global__ __launch_bounds__(256) void join_few_kernel(AttendParams p, int most_rows) {
     const int wave = (int)threadIdx.x >> 6;
-    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads), s = (int)(blockIdx.x / (uint32_t)p.kv_heads);
+    const uint32_t unit = p.first_block + blockIdx.x;
+    const int head = (int)(unit % (uint32_t)p.kv_heads), s = (int)(unit / (uint32_t)p.kv_heads);
     const Seq seq = seq_of(p.batch, s);
     const int tiles = few_tiles(p, seq, most_rows);
     if (tiles == 0) return;
@@ -843,8 +846,9 @@ constexpr int kJoinRows = 8;
 template <int DT>
 __global__ __launch_bounds__(256) void join_many_kernel(AttendParams p) {
     const int wave = (int)threadIdx.x >> 6;
-    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads);
-    const uint32_t rest = blockIdx.x / (uint32_t)p.kv_heads;
+    const uint32_t unit = p.first_block + blockIdx.x;
+    const int head = (int)(unit % (uint32_t)p.kv_heads);
+    const uint32_t rest = unit / (uint32_t)p.kv_heads;
     const Cut cut{p.cut[0], p.cut[1]};
     int s, block;
     if (cut.n == 1 || !find_unit(p, (int)(rest / (kManyRows / kJoinRows)), s, block)) return;
@@ -932,7 +936,7 @@ void launch(const AttendParams& base, const Plan& plan, float* workspace, hipStr
         }
         if (plan.nt == 1) hipLaunchKernelGGL((few_kernel<DT, DP, 1>), grid, dim3(256), 0, stream, p);
         if (plan.few_groups > 1)
-            hipLaunchKernelGGL(join_few_kernel<DT>, dim3(heads * (uint32_t)p.batch.n_seqs), dim3(256), 0, stream, p, 16 * plan.nt);
+            launch_blocks(join_few_kernel<DT>, (uint64_t)heads * (uint32_t)p.batch.n_seqs, 256, 0, stream, p, 16 * plan.nt);
     }
     if (plan.many) {
         if (plan.splits > 1) {
@@ -940,10 +944,10 @@ void launch(const AttendParams& base, const Plan& plan, float* workspace, hipStr
             p.partial = workspace + kCutFloats;
         }
         const uint32_t units = (uint32_t)plan.many_units * heads;
-        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((uint32_t)plan.many_groups), dim3(256), 0, stream, p); };
-        if (p.batch.page_tokens % (many_tile(DP) / 4) == 0 && p.head_dim == DP) go(many_kernel<DT, DP, true>);
-        else go(many_kernel<DT, DP, false>);
-        if (p.splits > 1) hipLaunchKernelGGL(join_many_kernel<DT>, dim3(units * (kManyRows / kJoinRows)), dim3(256), 0, stream, p);
+        const bool even = p.batch.page_tokens % (many_tile(DP) / 4) == 0 && p.head_dim == DP;
+        launch_blocks(even ? many_kernel<DT, DP, true> : many_kernel<DT, DP, false>, (uint64_t)plan.many_groups, 256, 0, stream, p);
+        if (p.splits > 1)
+            launch_blocks(join_many_kernel<DT>, (uint64_t)units * (kManyRows / kJoinRows), 256, 0, stream, p);
     }
 }
 

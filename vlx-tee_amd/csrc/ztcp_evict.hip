@@ -24,6 +24,7 @@ struct EvictParams {
     int32_t* out_lens;
     int32_t* evicted;
     int32_t* n_evicted;
+    uint32_t first_block;               // of this launch
 };
 
 // A number's place among all doubles as an unsigned whole number; the two
@@ -95,7 +96,7 @@ __global__ __launch_bounds__(THREADS) void evict_kernel(EvictParams p) {
     __shared__ uint64_t ends[2][kWaves];
     __shared__ uint64_t few[kFew];
     __shared__ int found[3], n_few;
-    const int64_t s = blockIdx.x;
+    const int64_t s = (int64_t)p.first_block + blockIdx.x;
     const int tid = (int)threadIdx.x, lane = tid & 63;
     const float* mass = p.mass + s * p.heads * p.max_pages;
     const int32_t* table = p.table + s * p.table_stride;
@@ -325,7 +326,7 @@ extern "C" int ztcp_evict_pages(const float* mass, const int32_t* page_table, in
             hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
                                 kKeysInLds * (int)sizeof(uint64_t)) != hipSuccess)
             return ZTCP_EHIP;
-        hipLaunchKernelGGL(kernel, dim3((uint32_t)n_seqs), dim3(threads), lds, (hipStream_t)stream, p);
+        launch_blocks(kernel, (uint64_t)n_seqs, threads, lds, (hipStream_t)stream, p);
         return hipGetLastError() == hipSuccess ? ZTCP_OK : ZTCP_EHIP;
     };
     if (max_pages <= 1024) return go(evict_kernel<256, true>, 256u);

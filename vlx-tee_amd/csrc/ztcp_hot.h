@@ -53,6 +53,19 @@ inline DivBy div_by(uint32_t d) {
     return DivBy{(uint32_t)(((uint64_t)1 << (31 + s)) / d + 1), 31 + s};
 }
 
+// Launches `blocks` workgroups.  A launch takes fewer than 2^32 threads, so more workgroups than that come in parts, each
+// with its first one's number in p.first_block.
+template <class Params, class... More>
+inline void launch_blocks(void (*kernel)(Params, More...), uint64_t blocks, uint32_t threads, size_t lds, hipStream_t stream,
+                          Params p, More... more) {
+    const uint64_t most = 0xFFFFFFFFull / threads;
+    for (uint64_t first = 0; first < blocks; first += most) {
+        p.first_block = (uint32_t)first;
+        const uint64_t n = blocks - first < most ? blocks - first : most;
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)n), dim3(threads), lds, stream, p, more...);
+    }
+}
+
 // Compute units of the current device.
 inline int cu_count(int& cus) {
     int dev = 0;

@@ -28,6 +28,7 @@ struct MassParams {
     int32_t group_pages;             // pages of a tile: as many as the kernel's keys hold, one at least
     DivBy group_div;
     float scale_log2, decay;
+    uint32_t first_block;            // of this launch
 };
 
 // (a page may have so many tokens that a length and a page's tokens together pass 2^31)
@@ -249,8 +250,9 @@ void mass_many_kernel(MassParams p) {
     const int lane = (int)threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int row_half = wave >> 1;
-    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads);
-    const uint32_t rest = blockIdx.x / (uint32_t)p.kv_heads;
+    const uint32_t unit = p.first_block + blockIdx.x;
+    const int head = (int)(unit % (uint32_t)p.kv_heads);
+    const uint32_t rest = unit / (uint32_t)p.kv_heads;
     const int s = (int)(rest % (uint32_t)p.batch.n_seqs);
     const int tile = (int)(rest / (uint32_t)p.batch.n_seqs);  // early keys, which most rows see, first
     const Seq seq = uniform(seq_of(p.batch, s));
@@ -464,7 +466,7 @@ void launch(MassParams p, int64_t most_rows, int cus, hipStream_t stream) {
     }
     if (many) {
         const int64_t tiles = p.batch.n_seqs * tiles_of(kManyKeys);
-        hipLaunchKernelGGL((mass_many_kernel<DT, DP>), dim3((uint32_t)(tiles * heads)), dim3(256), 0, stream, p);
+        launch_blocks(mass_many_kernel<DT, DP>, (uint64_t)(tiles * heads), 256, 0, stream, p);
     }
 }
 
