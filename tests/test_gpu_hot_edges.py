@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import hot_reference as R
-from test_gpu_hot_ops import A, BF, FP, _batch, _check_attend, _close, _say  # noqa: F401  (A: the module's fixture)
+from test_gpu_hot_ops import A, BF, FP, _attend, _batch, _check_attend, _check_mass, _close, _say  # noqa: F401  (A: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -149,3 +149,23 @@ def test_an_eviction_of_more_sequences_than_a_launch_has(A):
     assert bool((e.n_evicted == 1).all()) and bool((e.kv_lens == 4).all())
     assert torch.equal(e.evicted[:, 0], table[:, 0]) and torch.equal(e.page_table[:, 0], table[:, 1])
     assert torch.equal(e.mass[:, 0, 0], mass[:, 0, 1]) and bool((e.page_table[:, 1] == -1).all())
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("which", ["q", "k"])
+def test_a_row_without_a_weight_reaches_the_pages_it_sees_only(A, which, d):
+    """A NaN in one new token's query, or in its key, makes its rows' log-sum-exp NaN (and those of the rows behind it,
+    for the key): the pages that these rows see have NaN accounts of that head, all others the 64-bit form's."""
+    _say("NaN rows", which, d)
+    for lens in ([(4, 300)], [(150, 400), (1, 60)], [(200, 200)]):
+        for token in (1, lens[0][0] // 2):
+            b = _batch(lens, 3, 2, d, 16, BF, seed=d)
+            key = lens[0][1] - lens[0][0] + token
+            if which == "q":
+                b["q"][token, 4] = float("nan")                # a head of the second KV head
+            else:
+                b["kp"][int(b["table"][0, key // 16]), key % 16, 1] = float("nan")
+            for hint in (True, False):
+                _, lse = _attend(A, b, hint)
+                assert bool(torch.isnan(lse[token, 4])) and not bool(torch.isnan(lse[:, :3]).any())
+                _check_mass(A, b, lse, (which, d, lens, token, hint), hint=hint)

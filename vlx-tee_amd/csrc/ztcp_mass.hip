@@ -355,6 +355,12 @@ void mass_many_kernel(MassParams p) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (8 * (i / 4) + i % 4 >= seen) sc[u][i] = -INFINITY;
+                if (base[u] != base[u]) {                        // a NaN goes to the tokens that its row sees
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (8 * (i / 4) + i % 4 < seen) sc[u][i] = base[u];
+                    base[u] = 0.f;
+                }
             }
         };
         auto weigh = [&](const f32x16 (&sc)[kSub], int w) {
