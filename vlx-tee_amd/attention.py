@@ -19,7 +19,8 @@ of ``q``.
 Every call is enqueued on the current stream of its tensors' device,
 synchronizes nothing, and can be recorded into a graph.  No operator has a
 gradient (they serve, as the codec does): a tensor that requires one is
-refused outside ``torch.no_grad()``.  Wrong arguments raise ``ValueError``;
+refused outside ``torch.no_grad()``, and one that carries a forward-mode
+tangent everywhere.  Wrong arguments raise ``ValueError``;
 indexes on the device are bounded by the kernels as include/ztcp.h says
 (ztcp_append_tokens and the entries after it).
 """

@@ -10,6 +10,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -44,6 +45,8 @@ const at::Tensor* tensor(PyObject* o, const char* name) {
     const at::Tensor* t = &THPVariable_Unpack(o);
     if (at::GradMode::is_enabled() && t->requires_grad())
         throw Refused(std::string(name) + " requires a gradient, which this operator does not have (torch.no_grad())");
+    if (t->_fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        throw Refused(std::string(name) + " carries a tangent, which this operator would drop");
     return t;
 }
 const at::Tensor* tensor_or_none(PyObject* o, const char* name) { return o == Py_None ? nullptr : tensor(o, name); }
