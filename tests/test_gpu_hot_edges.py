@@ -169,3 +169,46 @@ def test_a_row_without_a_weight_reaches_the_pages_it_sees_only(A, which, d):
                 _, lse = _attend(A, b, hint)
                 assert bool(torch.isnan(lse[token, 4])) and not bool(torch.isnan(lse[:, :3]).any())
                 _check_mass(A, b, lse, (which, d, lens, token, hint), hint=hint)
+
+
+def _serving_calls(A):
+    """The tensors that each call writes, and the call."""
+    b = _batch([(1, 40), (3, 70)], 4, 2, 128, 16, BF, seed=1)
+    out, mass = torch.zeros_like(b["q"]), torch.zeros((2, 2, b["table"].shape[1]), device="cuda")
+    _, lse = _attend(A, b)
+    k, v = torch.randn((2, 4, 2, 128), device="cuda").to(BF)
+    slots, pos, rope = torch.arange(4, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda"), A.rope_table(9, 64)
+    rest = [b[x] for x in ("q", "kp", "vp", "table", "lens", "starts")]
+    yield [b["q"], b["kp"], b["vp"]], lambda: A.append_tokens(b["q"], k, v, b["kp"], b["vp"], slots, pos, rope, q_out=b["q"])
+    yield [out], lambda: A.paged_attention(*rest, out=out)
+    yield [mass], lambda: A.attention_mass(b["q"], lse, b["kp"], b["table"], b["lens"], b["starts"], mass, out=mass)
+    yield [mass, b["table"], b["lens"]], lambda: A.evict_pages(mass, b["table"], b["lens"], page_tokens=16, budget=2,
+                                                               in_place=True)
+
+
+def test_tensors_that_are_written_have_a_new_version(A):
+    """torch tells by a tensor's version that one saved for a gradient has been overwritten since."""
+    _say("versions")
+    for written, call in _serving_calls(A):
+        before = [t._version for t in written]
+        call()
+        assert all(t._version > x for t, x in zip(written, before))
+    scale = torch.ones((), device="cuda", dtype=BF, requires_grad=True)
+    written, call = next(_serving_calls(A))
+    y = (scale * written[1]).sum()                             # saves the pages
+    with torch.no_grad():
+        call()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_tensors_of_inference_mode_are_written(A):
+    """They have no versions, inside and outside of that mode."""
+    _say("inference mode")
+    with torch.inference_mode():
+        calls = list(_serving_calls(A))
+        for _, call in calls:
+            call()
+    for written, call in calls:
+        assert all(t.is_inference() for t in written)
+        call()

@@ -77,6 +77,12 @@ bool truth(PyObject* o, const char* name) {
     return x != 0;
 }
 
+// A tensor that the caller holds has been written: what torch saved of it for a gradient is no longer what it was.
+// (Tensors of inference mode have no versions.)
+void written(const at::Tensor* t) {
+    if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 void* stream_of(const at::Device& d) { return (void*)c10::hip::getCurrentHIPStream(d.index()).stream(); }
 
 at::Tensor make(at::IntArrayRef shape, at::ScalarType type, const at::Device& d) {
@@ -183,6 +189,7 @@ PyObject* append_tokens(PyObject* const* a) {
                             (const float*)rope_ptr, rope->size(0), w[0], wl[0], w[1], wl[1], eps, truth(a[11], "interleaved"),
                             stream_of(d)),
          "append_tokens");
+    for (const at::Tensor* t : {given, k_pages, v_pages}) written(t);
     return THPVariable_Wrap(out);
 }
 
@@ -212,6 +219,7 @@ PyObject* paged_attention(PyObject* const* a) {
     done(ztcp_paged_attention(q->data_ptr(), qs, out.data_ptr(), want_lse ? (float*)lse.data_ptr() : nullptr, heads, &p.pool,
                               &batch, &p.g, scale, bytes ? work.data_ptr() : nullptr, bytes, stream_of(d)),
          "paged_attention");
+    written(given);
     PyObject* o = THPVariable_Wrap(out);
     if (!want_lse || !o) return o;
     PyObject* l = THPVariable_Wrap(lse);
@@ -240,6 +248,7 @@ PyObject* attention_mass(PyObject* const* a) {
     done(ztcp_attention_mass(q->data_ptr(), qs, (const float*)lse_ptr, heads, &p.pool, &batch, &p.g, scale,
                              (const float*)mass_ptr, decay, (float*)out.data_ptr(), stream_of(d)),
          "attention_mass");
+    written(given);
     return THPVariable_Wrap(out);
 }
 
@@ -265,6 +274,7 @@ PyObject* evict_pages(PyObject* const* a) {
                           (float*)out[1].data_ptr(), (int32_t*)out[2].data_ptr(), (int32_t*)out[3].data_ptr(),
                           (int32_t*)out[4].data_ptr(), stream_of(d)),
          "evict_pages");
+    for (const at::Tensor* t : {table, mass, lens}) written(in_place ? t : nullptr);
     PyObject* all = PyTuple_New(5);
     for (int i = 0; all && i < 5; ++i) {
         PyObject* o = THPVariable_Wrap(out[i]);
