@@ -14,7 +14,8 @@ counts (start-up, waits of each wave role, end) into a device buffer that
 it; the product library carries no timer code.
 
 ``_ztcp_torch.so`` (binding/ztcp_torch.cpp, host code) takes torch tensors to
-the operators on hot pages for ``attention.py``.
+the operators on hot pages for ``attention.py``; it is left out where torch
+is not installed, which the C ABI does not need.
 
 Flags: ``-ffp-contract=off`` and no fast-math (the quantizer's fp32 rounding
 order must match the reference's), packed-FP32 instructions disabled.
@@ -22,6 +23,7 @@ order must match the reference's), packed-FP32 instructions disabled.
 from __future__ import annotations
 
 import os
+import shutil
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -95,20 +97,26 @@ def build(verbose: bool = False, timers: bool = True) -> Path:
                 f.result()
             _link(hipcc, objs, out, verbose)
     _build_example(hipcc, verbose)
-    _build_binding(verbose)
+    _build_binding(hipcc, verbose)
     return LIB
 
 
-def _build_binding(verbose: bool) -> None:
+def _build_binding(hipcc: str, verbose: bool) -> None:
     import sysconfig
 
-    import torch
-
+    try:
+        import torch
+    except ImportError:
+        print("torch is not installed: torch binding left out", file=sys.stderr)
+        return
+    rocm_bin = Path(shutil.which(hipcc) or hipcc).resolve().parent
+    rocm = Path(os.environ.get("ROCM_PATH") or rocm_bin.parent)
+    cxx = os.environ.get("CXX") or shutil.which("g++") or str(rocm_bin / "amdclang++")
     root = Path(torch.__file__).resolve().parent
     tmp = BINDING.with_suffix(".so.tmp")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-isystem", str(root / "include"), "-isystem", "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"],
+           "-isystem", str(root / "include"), "-isystem", str(rocm / "include"), "-isystem", sysconfig.get_paths()["include"],
            str(BINDING_SRC), "-o", str(tmp), f"-L{HERE}", "-lztcp_hip", f"-L{root / 'lib'}", "-lc10", "-lc10_hip",
            "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     if verbose:
