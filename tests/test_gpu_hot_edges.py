@@ -212,3 +212,27 @@ def test_tensors_of_inference_mode_are_written(A):
     for written, call in calls:
         assert all(t.is_inference() for t in written)
         call()
+
+
+@pytest.mark.parametrize("t", [16, 300])
+@pytest.mark.parametrize("group", [5, 20])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_accounts_with_a_hint_too_small(A, d, group, t):
+    """Sequences of many more rows than ``max_q_len`` says: the rows come again for every block of keys."""
+    _say("accounts, hint", d, group, t)
+    b = _batch([(70, 200), (33, 33), (1, 90), (41, 1000)], group, 2, d, t, BF, seed=8)
+    _, lse = _attend(A, b)
+    b["most"] = 1
+    _check_mass(A, b, lse, (d, group, t))
+
+
+def test_accounts_of_wrong_lengths_and_hints(A):
+    """Lengths below 0 and behind the table, with rows that see nothing, and a hint that is too small."""
+    _say("accounts, wrong lengths")
+    b = _batch([(3, 50), (4, 60), (9, 70)], 4, 2, 64, 16, BF, seed=6)
+    for lens in ([-5, 60, 2 ** 31 - 1], [0, 0, 0], [2, 3, 70]):
+        b["lens"] = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        for most in (1, 100):
+            b["most"] = most
+            _, lse = _check_attend(A, b, (lens, most))
+            _check_mass(A, b, lse, (lens, most))
