@@ -236,3 +236,35 @@ def test_accounts_of_wrong_lengths_and_hints(A):
             b["most"] = most
             _, lse = _check_attend(A, b, (lens, most))
             _check_mass(A, b, lse, (lens, most))
+
+
+def test_captured_chunks_and_evictions_of_long_tables(A):
+    """A graph of chunks in pieces beside decoding sequences, their accounts and evictions from tables of 8,000 and 20,000
+    pages, replayed as lengths and numbers change, beside eager calls."""
+    _say("captured chunks")
+    b = _batch([(1, 700), (60, 2100), (1, 90), (140, 1500)], 2, 1, 128, 16, FP, seed=8)
+    mass = torch.zeros((4, 1, b["table"].shape[1]), device="cuda")
+    long = [(torch.rand((2, 1, n), device="cuda"), torch.arange(2 * n, dtype=torch.int32, device="cuda").view(2, n),
+             torch.tensor([n * 16, n * 8], dtype=torch.int32, device="cuda")) for n in (8000, 20000)]
+
+    def step():
+        out, lse = _attend(A, b)
+        m = A.attention_mass(b["q"], lse, b["kp"], b["table"], b["lens"], b["starts"], mass, decay=0.5)
+        return [out, lse, m, *(x for t in long for x in A.evict_pages(*t, page_tokens=16, budget=3000))]
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for i in range(4):
+        b["q"].normal_()
+        b["lens"].copy_(torch.tensor([700 - i, 2100 - 500 * i, 90, 140 + 300 * i], dtype=torch.int32))
+        for m, _, _ in long:
+            m.uniform_()
+        want = [x.clone() for x in step()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, w in zip(outs, want):
+            assert torch.equal(got, w), i
