@@ -382,7 +382,8 @@ ZTCP_API int ztcp_append_tokens(const void* q, int64_t q_stride, void* q_out, in
                        int32_t interleaved, void* stream);
 
 /* Attention of the batch's new tokens over its hot pages: softmax of scale * q . k
- * over the tokens a row sees, times V, in one pass with fp32 statistics.
+ * over the tokens a row sees, times V, in one pass with fp32 statistics.  For pages
+ * with K and V: single-buffer pages are refused.
  *   q [n_rows, q_heads, head_dim], tokens q_stride elements apart; query head h
  *   reads KV head h / (q_heads / num_heads); head_dim at most 256.
  *   out [n_rows, q_heads, head_dim] of the hot dtype.
@@ -390,8 +391,9 @@ ZTCP_API int ztcp_append_tokens(const void* q, int64_t q_stride, void* q_out, in
  *   exponentials, as ztcp_attention_mass takes it.
  * A row that sees no token gets zeros and -infinity.  What stands in pages behind
  * a sequence's length or after a row's own token, NaN and infinities among it,
- * does not reach the row.  workspace: ztcp_paged_attention_workspace(...) bytes
- * (may be 0; (size_t)-1 for arguments that the call refuses), needed until the
+ * does not reach the row; an infinity or a NaN of V that a row sees makes its column
+ * of the result infinite or NaN.  workspace: ztcp_paged_attention_workspace(...)
+ * bytes (may be 0; (size_t)-1 for arguments that the call refuses), needed until the
  * call's work is done, by one call at a time. */
 ZTCP_API size_t ztcp_paged_attention_workspace(const ztcp_paged_batch* batch, const ztcp_page_pool* pool,
                                       const ztcp_geometry* g, int64_t q_heads);
@@ -405,8 +407,8 @@ ZTCP_API int ztcp_paged_attention(const void* q, int64_t q_stride, void* out, fl
  *   out[s, h, p] = decay * mass[s, h, p] + sum of exp(scale * q . k - lse) over the
  *   rows of KV head h's query heads and the tokens of page p that they see.
  * mass, out [n_seqs, num_heads, max_pages] fp32; out may be mass itself.  lse as
- * ztcp_paged_attention gives it; a row with -infinity adds nothing.  The pool's v is
- * not read and may be NULL.  Sums are in fp32, in an order that the call fixes. */
+ * ztcp_paged_attention gives it; a row with -infinity adds nothing.  head_dim at most
+ * 256.  The pool's v is not read and may be NULL.  Sums are in fp32, in an order that the call fixes. */
 ZTCP_API int ztcp_attention_mass(const void* q, int64_t q_stride, const float* lse, int64_t q_heads,
                         const ztcp_page_pool* pool, const ztcp_paged_batch* batch,
                         const ztcp_geometry* g, float scale, const float* mass, float decay,

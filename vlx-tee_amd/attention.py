@@ -8,6 +8,10 @@ pages than its budget gives up those with the least weight (``evict_pages``);
 their ids select the descriptors that ``pages.egress`` takes to the cold tier,
 and pages that ``pages.ingress`` brought back are read like any other.
 
+``append_tokens`` and ``evict_pages`` take single-buffer (latent) pages too;
+``paged_attention`` is for pages with K and V, and it and ``attention_mass`` for a
+head_dim of at most 256.
+
 Pages are the codec's hot pages: a pool ``[n_pages, page_tokens, kv_heads,
 head_dim]`` of float16 or bfloat16, each page contiguous (pages may be padded
 or interleaved), RoPE columns leading.  Row ``s`` of ``page_table`` lists

@@ -58,7 +58,7 @@ __device__ __forceinline__ uint4 pack_chunk(const Chunk& c) {
 // reads and writes every element once and is bound by that: the angles and weights are loaded once for a wave's
 // vectors, the next turns' loads are in flight during a turn, the sum of squares is a butterfly over the group, and
 // the partner of a rotated pair sits rope_dim / 16 lanes away (or in the same lane when interleaved), so a vector
-// never leaves registers.  Prompt of 16,384 tokens of 32 + 8 + 8 vectors of 128 (407 MB): 88 to 92 us, 4.5 TB/s where a
+// never leaves registers.  Prompt of 16,384 tokens of 32 + 8 + 8 vectors of 128 (407 MB): 91 to 92 us, 4.45 TB/s where a
 // large copy has 5.0; with loads that leave a trace in the caches 99 us, and a wave for every four vectors, with
 // angles and weights of its own, 147 us.
 template <int DT, int LANES, int CHUNKS, int AHEAD>

@@ -97,7 +97,7 @@ __device__ __forceinline__ f32x4 only_not_finite(const AttendParams& p, const Pl
 // sequence.
 //
 // 64 sequences of 500 to 16,384 tokens, 4 query heads to each of 8 KV heads of
-// 128, pages of 16 (1.16 GB): 198 to 203 us, 5.8 TB/s where a kernel that only reads has
+// 128, pages of 16 (1.16 GB): 197 to 203 us, 5.8 TB/s where a kernel that only reads has
 // 6.35.  Loads of whole rows that leave no trace in the caches made it that: with
 // K in 64-byte parts of rows and ordinary loads it took 237 (V's alone without
 // trace: 222; K's parts too: 234, each line fetched twice), and cut by sequence
@@ -401,10 +401,10 @@ void few_kernel(AttendParams p) {
 // vector units have work at the same time, with two waves on a SIMD.
 //
 // Two prompts' second 4,096 tokens over 8,192, 32 + 8 heads of 128, pages of 64
-// (825 GFLOP): 851 to 900 us, 970 to 920 TFLOP/s, where the library's largest
+// (825 GFLOP): 840 to 900 us, 980 to 920 TFLOP/s, where the library's largest
 // products have 1194.  Through registers, one tile after the other, 2067 us;
 // straight to LDS 925.  Matrix units are busy for 46% of the clocks and the vector
-// units issue for 42%, which two waves a SIMD overlap in part only; registers
+// units issue for 43%, which two waves a SIMD overlap in part only; registers
 // allow no third.  The spread is the clock's, about 2.0 GHz in such a kernel.
 
 constexpr int kManyRows = 128;

@@ -84,9 +84,10 @@ __device__ __forceinline__ int pages_of(const EvictParams& p, int32_t len) {
 // It is bound by latencies: what one compute unit has in flight brings about 16
 // bytes a nanosecond.  8 sequences of 256 pages and 8 heads: 9.2 us by 256
 // threads (13.4 by 1024, whose barriers and redundant scans cost more).  128
-// sequences of up to 8,192 pages: 47.6 us, of which the keys take 16, finding
-// what goes 9, the walk 20 with two pages a thread (51 with one; four spill); as
-// three kernels, with keys and accounts moved by all compute units, 50.5.
+// sequences of up to 8,192 pages: 52 us a pass, 47.4 of them the kernel's (the
+// profiler's time), of which the keys take 16, finding what goes 9, the walk 20
+// with two pages a thread (51 with one; four spill); as three kernels, with keys
+// and accounts moved by all compute units, 50.5 beside 47.6.
 template <int THREADS, bool IN_LDS>
 __global__ __launch_bounds__(THREADS) void evict_kernel(EvictParams p) {
     constexpr int kWaves = THREADS / 64, kOwn = kBins / THREADS, kOwnPages = THREADS == 1024 ? 2 : 1;

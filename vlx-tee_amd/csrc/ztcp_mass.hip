@@ -232,11 +232,12 @@ void mass_few_kernel(MassParams p) {
 // the card ends evenly.  Every page's account has one writer and one order of additions.
 //
 // Two prompts' second 2,048 tokens over 4,096, 32 + 8 heads of 128, pages of 16
-// (103 GFLOP): 154 to 165 us, 670 to 625 TFLOP/s; with the rows read from memory
-// by every wave and the exponentials after the products 408.  The 403 million
-// exponentials with their scaling and sums bound it: the matrix units are busy
-// for 28% of the clocks, the vector units issue for 44% and, an exponential
-// taking the time of four instructions, work for more.
+// (103 GFLOP): 153 to 158 us, 675 to 655 TFLOP/s; with the rows read from memory
+// by every wave and the exponentials after the products 408.  Vector work bounds
+// it: the matrix units are busy for 28% of the clocks, the vector units, with
+// the time of four instructions for an exponential, for 65%: 42% the 403 million
+// exponentials with their scaling and sums, 23% everything else (scores begun at
+// zero, masks, the rows' references, addresses).
 
 template <int DT, int DP>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1)))
