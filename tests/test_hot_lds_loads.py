@@ -4,7 +4,11 @@ Such a load takes its LDS address from m0, and needs a wait state behind the
 instruction that writes m0: without one it may still see the previous load's
 address.  Inside an asm statement the compiler neither adds the wait state nor
 knows that m0 is overwritten, so the compiled code must show both: something
-between the write and the load, and no other use of m0.
+between the write and the load, and no other use of m0.  Nor does it know that
+a load inside asm reads a scalar base, which needs five wait states behind a
+vector instruction (v_readfirstlane) that wrote it, whatever the compiler puts
+in front of the asm; behind a scalar instruction, which waits for a vector
+instruction's result by itself, it needs none.
 """
 import re
 import shutil
@@ -46,7 +50,7 @@ def test_a_load_waits_for_its_address(listings, name):
     loads = [i for i, x in enumerate(lines) if x.startswith("global_load_lds")]
     assert loads
     for i in loads:
-        assert lines[i - 1].startswith("s_nop") and lines[i - 2].startswith("s_mov_b32 m0,"), lines[i - 3:i + 1]
+        assert lines[i - 2].startswith("s_mov_b32 m0,") and re.match(r"s_nop|s_mov_b64", lines[i - 1]), lines[i - 3:i + 1]
 
 
 @pytest.mark.parametrize("name", SOURCES)
@@ -56,3 +60,12 @@ def test_nothing_else_uses_m0(listings, name):
     loads = [i for i, x in enumerate(lines) if x.startswith("global_load_lds")]
     assert loads and len(writes) == len(loads)
     assert all(lines[i].startswith("s_mov_b32 m0,") for i in writes)
+
+
+@pytest.mark.parametrize("name", SOURCES)
+def test_a_load_waits_for_its_scalar_base(listings, name):
+    lines = listings[name]
+    bases = {i: m[1] for i, x in enumerate(lines) if (m := re.match(r"global_load_lds\S*\s+v\S+,\s*(s\[\S+\])", x))}
+    assert bases
+    for i, base in bases.items():
+        assert re.match(r"s_mov_b64 " + re.escape(base) + ",", lines[i - 1]), lines[i - 2:i + 1]

@@ -222,15 +222,19 @@ __device__ __forceinline__ Place place_of(const PagedView& v, const Seq& q, int 
 
 // 64 pieces of 16 bytes from global memory to LDS, a wave's piece i to lds + 16 i, without passing through registers;
 // done once vmcnt says so.  Written in asm because the compiler, which cannot tell two buffers apart, would wait for
-// the next tile's loads before this tile's reads.  A load to LDS needs one wait state behind the write of m0 that it
-// uses, which the compiler does not add inside asm.  There is no output register.  m0 is reserved, so that it cannot
-// be listed as overwritten and the compiler keeps nothing in it; nothing else in these kernels' code uses it, which
-// tests/test_hot_lds_loads.py checks.  The second form takes a base of the wave and each lane's offset.
+// the next tile's loads before this tile's reads.  It has no output that the load writes.  What the compiler does not
+// add inside asm: a load to LDS needs one wait state behind the write of m0 that it uses, and five behind a vector
+// instruction (readfirstlane) that wrote its scalar base; a scalar copy of the base, which waits for that by itself, is
+// both.  m0 is reserved: it cannot be listed as overwritten, and the compiler keeps nothing in it; nothing else in
+// these kernels' code uses it, which tests/test_hot_lds_loads.py checks.  The second form takes a base of the wave and
+// each lane's offset.
 __device__ __forceinline__ void load_lds16(const uint8_t* src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(uniform((int)lds)), "v"(src) : "memory");
 }
 __device__ __forceinline__ void load_lds16(const uint8_t* base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(uniform((int)lds)), "v"(offset), "s"(uniform(base)) : "memory");
+    uint64_t copy;
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0"
+                 : "=&s"(copy) : "s"(uniform((int)lds)), "v"(offset), "s"(uniform(base)) : "memory");
 }
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
