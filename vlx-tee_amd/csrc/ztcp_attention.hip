@@ -401,7 +401,7 @@ void few_kernel(AttendParams p) {
 // vector units have work at the same time, with two waves on a SIMD.
 //
 // Two prompts' second 4,096 tokens over 8,192, 32 + 8 heads of 128, pages of 64
-// (825 GFLOP): 840 to 900 us, 980 to 920 TFLOP/s, where the library's largest
+// (825 GFLOP): 840 to 870 us, 980 to 950 TFLOP/s, where the library's largest
 // products have 1194.  Through registers, one tile after the other, 2067 us;
 // straight to LDS 925.  Matrix units are busy for 46% of the clocks and the vector
 // units issue for 43%, which two waves a SIMD overlap in part only; registers
