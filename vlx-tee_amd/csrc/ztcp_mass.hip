@@ -232,7 +232,7 @@ void mass_few_kernel(MassParams p) {
 // the card ends evenly.  Every page's account has one writer and one order of additions.
 //
 // Two prompts' second 2,048 tokens over 4,096, 32 + 8 heads of 128, pages of 16
-// (103 GFLOP): 151 us, 684 TFLOP/s; with the rows read from memory
+// (103 GFLOP): 151 to 153 us, 684 to 675 TFLOP/s; with the rows read from memory
 // by every wave and the exponentials after the products 408.  Vector work bounds
 // it: the matrix units are busy for 29% of the clocks, the vector units, with
 // the time of four instructions for an exponential, for 67%: 43% the 403 million
