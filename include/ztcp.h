@@ -432,6 +432,46 @@ ZTCP_API int ztcp_evict_pages(const float* mass, const int32_t* page_table, int6
                      int32_t* out_table, int64_t out_table_stride, float* out_mass, int32_t* out_lens,
                      int32_t* evicted, int32_t* n_evicted, void* stream);
 
+/* Pages for a step's new tokens, with the step's row starts, slots and positions,
+ * from what the sequences hold and ask for.  With L = kv_lens[s] (cut to
+ * 0 .. max_pages * num_tokens) and q = q_lens[s] (negative: 0; 0 too where L + q tokens
+ * have no room in the table's columns), sequence s needs
+ * ceil((L + q) / num_tokens) - ceil(L / num_tokens) pages.  It gets all or nothing:
+ * R and P being the sums of the rows and pages asked for by it and the sequences in
+ * front (served or not), it is served if R <= max_rows and either it needs no page or
+ * P <= n_free (cut to 0 .. capacity).
+ *   free_pages [capacity] is a stack of which the first n_free[0] entries are there;
+ *   sequence s's i-th new page is entry n_free - 1 - (P - needed) - i, which is written
+ *   into its column of the table.  The other entries of the table are left.
+ *   out_lens [n_seqs] = L + granted, out_n_free [1], both may be the inputs themselves;
+ *   q_starts [n_seqs + 1]: sums of granted [n_seqs], which is q or 0;
+ *   slots, positions [max_rows]: of sequence s's i-th new token, which is token L + i,
+ *   page * num_tokens + token in page (-1 where its entry is negative), and
+ *   next_positions[s] + i (NULL: L + i); -1 and 0 behind the last row;
+ *   out_next_positions [n_seqs] = next_positions + granted (may be next_positions).
+ * workspace: ztcp_allot_pages_workspace(n_seqs) bytes ((size_t)-1 if the call refuses
+ * n_seqs), needed until the call's work is done, by one call at a time. */
+ZTCP_API size_t ztcp_allot_pages_workspace(int64_t n_seqs);
+ZTCP_API int ztcp_allot_pages(int32_t* page_table, int64_t table_stride, int64_t max_pages, const int32_t* kv_lens,
+                     const int32_t* q_lens, int64_t n_seqs, const int32_t* free_pages, int64_t capacity,
+                     const int32_t* n_free, const int32_t* next_positions, int64_t num_tokens, int64_t max_rows,
+                     int32_t* out_lens, int32_t* out_n_free, int32_t* out_next_positions, int32_t* q_starts,
+                     int64_t* slots, int32_t* positions, int32_t* granted, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* Pages given back: of every sequence the entries in columns from
+ * ceil(kv_lens[s] / num_tokens) on that are not negative go onto the stack
+ * (free_pages, n_free as above), sequence after sequence in the columns' order, and
+ * out_table has -1 in their place and is page_table elsewhere.  What the stack has no
+ * room for stays in the table.  out_n_free [1], n_released [n_seqs].  out_table and
+ * out_n_free may be the inputs themselves.  An entry that occurs twice is given back
+ * twice.  workspace: ztcp_release_pages_workspace(...) bytes, as above. */
+ZTCP_API size_t ztcp_release_pages_workspace(int64_t n_seqs, int64_t max_pages);
+ZTCP_API int ztcp_release_pages(const int32_t* page_table, int64_t table_stride, int64_t max_pages, const int32_t* kv_lens,
+                       int64_t n_seqs, int64_t num_tokens, int32_t* free_pages, int64_t capacity,
+                       const int32_t* n_free, int32_t* out_table, int64_t out_table_stride, int32_t* out_n_free,
+                       int32_t* n_released, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Short description of a return code. */
 ZTCP_API const char* ztcp_strerror(int code);
 

@@ -132,3 +132,52 @@ def evict_pages(mass: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Ten
     cold already (a page that is not there) has its account and its turn like
     any other, and is listed as the table had it."""
     return Eviction._make(_call().evict_pages(mass, page_table, kv_lens, page_tokens, budget, sink, recent, in_place))
+
+
+class Allotment(NamedTuple):
+    """What ``allot_pages`` leaves of the sequences and what a step's calls take."""
+
+    kv_lens: torch.Tensor                # [sequences] int32: the new tokens among them
+    n_free: torch.Tensor                 # [1] int32: free pages left
+    q_starts: torch.Tensor               # [sequences + 1] int32
+    slots: torch.Tensor                  # [max_rows] int64: -1 behind the last row
+    positions: torch.Tensor              # [max_rows] int32: 0 behind the last row
+    granted: torch.Tensor                # [sequences] int32: q_lens, or 0 for a sequence that has to wait
+    next_positions: torch.Tensor | None  # [sequences] int32, if they were given
+
+
+def allot_pages(page_table: torch.Tensor, kv_lens: torch.Tensor, q_lens: torch.Tensor, free_pages: torch.Tensor,
+                n_free: torch.Tensor, *, page_tokens: int, max_rows: int, next_positions: torch.Tensor | None = None,
+                in_place: bool = False) -> Allotment:
+    """Gives every sequence the pages that its ``q_lens`` new tokens need, behind the ``kv_lens`` that it has, and lays
+    out the step: where each sequence's rows start, each row's slot and position, as ``append_tokens`` and the
+    attention calls take them.
+
+    ``free_pages`` [any number] is a stack of page ids of which the first ``n_free`` [1] are there; pages are taken from
+    its end and written into ``page_table``.  A sequence gets all or nothing: it waits (``granted`` 0) if the rows that
+    it and the sequences in front ask for exceed ``max_rows``, if it needs a page and the pages that they ask for exceed
+    ``n_free``, or if its table row has no column left.  Positions go on from ``next_positions`` (after an eviction a
+    sequence's own count is more than its length), from ``kv_lens`` if there are none.  A new token whose page is not
+    there (its last page is cold) has slot -1.
+
+    ``page_table`` is written in either case; ``in_place`` updates ``kv_lens``, ``n_free`` and ``next_positions`` too."""
+    return Allotment._make(_call().allot_pages(page_table, kv_lens, q_lens, free_pages, n_free, page_tokens, max_rows,
+                                               next_positions, in_place))
+
+
+class Release(NamedTuple):
+    """What ``release_pages`` leaves."""
+
+    page_table: torch.Tensor   # [sequences, pages] int32: -1 where a page was given back
+    n_free: torch.Tensor       # [1] int32
+    n_released: torch.Tensor   # [sequences] int32
+
+
+def release_pages(page_table: torch.Tensor, kv_lens: torch.Tensor, free_pages: torch.Tensor, n_free: torch.Tensor, *,
+                  page_tokens: int, in_place: bool = False) -> Release:
+    """Puts the pages that ``kv_lens`` tokens do not reach back onto the stack ``free_pages``, ``n_free`` (written in
+    either case): those of a sequence that has ended (``kv_lens`` 0), or of drafted tokens that were not accepted.  Pages
+    go in the order of sequences and columns; negative entries are no pages; what the stack has no room for stays in the
+    table.  The ids that ``evict_pages`` lists are given back, once they have been written out, by
+    ``release_pages(cold.evicted, torch.zeros_like(kv_lens), ...)``.  ``in_place`` updates ``page_table`` and ``n_free``."""
+    return Release._make(_call().release_pages(page_table, kv_lens, free_pages, n_free, page_tokens, in_place))

@@ -287,6 +287,88 @@ PyObject* evict_pages(PyObject* const* a) {
     return all;
 }
 
+PyObject* tuple_of(const at::Tensor* out, int n) {   // None for an undefined one
+    PyObject* all = PyTuple_New(n);
+    for (int i = 0; all && i < n; ++i) {
+        PyObject* o = Py_None;
+        if (out[i].defined()) o = THPVariable_Wrap(out[i]);
+        else Py_INCREF(o);
+        if (!o) {
+            Py_DECREF(all);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(all, i, o);
+    }
+    return all;
+}
+
+PyObject* allot_pages(PyObject* const* a) {
+    const at::Tensor *table = tensor(a[0], "page_table"), *lens = tensor(a[1], "kv_lens"), *wanted = tensor(a[2], "q_lens");
+    const at::Tensor *free_pages = tensor(a[3], "free_pages"), *n_free = tensor(a[4], "n_free");
+    const at::Tensor* counts = tensor_or_none(a[7], "next_positions");
+    const int64_t tokens = whole(a[5], "page_tokens"), rows = whole(a[6], "max_rows");
+    const bool in_place = truth(a[8], "in_place");
+    need(table->is_cuda(), "page_table must be a HIP tensor");
+    const at::Device d = table->device();
+    const int64_t stride = Pool::table(*table, d), s = table->size(0), mp = table->size(1);
+    const void* lens_ptr = Pool::plain(*lens, "kv_lens", at::kInt, {s}, d);
+    const void* wanted_ptr = Pool::plain(*wanted, "q_lens", at::kInt, {s}, d);
+    const void* free_ptr = Pool::plain(*free_pages, "free_pages", at::kInt, {free_pages->numel()}, d);
+    const void* n_free_ptr = Pool::plain(*n_free, "n_free", at::kInt, {1}, d);
+    const void* counts_ptr = counts ? Pool::plain(*counts, "next_positions", at::kInt, {s}, d) : nullptr;
+    need(rows >= 0, "max_rows must not be negative");
+    at::Tensor out[7];
+    out[0] = in_place ? *lens : make({s}, at::kInt, d);
+    out[1] = in_place ? *n_free : make({1}, at::kInt, d);
+    out[2] = make({s + 1}, at::kInt, d);
+    out[3] = make({rows}, at::kLong, d);
+    out[4] = make({rows}, at::kInt, d);
+    out[5] = make({s}, at::kInt, d);
+    if (counts) out[6] = in_place ? *counts : make({s}, at::kInt, d);
+    const c10::DeviceGuard guard(d);
+    const size_t bytes = ztcp_allot_pages_workspace(s);
+    need(bytes != (size_t)-1, "too many sequences");
+    const at::Tensor work = make({(int64_t)bytes}, at::kByte, d);
+    done(ztcp_allot_pages((int32_t*)table->data_ptr(), stride, mp, (const int32_t*)lens_ptr, (const int32_t*)wanted_ptr, s,
+                          (const int32_t*)free_ptr, free_pages->numel(), (const int32_t*)n_free_ptr, (const int32_t*)counts_ptr,
+                          tokens, rows, (int32_t*)out[0].data_ptr(), (int32_t*)out[1].data_ptr(),
+                          counts ? (int32_t*)out[6].data_ptr() : nullptr, (int32_t*)out[2].data_ptr(),
+                          (int64_t*)out[3].data_ptr(), (int32_t*)out[4].data_ptr(), (int32_t*)out[5].data_ptr(), work.data_ptr(),
+                          bytes, stream_of(d)),
+         "allot_pages");
+    written(table);
+    for (const at::Tensor* t : {lens, n_free, counts}) written(in_place ? t : nullptr);
+    return tuple_of(out, 7);
+}
+
+PyObject* release_pages(PyObject* const* a) {
+    const at::Tensor *table = tensor(a[0], "page_table"), *lens = tensor(a[1], "kv_lens");
+    const at::Tensor *free_pages = tensor(a[2], "free_pages"), *n_free = tensor(a[3], "n_free");
+    const int64_t tokens = whole(a[4], "page_tokens");
+    const bool in_place = truth(a[5], "in_place");
+    need(table->is_cuda(), "page_table must be a HIP tensor");
+    const at::Device d = table->device();
+    const int64_t stride = Pool::table(*table, d), s = table->size(0), mp = table->size(1);
+    const void* lens_ptr = Pool::plain(*lens, "kv_lens", at::kInt, {s}, d);
+    void* free_ptr = Pool::plain(*free_pages, "free_pages", at::kInt, {free_pages->numel()}, d);
+    const void* n_free_ptr = Pool::plain(*n_free, "n_free", at::kInt, {1}, d);
+    at::Tensor out[3];
+    out[0] = in_place ? *table : make({s, mp}, at::kInt, d);
+    out[1] = in_place ? *n_free : make({1}, at::kInt, d);
+    out[2] = make({s}, at::kInt, d);
+    const c10::DeviceGuard guard(d);
+    const size_t bytes = ztcp_release_pages_workspace(s, mp);
+    need(bytes != (size_t)-1, "too many sequences or pages");
+    const at::Tensor work = make({(int64_t)bytes}, at::kByte, d);
+    done(ztcp_release_pages((const int32_t*)table->data_ptr(), stride, mp, (const int32_t*)lens_ptr, s, tokens, (int32_t*)free_ptr,
+                            free_pages->numel(), (const int32_t*)n_free_ptr, (int32_t*)out[0].data_ptr(), in_place ? stride : mp,
+                            (int32_t*)out[1].data_ptr(), (int32_t*)out[2].data_ptr(), work.data_ptr(), bytes, stream_of(d)),
+         "release_pages");
+    written(free_pages);
+    for (const at::Tensor* t : {table, n_free}) written(in_place ? t : nullptr);
+    return tuple_of(out, 3);
+}
+
 // No C++ exception leaves a C entry.
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -315,7 +397,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 #define ZT_FUNCTION(name, n) {#name, (PyCFunction)(void*)entry<name, n>, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {ZT_FUNCTION(append_tokens, 13), ZT_FUNCTION(paged_attention, 10), ZT_FUNCTION(attention_mass, 11),
-                          ZT_FUNCTION(evict_pages, 8), {nullptr, nullptr, 0, nullptr}};
+                          ZT_FUNCTION(evict_pages, 8), ZT_FUNCTION(allot_pages, 9), ZT_FUNCTION(release_pages, 6), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_ztcp_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
