@@ -402,6 +402,19 @@ ZTCP_API int ztcp_paged_attention(const void* q, int64_t q_stride, void* out, fl
                          const ztcp_geometry* g, float scale, void* workspace, size_t workspace_bytes,
                          void* stream);
 
+/* Attention of drafted tokens that form a tree: as ztcp_paged_attention, but the i-th
+ * of a sequence's n new tokens sees all kv_lens[s] - n tokens in front of the new ones
+ * and, of the new ones, the j-th if bit j % 64 of word j / 64 of its mask is set (itself
+ * too only if it is; bits from n on are not looked at, new tokens behind the last word
+ * not seen).  tree_mask [n_rows, tree_words], 8-byte aligned.  For a tree a token's mask is
+ * itself and the line of its ancestors; any other mask is as good. */
+ZTCP_API size_t ztcp_tree_attention_workspace(const ztcp_paged_batch* batch, const ztcp_page_pool* pool,
+                                     const ztcp_geometry* g, int64_t q_heads);
+ZTCP_API int ztcp_tree_attention(const void* q, int64_t q_stride, void* out, float* lse, int64_t q_heads,
+                        const ztcp_page_pool* pool, const ztcp_paged_batch* batch,
+                        const ztcp_geometry* g, const uint64_t* tree_mask, int64_t tree_words, float scale,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
 /* The attention weight that each page of the batch received from its new tokens,
  * added to the accounts:
  *   out[s, h, p] = decay * mass[s, h, p] + sum of exp(scale * q . k - lse) over the

@@ -97,6 +97,17 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return _call().paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts, scale, max_q_len, return_lse, out)
 
 
+def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                   kv_lens: torch.Tensor, q_starts: torch.Tensor, tree_mask: torch.Tensor, *, scale: float | None = None,
+                   max_q_len: int | None = None, return_lse: bool = False, out: torch.Tensor | None = None):
+    """``paged_attention`` of drafted tokens that form a tree: each of a sequence's n new tokens sees all tokens in
+    front of the new ones and, of these, the j-th if bit ``j % 64`` of word ``j // 64`` of its row of ``tree_mask``
+    [rows, words] (int64) is set: itself and its ancestors.  Bits from n on are not looked at; new tokens behind the last
+    word are not seen; a token whose own bit is not set does not see itself."""
+    return _call().tree_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts, tree_mask, scale, max_q_len, return_lse,
+                                  out)
+
+
 def attention_mass(q: torch.Tensor, lse: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor,
                    kv_lens: torch.Tensor, q_starts: torch.Tensor, mass: torch.Tensor, *, scale: float | None = None,
                    decay: float = 1.0, max_q_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:

@@ -197,36 +197,53 @@ float scale_of(PyObject* o, int64_t head_dim) {
     return o == Py_None ? (float)(1.0 / std::sqrt((double)head_dim)) : (float)number(o, "scale");
 }
 
-PyObject* paged_attention(PyObject* const* a) {
-    need(a[2] != Py_None, "paged_attention needs K and V pages (single-buffer pages have none)");
-    const at::Tensor *q = tensor(a[0], "q"), *k_pages = tensor(a[1], "k_pages"), *v_pages = tensor(a[2], "v_pages");
-    const at::Tensor *table = tensor(a[3], "page_table"), *lens = tensor(a[4], "kv_lens"), *starts = tensor(a[5], "q_starts");
-    const bool want_lse = truth(a[8], "return_lse");
-    const at::Tensor* given = tensor_or_none(a[9], "out");
-    const Pool p(k_pages, v_pages, 0);
-    const at::Device d = p.device();
-    const int64_t qs = p.tokens(*q, "q"), n = q->size(0), heads = q->size(1);
-    const ztcp_paged_batch batch = p.batch(*table, *lens, *starts, n, a[7]);
-    const at::Tensor out = given ? *given : make(q->sizes(), q->scalar_type(), d);
-    if (given) p.array(out, "out", q->scalar_type(), q->sizes());
-    const at::Tensor lse = want_lse ? make({n, heads}, at::kFloat, d) : at::Tensor();
-    const float scale = scale_of(a[6], k_pages->size(3));
-    const c10::DeviceGuard guard(d);
-    const size_t bytes = ztcp_paged_attention_workspace(&batch, &p.pool, &p.g, heads);
-    if (bytes == (size_t)-1) done(*ztcp_last_error() ? ZTCP_EINVAL : ZTCP_EHIP, "paged_attention");
-    // the caching allocator gives it to later work of this stream only
-    const at::Tensor work = bytes ? make({(int64_t)bytes}, at::kByte, d) : at::Tensor();
-    done(ztcp_paged_attention(q->data_ptr(), qs, out.data_ptr(), want_lse ? (float*)lse.data_ptr() : nullptr, heads, &p.pool,
-                              &batch, &p.g, scale, bytes ? work.data_ptr() : nullptr, bytes, stream_of(d)),
-         "paged_attention");
-    written(given);
+PyObject* with_lse(const at::Tensor& out, const at::Tensor* lse) {
     PyObject* o = THPVariable_Wrap(out);
-    if (!want_lse || !o) return o;
-    PyObject* l = THPVariable_Wrap(lse);
+    if (!lse || !o) return o;
+    PyObject* l = THPVariable_Wrap(*lse);
     PyObject* both = l ? PyTuple_Pack(2, o, l) : nullptr;
     Py_DECREF(o);
     Py_XDECREF(l);
     return both;
+}
+
+// paged_attention, and with TREE tree_attention, which has the mask behind q_starts
+template <bool TREE>
+PyObject* attention(PyObject* const* a) {
+    constexpr const char* name = TREE ? "tree_attention" : "paged_attention";
+    need(a[2] != Py_None, name, " needs K and V pages (single-buffer pages have none)");
+    const at::Tensor *q = tensor(a[0], "q"), *k_pages = tensor(a[1], "k_pages"), *v_pages = tensor(a[2], "v_pages");
+    const at::Tensor *table = tensor(a[3], "page_table"), *lens = tensor(a[4], "kv_lens"), *starts = tensor(a[5], "q_starts");
+    const at::Tensor* mask = TREE ? tensor(a[6], "tree_mask") : nullptr;
+    PyObject* const* b = a + (TREE ? 7 : 6);   // scale, max_q_len, return_lse, out
+    const bool want_lse = truth(b[2], "return_lse");
+    const at::Tensor* given = tensor_or_none(b[3], "out");
+    const Pool p(k_pages, v_pages, 0);
+    const at::Device d = p.device();
+    const int64_t qs = p.tokens(*q, "q"), n = q->size(0), heads = q->size(1);
+    const ztcp_paged_batch batch = p.batch(*table, *lens, *starts, n, b[1]);
+    need(!TREE || (mask->dim() == 2 && mask->size(1) > 0), "tree_mask must have shape [rows, words]");
+    const int64_t words = TREE ? mask->size(1) : 0;
+    const void* mask_ptr = TREE ? p.array(*mask, "tree_mask", at::kLong, {n, words}) : nullptr;
+    const at::Tensor out = given ? *given : make(q->sizes(), q->scalar_type(), d);
+    if (given) p.array(out, "out", q->scalar_type(), q->sizes());
+    const at::Tensor lse = want_lse ? make({n, heads}, at::kFloat, d) : at::Tensor();
+    const float scale = scale_of(b[0], k_pages->size(3));
+    const c10::DeviceGuard guard(d);
+    const size_t bytes = TREE ? ztcp_tree_attention_workspace(&batch, &p.pool, &p.g, heads)
+                              : ztcp_paged_attention_workspace(&batch, &p.pool, &p.g, heads);
+    if (bytes == (size_t)-1) done(*ztcp_last_error() ? ZTCP_EINVAL : ZTCP_EHIP, name);
+    // the caching allocator gives it to later work of this stream only
+    const at::Tensor work = bytes ? make({(int64_t)bytes}, at::kByte, d) : at::Tensor();
+    void* work_ptr = bytes ? work.data_ptr() : nullptr;
+    float* lse_ptr = want_lse ? (float*)lse.data_ptr() : nullptr;
+    done(TREE ? ztcp_tree_attention(q->data_ptr(), qs, out.data_ptr(), lse_ptr, heads, &p.pool, &batch, &p.g,
+                                    (const uint64_t*)mask_ptr, words, scale, work_ptr, bytes, stream_of(d))
+              : ztcp_paged_attention(q->data_ptr(), qs, out.data_ptr(), lse_ptr, heads, &p.pool, &batch, &p.g, scale, work_ptr,
+                                     bytes, stream_of(d)),
+         name);
+    written(given);
+    return with_lse(out, want_lse ? &lse : nullptr);
 }
 
 PyObject* attention_mass(PyObject* const* a) {
@@ -396,7 +413,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 #define ZT_FUNCTION(name, n) {#name, (PyCFunction)(void*)entry<name, n>, METH_FASTCALL, nullptr}
-PyMethodDef kMethods[] = {ZT_FUNCTION(append_tokens, 13), ZT_FUNCTION(paged_attention, 10), ZT_FUNCTION(attention_mass, 11),
+PyMethodDef kMethods[] = {ZT_FUNCTION(append_tokens, 13), {"paged_attention", (PyCFunction)(void*)entry<attention<false>, 10>, METH_FASTCALL, nullptr},
+                          {"tree_attention", (PyCFunction)(void*)entry<attention<true>, 11>, METH_FASTCALL, nullptr}, ZT_FUNCTION(attention_mass, 11),
                           ZT_FUNCTION(evict_pages, 8), ZT_FUNCTION(allot_pages, 9), ZT_FUNCTION(release_pages, 6), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_ztcp_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
