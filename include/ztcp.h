@@ -445,6 +445,48 @@ ZTCP_API int ztcp_evict_pages(const float* mass, const int32_t* page_table, int6
                      int32_t* out_table, int64_t out_table_stride, float* out_mass, int32_t* out_lens,
                      int32_t* evicted, int32_t* n_evicted, void* stream);
 
+/* Bounds of pages' keys: bounds [n_pages, 2, num_heads, head_dim] of the hot dtype, pages
+ * bounds_stride elements apart (a multiple of 8, 16-byte aligned), hold for each column
+ * the least and the greatest number of the page's keys.  Written for the pages that hold
+ * new tokens of the batch, over all of a page's tokens up to kv_lens[s]; a page with a
+ * NaN in a column has NaN as both its bounds.  The pool's v is not read and may be NULL;
+ * head_dim at most 1024.  A page that two sequences list has the bounds that one of them
+ * gives it. */
+ZTCP_API int ztcp_page_bounds(const ztcp_page_pool* pool, const ztcp_paged_batch* batch, const ztcp_geometry* g,
+                     void* bounds, int64_t bounds_stride, void* stream);
+
+/* Which pages each new token attends over, for each KV head: `budget` of those that it
+ * sees (page p if p * num_tokens <= kv_lens[s] - n + i, and its entry is a page of the
+ * pool): the first `sink` and the last `recent` (>= 1) of the columns that it sees, and
+ * of the others those with the highest scores.  The score of a page for query head h is
+ *   sum over the columns of max(q, 0) * hi + min(q, 0) * lo
+ * of the page's bounds, which no q . k of the page exceeds, and for a KV head the greatest
+ * of its query heads' scores.  Pages are ranked by their scores in 64 bits; NaN counts as
+ * more than every number, of equal ones the first is taken.
+ *   q as in ztcp_paged_attention; bounds as ztcp_page_bounds writes them, of n_pages pages;
+ *   out [n_rows, num_heads, budget]: columns of the page table, ascending, -1 behind them.
+ * sink + recent <= budget.  Rows that no sequence has are left.  workspace:
+ * ztcp_select_pages_workspace bytes ((size_t)-1 for arguments that the call refuses),
+ * needed until the call's work is done, by one call at a time. */
+ZTCP_API size_t ztcp_select_pages_workspace(const ztcp_paged_batch* batch, int64_t n_pages, const ztcp_geometry* g,
+                                   int64_t q_heads);
+ZTCP_API int ztcp_select_pages(const void* q, int64_t q_stride, int64_t q_heads, const void* bounds,
+                      int64_t bounds_stride, int64_t n_pages, const ztcp_paged_batch* batch,
+                      const ztcp_geometry* g, int64_t budget, int64_t sink, int64_t recent, int32_t* out,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of new tokens over listed pages: as ztcp_paged_attention, but a row's sums
+ * for the query heads of KV head h are over the tokens that it sees of the pages in
+ * columns selected[row, h, 0 .. listed - 1] of its sequence's table row.  Entries outside
+ * the table's columns list nothing; a column listed twice counts twice.
+ * selected [n_rows, num_heads, listed]; listed * num_tokens at most 2^31 - 4096. */
+ZTCP_API size_t ztcp_selected_attention_workspace(const ztcp_paged_batch* batch, const ztcp_page_pool* pool,
+                                         const ztcp_geometry* g, int64_t q_heads, int64_t listed);
+ZTCP_API int ztcp_selected_attention(const void* q, int64_t q_stride, void* out, float* lse, int64_t q_heads,
+                            const ztcp_page_pool* pool, const ztcp_paged_batch* batch,
+                            const ztcp_geometry* g, const int32_t* selected, int64_t listed, float scale,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 /* Pages for a step's new tokens, with the step's row starts, slots and positions,
  * from what the sequences hold and ask for.  With L = kv_lens[s] (cut to
  * 0 .. max_pages * num_tokens) and q = q_lens[s] (negative: 0; 0 too where L + q tokens

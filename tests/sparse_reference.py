@@ -67,3 +67,70 @@ def tree(q, k_pages, v_pages, table, lens, starts, mask, scale):
             for full, part in zip(res, softmax_rows(q[r0:r0 + n, h].double(), k, v, seen, scale, q.dtype)):
                 full[r0:r0 + n, h] = part
     return res
+
+
+def bounds(k_pages, out, table, lens, starts, rows=1 << 30):
+    """``out`` with the bounds of the pages that hold new tokens."""
+    k_pages, out, table, lens, starts = (x.cpu() for x in (k_pages, out.clone(), table, lens, starts))
+    t = k_pages.shape[1]
+    for s in range(lens.numel()):
+        _, n = _rows_of(starts, s, rows)
+        length = min(max(int(lens[s]), 0), table.shape[1] * t)
+        for p in range(max(length - n, 0) // t, -(-length // t)) if n else ():
+            if 0 <= int(table[s, p]) < k_pages.shape[0]:
+                keys = k_pages[int(table[s, p]), :min(t, length - p * t)]
+                out[int(table[s, p]), 0], out[int(table[s, p]), 1] = keys.amin(0), keys.amax(0)   # NaN if there is one
+    return out
+
+
+def select(q, bounds_, table, lens, starts, page_tokens, budget, sink, recent, out):
+    """``out`` with the rows that sequences have."""
+    q, b, table, lens, starts, out = (x.cpu() for x in (q, bounds_, table, lens, starts, out.clone()))
+    rows, heads, _ = q.shape
+    kv = b.shape[2]
+    for s in range(lens.numel()):
+        r0, n = _rows_of(starts, s, rows)
+        length = min(max(int(lens[s]), 0), table.shape[1] * page_tokens)
+        ids = table[s].long()
+        there = (ids >= 0) & (ids < b.shape[0])
+        at = b[torch.where(there, ids, 0)].double()
+        for i in range(n):
+            limit = length - n + i + 1
+            pages = -(-limit // page_tokens) if limit > 0 else 0
+            for h in range(kv):
+                x = q[r0 + i, h * (heads // kv):(h + 1) * (heads // kv)].double()
+                high, low = at[:pages, 1, h], at[:pages, 0, h]
+                sign = torch.signbit(x)   # NaN goes to either side and stays NaN
+                score = (torch.where(sign, 0.0, x)[:, None] * high + torch.where(sign, x, 0.0)[:, None] * low).sum(-1).amax(0).tolist()
+                seen = [p for p in range(pages) if there[p]]
+                always = [p for p in seen if p < sink or p >= pages - recent]
+                rest = sorted((p for p in seen if p not in always),
+                              key=lambda p: (score[p] == score[p], -score[p] if score[p] == score[p] else 0.0, p))
+                chosen = sorted(always + rest[:budget - len(always)])
+                out[r0 + i, h] = torch.tensor(chosen + [-1] * (budget - len(chosen)), dtype=torch.int32)
+    return out
+
+
+def selected(q, k_pages, v_pages, table, lens, starts, picked, scale):
+    """out, lse [rows, heads] and their bounds."""
+    q, k_pages, v_pages, table, lens, starts, picked = (x.cpu() for x in (q, k_pages, v_pages, table, lens, starts, picked))
+    rows, heads, d = q.shape
+    t, kv = k_pages.shape[1:3]
+    g = heads // kv
+    res = _blank(rows, heads, d)
+    for s in range(lens.numel()):
+        r0, n = _rows_of(starts, s, rows)
+        length = min(max(int(lens[s]), 0), table.shape[1] * t)
+        for row in range(r0, r0 + n):
+            limit = length - n + row - r0 + 1
+            for h in range(kv):
+                pages = [p for p in picked[row, h].tolist() if 0 <= p < table.shape[1] and 0 <= int(table[s, p]) < k_pages.shape[0]]
+                where = [(int(table[s, p]), j) for p in pages for j in range(t) if p * t + j < limit]
+                if not where:
+                    continue
+                ids, j = torch.tensor(where).T
+                k, v = (x[ids, j, h].double() for x in (k_pages, v_pages))
+                seen = torch.ones(g, len(where), dtype=torch.bool)
+                for full, part in zip(res, softmax_rows(q[row, h * g:(h + 1) * g].double(), k, v, seen, scale, q.dtype)):
+                    full[row, h * g:(h + 1) * g] = part
+    return res

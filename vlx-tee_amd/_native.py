@@ -32,6 +32,8 @@ EXPORTS = (
     "ztcp_wire_ring_wait", "ztcp_wire_ring_destroy", "ztcp_append_tokens",
     "ztcp_paged_attention_workspace", "ztcp_paged_attention", "ztcp_attention_mass", "ztcp_evict_pages",
     "ztcp_tree_attention_workspace", "ztcp_tree_attention",
+    "ztcp_page_bounds", "ztcp_select_pages_workspace", "ztcp_select_pages",
+    "ztcp_selected_attention_workspace", "ztcp_selected_attention",
     "ztcp_allot_pages_workspace", "ztcp_allot_pages", "ztcp_release_pages_workspace", "ztcp_release_pages",
 )
 
@@ -176,6 +178,16 @@ def lib() -> C.CDLL:
     L.ztcp_tree_attention_workspace.restype = C.c_size_t
     L.ztcp_tree_attention.argtypes = [P, i64, P, P, i64, PP, PB, G, P, i64, f32, P, C.c_size_t, P]
     L.ztcp_tree_attention.restype = i32
+    L.ztcp_page_bounds.argtypes = [PP, PB, G, P, i64, P]
+    L.ztcp_page_bounds.restype = i32
+    L.ztcp_select_pages_workspace.argtypes = [PB, i64, G, i64]
+    L.ztcp_select_pages_workspace.restype = C.c_size_t
+    L.ztcp_select_pages.argtypes = [P, i64, i64, P, i64, i64, PB, G, i64, i64, i64, P, P, C.c_size_t, P]
+    L.ztcp_select_pages.restype = i32
+    L.ztcp_selected_attention_workspace.argtypes = [PB, PP, G, i64, i64]
+    L.ztcp_selected_attention_workspace.restype = C.c_size_t
+    L.ztcp_selected_attention.argtypes = [P, i64, P, P, i64, PP, PB, G, P, i64, f32, P, C.c_size_t, P]
+    L.ztcp_selected_attention.restype = i32
     L.ztcp_allot_pages_workspace.argtypes = [i64]
     L.ztcp_allot_pages_workspace.restype = C.c_size_t
     L.ztcp_allot_pages.argtypes = [P, i64, i64, P, P, i64, P, i64, P, P, i64, i64, P, P, P, P, P, P, P, P, C.c_size_t, P]

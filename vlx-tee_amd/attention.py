@@ -108,6 +108,37 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                                   out)
 
 
+def page_bounds(k_pages: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
+                q_starts: torch.Tensor, *, max_q_len: int | None = None) -> torch.Tensor:
+    """Brings ``bounds`` [n_pages, 2, kv_heads, d] (the pages' dtype) up to date for the pages that hold the step's new
+    tokens: the least and the greatest number of each column of a page's keys, over all of its tokens; NaN where a key's
+    is.  Other pages' bounds are left.  Returns ``bounds``."""
+    return _call().page_bounds(k_pages, bounds, page_table, kv_lens, q_starts, max_q_len)
+
+
+def select_pages(q: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
+                 q_starts: torch.Tensor, *, page_tokens: int, budget: int, sink: int = 1, recent: int = 1,
+                 max_q_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The pages that each new token attends over, for each KV head: [rows, kv_heads, budget] int32 columns of the page
+    table, ascending, -1 behind them.  Of the pages that the token sees its first ``sink`` and last ``recent`` are always
+    taken, and of the others those with the highest scores: for a query head the most that ``q . k`` can be within the
+    page's ``bounds``, the sum of ``max(q, 0) * hi + min(q, 0) * lo``, for a KV head the greatest of its query heads'.
+    Scores count in 64 bits, NaN as more than every number; of equal ones the first page is taken.  Pages that are not
+    there are not taken.  Rows of no sequence keep what ``out`` holds (in one allocated here, anything)."""
+    return _call().select_pages(q, bounds, page_table, kv_lens, q_starts, page_tokens, budget, sink, recent, max_q_len, out)
+
+
+def selected_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                       kv_lens: torch.Tensor, q_starts: torch.Tensor, selected: torch.Tensor, *, scale: float | None = None,
+                       max_q_len: int | None = None, return_lse: bool = False, out: torch.Tensor | None = None):
+    """``paged_attention`` over a part of the pages: a row's query heads of KV head h see, of the tokens that they would
+    see, those of the pages in columns ``selected[row, h]`` ([rows, kv_heads, any number] int32, as ``select_pages`` gives
+    them, in any order).  Entries outside the table's columns list nothing, a column listed twice counts twice.  The
+    log-sum-exp is over what the row sees here."""
+    return _call().selected_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts, selected, scale, max_q_len,
+                                      return_lse, out)
+
+
 def attention_mass(q: torch.Tensor, lse: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor,
                    kv_lens: torch.Tensor, q_starts: torch.Tensor, mass: torch.Tensor, *, scale: float | None = None,
                    decay: float = 1.0, max_q_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:

@@ -246,6 +246,100 @@ PyObject* attention(PyObject* const* a) {
     return with_lse(out, want_lse ? &lse : nullptr);
 }
 
+PyObject* selected_attention(PyObject* const* a) {
+    constexpr const char* name = "selected_attention";
+    need(a[2] != Py_None, name, " needs K and V pages (single-buffer pages have none)");
+    const at::Tensor *q = tensor(a[0], "q"), *k_pages = tensor(a[1], "k_pages"), *v_pages = tensor(a[2], "v_pages");
+    const at::Tensor *table = tensor(a[3], "page_table"), *lens = tensor(a[4], "kv_lens"), *starts = tensor(a[5], "q_starts");
+    const at::Tensor* selected = tensor(a[6], "selected");
+    const bool want_lse = truth(a[9], "return_lse");
+    const at::Tensor* given = tensor_or_none(a[10], "out");
+    const Pool p(k_pages, v_pages, 0);
+    const at::Device d = p.device();
+    const int64_t qs = p.tokens(*q, "q"), n = q->size(0), heads = q->size(1);
+    const ztcp_paged_batch batch = p.batch(*table, *lens, *starts, n, a[8]);
+    need(selected->dim() == 3 && selected->size(2) > 0, "selected must have shape [rows, kv_heads, listed]");
+    const int64_t listed = selected->size(2);
+    const void* selected_ptr = p.array(*selected, "selected", at::kInt, {n, k_pages->size(2), listed});
+    const at::Tensor out = given ? *given : make(q->sizes(), q->scalar_type(), d);
+    if (given) p.array(out, "out", q->scalar_type(), q->sizes());
+    const at::Tensor lse = want_lse ? make({n, heads}, at::kFloat, d) : at::Tensor();
+    const float scale = scale_of(a[7], k_pages->size(3));
+    const c10::DeviceGuard guard(d);
+    const size_t bytes = ztcp_selected_attention_workspace(&batch, &p.pool, &p.g, heads, listed);
+    if (bytes == (size_t)-1) done(*ztcp_last_error() ? ZTCP_EINVAL : ZTCP_EHIP, name);
+    const at::Tensor work = bytes ? make({(int64_t)bytes}, at::kByte, d) : at::Tensor();
+    done(ztcp_selected_attention(q->data_ptr(), qs, out.data_ptr(), want_lse ? (float*)lse.data_ptr() : nullptr, heads, &p.pool,
+                                 &batch, &p.g, (const int32_t*)selected_ptr, listed, scale, bytes ? work.data_ptr() : nullptr,
+                                 bytes, stream_of(d)),
+         name);
+    written(given);
+    return with_lse(out, want_lse ? &lse : nullptr);
+}
+
+// Bounds [n_pages, 2, kv_heads, head_dim], each page's contiguous: elements between pages.
+int64_t bounds_step(const at::Tensor& t) {
+    need(t.dim() == 4 && t.size(1) == 2, "bounds must have shape [n_pages, 2, kv_heads, head_dim]");
+    need(t.is_cuda() && (t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16),
+         "bounds must be a HIP float16 or bfloat16 tensor");
+    const int64_t h = t.size(2), d = t.size(3);
+    need(t.numel() > 0 && (d == 1 || t.stride(3) == 1) && (h == 1 || t.stride(2) == d) && t.stride(1) == h * d,
+         "bounds: each page's must be contiguous");
+    return t.size(0) > 1 ? t.stride(0) : 2 * h * d;
+}
+
+PyObject* page_bounds(PyObject* const* a) {
+    const at::Tensor *k_pages = tensor(a[0], "k_pages"), *bounds = tensor(a[1], "bounds");
+    const at::Tensor *table = tensor(a[2], "page_table"), *lens = tensor(a[3], "kv_lens"), *starts = tensor(a[4], "q_starts");
+    const Pool p(k_pages, nullptr, 0);
+    const at::Device d = p.device();
+    const int64_t step = bounds_step(*bounds);
+    need(bounds->device() == d && bounds->scalar_type() == k_pages->scalar_type() && bounds->size(0) == k_pages->size(0) &&
+             bounds->size(2) == k_pages->size(2) && bounds->size(3) == k_pages->size(3),
+         "bounds must match the pages in number, heads, head_dim, dtype and device");
+    // how many rows there are, the device knows
+    const ztcp_paged_batch batch = p.batch(*table, *lens, *starts, (((int64_t)1 << 31) - 1024) / p.g.num_heads, a[5]);
+    const c10::DeviceGuard guard(d);
+    done(ztcp_page_bounds(&p.pool, &batch, &p.g, bounds->data_ptr(), step, stream_of(d)), "page_bounds");
+    written(bounds);
+    return THPVariable_Wrap(*bounds);
+}
+
+PyObject* select_pages(PyObject* const* a) {
+    const at::Tensor *q = tensor(a[0], "q"), *bounds = tensor(a[1], "bounds");
+    const at::Tensor *table = tensor(a[2], "page_table"), *lens = tensor(a[3], "kv_lens"), *starts = tensor(a[4], "q_starts");
+    const at::Tensor* given = tensor_or_none(a[10], "out");
+    const int64_t tokens = whole(a[5], "page_tokens"), budget = whole(a[6], "budget"), sink = whole(a[7], "sink"),
+                  recent = whole(a[8], "recent"), most = a[9] == Py_None ? 0 : whole(a[9], "max_q_len");
+    need(most >= 0, "max_q_len must not be negative");
+    const int64_t step = bounds_step(*bounds);
+    const at::Device d = bounds->device();
+    const int64_t kv = bounds->size(2), width = bounds->size(3);
+    need(q->dim() == 3 && q->scalar_type() == bounds->scalar_type() && q->device() == d && q->size(2) == width,
+         "q must have shape [tokens, heads, head_dim] and match bounds in dtype, device and head_dim");
+    need(q->numel() == 0 || ((width == 1 || q->stride(2) == 1) && (q->size(1) <= 1 || q->stride(1) == width)),
+         "q: a token's heads must be contiguous");
+    const int64_t n = q->size(0), heads = q->size(1), qs = n > 1 ? q->stride(0) : heads * width;
+    const ztcp_geometry g{tokens, kv, width, 0, q->scalar_type() == at::kBFloat16 ? ZTCP_HOT_BF16 : ZTCP_HOT_FP16, 1};
+    const int64_t stride = Pool::table(*table, d), s = table->size(0);
+    const ztcp_paged_batch batch{(const int32_t*)table->data_ptr(), stride, table->size(1),
+                                 (const int32_t*)Pool::plain(*lens, "kv_lens", at::kInt, {s}, d),
+                                 (const int32_t*)Pool::plain(*starts, "q_starts", at::kInt, {s + 1}, d), s, n, most};
+    need(budget > 0, "budget must be positive");
+    const int64_t shape[3] = {n, kv, budget};
+    if (given) Pool::plain(*given, "out", at::kInt, shape, d);
+    const c10::DeviceGuard guard(d);
+    const size_t bytes = ztcp_select_pages_workspace(&batch, bounds->size(0), &g, heads);
+    if (bytes == (size_t)-1) done(ZTCP_EINVAL, "select_pages");
+    const at::Tensor out = given ? *given : make(shape, at::kInt, d);
+    const at::Tensor work = make({(int64_t)bytes}, at::kByte, d);
+    done(ztcp_select_pages(q->data_ptr(), qs, heads, bounds->data_ptr(), step, bounds->size(0), &batch, &g, budget, sink, recent,
+                           (int32_t*)out.data_ptr(), work.data_ptr(), bytes, stream_of(d)),
+         "select_pages");
+    written(given);
+    return THPVariable_Wrap(out);
+}
+
 PyObject* attention_mass(PyObject* const* a) {
     const at::Tensor *q = tensor(a[0], "q"), *lse = tensor(a[1], "lse"), *k_pages = tensor(a[2], "k_pages");
     const at::Tensor *table = tensor(a[3], "page_table"), *lens = tensor(a[4], "kv_lens"), *starts = tensor(a[5], "q_starts");
@@ -415,7 +509,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 #define ZT_FUNCTION(name, n) {#name, (PyCFunction)(void*)entry<name, n>, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {ZT_FUNCTION(append_tokens, 13), {"paged_attention", (PyCFunction)(void*)entry<attention<false>, 10>, METH_FASTCALL, nullptr},
                           {"tree_attention", (PyCFunction)(void*)entry<attention<true>, 11>, METH_FASTCALL, nullptr}, ZT_FUNCTION(attention_mass, 11),
-                          ZT_FUNCTION(evict_pages, 8), ZT_FUNCTION(allot_pages, 9), ZT_FUNCTION(release_pages, 6), {nullptr, nullptr, 0, nullptr}};
+                          ZT_FUNCTION(evict_pages, 8), ZT_FUNCTION(page_bounds, 6), ZT_FUNCTION(select_pages, 11),
+                          ZT_FUNCTION(selected_attention, 11), ZT_FUNCTION(allot_pages, 9), ZT_FUNCTION(release_pages, 6), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_ztcp_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1034,6 +1034,10 @@ int attend(const void* q, int64_t q_stride, void* out, float* lse, int64_t q_hea
                !rows_overlap(x, 1, bytes, bytes, pool->v, pool->n_pages, page, 2 * pool->v_stride);
     };
     const int64_t out_bytes = 2 * batch->n_rows * row, lse_bytes = lse ? 4 * batch->n_rows * q_heads : 0;
+    constexpr const char* kOverlap = TREE ? "out, lse and workspace must not overlap q, tree_mask, the pages or each other"
+                                          : "out, lse and workspace must not overlap q, the pages or each other";
+    if (!misses(out, out_bytes) || !misses(lse, lse_bytes) || bytes_overlap(out, out_bytes, lse, lse_bytes))
+        return arg_result(ZTCP_EOVERLAP, kOverlap);
     int cus = 0;
     if (cu_count(cus) != ZTCP_OK) return ZTCP_EHIP;
     const Plan plan = plan_call(batch, g, q_heads, cus);
@@ -1041,11 +1045,9 @@ int attend(const void* q, int64_t q_stride, void* out, float* lse, int64_t q_hea
     if (need > 0 && (!workspace || (int64_t)workspace_bytes < need || !hot_aligned(workspace)))
         return arg_result(ZTCP_EINVAL, TREE ? "workspace must hold ztcp_tree_attention_workspace bytes, 16-byte aligned"
                                             : "workspace must hold ztcp_paged_attention_workspace bytes, 16-byte aligned");
-    if (!misses(out, out_bytes) || !misses(lse, lse_bytes) || !misses(need ? workspace : nullptr, need) ||
-        bytes_overlap(out, out_bytes, lse, lse_bytes) || bytes_overlap(workspace, need, out, out_bytes) ||
+    if (!misses(need ? workspace : nullptr, need) || bytes_overlap(workspace, need, out, out_bytes) ||
         bytes_overlap(workspace, need, lse, lse_bytes))
-        return arg_result(ZTCP_EOVERLAP, TREE ? "out, lse and workspace must not overlap q, tree_mask, the pages or each other"
-                                              : "out, lse and workspace must not overlap q, the pages or each other");
+        return arg_result(ZTCP_EOVERLAP, kOverlap);
     const int64_t most = (int64_t)1 << 31, tiles = batch->n_seqs * (p.batch.max_tokens / kFewTile + 1);
     if (g->num_heads * plan.many_units * (kManyRows / kJoinRows) >= most ||
         g->num_heads * batch->n_seqs >= most || tiles >= most)

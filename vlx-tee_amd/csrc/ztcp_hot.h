@@ -205,6 +205,21 @@ __device__ __forceinline__ int find_tile(const PagedView& v, int& tile, F&& tile
     return v.n_seqs;
 }
 
+// The first of n ascending ends that is above x, n if none is; every lane of the wave asks for the same x.
+__device__ __forceinline__ int find_above(const int32_t* ends, int n, int x) {
+    const int lane = (int)threadIdx.x & 63;
+    int low = 0, high = n;                                    // it is in low .. high
+    while (low < high) {
+        const int step = (high - low - 1) / 64 + 1, at = low + (lane + 1) * step - 1;
+        const uint64_t past = __ballot(at >= high || ends[at] > x);
+        if (past == 0) return high;
+        const int first = __ffsll((unsigned long long)past) - 1;
+        high = min(low + (first + 1) * step - 1, high);
+        low += first * step;
+    }
+    return low;
+}
+
 // Where token `key` (below `stop`) is: its page, -1 if there is none, and its row in the page.
 struct Place {
     int page, row;

@@ -162,21 +162,6 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(AllotParams p) {
     }
 }
 
-// The first s with starts[s + 1] > row (there is one), all lanes of the wave asking for the same row.
-__device__ __forceinline__ int find_row(const int32_t* starts, int n_seqs, int row) {
-    const int lane = (int)threadIdx.x & 63;
-    int low = 0, high = n_seqs - 1;                          // it is in low .. high
-    while (low < high) {
-        const int step = (high - low) / 64 + 1, at = min(low + (lane + 1) * step - 1, high);
-        const uint64_t past = __ballot(starts[at + 1] > row);
-        const int first = __ffsll((unsigned long long)past) - 1;
-        const int new_low = low + first * step;
-        high = min(new_low + step - 1, high);
-        low = new_low;
-    }
-    return low;
-}
-
 constexpr int kRowsABlock = 1024;
 
 __global__ __launch_bounds__(256) void rows_kernel(AllotParams p) {
@@ -184,8 +169,8 @@ __global__ __launch_bounds__(256) void rows_kernel(AllotParams p) {
     const int total = p.starts[p.n_seqs], had = *p.had;
     int low0 = 0, high0 = 0;
     if (row0 < total) {
-        low0 = find_row(p.starts, p.n_seqs, (int)row0);
-        high0 = find_row(p.starts, p.n_seqs, (int)min(row0 + kRowsABlock, (int64_t)total) - 1);
+        low0 = find_above(p.starts + 1, p.n_seqs, (int)row0);
+        high0 = find_above(p.starts + 1, p.n_seqs, (int)min(row0 + kRowsABlock, (int64_t)total) - 1);
     }
 #pragma unroll
     for (int i = 0; i < kRowsABlock / 256; ++i) {
