@@ -99,7 +99,8 @@ def test_tree(A, lens, kv, group, d, t, dtype):
 
 
 def test_a_line_is_paged_attention(A):
-    """A tree without branches is a chunk: the results are those of paged_attention, bit for bit."""
+    """A tree without branches is a chunk: the results are those of paged_attention.  The two may cut the tokens into other
+    pieces, so each may be off by the formula's bound."""
     _say("tree as a line")
     for lens in ([(6, 500), (3, 20)], [(70, 900), (12, 12)]):
         c = _case(lens, 2, 4, 128, 16, BF)
@@ -110,7 +111,9 @@ def test_a_line_is_paged_attention(A):
                 c["mask"][int(c["starts"][s]) + i] = torch.tensor([x - 2 ** 64 if x >= 2 ** 63 else x for x in words])
         out, lse = _run(A, c)
         want = A.paged_attention(c["q"], c["k"], c["v"], c["table"], c["lens"], c["starts"], return_lse=True)
-        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        _, _, out_tol, lse_tol = R.tree(c["q"], c["k"], c["v"], c["table"], c["lens"], c["starts"], c["mask"], 128 ** -0.5)
+        _close(out, want[0].cpu().double(), 2 * out_tol, ("line", "out"))
+        _close(lse, want[1].cpu().double(), 2 * lse_tol, ("line", "lse"))
 
 
 def test_masks_that_leave_nothing(A):

@@ -482,6 +482,37 @@ __device__ __forceinline__ Cut cut_of(const AttendParams& p) {
     return Cut{n, ((longest + n - 1) / n + 127) / 128 * 128};
 }
 
+// A tree's rows are few blocks over contexts of any length, and a workgroup for each of these would leave the longest
+// one to itself: pieces of equal work instead, as many in all as the card holds at once beside one for each block, of
+// 128 tokens at least, laid out sequence behind sequence.  Drafts of 24 to 64 tokens of 32 sequences of 500 to 8,192
+// tokens: 257 us with a workgroup for each block, 174 now (half as many pieces 192 us, twice as many 182); a draft of 37
+// over 1,501: 32 us in pieces of 512 tokens, 22 now.
+constexpr int kTreePiece = 128;
+__device__ __forceinline__ int blocks_of(const AttendParams& p, const Seq& q) {
+    const int rows = q.n_new * p.group;
+    return rows > p.few_rows ? (rows + kManyRows - 1) / kManyRows : 0;
+}
+__device__ __forceinline__ Cut tree_cut(const AttendParams& p) {
+    if (p.splits == 1) return Cut{1, p.batch.max_tokens};
+    const int lane = (int)threadIdx.x & 63;
+    int64_t work = 0;                                         // tokens of all blocks
+    int longest = 1;
+    for (int base = 0; base < p.batch.n_seqs; base += 64) {
+        if (base + lane >= p.batch.n_seqs) continue;
+        const Seq q = seq_of(p.batch, base + lane);
+        const int blocks = blocks_of(p, q);
+        work += (int64_t)blocks * q.len;
+        if (blocks > 0) longest = max(longest, q.len);
+    }
+    for (int m = 1; m < 64; m <<= 1) {
+        work += (int64_t)__shfl_xor((long long)work, m);
+        longest = max(longest, __shfl_xor(longest, m));
+    }
+    const int64_t share = work * p.kv_heads * 2 / (3 * (int64_t)p.resident), least = ((int64_t)longest + p.splits - 1) / p.splits;
+    const int64_t tokens = max(max(share, least), (int64_t)1);
+    return Cut{p.splits, uniform((int)((tokens + kTreePiece - 1) / kTreePiece * kTreePiece))};
+}
+
 // Zeros that the tile loads read in the place of tokens that are not there: a row of 256 elements.
 __device__ __attribute__((aligned(16))) uint32_t g_zeros[128];
 
@@ -502,11 +533,20 @@ void many_kernel(AttendParams p) {
     const uint32_t unit = p.first_block + blockIdx.x;
     const int head = (int)(unit % (uint32_t)p.kv_heads);
     const uint32_t rest = unit / (uint32_t)p.kv_heads;
-    const Cut cut = cut_of(p);
+    const Cut cut = TREE ? tree_cut(p) : cut_of(p);
     if (unit == 0 && threadIdx.x == 0 && p.splits > 1) p.cut[0] = cut.n, p.cut[1] = cut.tokens;
-    const int split = (int)(rest % (uint32_t)cut.n);
+    int split = (int)(rest % (uint32_t)cut.n);
     int s, block;
-    if (!find_unit(p, (int)(rest / (uint32_t)cut.n), s, block)) return;
+    if constexpr (TREE) {
+        int at = (int)rest;
+        s = find_tile(p.batch, at, [&](const Seq& q) { return blocks_of(p, q) * pieces_of(q.len, cut.tokens); });
+        if (s >= p.batch.n_seqs) return;
+        const int pieces = pieces_of(seq_of(p.batch, s).len, cut.tokens);
+        split = uniform(at % pieces);
+        block = at / pieces;
+    } else {
+        if (!find_unit(p, (int)(rest / (uint32_t)cut.n), s, block)) return;
+    }
     s = uniform(s);
     block = uniform(block);
     const Seq seq = uniform(seq_of(p.batch, s));
@@ -793,7 +833,7 @@ void many_kernel(AttendParams p) {
     if (r >= rows) return;
     const int64_t row_head = (int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head;
     const float base = m == -INFINITY ? 0.f : m;
-    if (cut.n > 1) {
+    if (TREE ? pieces_of(seq.len, cut.tokens) > 1 : cut.n > 1) {
         float* dst = many_partial(p, seq.row0 + token, q_head, split);
 #pragma unroll
         for (int n = 0; n < DP / 32; ++n)
@@ -880,7 +920,7 @@ __global__ __launch_bounds__(256) void join_few_kernel(AttendParams p, int most_
 // took 60 us where their attention had taken 40.
 constexpr int kJoinRows = 8;
 
-template <int DT>
+template <int DT, bool TREE>
 __global__ __launch_bounds__(256) void join_many_kernel(AttendParams p) {
     const int wave = (int)threadIdx.x >> 6;
     const uint32_t unit = p.first_block + blockIdx.x;
@@ -891,6 +931,7 @@ __global__ __launch_bounds__(256) void join_many_kernel(AttendParams p) {
     if (cut.n == 1 || !find_unit(p, (int)(rest / (kManyRows / kJoinRows)), s, block)) return;
     const Seq seq = seq_of(p.batch, s);
     const int rows = seq.n_new * p.group, n = pieces_of(seq.len, cut.tokens);
+    if (TREE && n == 1) return;
     const int r0 = block * kManyRows + (int)(rest % (kManyRows / kJoinRows)) * kJoinRows;
     for (int r = r0 + wave; r < min(rows, r0 + kJoinRows); r += 4) {
         const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
@@ -915,7 +956,7 @@ struct Plan {
     int64_t workspace;              // floats
 };
 
-Plan plan_call(const ztcp_paged_batch* b, const ztcp_geometry* g, int64_t q_heads, int cus) {
+Plan plan_call(const ztcp_paged_batch* b, const ztcp_geometry* g, int64_t q_heads, int cus, bool tree) {
     Plan plan{};
     const int64_t heads = g->num_heads, group = q_heads / heads, piece = g->head_dim + 2;
     const int64_t most_q = b->max_q_len > 0 && b->max_q_len < b->n_rows ? b->max_q_len : b->n_rows;
@@ -946,11 +987,17 @@ Plan plan_call(const ztcp_paged_batch* b, const ztcp_geometry* g, int64_t q_head
         const int64_t blocks = (b->n_rows * group + kManyRows - 1) / kManyRows * heads, most = (max_tokens + 511) / 512;
         int64_t n = plan.resident / blocks;
         n = n < most ? n : most;
+        if (tree) {   // up to twice what fills the card, and as the longest of many contexts 8
+            n = 2 * plan.resident / blocks;
+            n = n > 8 ? n : 8;
+            n = n < (max_tokens + kTreePiece - 1) / kTreePiece ? n : (max_tokens + kTreePiece - 1) / kTreePiece;
+        }
         n = n < 64 ? n : 64;
         plan.splits = (int)(n > 1 ? n : 1);
         plan.many_groups = plan.many_units * heads;
+        if (tree && plan.splits > 1) plan.many_groups += (2 * plan.resident + heads - 1) / heads * heads;
         const int64_t pieces = (plan.resident + heads - 1) / heads * heads;
-        if (plan.splits > 1 && plan.many_groups < pieces) plan.many_groups = pieces;
+        if (!tree && plan.splits > 1 && plan.many_groups < pieces) plan.many_groups = pieces;
         const int64_t need = plan.splits > 1 ? b->n_rows * q_heads * plan.splits * piece + kCutFloats : 0;
         plan.workspace = need > plan.workspace ? need : plan.workspace;
     }
@@ -985,7 +1032,7 @@ void launch(const AttendParams& base, const Plan& plan, float* workspace, hipStr
         launch_blocks(even ? many_kernel<DT, DP, true, TREE> : many_kernel<DT, DP, false, TREE>, (uint64_t)plan.many_groups, 256, 0,
                       stream, p);
         if (p.splits > 1)
-            launch_blocks(join_many_kernel<DT>, (uint64_t)units * (kManyRows / kJoinRows), 256, 0, stream, p);
+            launch_blocks(join_many_kernel<DT, TREE>, (uint64_t)units * (kManyRows / kJoinRows), 256, 0, stream, p);
     }
 }
 
@@ -995,7 +1042,7 @@ const char* check_all(const ztcp_paged_batch* b, const ztcp_page_pool* pool, con
     return check_batch(b, pool, g, q_heads, view);
 }
 
-size_t workspace_of(const ztcp_paged_batch* batch, const ztcp_page_pool* pool, const ztcp_geometry* g, int64_t q_heads) {
+size_t workspace_of(const ztcp_paged_batch* batch, const ztcp_page_pool* pool, const ztcp_geometry* g, int64_t q_heads, bool tree) {
     arg_result(ZTCP_OK, "");
     PagedView view;
     if (const char* why = check_all(batch, pool, g, q_heads, view)) {
@@ -1004,7 +1051,7 @@ size_t workspace_of(const ztcp_paged_batch* batch, const ztcp_page_pool* pool, c
     }
     int cus = 0;
     if (cu_count(cus) != ZTCP_OK) return (size_t)-1;
-    const Plan plan = plan_call(batch, g, q_heads, cus);
+    const Plan plan = plan_call(batch, g, q_heads, cus, tree);
     return (size_t)plan.workspace * sizeof(float);
 }
 
@@ -1040,7 +1087,7 @@ int attend(const void* q, int64_t q_stride, void* out, float* lse, int64_t q_hea
         return arg_result(ZTCP_EOVERLAP, kOverlap);
     int cus = 0;
     if (cu_count(cus) != ZTCP_OK) return ZTCP_EHIP;
-    const Plan plan = plan_call(batch, g, q_heads, cus);
+    const Plan plan = plan_call(batch, g, q_heads, cus, TREE);
     const int64_t need = plan.workspace * (int64_t)sizeof(float);
     if (need > 0 && (!workspace || (int64_t)workspace_bytes < need || !hot_aligned(workspace)))
         return arg_result(ZTCP_EINVAL, TREE ? "workspace must hold ztcp_tree_attention_workspace bytes, 16-byte aligned"

@@ -5,7 +5,7 @@
 
 extern "C" size_t ztcp_tree_attention_workspace(const ztcp_paged_batch* batch, const ztcp_page_pool* pool,
                                                 const ztcp_geometry* g, int64_t q_heads) {
-    return workspace_of(batch, pool, g, q_heads);
+    return workspace_of(batch, pool, g, q_heads, true);
 }
 
 extern "C" int ztcp_tree_attention(const void* q, int64_t q_stride, void* out, float* lse, int64_t q_heads,
