@@ -594,7 +594,7 @@ void many_kernel(AttendParams p) {
     };
     auto fetch = [&](int kb) {
         const int key = kb + (lane & (kTile - 1));
-        return key < stop ? seq.table[div_page(key, p.batch.page_div)] : -1;
+        return key < stop ? seq.entry(div_page(key, p.batch.page_div)) : -1;
     };
     auto where = [&](int entry, int kb) {
         const int key = kb + (lane & (kTile - 1));

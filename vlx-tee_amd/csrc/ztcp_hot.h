@@ -149,6 +149,9 @@ __device__ __forceinline__ int div_page(int x, DivBy d) { return (int)(((uint64_
 struct Seq {
     int row0, n_new, len;
     const int32_t* table;
+    // Of global memory: the compiler, which has lost sight of that, would take a load that may be of LDS too, and a wait
+    // for any LDS read behind it would wait for the entry, and for the loads in front of it.
+    __device__ __forceinline__ int entry(int at) const { return ((const __attribute__((address_space(1))) int32_t*)table)[at]; }
 };
 __device__ __forceinline__ Seq uniform(Seq q) {
     return Seq{uniform(q.row0), uniform(q.n_new), uniform(q.len), uniform(q.table)};
@@ -228,7 +231,7 @@ __device__ __forceinline__ Place place_of(const PagedView& v, const Seq& q, int 
     Place p{-1, 0};
     if (key < stop) {
         const int at = div_page(key, v.page_div);
-        const int id = q.table[at];
+        const int id = q.entry(at);
         if (id >= 0 && id < v.n_pages) p.page = id;
         p.row = key - at * v.page_tokens;
     }

@@ -141,7 +141,7 @@ void mass_few_kernel(MassParams p) {
         int entry = -1;                                       // of key lane % 32 of the wave's share of the block to be loaded
         auto look_up = [&](int kb) {
             const int key = kb + 32 * wave + (lane & 31);
-            return key < key_end ? seq.table[div_page(key, p.batch.page_div)] : -1;
+            return key < key_end ? seq.entry(div_page(key, p.batch.page_div)) : -1;
         };
         auto load = [&](int kb) {
             const int key = kb + 32 * wave + (lane & 31);

@@ -57,7 +57,7 @@ __device__ __forceinline__ void bounds_of(const BoundsParams& p, int64_t run0, i
             const int tokens = min(p.batch.page_tokens, seq.len - first);
             const bool mine = row == seq.row0 || place == first;
             row += p.batch.page_tokens - (place - first);         // the next page's first token
-            const int id = seq.table[at];
+            const int id = seq.entry(at);
             if (!mine || id < 0 || id >= p.batch.n_pages) continue;
             const uint8_t* src = p.k_pool + 2 * ((int64_t)id * p.k_page + column);
             float lo[8], hi[8];
@@ -115,9 +115,15 @@ __global__ __launch_bounds__(256) void bounds_kernel(BoundsParams p) {
 }
 // ---- scores -----------------------------------------------------------------------
 // In fp32: pages are the rows of the products, (token, query head) pairs their columns,
-// as many heads to a token as leave no column idle.  A wave keeps 16 pages' bounds of one
-// KV head in registers and goes over a block of its sequence's new tokens; the greatest
+// as many heads to a token as leave no column idle.  A unit is 64 pages of a sequence,
+// 16 a wave, and a block of its new tokens; units lie sequence behind sequence, and the
+// workgroups of a KV head take equal shares of them, with the loads of the next unit's
+// bounds, by whole rows through LDS of the wave's own, in flight meanwhile.  The greatest
 // score of the KV head's query heads is what counts.
+//
+// 32 sequences of 512 to 8,192 pages, 4 query heads to each of 8 KV heads of 128 (375 MB
+// of bounds): 114 us a workgroup for each unit and bounds as the products want them, 84
+// now, of which the loads alone take 74 and all else alone 41.
 
 constexpr int kTilePages = 64;      // of a workgroup
 constexpr int kBlockTokens = 64;
@@ -132,6 +138,8 @@ struct SelectParams {
     int32_t budget, sink, recent;
     int32_t score_stride, tops;      // floats of a row's scores (a multiple of 4), of a sequence's tops for a head
     float* scores;                   // [rows, kv_heads, score_stride]; NaN: no finite number
+    int32_t score_groups;            // score kernel: workgroups of a KV head
+    int32_t few_pages;               // pick kernel: rows of at most so many pages are another kernel's
     float* top;                      // [n_seqs, kv_heads, tops]: the greatest bound of 16 pages, by magnitude
     int32_t* out;
     uint32_t first_block;
@@ -143,90 +151,197 @@ __device__ __forceinline__ int pages_seen(const SelectParams& p, const Seq& q, i
     return limit > 0 ? div_page(limit - 1, p.batch.page_div) + 1 : 0;
 }
 
+// The greatest of the 16 lanes of a row, or of as many of them as an aligned 2^log are; a lane's partners by DPP.
+template <int CTRL>
+__device__ __forceinline__ float partner(float x) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float row_max(float x, int log) {
+    if (log > 0) x = fmaxf(x, partner<0xB1>(x));              // lane ^ 1
+    if (log > 1) x = fmaxf(x, partner<0x4E>(x));              // lane ^ 2
+    if (log > 2) x = fmaxf(x, partner<0x141>(x));             // 7 - lane, within 8
+    if (log > 3) x = fmaxf(x, partner<0x140>(x));             // 15 - lane
+    return x;
+}
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
 template <int DT, int DP>
 __global__ __launch_bounds__(256) void score_kernel(SelectParams p) {
-    constexpr int kSteps = DP / 32;
+    constexpr int kSteps = DP / 32, kChunks = DP / 8;         // products of depth 32; 16-byte pieces of a row
+    constexpr int kLoadRows = 64 / kChunks, kLoads = 16 / kLoadRows;   // rows of a load; loads of 16 pages' lower, or upper, bounds
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4][32 * DP * 2];
     const int lane = (int)threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, quad = lane >> 4;
-    const uint32_t unit = p.first_block + blockIdx.x;
-    const int head = (int)(unit % (uint32_t)p.kv_heads);
-    int tile = (int)(unit / (uint32_t)p.kv_heads);
+    const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads), group = (int)(blockIdx.x / (uint32_t)p.kv_heads);
     auto tiles_of = [&](const Seq& q) { return (pages_seen(p, q, q.n_new) + kTilePages - 1) / kTilePages; };
-    auto units_of = [&](const Seq& q) { return q.n_new > 0 ? tiles_of(q) * ((q.n_new - 1) / kBlockTokens + 1) : 0; };
-    const int s = uniform(find_tile(p.batch, tile, units_of));
-    if (s >= p.batch.n_seqs) return;
-    const Seq seq = uniform(seq_of(p.batch, s));
-    const int n_tiles = tiles_of(seq);
-    if (tile < 0 || tile >= units_of(seq)) return;            // (starts that do not ascend)
-    const int block = uniform(tile / n_tiles);
-    const int page0 = uniform(tile % n_tiles) * kTilePages + wave * 16;
-    const int token0 = block * kBlockTokens, tokens = min(seq.n_new - token0, kBlockTokens);
-    if (page0 >= pages_seen(p, seq, token0 + tokens)) return;
-
-    uint4 lo[kSteps], hi[kSteps];
-    {
-        const int at = page0 + col;
-        const int id = at < pages_seen(p, seq, seq.n_new) ? seq.table[at] : -1;
-        const bool there = id >= 0 && id < p.batch.n_pages;
-        const uint8_t* src = p.bounds + 2 * ((int64_t)(there ? id : 0) * p.bounds_page + (int64_t)head * p.head_dim);
-        const int64_t step = 2 * (int64_t)p.kv_heads * p.head_dim;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            const int d = 32 * i + 8 * quad;
-            const bool has = there && d < p.head_dim;
-            lo[i] = has ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
-            hi[i] = has ? ldg16(src + step + 2 * d) : make_uint4(0, 0, 0, 0);
+    auto blocks_of = [&](const Seq& q) { return q.n_new > 0 ? (q.n_new - 1) / kBlockTokens + 1 : 0; };
+    auto units_of = [&](const Seq& q) { return tiles_of(q) * blocks_of(q); };
+    struct Unit {
+        int s, tile, block, tiles, pages;
+        Seq seq;
+    };
+    int none;
+    const int total = uniform(count_tiles(p.batch, 0, none, units_of));
+    const int quota = (total + p.score_groups - 1) / p.score_groups;
+    if ((int64_t)group * quota >= total) return;
+    int first = group * quota;
+    int left = min(quota, total - first);
+    auto open = [&](Unit& u) {       // u.s's sequence, or the next one that has units
+        for (; u.s < p.batch.n_seqs; ++u.s) {
+            u.seq = uniform(seq_of(p.batch, u.s));
+            u.pages = uniform(pages_seen(p, u.seq, u.seq.n_new));
+            u.tiles = (u.pages + kTilePages - 1) / kTilePages;
+            if (u.seq.n_new > 0 && u.tiles > 0) return;
         }
-    }
-    if (token0 + tokens == seq.n_new) {   // the block that sees every page
-        uint32_t most = 0;
+    };
+    auto advance = [&](Unit& u) {
+        if (++u.tile < u.tiles) return;
+        u.tile = 0;
+        if (++u.block < blocks_of(u.seq)) return;
+        u.block = 0;
+        ++u.s;
+        open(u);
+    };
+    auto ids = [&](const Unit& u) {  // of page lane % 16 of this wave's, as it was read; looked at when it is loaded from
+        const int at = u.tile * kTilePages + wave * 16 + col;
+        return u.s < p.batch.n_seqs && at < u.pages ? u.seq.entry(at) : -1;
+    };
+    uint8_t* mine = lds[wave];
+    auto swizzle = [](int row, int chunk) { return chunk ^ (row & (kChunks < 16 ? kChunks - 1 : 15)); };
+    const int load_row = lane / kChunks, load_chunk = lane % kChunks;
+    const int64_t upper = 2 * (int64_t)p.kv_heads * p.head_dim, in_page = 2 * ((int64_t)head * p.head_dim + 8 * load_chunk);
+    uint4 raw[2][kLoads];
+    uint32_t there = 0;              // of this lane's loads: what they bring counts (a look at it here would wait for them)
+    auto load = [&](int id, bool once) {
+        const uint8_t* src[kLoads];
+        there = 0;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            const uint32_t w[8] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w, hi[i].x, hi[i].y, hi[i].z, hi[i].w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) most = max(most, max(w[j] & 0x7FFFu, w[j] >> 16 & 0x7FFFu));
+        for (int i = 0; i < kLoads; ++i) {
+            const int from = __shfl(id, i * kLoadRows + load_row);
+            const bool has = (uint32_t)from < (uint32_t)p.batch.n_pages && load_chunk * 8 < p.head_dim;
+            src[i] = p.bounds + 2 * ((int64_t)(has ? from : 0) * p.bounds_page) + (has ? in_page : 0);
+            there |= has ? 1u << i : 0u;
         }
-        for (int m = 1; m < 64; m <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, m));
-        if (lane == 0) p.top[((int64_t)s * p.kv_heads + head) * p.tops + page0 / 16] = hot_lo<DT>(most);
-    }
-    int heads_log = 4;                    // 2^heads_log heads and 2^(4 - heads_log) tokens are the 16 columns
-    while (heads_log > 0 && tokens > 16 >> heads_log) --heads_log;
-    const int heads = 1 << heads_log, token_step = 16 >> heads_log;
-    const int col_token = col >> heads_log, col_head = col & (heads - 1);
-    for (int t0 = 0; t0 < tokens; t0 += token_step) {
-        const int token = token0 + min(t0 + col_token, tokens - 1);
-        const uint8_t* row = p.q + 2 * ((int64_t)(seq.row0 + token) * p.q_stride + (int64_t)head * p.group * p.head_dim);
-        float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        for (int h0 = 0; h0 < p.group; h0 += heads) {
-            const uint8_t* src = row + 2 * (int64_t)min(h0 + col_head, p.group - 1) * p.head_dim;
-            uint4 x[kSteps];
+        if (once) {
+#pragma unroll
+            for (int i = 0; i < 2 * kLoads; ++i) raw[i % 2][i / 2] = ldg16_once(src[i / 2] + i % 2 * upper);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2 * kLoads; ++i) raw[i % 2][i / 2] = ldg16(src[i / 2] + i % 2 * upper);
+        }
+    };
+    Unit unit;
+    unit.s = uniform(find_tile(p.batch, first, units_of));
+    if (unit.s >= p.batch.n_seqs) return;
+    open(unit);
+    unit.block = uniform(first) / unit.tiles;
+    unit.tile = uniform(first) - unit.block * unit.tiles;
+    if (unit.s >= p.batch.n_seqs || unit.block >= blocks_of(unit.seq)) return;   // (starts that do not ascend)
+    load(ids(unit), unit.seq.n_new <= kBlockTokens);
+    Unit next = unit;
+    advance(next);
+    int next_ids = ids(next);
+    uint4 neg[kSteps], pos[kSteps];                           // columns of a product
+    int have = -1;                                            // whose: the sequence's, if it has one product only
+    for (; left > 0 && unit.s < p.batch.n_seqs; --left) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int row = i * kLoadRows + load_row;
+                *reinterpret_cast<uint4*>(mine + (16 * u + row) * DP * 2 + swizzle(row, load_chunk) * 16) =
+                    there >> i & 1 ? raw[u][i] : make_uint4(0, 0, 0, 0);
+            }
+        const Seq seq = unit.seq;
+        const int s = unit.s, page0 = unit.tile * kTilePages + wave * 16, token0 = unit.block * kBlockTokens;
+        const int tokens = min(seq.n_new - token0, kBlockTokens);
+        const bool last_block = token0 + tokens == seq.n_new;
+        const int pages = last_block ? unit.pages : pages_seen(p, seq, token0 + tokens);
+        int heads_log = 4;                    // 2^heads_log heads and 2^(4 - heads_log) tokens are the 16 columns
+        while (heads_log > 0 && tokens > 16 >> heads_log) --heads_log;
+        const int heads = 1 << heads_log, token_step = 16 >> heads_log;
+        const int col_token = col >> heads_log, col_head = col & (heads - 1);
+        uint4 x[kSteps];
+        auto load_q = [&](int t0, int h0) {
+            const int token = token0 + min(t0 + col_token, tokens - 1), h = min(h0 + col_head, p.group - 1);
+            const uint8_t* src = p.q + 2 * ((int64_t)(seq.row0 + token) * p.q_stride + ((int64_t)head * p.group + h) * p.head_dim);
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 const int d = 32 * i + 8 * quad;
                 x[i] = d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
             }
-            f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+        };
+        auto split = [&]() {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-                uint32_t neg[4];
+                uint32_t n[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) neg[j] = w[j] & ((w[j] >> 15 & 0x00010001u) * 0xFFFFu);
-                sc = mfma16<DT>(lo[i], make_uint4(neg[0], neg[1], neg[2], neg[3]), sc);
-                sc = mfma16<DT>(hi[i], make_uint4(w[0] ^ neg[0], w[1] ^ neg[1], w[2] ^ neg[2], w[3] ^ neg[3]), sc);
+                for (int j = 0; j < 4; ++j) n[j] = w[j] & ((w[j] >> 15 & 0x00010001u) * 0xFFFFu);
+                neg[i] = make_uint4(n[0], n[1], n[2], n[3]);
+                pos[i] = make_uint4(w[0] ^ n[0], w[1] ^ n[1], w[2] ^ n[2], w[3] ^ n[3]);
             }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) best[e] = fmaxf(best[e], fabsf(sc[e]) < INFINITY ? sc[e] : INFINITY);
+        };
+        const bool one = tokens <= token_step && p.group <= heads && seq.n_new == tokens;
+        const bool keeps = one && have == s;
+        if (!keeps) load_q(0, 0);             // ahead of the next unit's bounds, which a wait for it would include
+        if (left > 1) load(next_ids, next.seq.n_new <= kBlockTokens);
+        unit = next;
+        if (left > 1) {
+            advance(next);
+            next_ids = ids(next);
         }
-        for (int m = 1; m < heads; m <<= 1)
+        if (page0 >= pages) continue;
+        uint4 lo[kSteps], hi[kSteps];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) best[e] = fmaxf(best[e], __shfl_xor(best[e], m));
-        const int at = page0 + 4 * quad;
-        if (col_head == 0 && t0 + col_token < tokens && at < p.score_stride) {
-            float* dst = p.scores + ((int64_t)(seq.row0 + token) * p.kv_heads + head) * p.score_stride + at;
+        for (int i = 0; i < kSteps; ++i) {
+            lo[i] = *reinterpret_cast<const uint4*>(mine + col * DP * 2 + swizzle(col, 4 * i + quad) * 16);
+            hi[i] = *reinterpret_cast<const uint4*>(mine + (16 + col) * DP * 2 + swizzle(col, 4 * i + quad) * 16);
+        }
+        if (last_block) {                     // it sees every page
+            u16x2 most = {0, 0};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) best[e] = best[e] < INFINITY ? best[e] : NAN;
-            *reinterpret_cast<float4*>(dst) = make_float4(best[0], best[1], best[2], best[3]);
+            for (int i = 0; i < kSteps; ++i) {
+                const uint32_t w[8] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w, hi[i].x, hi[i].y, hi[i].z, hi[i].w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[j] & 0x7FFF7FFFu));
+            }
+            // numbers of one sign are ordered as their bits are; NaN is above infinity
+            float top = __int_as_float((int)max((uint32_t)most.x, (uint32_t)most.y) << 8);
+            top = row_max(top, 4);
+            const int all = max(max(__builtin_amdgcn_readlane(__float_as_int(top), 0), __builtin_amdgcn_readlane(__float_as_int(top), 16)),
+                                max(__builtin_amdgcn_readlane(__float_as_int(top), 32), __builtin_amdgcn_readlane(__float_as_int(top), 48)));
+            if (lane == 0) p.top[((int64_t)s * p.kv_heads + head) * p.tops + page0 / 16] = hot_lo<DT>((uint32_t)all >> 8);
+        }
+        for (int t0 = 0; t0 < tokens; t0 += token_step) {
+            float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            for (int h0 = 0; h0 < p.group; h0 += heads) {
+                if (!keeps) split();
+                have = one ? s : -1;
+                const bool same_tokens = h0 + heads < p.group;
+                if (same_tokens || t0 + token_step < tokens) load_q(same_tokens ? t0 : t0 + token_step, same_tokens ? h0 + heads : 0);
+                f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    sc = mfma16<DT>(lo[i], neg[i], sc);
+                    sc = mfma16<DT>(hi[i], pos[i], sc);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) best[e] = fmaxf(best[e], fabsf(sc[e]) < INFINITY ? sc[e] : INFINITY);
+            }
+            // (columns behind the group's heads repeat its last one)
+            const int log = p.group <= 1 ? 0 : min(heads_log, 32 - __clz(p.group - 1));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) best[e] = row_max(best[e], log);
+            const int at = page0 + 4 * quad;
+            if (col_head == 0 && t0 + col_token < tokens && at < p.score_stride) {
+                const int token = token0 + t0 + col_token;
+                float* dst = p.scores + ((int64_t)(seq.row0 + token) * p.kv_heads + head) * p.score_stride + at;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) best[e] = best[e] < INFINITY ? best[e] : NAN;
+                *reinterpret_cast<float4*>(dst) = make_float4(best[0], best[1], best[2], best[3]);
+            }
         }
     }
 }
@@ -257,30 +372,96 @@ __device__ __forceinline__ uint64_t order_of(double x) {
     return b >> 63 ? ~b : b | 1ull << 63;
 }
 
-struct PickShared {
-    int bins[kBins];
-    uint64_t few[kFew];
-    int few_page[kFew];
-    uint64_t ends[2][4];
-    int scan[4];
-    float sums[2][4];
-    int found[3], n_few;
-    uint64_t kth;
+struct PickSums {
+    uint32_t least, most;            // keys of open pages
+    int forced, open, unknown;       // pages
+    float sum, top;                  // |q|_1, the greatest bound
 };
 
-__device__ __forceinline__ int block_total(int x, int* lds) {
-    for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m);
+template <int THREADS>
+struct PickShared {
+    static constexpr int kThreads = THREADS, kWaves = THREADS / 64;
+    int bins[kBins];
+    uint64_t few[THREADS];
+    int few_page[kFew];
+    uint64_t ends[2][kWaves];
+    int scan[kWaves];
+    PickSums sums[kWaves];
+    int found[3], n_few, n_near;
+    uint32_t kth;
+};
+
+// The bin where a count from bin 0 on reaches `left`: its number, what lies in the bins before it, what is in it.
+template <class Shared>
+__device__ __forceinline__ void find_bin(Shared& sh, int left) {
+    constexpr int kOwn = kBins / Shared::kThreads;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int of[kOwn], own = 0;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) own += of[j] = sh.bins[kOwn * tid + j];
+    int x = own;
+    for (int m = 1; m < 64; m <<= 1) {
+        const int y = __shfl_up(x, m);
+        x += lane >= m ? y : 0;
+    }
+    if (lane == 63) sh.scan[wave] = x;
     __syncthreads();
-    if ((threadIdx.x & 63u) == 0) lds[threadIdx.x / 64] = x;
+    int before = x - own;
+    for (int w = 0; w < wave; ++w) before += sh.scan[w];
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+        if (before < left && left <= before + of[j]) sh.found[0] = kOwn * tid + j, sh.found[1] = before, sh.found[2] = of[j];
+        before += of[j];
+    }
     __syncthreads();
-    return lds[0] + lds[1] + lds[2] + lds[3];
+}
+
+// The left-th highest of the keys from least to most, which are n keys' range of open pages; bins are 0 and n_few is.
+// Two turns at most with a few hundred keys in a bin of the first: these are ranked by counting.
+template <class Shared>
+__device__ __forceinline__ uint32_t kth_key(Shared& sh, const uint32_t* keys, int n, uint32_t least, uint32_t most, int left) {
+    constexpr int kThreads = Shared::kThreads;
+    const int tid = (int)threadIdx.x;
+    while (least != most) {
+        const int bits = 32 - __clz((int)(most - least)), shift = bits > 11 ? bits - 11 : 0;
+        for (int i = tid; i < n; i += kThreads) {
+            const uint32_t k = keys[i];
+            if (k >= least && k <= most) atomicAdd(&sh.bins[(most - k) >> shift], 1);        // bin 0: the highest
+        }
+        __syncthreads();
+        find_bin(sh, left);
+        most -= (uint32_t)sh.found[0] << shift;
+        least = max(least, most - min(most, (uint32_t)((1ull << shift) - 1)));
+        left -= sh.found[1];
+        const int inside = sh.found[2];
+        if (inside <= kFew) {
+            for (int i = tid; i < n; i += kThreads) {
+                const uint32_t k = keys[i];
+                if (k >= least && k <= most) sh.few[atomicAdd(&sh.n_few, 1)] = k;
+            }
+            __syncthreads();
+            if (tid < inside) {
+                const uint64_t mine = sh.few[tid];
+                int more = 0, same = 0;
+#pragma unroll 8
+                for (int j = 0; j < inside; ++j) more += sh.few[j] > mine, same += sh.few[j] == mine;
+                if (more < left && left <= more + same) sh.kth = (uint32_t)mine;
+            }
+            __syncthreads();
+            return sh.kth;
+        }
+        for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
+        __syncthreads();
+    }
+    return least;
 }
 
 // Closing in on the `left`-th highest of some keys.  visit(f) calls f(key) for each, all threads taking part.  On
 // return keys above `high` are among the highest, and `left` of those from low to high, which are all equal or as
 // many as that (then `left` is 0 below: all of them).
-template <class Key, class Visit>
-__device__ __forceinline__ void close_in(PickShared& sh, Visit&& visit, Key& low, Key& high, int& left) {
+template <class Shared, class Key, class Visit>
+__device__ __forceinline__ void close_in(Shared& sh, Visit&& visit, Key& low, Key& high, int& left) {
+    constexpr int kThreads = Shared::kThreads;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (;;) {
         uint64_t least = ~0ull, most = 0;
@@ -293,11 +474,11 @@ __device__ __forceinline__ void close_in(PickShared& sh, Visit&& visit, Key& low
         }
         __syncthreads();
         if (lane == 0) sh.ends[0][wave] = least, sh.ends[1][wave] = most;
-        for (int i = tid; i < kBins; i += 256) sh.bins[i] = 0;
+        for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
         __syncthreads();
         least = sh.ends[0][0], most = sh.ends[1][0];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) {
+        for (int w = 1; w < Shared::kWaves; ++w) {
             least = sh.ends[0][w] < least ? sh.ends[0][w] : least;
             most = sh.ends[1][w] > most ? sh.ends[1][w] : most;
         }
@@ -309,29 +490,23 @@ __device__ __forceinline__ void close_in(PickShared& sh, Visit&& visit, Key& low
             if (k >= low && k <= high) atomicAdd(&sh.bins[(int)((uint64_t)(high - k) >> shift)], 1);   // bin 0: the highest
         });
         __syncthreads();
-        int of[kBins / 256], own = 0;
-#pragma unroll
-        for (int j = 0; j < kBins / 256; ++j) own += of[j] = sh.bins[kBins / 256 * tid + j];
-        int x = own;
-        for (int m = 1; m < 64; m <<= 1) {
-            const int y = __shfl_up(x, m);
-            x += lane >= m ? y : 0;
-        }
-        if (lane == 63) sh.scan[wave] = x;
-        __syncthreads();
-        int before = x - own;
-        for (int w = 0; w < wave; ++w) before += sh.scan[w];
-#pragma unroll
-        for (int j = 0; j < kBins / 256; ++j) {
-            if (before < left && left <= before + of[j]) sh.found[0] = kBins / 256 * tid + j, sh.found[1] = before, sh.found[2] = of[j];
-            before += of[j];
-        }
-        __syncthreads();
+        find_bin(sh, left);
         high = (Key)(most - ((uint64_t)sh.found[0] << shift));
         const uint64_t width = ((uint64_t)1 << shift) - 1;
         if ((uint64_t)high - (uint64_t)low > width) low = (Key)((uint64_t)high - width);
         left -= sh.found[1];
     }
+}
+
+// The keys from low to high are those that fp32 sums cannot tell from the k-th highest.
+__device__ __forceinline__ void border(const SelectParams& p, float sum, float top, uint32_t kth_key, uint32_t& low, uint32_t& high) {
+    // (a hundredth more than E for the rounding of the sum, of E itself and of the borders)
+    const float err = 2.02f * (float)p.head_dim * (0x1p-23f * sum * top + 0x1p-125f * (1.f + sum + top));
+    const float kth = number_of(kth_key), reach = 2.f * err + 0x1p-22f * fabsf(kth);
+    if (!(reach < INFINITY)) return;
+    const float a = kth - reach, b = kth + reach;
+    low = a > -INFINITY ? order_of(a) : 1u;
+    high = b < INFINITY ? order_of(b) : kChosen - 1;
 }
 
 // A page's score in fp64 as a number's place among all: the wave's lanes lie along the columns, and what is left of
@@ -373,10 +548,11 @@ __device__ __forceinline__ uint64_t exact_key(const SelectParams& p, const uint8
 }
 
 // One workgroup for a row and KV head.  Keys are in LDS, or (IN_LDS false) in the place of the scores.
-template <int DT, bool IN_LDS>
-__global__ __launch_bounds__(256) void pick_kernel(SelectParams p) {
+template <int DT, int THREADS, bool IN_LDS>
+__global__ __launch_bounds__(THREADS) void pick_kernel(SelectParams p) {
     extern __shared__ uint32_t lds_keys[];
-    __shared__ PickShared sh;
+    constexpr int kWaves = THREADS / 64;
+    __shared__ PickShared<THREADS> sh;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int64_t unit = (int64_t)p.first_block + blockIdx.x;
     const int row = (int)(unit / p.kv_heads), head = (int)(unit % p.kv_heads);
@@ -385,6 +561,7 @@ __global__ __launch_bounds__(256) void pick_kernel(SelectParams p) {
     const Seq seq = uniform(seq_of(p.batch, s));
     if (row < seq.row0 || row >= seq.row0 + seq.n_new) return;
     const int n = pages_seen(p, seq, row - seq.row0 + 1);
+    if (n <= p.few_pages) return;
     float* scores = p.scores + unit * p.score_stride;
     uint32_t* keys;
     if constexpr (IN_LDS) keys = lds_keys;
@@ -392,125 +569,86 @@ __global__ __launch_bounds__(256) void pick_kernel(SelectParams p) {
     const uint8_t* q = p.q + 2 * ((int64_t)row * p.q_stride + (int64_t)head * p.group * p.head_dim);
     int32_t* out = p.out + unit * p.budget;
 
-    int forced = 0, open = 0, unknown = 0;
-    for (int i = tid; i < n; i += 256) {
-        const float x = scores[i];
-        const int id = seq.table[i];
-        const bool there = id >= 0 && id < p.batch.n_pages, always = there && (i < p.sink || i >= n - p.recent);
-        const bool known = x == x;
-        keys[i] = always ? kChosen : there ? (known ? order_of(x) : 1u) : 0u;
-        forced += always, open += there && !always, unknown += there && !always && !known;
+    for (int i = tid; i < kBins; i += THREADS) sh.bins[i] = 0;
+    if (tid == 0) sh.n_few = sh.n_near = 0;
+    PickSums all{kChosen, 0, 0, 0, 0, 0.f, 0.f};
+    auto larger = [](float a, float b) { return a > b || a != a ? a : b; };   // NaN above all
+    for (int h = wave; h < p.group; h += kWaves) {
+        float x = 0.f;
+        for (int d = 2 * lane; d < p.head_dim; d += 128) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(q + 2 * ((int64_t)h * p.head_dim + d));
+            x += fabsf(hot_lo<DT>(w)) + fabsf(hot_hi<DT>(w));
+        }
+        all.sum = larger(xor_sum(x, 64), all.sum);
     }
-    forced = block_total(forced, sh.scan);
-    open = block_total(open, sh.scan);
-    unknown = block_total(unknown, sh.scan);
-    const int wanted = p.budget - forced;
-    if (open <= wanted) {                                     // all of them
-        for (int i = tid; i < n; i += 256)
-            if (keys[i] != 0) keys[i] = kChosen;
-    } else if (wanted > 0) {
-        // the fp32 scores' k-th highest, and how far from it fp32 sums cannot tell
-        uint32_t low = 1, high = kChosen - 1;                 // keys of pages that may or may not be taken
-        int left = wanted;
-        if (unknown == 0) {
-            uint32_t least = 1, most = kChosen - 1;
-            close_in(sh, [&](auto&& f) { for (int i = tid; i < n; i += 256) f(keys[i]); }, least, most, left);
-            float sum = 0.f, top = 0.f;
-            for (int h = wave; h < p.group; h += 4) {
-                float x = 0.f;
-                for (int d = 2 * lane; d < p.head_dim; d += 128) {
-                    const uint32_t w = *reinterpret_cast<const uint32_t*>(q + 2 * ((int64_t)h * p.head_dim + d));
-                    x += fabsf(hot_lo<DT>(w)) + fabsf(hot_hi<DT>(w));
-                }
-                x = xor_sum(x, 64);
-                sum = x > sum || x != x ? x : sum;
-            }
-            const float* tops = p.top + ((int64_t)s * p.kv_heads + head) * p.tops;
-            for (int i = tid; i < (n + 15) / 16; i += 256) {
-                const float x = tops[i];
-                top = x > top || x != x ? x : top;
-            }
-            for (int m = 1; m < 64; m <<= 1) {
-                const float x = __shfl_xor(top, m);
-                top = x > top || x != x ? x : top;
-            }
-            __syncthreads();
-            if (lane == 0) sh.sums[0][wave] = sum, sh.sums[1][wave] = top;
-            __syncthreads();
+    const float* tops = p.top + ((int64_t)s * p.kv_heads + head) * p.tops;
+    for (int i = tid; i < (n + 15) / 16; i += THREADS) all.top = larger(tops[i], all.top);
+    for (int base = 0; base < n; base += 4 * THREADS) {       // four loads in flight
+        float x[4];
+        int id[4];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                sum = sh.sums[0][w] > sum || sh.sums[0][w] != sh.sums[0][w] ? sh.sums[0][w] : sum;
-                top = sh.sums[1][w] > top || sh.sums[1][w] != sh.sums[1][w] ? sh.sums[1][w] : top;
-            }
-            // (a hundredth more than E for the rounding of the sum, of E itself and of the borders)
-            const float err = 2.02f * (float)p.head_dim * (0x1p-23f * sum * top + 0x1p-125f * (1.f + sum + top));
-            const float kth = number_of(least), reach = 2.f * err + 0x1p-22f * fabsf(kth);
-            if (reach < INFINITY) {
-                const float a = kth - reach, b = kth + reach;
-                low = a > -INFINITY ? order_of(a) : 1u;
-                high = b < INFINITY ? order_of(b) : kChosen - 1;
+        for (int j = 0; j < 4; ++j) {
+            const int i = base + j * THREADS + tid;
+            x[j] = i < n ? scores[i] : 0.f;
+            id[j] = i < n ? seq.entry(i) : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = base + j * THREADS + tid;
+            const bool there = id[j] >= 0 && id[j] < p.batch.n_pages, always = there && (i < p.sink || i >= n - p.recent);
+            const bool may = there && !always, known = x[j] == x[j];
+            const uint32_t k = always ? kChosen : may ? (known ? order_of(x[j]) : 1u) : 0u;
+            if (i < n) keys[i] = k;
+            if (may) all.least = min(all.least, k), all.most = max(all.most, k);
+            all.forced += __popcll(__ballot(always)), all.open += __popcll(__ballot(may)), all.unknown += __popcll(__ballot(may && !known));
+        }
+    }
+    auto join = [&](int width, bool counts) {
+        for (int m = 1; m < width; m <<= 1) {
+            all.least = min(all.least, (uint32_t)__shfl_xor((int)all.least, m));
+            all.most = max(all.most, (uint32_t)__shfl_xor((int)all.most, m));
+            all.top = larger(__shfl_xor(all.top, m), all.top);
+            if (!counts) continue;
+            all.sum = larger(__shfl_xor(all.sum, m), all.sum);
+            all.forced += __shfl_xor(all.forced, m);
+            all.open += __shfl_xor(all.open, m);
+            all.unknown += __shfl_xor(all.unknown, m);
+        }
+    };
+    join(64, false);
+    if (lane == 0) sh.sums[wave] = all;
+    __syncthreads();
+    all = sh.sums[lane % kWaves];
+    join(kWaves, true);
+    const int wanted = p.budget - all.forced;
+    bool every = all.open <= wanted;                          // what is neither 0 nor kChosen by the end is taken
+    if (!every && wanted > 0) {
+        uint32_t low = 1, high = kChosen - 1;                 // keys of pages that may or may not be taken
+        // the fp32 scores' k-th highest, and how far from it fp32 sums cannot tell
+        if (all.unknown == 0) border(p, all.sum, all.top, kth_key(sh, keys, n, all.least, all.most, wanted), low, high);
+        int above = 0;
+        for (int base = 0; base < n; base += THREADS) {
+            const int i = base + tid;
+            const uint32_t k = i < n ? keys[i] : 0u;
+            const bool over = k > high && k != kChosen;
+            above += __popcll(__ballot(over));
+            if (over) keys[i] = kChosen;
+            if (k >= low && k <= high) {
+                const int at = atomicAdd(&sh.n_near, 1);
+                if (at < kFew) sh.few_page[at] = i;
             }
         }
-        int above = 0, near = 0;
-        for (int i = tid; i < n; i += 256) {
-            const uint32_t k = keys[i];
-            above += k > high && k != kChosen;
-            near += k >= low && k <= high;
-        }
-        above = block_total(above, sh.scan);
-        near = block_total(near, sh.scan);
-        left = wanted - above;
-        // above `high`: taken; below `low`: not
-        if (near <= left || near > kFew) {
-            uint64_t exact_low = 1, exact_high = ~0ull;       // (a score's place is never 0)
-            int ties = 0x7FFFFFFF;
-            auto chunk = [&](int base) {                      // of 256 pages: the scores of those near the border, 0 for the others
-                __syncthreads();
-                for (int j = wave; j < 256; j += 4) {
-                    const int i = base + j;
-                    const uint32_t k = i < n ? keys[i] : 0u;
-                    const bool is = k >= low && k <= high;
-                    const uint64_t x = is ? exact_key<DT>(p, q, seq.table[i], head) : 0ull;
-                    if (lane == 0) sh.few[j] = x;
-                }
-                __syncthreads();
-                return sh.few[tid];
-            };
-            if (near > left) {
-                ties = left;
-                close_in(sh, [&](auto&& f) { for (int base = 0; base < n; base += 256) f(chunk(base)); }, exact_low, exact_high, ties);
-            } else {
-                exact_high = 0;                               // all that are near
-            }
-            int tied = 0;
-            for (int base = 0; base < n; base += 256) {
-                const int i = base + tid;
-                const uint32_t k = i < n ? keys[i] : 0u;
-                const bool is = k >= low && k <= high;
-                const uint64_t x = near > left ? chunk(base) : is ? 1ull : 0ull;
-                const bool tie = near > left && is && x >= exact_low && x <= exact_high;
-                const uint64_t all = __ballot(tie);
-                __syncthreads();
-                if (lane == 0) sh.scan[wave] = __popcll(all);
-                __syncthreads();
-                int rank = tied + __popcll(all & ((1ull << lane) - 1));
-                for (int w = 0; w < 4; ++w) {
-                    rank += w < wave ? sh.scan[w] : 0;
-                    tied += sh.scan[w];
-                }
-                if (i < n && k != kChosen) keys[i] = k > high || (is && x > exact_high) || (tie && rank < ties) ? kChosen : 0u;
-            }
-        } else {
-            if (tid == 0) sh.n_few = 0;
-            __syncthreads();
-            for (int i = tid; i < n; i += 256) {
-                const uint32_t k = keys[i];
-                if (k >= low && k <= high) sh.few_page[atomicAdd(&sh.n_few, 1)] = i;
-                if (k != kChosen) keys[i] = k > high ? kChosen : 0u;
-            }
-            __syncthreads();
-            for (int j = wave; j < near; j += 4) {
-                const uint64_t x = exact_key<DT>(p, q, seq.table[sh.few_page[j]], head);
+        if (lane == 0) sh.scan[wave] = above;
+        __syncthreads();
+        above = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) above += sh.scan[w];
+        const int left = wanted - above, near = sh.n_near;
+        if (near <= left) {                                   // all that are near, and of the others none
+            for (int i = tid; i < n; i += THREADS) keys[i] = keys[i] >= low ? kChosen : 0u;
+        } else if (near <= kFew) {
+            for (int j = wave; j < near; j += kWaves) {
+                const uint64_t x = exact_key<DT>(p, q, seq.entry(sh.few_page[j]), head);
                 if (lane == 0) sh.few[j] = x;
             }
             __syncthreads();
@@ -521,28 +659,229 @@ __global__ __launch_bounds__(256) void pick_kernel(SelectParams p) {
                 for (int j = 0; j < near; ++j) rank += sh.few[j] > mine || (sh.few[j] == mine && sh.few_page[j] < page);
                 if (rank < left) keys[page] = kChosen;
             }
+        } else {
+            uint64_t exact_low = 1, exact_high = ~0ull;       // (a score's place is never 0)
+            int ties = left;
+            auto chunk = [&](int base) {                      // of THREADS pages: the scores of those near the border, 0 for the others
+                __syncthreads();
+                for (int j = wave; j < THREADS; j += kWaves) {
+                    const int i = base + j;
+                    const uint32_t k = i < n ? keys[i] : 0u;
+                    const bool is = k >= low && k <= high;
+                    const uint64_t x = is ? exact_key<DT>(p, q, seq.entry(i), head) : 0ull;
+                    if (lane == 0) sh.few[j] = x;
+                }
+                __syncthreads();
+                return sh.few[tid];
+            };
+            close_in(sh, [&](auto&& f) { for (int base = 0; base < n; base += THREADS) f(chunk(base)); }, exact_low, exact_high, ties);
+            int tied = 0;
+            for (int base = 0; base < n; base += THREADS) {
+                const int i = base + tid;
+                const uint32_t k = i < n ? keys[i] : 0u;
+                const uint64_t x = chunk(base);               // 0 for pages that are not near
+                const bool tie = x >= exact_low && x <= exact_high;
+                const uint64_t all_ties = __ballot(tie);
+                __syncthreads();
+                if (lane == 0) sh.scan[wave] = __popcll(all_ties);
+                __syncthreads();
+                int rank = tied + __popcll(all_ties & ((1ull << lane) - 1));
+                for (int w = 0; w < kWaves; ++w) {
+                    rank += w < wave ? sh.scan[w] : 0;
+                    tied += sh.scan[w];
+                }
+                if (i < n && k != kChosen) keys[i] = x > exact_high || (tie && rank < ties) ? kChosen : 0u;
+            }
         }
-    } else {
-        for (int i = tid; i < n; i += 256)
-            if (keys[i] != kChosen) keys[i] = 0u;
     }
     __syncthreads();
-    int at = 0;
-    for (int base = 0; base < n; base += 256) {
-        const int i = base + tid;
-        const bool taken = i < n && keys[i] == kChosen;
-        const uint64_t all = __ballot(taken);
-        __syncthreads();
-        if (lane == 0) sh.scan[wave] = __popcll(all);
-        __syncthreads();
-        int to = at + __popcll(all & ((1ull << lane) - 1));
-        for (int w = 0; w < 4; ++w) {
-            to += w < wave ? sh.scan[w] : 0;
-            at += sh.scan[w];
-        }
-        if (taken && to < p.budget) out[to] = i;
+    // a wave has a run of pages
+    const int run = (n + THREADS - 1) / THREADS * 64, run0 = wave * run, run1 = min(run0 + run, n);
+    int mine = 0;
+    auto is_taken = [&](int i) { return i < run1 && (keys[i] == kChosen || (every && keys[i] != 0)); };
+    for (int base = run0; base < run1; base += 64) mine += __popcll(__ballot(is_taken(base + lane)));
+    if (lane == 0) sh.scan[wave] = mine;
+    __syncthreads();
+    int at = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        at += w < wave ? sh.scan[w] : 0;
+        total += sh.scan[w];
     }
-    for (int i = at + tid; i < p.budget; i += 256) out[i] = -1;
+    for (int base = run0; base < run1; base += 64) {
+        const bool taken = is_taken(base + lane);
+        const uint64_t mask = __ballot(taken);
+        const int to = at + __popcll(mask & ((1ull << lane) - 1));
+        if (taken && to < p.budget) out[to] = base + lane;
+        at += __popcll(mask);
+    }
+    for (int i = total + tid; i < p.budget; i += THREADS) out[i] = -1;
+}
+
+// The same for rows of at most 1,024 pages: one wave for a row and KV head, its keys in registers, which pages are taken
+// in the bits of a word of each lane, and the k-th highest key found bit by bit.
+//
+// 4,000 rows of 5 KV heads over 525 pages: 205 us by workgroups, 57 so.
+constexpr int kFewPages = 1024;
+
+template <int DT, int OWN>
+__global__ __launch_bounds__(256) void pick_few_kernel(SelectParams p) {
+    constexpr int kOwn = OWN;                                 // pages of a lane: 64 OWN are enough for every row
+    const int lane = (int)threadIdx.x & 63;
+    const int64_t unit = ((int64_t)p.first_block + blockIdx.x) * 4 + uniform((int)threadIdx.x >> 6);
+    const int64_t wide_row = unit / p.kv_heads;
+    if (wide_row >= p.batch.n_rows) return;
+    const int row = (int)wide_row, head = (int)(unit % p.kv_heads);
+    const int s = uniform(find_above(p.batch.starts + 1, p.batch.n_seqs, row));
+    if (s >= p.batch.n_seqs) return;
+    const Seq seq = uniform(seq_of(p.batch, s));
+    if (row < seq.row0 || row >= seq.row0 + seq.n_new) return;
+    const int n = uniform(pages_seen(p, seq, row - seq.row0 + 1));
+    if (n > 64 * OWN) return;                                 // (another kernel's)
+    const float* scores = p.scores + unit * p.score_stride;
+    const uint8_t* q = p.q + 2 * ((int64_t)row * p.q_stride + (int64_t)head * p.group * p.head_dim);
+    int32_t* out = p.out + unit * p.budget;
+
+    // |q|_1, of four heads at once, and the greatest bound
+    float sum = 0.f, top = lane < (n + 15) / 16 ? p.top[((int64_t)s * p.kv_heads + head) * p.tops + lane] : 0.f;
+    for (int h0 = 0; h0 < p.group; h0 += 4) {
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int d = 2 * lane; d < p.head_dim; d += 128)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(q + 2 * ((int64_t)min(h0 + e, p.group - 1) * p.head_dim + d));
+                x[e] += fabsf(hot_lo<DT>(w)) + fabsf(hot_hi<DT>(w));
+            }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[e] = xor_sum(x[e], 64);
+            sum = x[e] > sum || x[e] != x[e] ? x[e] : sum;
+        }
+    }
+    for (int m = 1; m < 64; m <<= 1) {
+        const float x = __shfl_xor(top, m);
+        top = x > top || x != x ? x : top;
+    }
+    uint32_t key[kOwn], taken = 0, nears = 0;                 // key 0: not open; bit c: of page 64 c + lane
+    int forced = 0, open = 0, unknown = 0;
+    {
+        float x[kOwn];
+        int id[kOwn];
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c) {
+            const int i = min(64 * c + lane, n - 1);
+            x[c] = 64 * c < n ? scores[i] : 0.f;
+            id[c] = 64 * c < n ? seq.entry(i) : -1;
+        }
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c) {
+            key[c] = 0;
+            if (64 * c >= n) continue;
+            const int i = 64 * c + lane;
+            const bool there = i < n && id[c] >= 0 && id[c] < p.batch.n_pages, always = there && (i < p.sink || i >= n - p.recent);
+            const bool known = x[c] == x[c];
+            if (there && !always) key[c] = known ? order_of(x[c]) : 1u;
+            taken |= always ? 1u << c : 0u;
+            forced += __popcll(__ballot(always));
+            open += __popcll(__ballot(key[c] != 0));
+            unknown += __popcll(__ballot(key[c] == 1u));
+        }
+    }
+    auto count = [&](auto&& is) {
+        int total = 0;
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c) total += __popcll(__ballot(is(c)));
+        return total;
+    };
+    const int wanted = p.budget - forced;
+    if (open <= wanted) {
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c) taken |= key[c] != 0 ? 1u << c : 0u;
+    } else if (wanted > 0) {
+        uint32_t low = 1, high = kChosen - 1;
+        if (unknown == 0) {
+            uint32_t least = kChosen, most = 0;               // the k-th highest is one of these and those between
+#pragma unroll
+            for (int c = 0; c < kOwn; ++c) {
+                least = key[c] != 0 ? min(least, key[c]) : least;
+                most = max(most, key[c]);
+            }
+            for (int m = 1; m < 64; m <<= 1) {
+                least = min(least, (uint32_t)__shfl_xor((int)least, m));
+                most = max(most, (uint32_t)__shfl_xor((int)most, m));
+            }
+            least = (uint32_t)uniform((int)least), most = (uint32_t)uniform((int)most);
+            while (least < most) {
+                const uint32_t t = least + (most - least + 1) / 2;
+                const int reach = count([&](int c) { return key[c] >= t; });
+                if (reach >= wanted) least = t;
+                else most = t - 1;
+                if (reach != wanted) continue;
+                most = kChosen;                               // the least of these
+#pragma unroll
+                for (int c = 0; c < kOwn; ++c) most = key[c] >= t ? min(most, key[c]) : most;
+                for (int m = 1; m < 64; m <<= 1) most = min(most, (uint32_t)__shfl_xor((int)most, m));
+                least = most;
+            }
+            const uint32_t kth_key = least;
+            border(p, sum, top, kth_key, low, high);
+        }
+        int above = 0, near = 0;
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c) {
+            if (64 * c >= n) continue;
+            const bool over = key[c] > high, is = key[c] >= low && key[c] <= high;
+            above += __popcll(__ballot(over));
+            near += __popcll(__ballot(is));
+            taken |= over ? 1u << c : 0u;
+            nears |= is ? 1u << c : 0u;
+        }
+        const int left = wanted - above;
+        if (near <= left) {
+            taken |= nears;
+        } else {
+            uint64_t exact[kOwn];                             // of this lane's near pages; 0 for the others
+#pragma unroll
+            for (int c = 0; c < kOwn; ++c) {
+                exact[c] = 0;
+                if (64 * c >= n) continue;
+                for (uint64_t todo = __ballot(nears >> c & 1); todo; todo &= todo - 1) {
+                    const int from = __ffsll((unsigned long long)todo) - 1;
+                    const uint64_t x = exact_key<DT>(p, q, seq.entry(64 * c + from), head);
+                    if (lane == from) exact[c] = x;
+                }
+            }
+            uint64_t kth_key = 0;
+            int reach = near;
+            for (int bit = 63; bit >= 0 && reach != left; --bit) {
+                const uint64_t t = kth_key | 1ull << bit;
+                const int r = count([&](int c) { return exact[c] >= t; });
+                if (r >= left) kth_key = t, reach = r;
+            }
+            // those above are taken, and as many as are left of those equal to it
+            int ties = left - (reach == left ? left : count([&](int c) { return exact[c] > kth_key; }));
+#pragma unroll
+            for (int c = 0; c < kOwn; ++c) {
+                if (64 * c >= n) continue;
+                const bool tie = reach != left && exact[c] == kth_key;
+                const uint64_t all = __ballot(tie);
+                const bool in = reach == left ? exact[c] >= kth_key && exact[c] != 0
+                                              : exact[c] > kth_key || (tie && __popcll(all & ((1ull << lane) - 1)) < ties);
+                taken |= in ? 1u << c : 0u;
+                ties -= min(ties, (int)__popcll(all));
+            }
+        }
+    }
+    int at = 0;
+#pragma unroll
+    for (int c = 0; c < kOwn; ++c) {
+        if (64 * c >= n) continue;
+        const uint64_t all = __ballot(taken >> c & 1);
+        const int to = at + __popcll(all & ((1ull << lane) - 1));
+        if ((taken >> c & 1) && to < p.budget) out[to] = 64 * c + lane;
+        at += __popcll(all);
+    }
+    for (int i = at + lane; i < p.budget; i += 64) out[i] = -1;
 }
 
 constexpr int kKeysInLds = 12288;   // 48 KiB
@@ -555,7 +894,7 @@ const char* check_bounds(const void* bounds, int64_t stride, const ztcp_geometry
 }
 
 struct SelectPlan {
-    int64_t stride, tops, units, floats;
+    int64_t stride, tops, units, floats;   // units: 64 pages and a block of tokens each, at most
 };
 SelectPlan plan_select(const ztcp_paged_batch* b, const ztcp_geometry* g) {
     SelectPlan plan;
@@ -663,14 +1002,27 @@ extern "C" int ztcp_select_pages(const void* q, int64_t q_stride, int64_t q_head
     p.top = (float*)workspace;
     p.scores = p.top + (batch->n_seqs * g->num_heads * plan.tops + 3) / 4 * 4;
     p.out = out;
+    int cus = 0;
+    if (cu_count(cus) != ZTCP_OK) return ZTCP_EHIP;
+    // as many as the card holds at once, and no more than units
+    const int64_t resident = (int64_t)cus * (d <= 64 ? 5 : d <= 128 ? 3 : 1), each = (resident + g->num_heads - 1) / g->num_heads;
+    p.score_groups = (int32_t)(each < plan.units ? each : plan.units);
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        const uint64_t units = (uint64_t)plan.units * (uint64_t)g->num_heads, picks = (uint64_t)batch->n_rows * (uint64_t)g->num_heads;
-        launch_blocks(d <= 64 ? score_kernel<DT, 64> : d <= 128 ? score_kernel<DT, 128> : score_kernel<DT, 256>, units, 256, 0,
-                      (hipStream_t)stream, p);
-        if (batch->max_pages <= kKeysInLds)
-            launch_blocks(pick_kernel<DT, true>, picks, 256, (size_t)batch->max_pages * 4, (hipStream_t)stream, p);
-        else launch_blocks(pick_kernel<DT, false>, picks, 256, 0, (hipStream_t)stream, p);
+        const dim3 grid((uint32_t)(g->num_heads * p.score_groups));
+        hipLaunchKernelGGL((d <= 64 ? score_kernel<DT, 64> : d <= 128 ? score_kernel<DT, 128> : score_kernel<DT, 256>), grid, dim3(256), 0,
+                           (hipStream_t)stream, p);
+        const uint64_t picks = (uint64_t)batch->n_rows * (uint64_t)g->num_heads;
+        const bool many = picks > 2 * (uint64_t)cus;          // rows: a wave each if their pages are few
+        if (batch->max_pages <= kFewPages || many)
+            launch_blocks(batch->max_pages <= 256 ? pick_few_kernel<DT, 4> : batch->max_pages <= 576 ? pick_few_kernel<DT, 9> : pick_few_kernel<DT, 16>,
+                          (picks + 3) / 4, 256, 0, (hipStream_t)stream, p);
+        if (batch->max_pages <= kFewPages) return;
+        p.few_pages = many ? kFewPages : 0;
+        const bool in_lds = batch->max_pages <= kKeysInLds;
+        const size_t lds = in_lds ? (size_t)batch->max_pages * 4 : 0;
+        if (many) launch_blocks(in_lds ? pick_kernel<DT, 256, true> : pick_kernel<DT, 256, false>, picks, 256, lds, (hipStream_t)stream, p);
+        else launch_blocks(in_lds ? pick_kernel<DT, 1024, true> : pick_kernel<DT, 1024, false>, picks, 1024, lds, (hipStream_t)stream, p);
     };
     if (g->hot_dtype == ZTCP_HOT_BF16) go(std::integral_constant<int, kHotBf16>{});
     else go(std::integral_constant<int, kHotFp16>{});

@@ -84,7 +84,7 @@ void selected_kernel(SelectedParams p) {
             at.row = key - nth * p.batch.page_tokens;
             const int page = picked[nth];
             if (page >= 0 && page < p.max_pages && page * p.batch.page_tokens + at.row < limit) {
-                const int id = seq.table[page];
+                const int id = seq.entry(page);
                 if (id >= 0 && id < p.batch.n_pages) at.page = id;
             }
         }
