@@ -477,8 +477,9 @@ ZTCP_API int ztcp_select_pages(const void* q, int64_t q_stride, int64_t q_heads,
 
 /* Attention of new tokens over listed pages: as ztcp_paged_attention, but a row's sums
  * for the query heads of KV head h are over the tokens that it sees of the pages in
- * columns selected[row, h, 0 .. listed - 1] of its sequence's table row.  Entries outside
- * the table's columns list nothing; a column listed twice counts twice.
+ * columns selected[row, h, 0 .. listed - 1] of its sequence's table row, which ascend:
+ * entries outside the table's columns list nothing, and neither does one that is not
+ * above all columns in front of it.
  * selected [n_rows, num_heads, listed]; listed * num_tokens at most 2^31 - 4096. */
 ZTCP_API size_t ztcp_selected_attention_workspace(const ztcp_paged_batch* batch, const ztcp_page_pool* pool,
                                          const ztcp_geometry* g, int64_t q_heads, int64_t listed);

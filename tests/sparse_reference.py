@@ -124,13 +124,20 @@ def selected(q, k_pages, v_pages, table, lens, starts, picked, scale):
         for row in range(r0, r0 + n):
             limit = length - n + row - r0 + 1
             for h in range(kv):
-                pages = [p for p in picked[row, h].tolist() if 0 <= p < table.shape[1] and 0 <= int(table[s, p]) < k_pages.shape[0]]
-                where = [(int(table[s, p]), j) for p in pages for j in range(t) if p * t + j < limit]
-                if not where:
+                pages, most = [], -1
+                for p in picked[row, h].tolist():
+                    if most < p < table.shape[1]:   # an entry that is not above all in front of it lists nothing
+                        most = p
+                        if 0 <= int(table[s, p]) < k_pages.shape[0]:
+                            pages.append(p)
+                pages = torch.tensor(pages, dtype=torch.int64)
+                place = (pages[:, None] * t + torch.arange(t)).flatten()
+                place = place[place < limit]
+                if place.numel() == 0:
                     continue
-                ids, j = torch.tensor(where).T
-                k, v = (x[ids, j, h].double() for x in (k_pages, v_pages))
-                seen = torch.ones(g, len(where), dtype=torch.bool)
+                ids = table[s, place // t].long()
+                k, v = (x[ids, place % t, h].double() for x in (k_pages, v_pages))
+                seen = torch.ones(g, place.numel(), dtype=torch.bool)
                 for full, part in zip(res, softmax_rows(q[row, h * g:(h + 1) * g].double(), k, v, seen, scale, q.dtype)):
                     full[row, h * g:(h + 1) * g] = part
     return res

@@ -208,6 +208,8 @@ def _attend_case(lens, kv, group, d, t, dtype, listed, *, seed=0, missing=0.0):
     q = torch.randn((rows, kv * group + 2, d), generator=gen).to(dtype).cuda()[:, :kv * group]
     k, v = (torch.randn((n_pages, t, kv, d), generator=gen).to(dtype).cuda() for _ in range(2))
     picked = torch.randint(-2, table.shape[1] + 2, (rows, kv, listed), generator=gen).int()
+    if seed % 3:   # ascending, and now and then not
+        picked = torch.where(torch.rand((rows, kv, 1), generator=gen) < 0.1, picked, picked.sort(-1).values)
     return dict(q=q, k=k, v=v, table=table, lens=length, starts=starts, picked=picked.cuda())
 
 
@@ -231,10 +233,14 @@ def _check_selected(A, c, what, **kw):
 @pytest.mark.parametrize("lens,kv,group,d,t,listed", [
     ([(1, 1)], 1, 1, 64, 16, 1), ([(1, 3000), (1, 40), (0, 17), (1, 900)], 2, 4, 128, 16, 40), ([(5, 700), (20, 300)], 3, 3, 96, 13, 7),
     ([(1, 600)], 2, 40, 16, 1, 100), ([(3, 900)], 1, 1, 256, 4, 33), ([(300, 1000), (1, 9)], 5, 2, 64, 64, 3), ([(250, 500)], 5, 1, 256, 16, 2),
-    ([(1, 20000)], 1, 8, 192, 8, 500), ([(2, 500)] * 70, 8, 4, 112, 16, 3), ([(1, 5000)], 1, 17, 128, 100, 30)])
+    ([(1, 20000)], 1, 8, 192, 8, 500), ([(2, 500)] * 70, 8, 4, 112, 16, 3), ([(1, 5000)], 1, 17, 128, 100, 30),
+    ([(300, 900), (250, 250)], 8, 4, 128, 16, 5), ([(520, 1300)], 8, 4, 64, 64, 4), ([(1100, 1111)], 8, 2, 128, 1, 30),
+    ([(300, 700), (0, 9), (260, 1100)], 8, 4, 256, 13, 6), ([(700, 2000)], 12, 2, 96, 100, 3), ([(150, 3000)], 3, 37, 128, 32, 20)])
 def test_selected(A, lens, kv, group, d, t, listed, dtype):
     _say("selected", lens[:3], kv, group, d, t, listed, dtype)
-    for seed, missing in enumerate((0.0, 0.15)):
+    for seed, missing in enumerate((0.0, 0.15, 0.0)):
+        if seed == 0 and sum(q for q, _ in lens) > 400:
+            continue   # lists in any order of many rows: the ascending ones with some that are not are enough
         c = _attend_case(lens, kv, group, d, t, dtype, listed, seed=seed, missing=missing)
         _check_selected(A, c, (lens[:3], seed), **({"scale": 0.3} if seed else {}))
 
@@ -243,7 +249,7 @@ def test_selected_nothing_twice_and_far_outside(A):
     _say("selected, odd lists")
     c = _attend_case([(3, 200), (2, 90)], 2, 2, 64, 16, BF, 6, seed=5)
     c["picked"][0] = -1
-    c["picked"][1, 0] = _i32([2, 2, 2, 0, 0, 5])
+    c["picked"][1, 0] = _i32([2, 2, 1 << 20, 0, 2, 5])
     c["picked"][2, 1] = _i32([2 ** 31 - 1, -2 ** 31, 1 << 27, 13, 12, 12])
     c["picked"][3] = 5   # pages behind the sequence's end
     out, lse = _check_selected(A, c, "odd lists")
@@ -281,6 +287,29 @@ def test_selected_numbers_that_are_not_seen(A):
         g = g.cpu().double()
         keep = ~bad[..., None].expand_as(w) if w.dim() == 3 else ~bad
         assert bool(((g == w) | (torch.isnan(g) & torch.isnan(w)) | ((g - w).abs() <= tol))[keep].all())
+
+
+def test_selected_numbers_that_others_see(A):
+    """Blocks of rows with lists of their own: NaN and infinities of V reach the rows that list their pages and no other of
+    the block, and where there are none the block is done once."""
+    _say("selected, NaN and infinities in blocks")
+    for d, t, dtype in ((128, 16, BF), (64, 13, FP)):
+        c = _attend_case([(300, 700), (260, 500)], 8, 4, d, t, dtype, 6, seed=10)
+        for page, token, pool, x in ((3, 2, "v", math.nan), (7, 1, "v", math.inf), (9, 0, "v", -math.inf), (5, 4, "k", math.nan),
+                                     (7, 3, "v", math.inf)):
+            c[pool][int(c["table"][0, page]), token, page % 8, 5] = x
+        for s, total in ((0, 700), (1, 500)):   # behind the end
+            if total % t:
+                for pool in ("k", "v"):
+                    c[pool][int(c["table"][s, total // t]), total % t:] = math.nan
+        out, lse = _attend(A, c)
+        want = _reference(c)
+        bad = torch.isnan(want[1])
+        assert bool(bad.any()) and bool(torch.isinf(want[0]).any()) and bool(torch.isnan(want[0])[~bad].any())
+        for g, w, tol in ((out, want[0], want[2]), (lse, want[1], want[3])):
+            g = g.cpu().double()
+            keep = ~bad[..., None].expand_as(w) if w.dim() == 3 else ~bad
+            assert bool(((g == w) | (torch.isnan(g) & torch.isnan(w)) | ((g - w).abs() <= tol))[keep].all()), d
 
 
 def test_selected_wrong_numbers_stay_inside(A):

@@ -132,9 +132,9 @@ def selected_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
                        kv_lens: torch.Tensor, q_starts: torch.Tensor, selected: torch.Tensor, *, scale: float | None = None,
                        max_q_len: int | None = None, return_lse: bool = False, out: torch.Tensor | None = None):
     """``paged_attention`` over a part of the pages: a row's query heads of KV head h see, of the tokens that they would
-    see, those of the pages in columns ``selected[row, h]`` ([rows, kv_heads, any number] int32, as ``select_pages`` gives
-    them, in any order).  Entries outside the table's columns list nothing, a column listed twice counts twice.  The
-    log-sum-exp is over what the row sees here."""
+    see, those of the pages in columns ``selected[row, h]`` ([rows, kv_heads, any number] int32, ascending as
+    ``select_pages`` gives them).  Entries outside the table's columns (-1) list nothing, and neither does one that is not
+    above all columns in front of it.  The log-sum-exp is over what the row sees here."""
     return _call().selected_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts, selected, scale, max_q_len,
                                       return_lse, out)
 

@@ -2,10 +2,13 @@
 // for each KV head, has picked.
 //
 // The formula is paged attention's with the sums over the tokens of the listed
-// pages that the row sees.  A row and KV head are a unit of their own: its query
-// heads are the columns of the products (16; a group of fewer leaves columns
-// idle, which costs nothing where reading K and V is the work), and all of them
-// see the same tokens.
+// pages that the row sees.
+//
+// Few rows (decoding): a row and KV head are a unit of their own, whose query heads
+// are the columns of the products (16; a group of fewer leaves columns idle, which
+// costs nothing where reading K and V is the work), and all of them see the same
+// tokens.  Many rows (chunks): a workgroup takes 128 rows of a KV head over the pages
+// that any of them lists, and each row's list says which of these it sees.
 #include <type_traits>
 
 #include "ztcp_hot.h"
@@ -32,6 +35,9 @@ struct SelectedParams {
     float scale_log2;                // scale * log2(e): exponentials are powers of two
     int32_t splits, piece;           // pieces of a unit's keys, and their keys
     float* partial;                  // results of pieces: sums [head_dim], maximum, total
+    int2* lists;                     // blocks: for each workgroup list_stride columns and pages that its rows list
+    uint32_t* masks;                 // and for each of these the tokens that list it
+    int64_t list_stride;
     uint32_t first_block;            // of this launch
 };
 
@@ -39,6 +45,7 @@ __device__ __forceinline__ float* partial_of(const SelectedParams& p, int row, i
     return p.partial + (((int64_t)row * p.kv_heads * p.group + q_head) * p.splits + split) * (p.head_dim + 2);
 }
 
+// ---- by rows ----------------------------------------------------------------------
 // A workgroup of WAVES waves takes a piece of a unit's keys, 32 a wave and turn, with a wave's loads of the next 32 in
 // flight while it works on these: K and V by whole rows through LDS of its own (K of vectors of more than 128 elements
 // as the products want it).  Scores are made transposed: a column is a query head.
@@ -66,6 +73,9 @@ void selected_kernel(SelectedParams p) {
     if (row < seq.row0 || row >= seq.row0 + seq.n_new) return;
     const int limit = max(0, seq.len - seq.n_new + (row - seq.row0) + 1);   // tokens that the row sees
     const int32_t* picked = p.selected + ((int64_t)row * p.kv_heads + head) * p.listed;
+    // An entry that is not above all (columns of the table) in front of it lists nothing.  Lists ascend: whether this one
+    // does is looked at while the first keys are on their way, and only if it does not are the entries in front looked at.
+    bool ascends = true;
     const int key0 = split * p.piece, stop = key0 + min(p.listed * p.batch.page_tokens - key0, p.piece);
     uint8_t* vt = lds + wave * kWaveBytes;
     uint8_t* kt = lds + (WAVES + wave) * kWaveBytes;          // (kKInLds)
@@ -83,7 +93,10 @@ void selected_kernel(SelectedParams p) {
             const int nth = div_page(key, p.batch.page_div);
             at.row = key - nth * p.batch.page_tokens;
             const int page = picked[nth];
-            if (page >= 0 && page < p.max_pages && page * p.batch.page_tokens + at.row < limit) {
+            bool counts = page >= 0 && page < p.max_pages && page * p.batch.page_tokens + at.row < limit;
+            if (!ascends)
+                for (int i = 0; i < nth; ++i) counts &= !(picked[i] >= page && picked[i] < p.max_pages);
+            if (counts) {
                 const int id = seq.entry(page);
                 if (id >= 0 && id < p.batch.n_pages) at.page = id;
             }
@@ -141,6 +154,25 @@ void selected_kernel(SelectedParams p) {
         if (kb < stop) {
             load(place(kb + (lane & 31)));
             at = place(kb + 32 * WAVES + (lane & 31));
+            if (h0 == 0) {
+                int most = -1;                                // of the entries in front
+                for (int base = 0; base < p.listed; base += 64) {
+                    const int x = base + lane < p.listed ? picked[base + lane] : -1;
+                    int upto = x < p.max_pages ? x : -1;
+                    const bool column = upto >= 0;
+                    for (int k = 1; k < 64; k <<= 1) {
+                        const int y = __shfl_up(upto, k);
+                        upto = lane >= k ? max(upto, y) : upto;
+                    }
+                    const int in_front = __shfl_up(upto, 1), before = max(most, lane > 0 ? in_front : -1);
+                    if (__any(column && x <= before)) ascends = false;
+                    most = max(most, __shfl(upto, 63));
+                }
+                if (!ascends) {
+                    load(place(kb + (lane & 31)));
+                    at = place(kb + 32 * WAVES + (lane & 31));
+                }
+            }
         }
         for (; kb < stop; kb += 32 * WAVES) {
             const uint32_t here = valid;
@@ -282,7 +314,7 @@ void selected_kernel(SelectedParams p) {
 
 // One wave per row and query head: the pieces' sums under one maximum.
 template <int DT>
-__global__ __launch_bounds__(256) void join_kernel(SelectedParams p) {
+__global__ __launch_bounds__(256) void join_selected_kernel(SelectedParams p) {
     const int lane = (int)threadIdx.x & 63, q_heads = p.kv_heads * p.group;
     const int64_t row_head = ((int64_t)p.first_block + blockIdx.x) * 4 + ((int)threadIdx.x >> 6);
     const int64_t row = row_head / q_heads;
@@ -314,16 +346,409 @@ __global__ __launch_bounds__(256) void join_kernel(SelectedParams p) {
     if (lane == 0 && p.lse) p.lse[row_head] = total == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
+// ---- by blocks --------------------------------------------------------------------
+// 128 rows (new token r / group, query head r % group) by eight waves of 16 rows each.
+// Keys are the tokens of the pages that the block's rows list, one behind the other;
+// tiles of 64 (32 where vectors have more than 128 elements) are loaded straight into
+// LDS, read by all waves whose rows see of them, the next one on its way meanwhile.
+// Few rows a wave, so that few waves have work to do for a page that few rows list: all
+// wait for those that have.
+//
+// Two chunks of 1,024 tokens, 16 pages of 64 picked at random for each of 8 KV heads of
+// 128, 4 query heads each: 440 us, 2 us a tile: the time that a wave with work
+// needs for it; 657 by rows, each of which brings its 512 KiB from the caches, 478 by
+// four waves of 32 rows.  Rows that pick alike share pages, which random ones hardly do.
+
+constexpr int kBlockWaves = 8, kBlockRows = 16 * kBlockWaves, kBlockThreads = 64 * kBlockWaves;
+constexpr int block_tile(int dp) { return dp <= 128 ? 64 : 32; }
+
+template <int DT>
+__device__ __forceinline__ bool not_finite16(uint32_t h) {
+    constexpr uint32_t e = DT == kHotBf16 ? 0x7F80u : 0x7C00u;
+    return (h & e) == e;
+}
+
+// Tokens that a block's rows can belong to, and words of a bit for each.
+__host__ __device__ inline int block_tokens(int group) { return kBlockRows % group == 0 ? kBlockRows / group : (kBlockRows - 1) / group + 2; }
+__host__ __device__ inline int block_words(int group) { return (block_tokens(group) + 31) / 32; }
+
+// A block's pages: in the order of their columns, each with its entry of the table and a bit for every token of the block
+// that lists it.  `bits` is LDS, two words for 32 columns; returns how many.  An entry of a token's list that is no column,
+// or not above all columns in front of it, lists nothing.
+constexpr int kMostColumns = 1 << 17;
+__device__ __forceinline__ int list_pages(const SelectedParams& p, const Seq& seq, int head, int block, uint32_t* bits, int2* list,
+                                          uint32_t* masks) {
+    __shared__ int32_t scan[kBlockWaves];
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, t = p.batch.page_tokens;
+    const int columns = seq.len > 0 ? div_page(seq.len - 1, p.batch.page_div) + 1 : 0, words = (columns + 31) / 32;
+    uint32_t* before = bits + words;                          // pages in the words in front
+    for (int i = tid; i < words; i += kBlockThreads) bits[i] = 0;
+    __syncthreads();
+    const int rows = seq.n_new * p.group, token0 = block * kBlockRows / p.group;
+    const int tokens = (min(rows, (block + 1) * kBlockRows) - 1) / p.group + 1 - token0;
+    auto each = [&](auto&& f) {                               // f(token of the block, column) for what the tokens list
+        for (int token = uniform(wave); token < tokens; token += kBlockWaves) {
+            const int limit = seq.len - seq.n_new + token0 + token + 1;
+            const int32_t* mine = p.selected + ((int64_t)(seq.row0 + token0 + token) * p.kv_heads + head) * p.listed;
+            int most = -1;                                    // of the entries in front
+            for (int base = 0; base < p.listed; base += 64) {
+                const int column = base + lane < p.listed ? mine[base + lane] : -1;
+                int upto = column < p.max_pages ? column : -1;
+                const bool is = upto >= 0;
+                for (int k = 1; k < 64; k <<= 1) {
+                    const int y = __shfl_up(upto, k);
+                    upto = lane >= k ? max(upto, y) : upto;
+                }
+                const int in_front = __shfl_up(upto, 1);
+                if (is && column > max(most, lane > 0 ? in_front : -1) && column < columns && column * t < limit) f(token, column);
+                most = max(most, __shfl(upto, 63));
+            }
+        }
+    };
+    each([&](int, int column) { atomicOr(&bits[column / 32], 1u << (column & 31)); });
+    __syncthreads();
+    // a thread has a run of words; of pages that are not there the bits go
+    const int run = (words + kBlockThreads - 1) / kBlockThreads, word0 = tid * run, word1 = min(word0 + run, words);
+    int own = 0;
+    for (int i = word0; i < word1; ++i) {
+        uint32_t left = bits[i];
+        for (uint32_t todo = left; todo; todo &= todo - 1) {
+            const int id = seq.entry(32 * i + __ffs((int)todo) - 1);
+            if (id < 0 || id >= p.batch.n_pages) left &= ~(todo & (0u - todo));
+        }
+        bits[i] = left;
+        own += __popc(left);
+    }
+    int upto = own;
+    for (int m = 1; m < 64; m <<= 1) {
+        const int y = __shfl_up(upto, m);
+        upto += lane >= m ? y : 0;
+    }
+    if (lane == 63) scan[wave] = upto;
+    __syncthreads();
+    int at = upto - own, total = 0;
+    for (int w = 0; w < kBlockWaves; ++w) {
+        at += w < wave ? scan[w] : 0;
+        total += scan[w];
+    }
+    const int mask_words = block_words(p.group);
+    for (int i = word0; i < word1; ++i) {
+        before[i] = (uint32_t)at;
+        for (uint32_t todo = bits[i]; todo; todo &= todo - 1) {
+            const int column = 32 * i + __ffs((int)todo) - 1;
+            list[at++] = make_int2(column, seq.entry(column));
+        }
+    }
+    for (int i = tid; i < total * mask_words; i += kBlockThreads) masks[i] = 0;
+    __syncthreads();
+    each([&](int token, int column) {
+        const uint32_t word = bits[column / 32], bit = 1u << (column & 31);
+        if (word & bit) atomicOr(&masks[((int)before[column / 32] + __popc(word & (bit - 1))) * mask_words + token / 32], 1u << (token & 31));
+    });
+    __syncthreads();                                          // lists and masks are there, and the bits have been read
+    return total;
+}
+
+// Zeros that the tile loads read in the columns behind head_dim: a row of 256 elements.
+__device__ __attribute__((aligned(16))) uint32_t g_no_columns[128];
+
+// EVEN: a wave's share of a tile never crosses a page and rows fill DP, so that the share's address is one scalar;
+// otherwise every lane has its own.  WORDS: of a page's tokens at most.
+template <int DT, int DP, bool EVEN, int WORDS>
+__global__ __launch_bounds__(kBlockThreads) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 4 : 2)))
+void block_kernel(SelectedParams p) {
+    constexpr int kTile = block_tile(DP), kShare = kTile / kBlockWaves, kSub = kTile / 16;
+    constexpr int kSteps = DP / 32, kChunks = DP / 8, kRowBytes = DP * 2, kTileBytes = kTile * kRowBytes;
+    constexpr int kLoadRows = 64 / kChunks, kLoads = kShare / kLoadRows;   // rows of a load; a wave's loads for a tile's K, and V
+    __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2][kTileBytes];   // [buffer][K, V]
+    const int lane = (int)threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+    const int col = lane & 15, quad = lane >> 4;
+    const uint32_t unit = p.first_block + blockIdx.x;
+    const int head = (int)(unit % (uint32_t)p.kv_heads);
+    int block = (int)(unit / (uint32_t)p.kv_heads);
+    const int s = uniform(find_tile(p.batch, block, [&](const Seq& q) { return (q.n_new * p.group + kBlockRows - 1) / kBlockRows; }));
+    if (s >= p.batch.n_seqs) return;
+    block = uniform(block);
+    const Seq seq = uniform(seq_of(p.batch, s));
+    const int rows = seq.n_new * p.group;
+    const int mask_words = block_words(p.group);
+    int2* list = p.lists + (int64_t)unit * p.list_stride;
+    uint32_t* masks = p.masks + (int64_t)unit * p.list_stride * mask_words;
+    const int stop = uniform(list_pages(p, seq, head, block, reinterpret_cast<uint32_t*>(&tiles[0][0][0]), list, masks)) * p.batch.page_tokens;
+    const int r = block * kBlockRows + wave * 16 + col;
+    const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
+    const int limit = r < rows ? max(0, seq.len - seq.n_new + token + 1) : 0;
+    const int nth_token = r < rows ? token - block * kBlockRows / p.group : 0;           // of the block
+    // 16-byte pieces are permuted within a row so that the rows of one read lie in different banks
+    auto k_swizzle = [](int row, int chunk) { return chunk ^ (row & (kChunks < 16 ? kChunks - 1 : 15)); };
+    auto v_swizzle = [](int row, int chunk) {
+        if constexpr (DP == 64) return chunk ^ (((row >> 1) & 3) << 1);
+        else return chunk ^ ((row & 7) << 1);
+    };
+    const int load_row = lane / kChunks, load_chunk = lane % kChunks;
+
+    uint4 qf[kSteps];
+    {
+        const uint8_t* src = p.q + 2 * ((int64_t)(seq.row0 + token) * p.q_stride + (int64_t)q_head * p.head_dim);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const int d = 32 * i + 8 * quad;
+            qf[i] = r < rows && d < p.head_dim ? ldg16(src + 2 * d) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    // Where a tile's keys are, lane = key: entries of the list as they were read, looked at a tile later.  What is not
+    // there is loaded from the page of the list's last entry and taken out of the V tile afterwards.
+    struct Entry {
+        int2 page;                                            // column, page
+        uint32_t mask[WORDS];
+    };
+    struct Where {
+        int page, row;                                        // EVEN: of this wave's share; else of the lane's key
+        int column, key_row;                                  // of the lane's key
+        uint64_t here;                                        // which keys are there
+        uint32_t mask[WORDS];                                 // tokens that list the lane's key's page
+    };
+    auto fetch = [&](int kb) {
+        const int key = kb + (lane & (kTile - 1)), nth = div_page(min(key, stop - 1), p.batch.page_div);
+        Entry x;
+        x.page = list[nth];
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) x.mask[w] = w < mask_words ? masks[nth * mask_words + w] : 0;
+        return x;
+    };
+    auto where = [&](const Entry& entry, int kb) {
+        const int key = kb + (lane & (kTile - 1));
+        const int row = key - div_page(key, p.batch.page_div) * p.batch.page_tokens;
+        Where x;
+        x.column = entry.page.x, x.key_row = row;
+        x.here = __ballot(key < stop && entry.page.x * p.batch.page_tokens + row < seq.len);
+        x.page = entry.page.y, x.row = row;
+        if constexpr (EVEN) x.page = __builtin_amdgcn_readlane(x.page, wave * kShare), x.row = __builtin_amdgcn_readlane(x.row, wave * kShare);
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) x.mask[w] = entry.mask[w];
+        return x;
+    };
+    // The keys of a tile that this lane's row sees
+    auto sees = [&](const Where& at, int keys) {
+        uint64_t mask = 0;
+        for (int j = 0; j < keys;) {                          // a page after another
+            const int column = __builtin_amdgcn_readlane(at.column, j), from = __builtin_amdgcn_readlane(at.key_row, j);
+            const int width = min(p.batch.page_tokens - from, kTile - j);
+            uint32_t word = (uint32_t)__builtin_amdgcn_readlane((int)at.mask[0], j);
+#pragma unroll
+            for (int w = 1; w < WORDS; ++w) {
+                const uint32_t x = (uint32_t)__builtin_amdgcn_readlane((int)at.mask[w], j);
+                word = nth_token / 32 == w ? x : word;
+            }
+            const int some = word >> (nth_token & 31) & 1u ? min(width, limit - (column * p.batch.page_tokens + from)) : 0;
+            if (some > 0) mask |= (some >= 64 ? ~0ull : (1ull << some) - 1) << j;
+            j += width;
+        }
+        return kTile == 32 ? mask | mask << 32 : mask;
+    };
+    constexpr uint64_t kAll = ~0ull;                          // (tiles of 32 keys: both halves of the lanes)
+    const uint32_t lds0 = lds_address(&tiles[0][0][0]);
+    const uint32_t row_bytes = 2u * (uint32_t)p.kv_heads * (uint32_t)p.head_dim;         // from a token to the next
+    // This wave's share of a tile of K (which = 0) or V (1) into a buffer
+    auto load = [&](const Where& at, int buffer, auto which) __attribute__((always_inline)) {
+        constexpr bool is_v = decltype(which)::value != 0;
+        const uint8_t* pool = is_v ? p.v_pool : p.k_pool;
+        const int64_t page_step = is_v ? p.v_page : p.k_page;
+        auto swizzle = [&](int row, int chunk) { return is_v ? v_swizzle(row, chunk) : k_swizzle(row, chunk); };
+        const uint32_t to = lds0 + (uint32_t)((2 * buffer + (is_v ? 1 : 0)) * kTileBytes + wave * kShare * kRowBytes);
+        if constexpr (EVEN) {
+            const uint8_t* src = pool + 2 * (at.page * page_step + (int64_t)(at.row * p.kv_heads + head) * DP);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                load_lds16(src + (uint64_t)(i * kLoadRows) * row_bytes,
+                           load_row * row_bytes + 16 * swizzle(wave * kShare + i * kLoadRows + load_row, load_chunk),
+                           to + i * kLoadRows * kRowBytes);
+        } else {
+            const uint64_t mine = (uint64_t)(pool + 2 * (at.page * page_step + (int64_t)(at.row * p.kv_heads + head) * p.head_dim));
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int from = wave * kShare + i * kLoadRows + load_row, chunk = swizzle(from, load_chunk);
+                const uint8_t* src = (const uint8_t*)__shfl(mine, from) + 16 * chunk;
+                if (chunk * 8 >= p.head_dim) src = reinterpret_cast<const uint8_t*>(g_no_columns);
+                load_lds16(src, to + i * kLoadRows * kRowBytes);
+            }
+        }
+    };
+    using IsK = std::integral_constant<int, 0>;
+    using IsV = std::integral_constant<int, 1>;
+    float m = -INFINITY, l = 0.f;
+    f32x4 o[DP / 16];
+#pragma unroll
+    for (int n = 0; n < DP / 16; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    bool careful = false, apart = false;                      // V is looked through; V numbers have to be added apart
+    // Every tile has keys that some rows see and others do not, and 0 * infinity and 0 * NaN are NaN, which stays: where no
+    // row has one, nothing has reached a row that it should not have; where one has, everything is done again with care:
+    // numbers of V that are not finite leave the products and are added afterwards to the rows that see them.
+    for (;;) {
+        Where at{}, next{};
+        Entry entry{};
+        if (stop > 0) {
+            at = where(fetch(0), 0);
+            load(at, 0, IsK{});
+            load(at, 0, IsV{});
+            entry = fetch(kTile);
+        }
+        for (int kb = 0, buffer = 0; kb < stop; kb += kTile, buffer ^= 1) {
+            next = where(entry, kb + kTile);
+            __builtin_amdgcn_s_waitcnt(0);                    // this wave's share of this tile
+            __syncthreads();                                  // everyone's; and what is loaded over has been read
+            entry = fetch(kb + 2 * kTile);
+            if (kb + kTile < stop) {
+                load(next, buffer ^ 1, IsK{});
+                load(next, buffer ^ 1, IsV{});
+            }
+            const uint64_t listed = sees(at, min(stop - kb, kTile)) & at.here;
+            if (at.here != kAll || careful) {
+                bool dropped = false;
+                for (int i = (int)threadIdx.x; i < kTileBytes / 16; i += kBlockThreads) {
+                    uint4* piece = reinterpret_cast<uint4*>(tiles[buffer][1]) + i;
+                    const uint4 x = *piece;
+                    uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                    if (!((at.here >> (i / kChunks)) & 1u)) {
+                        *piece = make_uint4(0, 0, 0, 0);
+                    } else if (careful) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (not_finite16<DT>(w[e])) w[e] &= 0xFFFF0000u, dropped = true;
+                            if (not_finite16<DT>(w[e] >> 16)) w[e] &= 0x0000FFFFu, dropped = true;
+                        }
+                        *piece = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                apart |= __syncthreads_or(dropped) != 0;
+            }
+            at = next;
+            if (!__any(listed != 0)) continue;
+            const uint8_t *kt = tiles[buffer][0], *vt = tiles[buffer][1];
+            f32x4 sc[kSub];
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+                sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i)
+                    sc[u] = mfma16<DT>(*reinterpret_cast<const uint4*>(kt + (16 * u + col) * kRowBytes + k_swizzle(col, 4 * i + quad) * 16), qf[i], sc[u]);
+            }
+            const uint64_t mine = listed >> (4 * quad);       // keys 16 u + i of this lane
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t bits = u < 2 ? (uint32_t)mine : (uint32_t)(mine >> 32);
+                    sc[u][i] = bits >> (16 * (u % 2) + i) & 1u ? sc[u][i] * p.scale_log2 : -INFINITY;
+                    top = fmaxf(top, sc[u][i]);
+                }
+            top = max_halves(top);
+            top = fmaxf(top, __shfl_xor(top, 16));
+            // the reference of the exponentials follows the maximum only when that has grown by 2^8: weights up to 256 lose
+            // nothing in fp32 sums and 16-bit operands
+            if (__any(top > m + 8.f)) {
+                const float m_new = fmaxf(m, top);
+                const float fade = m_new == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+                m = m_new;
+                l *= fade;
+#pragma unroll
+                for (int n = 0; n < DP / 16; ++n) o[n] *= fade;
+            }
+            const float base = m == -INFINITY ? 0.f : m;      // no key seen yet: every power is 0
+            uint4 pf[kSub / 2];
+#pragma unroll
+            for (int h = 0; h < kSub / 2; ++h) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(sc[2 * h + e / 4][e % 4] - base);
+                    l += x[e];
+                }
+                // weights are rounded to the hot dtype for the product with V (their total is not)
+                pf[h] = make_uint4(pack_hot<DT>(x[0], x[1]), pack_hot<DT>(x[2], x[3]), pack_hot<DT>(x[4], x[5]), pack_hot<DT>(x[6], x[7]));
+            }
+#pragma unroll
+            for (int n = 0; n < DP / 16; ++n)
+#pragma unroll
+                for (int h = 0; h < kSub / 2; ++h) {
+                    uint2 v[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int row = 32 * h + 16 * u + 4 * quad + col / 4, chunk = 2 * n + (col & 3) / 2;
+                        v[u] = lds_read_transposed(vt + row * kRowBytes + v_swizzle(row, chunk) * 16 + (col & 1) * 8);
+                    }
+                    o[n] = mfma16<DT>(make_uint4(v[0].x, v[0].y, v[1].x, v[1].y), pf[h], o[n]);
+                }
+        }
+        bool odd = false;
+#pragma unroll
+        for (int n = 0; n < DP / 16; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd |= o[n][e] != o[n][e];
+        if (careful || __syncthreads_or(odd && r < rows) == 0) break;
+        careful = true;
+        apart = false;
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int n = 0; n < DP / 16; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (careful && apart) {
+        for (int nth = 0; nth * p.batch.page_tokens < stop; ++nth) {
+            const int2 of = list[nth];
+            const bool lists = masks[nth * mask_words + nth_token / 32] >> (nth_token & 31) & 1u;
+            for (int row = 0; row < p.batch.page_tokens && of.x * p.batch.page_tokens + row < seq.len; ++row) {
+                const bool seen = lists && of.x * p.batch.page_tokens + row < limit;
+                const uint8_t* src = p.v_pool + 2 * (of.y * p.v_page + ((int64_t)row * p.kv_heads + head) * p.head_dim);
+#pragma unroll
+                for (int n = 0; n < DP / 16; ++n) {
+                    const int d = 16 * n + 4 * quad;
+                    if (d >= p.head_dim || !seen) continue;
+                    const uint2 w = *reinterpret_cast<const uint2*>(src + 2 * d);
+                    const float x[4] = {hot_lo<DT>(w.x), hot_hi<DT>(w.x), hot_lo<DT>(w.y), hot_hi<DT>(w.y)};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][e] += __builtin_fabsf(x[e]) < INFINITY ? 0.f : x[e];
+                }
+            }
+        }
+    }
+    l += __shfl_xor(l, 16);
+    l = sum_halves(l);
+    if (r >= rows) return;
+    const float base = m == -INFINITY ? 0.f : m, inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    const int64_t row_head = (int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head;
+#pragma unroll
+    for (int n = 0; n < DP / 16; ++n) {
+        const int d = 16 * n + 4 * quad;
+        if (d < p.head_dim)
+            *reinterpret_cast<uint2*>(p.out + 2 * (row_head * p.head_dim + d)) =
+                make_uint2(pack_hot<DT>(o[n][0] * inv, o[n][1] * inv), pack_hot<DT>(o[n][2] * inv, o[n][3] * inv));
+    }
+    if (quad == 0 && p.lse) p.lse[row_head] = l == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
 // ---- host -------------------------------------------------------------------------
 
 struct SelectedPlan {
-    int waves, splits;
-    int64_t piece, floats;
+    int waves, splits;               // rows: waves of a workgroup, pieces of a unit
+    int64_t piece;
+    int64_t units, list;             // blocks: workgroups (0: by rows), columns of a workgroup's list
+    int64_t bytes;                   // of the workspace
 };
 
 SelectedPlan plan_selected(const ztcp_paged_batch* b, const ztcp_geometry* g, int64_t q_heads, int64_t listed, int cus) {
-    SelectedPlan plan{1, 1, listed * g->num_tokens, 0};
-    const int64_t units = b->n_rows * g->num_heads, keys = listed * g->num_tokens;
+    SelectedPlan plan{1, 1, listed * g->num_tokens, 0, 0, 0};
+    const int64_t heads = g->num_heads, group = q_heads / heads, rows = b->n_rows * group;
+    // by blocks if these keep half of the compute units busy and are not mostly empty: a sequence's last one may be
+    if (rows / kBlockRows * heads >= cus / 2 && rows >= 64 * b->n_seqs && b->max_pages <= kMostColumns) {
+        const int64_t most = block_tokens((int)group) * listed;
+        plan.units = ((rows + kBlockRows - 1) / kBlockRows + b->n_seqs) * heads;
+        plan.list = ((most < b->max_pages ? most : b->max_pages) + 31) / 32 * 32;   // whole lines: none is two workgroups'
+        plan.bytes = plan.units * plan.list * ((int64_t)sizeof(int2) + 4 * block_words((int)group));
+        return plan;
+    }
+    const int64_t units = b->n_rows * heads, keys = listed * g->num_tokens;
     if (units < 4 * (int64_t)cus) {
         plan.waves = g->head_dim <= 128 ? 8 : 4;
         const int64_t turn = 32 * plan.waves, most = (keys + turn - 1) / turn;
@@ -333,7 +758,7 @@ SelectedPlan plan_selected(const ztcp_paged_batch* b, const ztcp_geometry* g, in
         n = n > 1 ? n : 1;
         plan.piece = ((keys + n - 1) / n + turn - 1) / turn * turn;
         plan.splits = (int)((keys + plan.piece - 1) / plan.piece);
-        if (plan.splits > 1) plan.floats = b->n_rows * q_heads * plan.splits * (g->head_dim + 2);
+        if (plan.splits > 1) plan.bytes = b->n_rows * q_heads * plan.splits * (g->head_dim + 2) * (int64_t)sizeof(float);
     }
     return plan;
 }
@@ -359,7 +784,7 @@ extern "C" size_t ztcp_selected_attention_workspace(const ztcp_paged_batch* batc
     }
     int cus = 0;
     if (cu_count(cus) != ZTCP_OK) return (size_t)-1;
-    return (size_t)plan_selected(batch, g, q_heads, listed, cus).floats * sizeof(float);
+    return (size_t)plan_selected(batch, g, q_heads, listed, cus).bytes;
 }
 
 extern "C" int ztcp_selected_attention(const void* q, int64_t q_stride, void* out, float* lse, int64_t q_heads,
@@ -390,7 +815,7 @@ extern "C" int ztcp_selected_attention(const void* q, int64_t q_stride, void* ou
     int cus = 0;
     if (cu_count(cus) != ZTCP_OK) return ZTCP_EHIP;
     const SelectedPlan plan = plan_selected(batch, g, q_heads, listed, cus);
-    const int64_t need = plan.floats * (int64_t)sizeof(float);
+    const int64_t need = plan.bytes;
     if (need > 0 && (!workspace || (int64_t)workspace_bytes < need || !hot_aligned(workspace)))
         return arg_result(ZTCP_EINVAL, "workspace must hold ztcp_selected_attention_workspace bytes, 16-byte aligned");
     if (!misses(need ? workspace : nullptr, need) || bytes_overlap(workspace, need, out, out_bytes) ||
@@ -414,13 +839,25 @@ extern "C" int ztcp_selected_attention(const void* q, int64_t q_stride, void* ou
     p.splits = plan.splits;
     p.piece = (int32_t)plan.piece;
     p.partial = (float*)workspace;
+    p.lists = (int2*)workspace;
+    p.masks = (uint32_t*)((int2*)workspace + plan.units * plan.list);
+    p.list_stride = plan.list;
+    if (plan.units >= (int64_t)1 << 31) return arg_result(ZTCP_EINVAL, "too many rows and heads in one call");
     auto go = [&](auto dt, auto dp) {
         constexpr int DT = decltype(dt)::value, DP = decltype(dp)::value, kMany = DP <= 128 ? 8 : 4;
+        if (plan.units > 0) {
+            const bool even = g->num_tokens % (block_tile(DP) / kBlockWaves) == 0 && d == DP;
+            const bool one = block_words(p.group) == 1;
+            launch_blocks(one ? even ? block_kernel<DT, DP, true, 1> : block_kernel<DT, DP, false, 1>
+                              : even ? block_kernel<DT, DP, true, 4> : block_kernel<DT, DP, false, 4>,
+                          (uint64_t)plan.units, kBlockThreads, 0, (hipStream_t)stream, p);
+            return;
+        }
         const uint64_t units = (uint64_t)batch->n_rows * (uint64_t)g->num_heads * (uint64_t)plan.splits;
         if (plan.waves == 1) launch_blocks(selected_kernel<DT, DP, 1>, units, 64, 0, (hipStream_t)stream, p);
         else launch_blocks(selected_kernel<DT, DP, kMany>, units, 64 * kMany, 0, (hipStream_t)stream, p);
         if (plan.splits > 1)
-            launch_blocks(join_kernel<DT>, ((uint64_t)batch->n_rows * (uint64_t)q_heads + 3) / 4, 256, 0, (hipStream_t)stream, p);
+            launch_blocks(join_selected_kernel<DT>, ((uint64_t)batch->n_rows * (uint64_t)q_heads + 3) / 4, 256, 0, (hipStream_t)stream, p);
     };
     auto by_width = [&](auto dt) {
         if (d <= 64) go(dt, std::integral_constant<int, 64>{});
