@@ -505,9 +505,10 @@ ZTCP_API int ztcp_selected_attention(const void* q, int64_t q_stride, void* out,
  *   page * num_tokens + token in page (-1 where its entry is negative), and
  *   next_positions[s] + i (NULL: L + i); -1 and 0 behind the last row;
  *   out_next_positions [n_seqs] = next_positions + granted (may be next_positions).
- * workspace: ztcp_allot_pages_workspace(n_seqs) bytes ((size_t)-1 if the call refuses
- * n_seqs), needed until the call's work is done, by one call at a time. */
-ZTCP_API size_t ztcp_allot_pages_workspace(int64_t n_seqs);
+ * workspace: ztcp_allot_pages_workspace(...) bytes (may be 0; (size_t)-1 for numbers that
+ * the call refuses), 16-byte aligned, needed until the call's work is done, by one call
+ * at a time. */
+ZTCP_API size_t ztcp_allot_pages_workspace(int64_t n_seqs, int64_t max_rows);
 ZTCP_API int ztcp_allot_pages(int32_t* page_table, int64_t table_stride, int64_t max_pages, const int32_t* kv_lens,
                      const int32_t* q_lens, int64_t n_seqs, const int32_t* free_pages, int64_t capacity,
                      const int32_t* n_free, const int32_t* next_positions, int64_t num_tokens, int64_t max_rows,
@@ -521,7 +522,7 @@ ZTCP_API int ztcp_allot_pages(int32_t* page_table, int64_t table_stride, int64_t
  * out_table has -1 in their place and is page_table elsewhere.  What the stack has no
  * room for stays in the table.  out_n_free [1], n_released [n_seqs].  out_table and
  * out_n_free may be the inputs themselves.  An entry that occurs twice is given back
- * twice.  workspace: ztcp_release_pages_workspace(...) bytes, as above. */
+ * twice.  workspace: ztcp_release_pages_workspace(...) bytes, 8-byte aligned, as above. */
 ZTCP_API size_t ztcp_release_pages_workspace(int64_t n_seqs, int64_t max_pages);
 ZTCP_API int ztcp_release_pages(const int32_t* page_table, int64_t table_stride, int64_t max_pages, const int32_t* kv_lens,
                        int64_t n_seqs, int64_t num_tokens, int32_t* free_pages, int64_t capacity,

@@ -74,6 +74,20 @@ def test_allot(A, seqs, cols, page, max_len, max_q, in_place):
                      (seqs, seed))
 
 
+def test_allot_where_only_some_wait(A):
+    """More sequences than one turn adds up: those of the first that need pages wait, the others' rows close up."""
+    _say("allot, waiting in an early turn")
+    seqs = 9000
+    lens = torch.full((seqs,), 5, dtype=torch.int32, device="cuda")
+    lens[::7] = 16                                   # these need a page for the next token
+    table = torch.arange(seqs * 2, dtype=torch.int32, device="cuda").reshape(seqs, 2).contiguous()
+    wanted = torch.ones_like(lens)
+    for rows in (seqs, seqs - 10, 3000):
+        for free in (0, 50, 700, seqs):
+            _check_allot(A, table.clone(), lens, wanted, torch.arange(seqs, dtype=torch.int32, device="cuda") + 10 ** 6, _i32([free]), 16,
+                         rows, what=(rows, free))
+
+
 def test_allot_wrong_numbers(A):
     """Negative and too large lengths and requests, a stack with fewer entries than n_free says, negative ids."""
     _say("allot, wrong numbers")

@@ -33,20 +33,21 @@ def _release(N, **kw):
 COMMON = [(dict(s=-1), "n_seqs"), (dict(s=1 << 24), "n_seqs"), (dict(t=0), "num_tokens"), (dict(cols=0), "num_tokens"),
           (dict(t=1 << 31), "num_tokens"), (dict(cols=1 << 27), "below 2^31"), (dict(stride=7), "cover"),
           (dict(table=None), "page_table"), (dict(cap=-1), "capacity"), (dict(cap=1 << 31), "capacity"), (dict(lens=None), "NULL"),
-          (dict(n_free=None), "NULL"), (dict(free=None), "NULL"), (dict(on=None), "NULL"), (dict(work=None), "workspace"),
-          (dict(work=B + 0xB0002), "workspace"), (dict(bytes=16), "workspace")]
+          (dict(n_free=None), "NULL"), (dict(free=None), "NULL"), (dict(on=None), "NULL")]
+WORK = [(dict(work=None), "workspace"), (dict(work=B + 0xB0002), "workspace"), (dict(bytes=16), "workspace")]
 
 
 @pytest.mark.parametrize("kw,why", COMMON + [
     (dict(rows=-1), "max_rows"), (dict(rows=(1 << 31) - 1024), "max_rows"), (dict(counts=B + 0xC0000), "both"),
     (dict(oc=B + 0xC0000), "both"), (dict(wanted=None), "NULL"), (dict(ol=None), "NULL"), (dict(starts=None), "NULL"),
-    (dict(slots=None), "NULL"), (dict(pos=None), "NULL"), (dict(granted=None), "NULL")])
+    (dict(slots=None), "NULL"), (dict(pos=None), "NULL"), (dict(granted=None), "NULL")]
+    + [(dict(kw, rows=5000), why) for kw, why in WORK])
 def test_allot_arguments(N, kw, why):
     rc, msg = _allot(N, **kw)
     assert rc == N.EINVAL and why in msg, msg
 
 
-@pytest.mark.parametrize("kw,why", COMMON + [(dict(ots=7), "cover"), (dict(ot=None), "NULL"), (dict(released=None), "NULL")])
+@pytest.mark.parametrize("kw,why", COMMON + WORK + [(dict(ots=7), "cover"), (dict(ot=None), "NULL"), (dict(released=None), "NULL")])
 def test_release_arguments(N, kw, why):
     rc, msg = _release(N, **kw)
     assert rc == N.EINVAL and why in msg, msg
@@ -54,7 +55,7 @@ def test_release_arguments(N, kw, why):
 
 def test_overlaps(N):
     for kw in (dict(ol=B + 0x20000), dict(ol=B + 0x10004), dict(on=B + 0x10000), dict(starts=B + 4), dict(slots=B + 0x30000),
-               dict(pos=B + 0x80008), dict(granted=B + 0x50000), dict(work=B + 0x70000), dict(free=B + 16), dict(lens=B),
+               dict(pos=B + 0x80008), dict(granted=B + 0x50000), dict(work=B + 0x70000, rows=5000), dict(free=B + 16), dict(lens=B),
                dict(counts=B + 0xC0000, oc=B + 0xC0004)):
         assert _allot(N, **kw)[0] == N.EOVERLAP, kw
     for kw in (dict(ot=B + 4), dict(ot=B, ots=16), dict(on=B), dict(released=B + 0x10000), dict(free=B + 8), dict(work=B + 0x30000),
@@ -64,7 +65,9 @@ def test_overlaps(N):
 
 def test_workspaces(N):
     L, bad = N.lib(), (1 << 64) - 1
-    assert L.ztcp_allot_pages_workspace(0) >= 4 and L.ztcp_allot_pages_workspace(-1) == bad == L.ztcp_allot_pages_workspace(1 << 24)
+    assert L.ztcp_allot_pages_workspace(0, 0) == 0 and L.ztcp_allot_pages_workspace(2000, 10) >= 16 * 2000
+    for args in ((-1, 1), (1 << 24, 1), (1, -1), (1, (1 << 31) - 1024)):
+        assert L.ztcp_allot_pages_workspace(*args) == bad
     assert L.ztcp_release_pages_workspace(3, 10) >= 8 * 4
     for args in ((-1, 1), (1 << 24, 1), (1, 0), (1, 1 << 31)):
         assert L.ztcp_release_pages_workspace(*args) == bad

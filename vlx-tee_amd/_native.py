@@ -188,7 +188,7 @@ def lib() -> C.CDLL:
     L.ztcp_selected_attention_workspace.restype = C.c_size_t
     L.ztcp_selected_attention.argtypes = [P, i64, P, P, i64, PP, PB, G, P, i64, f32, P, C.c_size_t, P]
     L.ztcp_selected_attention.restype = i32
-    L.ztcp_allot_pages_workspace.argtypes = [i64]
+    L.ztcp_allot_pages_workspace.argtypes = [i64, i64]
     L.ztcp_allot_pages_workspace.restype = C.c_size_t
     L.ztcp_allot_pages.argtypes = [P, i64, i64, P, P, i64, P, i64, P, P, i64, i64, P, P, P, P, P, P, P, P, C.c_size_t, P]
     L.ztcp_allot_pages.restype = i32

@@ -18,6 +18,7 @@
 #include <cmath>
 #include <stdexcept>
 #include <string>
+#include <vector>
 
 #include "../../include/ztcp.h"
 
@@ -398,6 +399,36 @@ PyObject* evict_pages(PyObject* const* a) {
     return all;
 }
 
+// Several outputs of one call in one allocation: the caching allocator takes most of a small call's host time.
+struct Together {
+    struct Part {
+        int64_t at;
+        std::vector<int64_t> shape;
+        at::ScalarType type;
+    };
+    std::vector<Part> parts;
+    int64_t bytes = 0;
+    at::Tensor all;
+    size_t add(at::IntArrayRef shape, at::ScalarType type) {
+        int64_t n = (int64_t)c10::elementSize(type);
+        for (int64_t x : shape) n *= x;
+        parts.push_back(Part{bytes, shape.vec(), type});
+        bytes += (n + 63) / 64 * 64;
+        return parts.size() - 1;
+    }
+    void allocate(const at::Device& d) { all = make({bytes > 0 ? bytes : 1}, at::kByte, d); }
+    void* data(size_t i) const { return (uint8_t*)all.data_ptr() + parts[i].at; }
+    at::Tensor tensor(size_t i) const {
+        const Part& x = parts[i];
+        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(),
+                                                                 c10::scalarTypeToTypeMeta(x.type));
+        c10::TensorImpl* impl = t.unsafeGetTensorImpl();
+        impl->set_storage_offset(x.at / (int64_t)c10::elementSize(x.type));
+        impl->set_sizes_contiguous(x.shape);
+        return t;
+    }
+};
+
 PyObject* tuple_of(const at::Tensor* out, int n) {   // None for an undefined one
     PyObject* all = PyTuple_New(n);
     for (int i = 0; all && i < n; ++i) {
@@ -428,25 +459,35 @@ PyObject* allot_pages(PyObject* const* a) {
     const void* n_free_ptr = Pool::plain(*n_free, "n_free", at::kInt, {1}, d);
     const void* counts_ptr = counts ? Pool::plain(*counts, "next_positions", at::kInt, {s}, d) : nullptr;
     need(rows >= 0, "max_rows must not be negative");
-    at::Tensor out[7];
-    out[0] = in_place ? *lens : make({s}, at::kInt, d);
-    out[1] = in_place ? *n_free : make({1}, at::kInt, d);
-    out[2] = make({s + 1}, at::kInt, d);
-    out[3] = make({rows}, at::kLong, d);
-    out[4] = make({rows}, at::kInt, d);
-    out[5] = make({s}, at::kInt, d);
-    if (counts) out[6] = in_place ? *counts : make({s}, at::kInt, d);
+    const size_t bytes = ztcp_allot_pages_workspace(s, rows);
+    need(bytes != (size_t)-1, "too many sequences or rows");
+    Together made;
+    made.add({rows}, at::kLong);   // in the order of `fields`
+    made.add({rows}, at::kInt);
+    made.add({s + 1}, at::kInt);
+    made.add({s}, at::kInt);
+    const int fields[4] = {3, 4, 2, 5};
+    if (!in_place) {
+        made.add({s}, at::kInt);
+        made.add({1}, at::kInt);
+        if (counts) made.add({s}, at::kInt);
+    }
     const c10::DeviceGuard guard(d);
-    const size_t bytes = ztcp_allot_pages_workspace(s);
-    need(bytes != (size_t)-1, "too many sequences");
-    const at::Tensor work = make({(int64_t)bytes}, at::kByte, d);
+    made.allocate(d);
+    const at::Tensor work = bytes ? make({(int64_t)bytes}, at::kByte, d) : at::Tensor();
     done(ztcp_allot_pages((int32_t*)table->data_ptr(), stride, mp, (const int32_t*)lens_ptr, (const int32_t*)wanted_ptr, s,
                           (const int32_t*)free_ptr, free_pages->numel(), (const int32_t*)n_free_ptr, (const int32_t*)counts_ptr,
-                          tokens, rows, (int32_t*)out[0].data_ptr(), (int32_t*)out[1].data_ptr(),
-                          counts ? (int32_t*)out[6].data_ptr() : nullptr, (int32_t*)out[2].data_ptr(),
-                          (int64_t*)out[3].data_ptr(), (int32_t*)out[4].data_ptr(), (int32_t*)out[5].data_ptr(), work.data_ptr(),
+                          tokens, rows, (int32_t*)(in_place ? lens->data_ptr() : made.data(4)),
+                          (int32_t*)(in_place ? n_free->data_ptr() : made.data(5)),
+                          (int32_t*)(!counts ? nullptr : in_place ? counts->data_ptr() : made.data(6)), (int32_t*)made.data(2),
+                          (int64_t*)made.data(0), (int32_t*)made.data(1), (int32_t*)made.data(3), bytes ? work.data_ptr() : nullptr,
                           bytes, stream_of(d)),
          "allot_pages");
+    at::Tensor out[7];
+    for (int i = 0; i < 4; ++i) out[fields[i]] = made.tensor(i);
+    out[0] = in_place ? *lens : made.tensor(4);
+    out[1] = in_place ? *n_free : made.tensor(5);
+    if (counts) out[6] = in_place ? *counts : made.tensor(6);
     written(table);
     for (const at::Tensor* t : {lens, n_free, counts}) written(in_place ? t : nullptr);
     return tuple_of(out, 7);
@@ -463,18 +504,27 @@ PyObject* release_pages(PyObject* const* a) {
     const void* lens_ptr = Pool::plain(*lens, "kv_lens", at::kInt, {s}, d);
     void* free_ptr = Pool::plain(*free_pages, "free_pages", at::kInt, {free_pages->numel()}, d);
     const void* n_free_ptr = Pool::plain(*n_free, "n_free", at::kInt, {1}, d);
-    at::Tensor out[3];
-    out[0] = in_place ? *table : make({s, mp}, at::kInt, d);
-    out[1] = in_place ? *n_free : make({1}, at::kInt, d);
-    out[2] = make({s}, at::kInt, d);
-    const c10::DeviceGuard guard(d);
     const size_t bytes = ztcp_release_pages_workspace(s, mp);
     need(bytes != (size_t)-1, "too many sequences or pages");
+    Together made;
+    made.add({s}, at::kInt);
+    if (!in_place) {
+        made.add({s, mp}, at::kInt);
+        made.add({1}, at::kInt);
+    }
+    const c10::DeviceGuard guard(d);
+    made.allocate(d);
     const at::Tensor work = make({(int64_t)bytes}, at::kByte, d);
-    done(ztcp_release_pages((const int32_t*)table->data_ptr(), stride, mp, (const int32_t*)lens_ptr, s, tokens, (int32_t*)free_ptr,
-                            free_pages->numel(), (const int32_t*)n_free_ptr, (int32_t*)out[0].data_ptr(), in_place ? stride : mp,
-                            (int32_t*)out[1].data_ptr(), (int32_t*)out[2].data_ptr(), work.data_ptr(), bytes, stream_of(d)),
+    done(ztcp_release_pages((int32_t*)table->data_ptr(), stride, mp, (const int32_t*)lens_ptr, s, tokens, (int32_t*)free_ptr,
+                            free_pages->numel(), (const int32_t*)n_free_ptr,
+                            (int32_t*)(in_place ? table->data_ptr() : made.data(1)), in_place ? stride : mp,
+                            (int32_t*)(in_place ? n_free->data_ptr() : made.data(2)), (int32_t*)made.data(0), work.data_ptr(), bytes,
+                            stream_of(d)),
          "release_pages");
+    at::Tensor out[3];
+    out[0] = in_place ? *table : made.tensor(1);
+    out[1] = in_place ? *n_free : made.tensor(2);
+    out[2] = made.tensor(0);
     written(free_pages);
     for (const at::Tensor* t : {table, n_free}) written(in_place ? t : nullptr);
     return tuple_of(out, 3);

@@ -16,6 +16,14 @@ namespace {
 // without gaps, page i of a sequence from place n_free - 1 - (P - needed) - i.
 //
 // Every new page begins with a new token, whose row writes the table's entry.
+//
+// All is latency: one workgroup, a few sequences to a thread, adds up once (sums that pass
+// 2^32 stay there, which no limit reaches), and only if some sequence has to wait once
+// more, for the rows granted.  Up to 4,096 rows it lays these out as well; more are laid
+// out by a second launch, whose workgroups find their sequences by what the first left
+// them.  64 decoding sequences: 4.6 us (9.6 a pass with an allocation for each output, 6.0
+// with one); 2,048 sequences of 246,000 rows: 8.6 and 6 us (12 and 9 with sums of 64 bits,
+// one sequence a thread, and searches in memory).
 
 struct AllotParams {
     int32_t* table;
@@ -35,19 +43,44 @@ struct AllotParams {
     int64_t* slots;
     int32_t* positions;
     int32_t* granted;
-    int32_t* before;                 // [n_seqs] pages taken by the sequences in front
-    int32_t* had;                    // free pages there were
+    int32_t* had;                    // for the second launch: free pages there were,
+    int32_t* hints;                  // the sequence of each block's first row,
+    int4* parts;                     // and of each sequence its first row, length, pages taken in front, count
     uint32_t first_block;            // of this launch
 };
 
-constexpr int kPlanThreads = 1024;
-constexpr int kOneLaunchRows = 4096;
+constexpr int kOneLaunchSeqs = 1024, kOneLaunchRows = 4096;
+constexpr int kRowsABlock = 1024;
 
-struct Sum2 {
-    int64_t rows, pages;
+// Sums of rows and pages; what passes 2^32 stays at its end.
+struct Sums {
+    uint32_t rows, pages;
 };
-__device__ __forceinline__ Sum2 up(Sum2 x, int m) {
-    return Sum2{(int64_t)__shfl_up((long long)x.rows, m), (int64_t)__shfl_up((long long)x.pages, m)};
+__device__ __forceinline__ uint32_t add(uint32_t a, uint32_t b) { return a + b < a ? ~0u : a + b; }
+__device__ __forceinline__ Sums add(Sums a, Sums b) { return Sums{add(a.rows, b.rows), add(a.pages, b.pages)}; }
+
+// The sum over the threads in front, and over all.
+template <int WAVES>
+__device__ __forceinline__ Sums sum_before(Sums x, Sums (&lds)[WAVES], Sums& all) {
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    Sums upto = x;
+    for (int m = 1; m < 64; m <<= 1) {
+        const Sums y{(uint32_t)__shfl_up((int)upto.rows, m), (uint32_t)__shfl_up((int)upto.pages, m)};
+        if (lane >= m) upto = add(upto, y);
+    }
+    const Sums last{(uint32_t)__shfl_up((int)upto.rows, 1), (uint32_t)__shfl_up((int)upto.pages, 1)};
+    __syncthreads();                                         // the sums of the turn before have been read
+    if (lane == 63) lds[wave] = upto;
+    __syncthreads();
+    Sums before = lane > 0 ? last : Sums{0, 0};
+    all = Sums{0, 0};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        const Sums y = lds[w];
+        if (w < wave) before = add(before, y);
+        all = add(all, y);
+    }
+    return before;
 }
 
 // Pages that hold so many tokens.
@@ -72,71 +105,87 @@ __device__ __forceinline__ void fill_row(const AllotParams& p, int64_t row, int 
     p.positions[row] = count + nth;
 }
 
-// Sums over the sequences, by one workgroup; ROWS: and the rows too (sequences fit into one turn).
-template <bool ROWS>
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(AllotParams p) {
-    __shared__ Sum2 waves[kPlanThreads / 64];
-    __shared__ int32_t granted_upto[ROWS ? kPlanThreads : kPlanThreads / 64];
-    __shared__ int32_t lens[ROWS ? kPlanThreads : 1], before_of[ROWS ? kPlanThreads : 1], counts[ROWS ? kPlanThreads : 1];
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// The sequence of a row among parts low .. high: the last that starts at it or in front.
+__device__ __forceinline__ int part_of(const int4* parts, int low, int high, int row) {
+    while (low < high) {
+        const int mid = (low + high + 1) >> 1;
+        if (parts[mid].x <= row) low = mid;
+        else high = mid - 1;
+    }
+    return low;
+}
+
+// ROWS: and the rows too (the sequences fit into one turn).
+template <int THREADS, bool ROWS>
+__global__ __launch_bounds__(THREADS) void plan_kernel(AllotParams p) {
+    constexpr int kOwn = 4, kWaves = THREADS / 64;           // sequences of a thread, side by side
+    __shared__ Sums lds[kWaves];
+    __shared__ int4 parts[ROWS ? kOneLaunchSeqs : 1];
+    const int tid = (int)threadIdx.x;
     const int had = (int)min((int64_t)max(*p.n_free, 0), p.capacity);
-    Sum2 base{0, 0};
+    Sums base{0, 0};
     int start = 0, taken = 0;                                // rows and pages granted in the turns before
-    for (int first = 0; first < p.n_seqs; first += kPlanThreads) {
-        const int s = first + tid;
-        const bool is = s < p.n_seqs;
-        const int len = is ? min(max(p.lens[s], 0), p.max_tokens) : 0;
-        int want = is ? max(p.wanted[s], 0) : 0;
-        if (want > p.max_tokens - len) want = 0;
-        const int count = is ? (p.counts ? p.counts[s] : len) : 0;
-        const int need = pages_for(p, len + want) - pages_for(p, len);
-        Sum2 x{want, need};
-        for (int m = 1; m < 64; m <<= 1) {
-            const Sum2 y = up(x, m);
-            if (lane >= m) x.rows += y.rows, x.pages += y.pages;
-        }
-        __syncthreads();                                     // the last turn's sums have been read
-        if (lane == 63) waves[wave] = x;
-        __syncthreads();
-        x.rows += base.rows, x.pages += base.pages;
+    for (int first = 0; first < p.n_seqs; first += THREADS * kOwn) {
+        const int s0 = first + tid * kOwn;
+        int len[kOwn], want[kOwn], count[kOwn], need[kOwn];
 #pragma unroll
-        for (int w = 0; w < kPlanThreads / 64; ++w) {
-            const Sum2 y = waves[w];
-            if (w < wave) x.rows += y.rows, x.pages += y.pages;
-            base.rows += y.rows, base.pages += y.pages;
+        for (int i = 0; i < kOwn; ++i) {
+            const bool is = s0 + i < p.n_seqs;
+            len[i] = is ? p.lens[s0 + i] : 0;
+            want[i] = is ? p.wanted[s0 + i] : 0;
+            count[i] = is && p.counts ? p.counts[s0 + i] : 0;
         }
-        const bool served = x.rows <= p.max_rows && (need == 0 || x.pages <= had);
-        const int grant = served ? want : 0, before = (int)min(x.pages - need, (int64_t)had);
-        // rows granted: a second sum, of at most max_rows
-        int g = grant;
-        for (int m = 1; m < 64; m <<= 1) {
-            const int y = __shfl_up(g, m);
-            if (lane >= m) g += y;
-        }
-        int most = served && need > 0 ? (int)x.pages : 0;    // pages taken up to the last one served
-        for (int m = 1; m < 64; m <<= 1) most = max(most, __shfl_xor(most, m));
-        __shared__ int32_t rows_of[kPlanThreads / 64], pages_of[kPlanThreads / 64];
-        if (lane == 63) rows_of[wave] = g, pages_of[wave] = most;
-        __syncthreads();
-        int from = start;
+        Sums own{0, 0};
 #pragma unroll
-        for (int w = 0; w < kPlanThreads / 64; ++w) {
-            if (w < wave) from += rows_of[w];
-            start += rows_of[w];
-            taken = max(taken, pages_of[w]);
+        for (int i = 0; i < kOwn; ++i) {
+            len[i] = min(max(len[i], 0), p.max_tokens);
+            want[i] = max(want[i], 0);
+            if (want[i] > p.max_tokens - len[i]) want[i] = 0;
+            if (!p.counts) count[i] = len[i];
+            need[i] = pages_for(p, len[i] + want[i]) - pages_for(p, len[i]);
+            own = add(own, Sums{(uint32_t)want[i], (uint32_t)need[i]});
         }
-        from += g - grant;
-        if (is) {
+        Sums all;
+        const Sums in_front = sum_before(own, lds, all);     // in this turn
+        Sums upto = add(base, in_front);
+        base = add(base, all);
+        int before[kOwn];
+        bool every = true;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            before[i] = (int)min(upto.pages, (uint32_t)had);
+            upto = add(upto, Sums{(uint32_t)want[i], (uint32_t)need[i]});
+            const bool served = upto.rows <= (uint64_t)p.max_rows && (need[i] == 0 || upto.pages <= (uint32_t)had);
+            every &= served;
+            if (!served) want[i] = need[i] = 0;
+        }
+        Sums granted = in_front, in_all = all;               // what is granted in front of this thread's, and to all, in this turn
+        if (!__syncthreads_and(every)) {
+            own = Sums{0, 0};
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) own = add(own, Sums{(uint32_t)want[i], (uint32_t)need[i]});
+            granted = sum_before(own, lds, in_all);
+        }
+        int from = start + (int)granted.rows;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            const int s = s0 + i;
+            if (s >= p.n_seqs) break;
             p.starts[s] = from;
-            p.granted[s] = grant;
-            p.out_lens[s] = len + grant;
-            if (p.out_counts) p.out_counts[s] = count + grant;
-            if (!ROWS) p.before[s] = before;
+            p.granted[s] = want[i];
+            p.out_lens[s] = len[i] + want[i];
+            if (p.out_counts) p.out_counts[s] = count[i] + want[i];
+            const int4 part = make_int4(from, len[i], before[i], count[i]);
+            if constexpr (ROWS) {
+                parts[s] = part;
+            } else {
+                p.parts[s] = part;
+                for (int block = (from + kRowsABlock - 1) / kRowsABlock; block * kRowsABlock < from + want[i]; ++block) p.hints[block] = s;
+            }
+            from += want[i];
         }
-        if constexpr (ROWS) {
-            granted_upto[tid] = from + grant;
-            lens[tid] = len, before_of[tid] = before, counts[tid] = count;
-        }
+        start += (int)in_all.rows;
+        taken += (int)in_all.pages;
     }
     if (tid == 0) {
         p.starts[p.n_seqs] = start;
@@ -145,32 +194,32 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(AllotParams p) {
     }
     if constexpr (ROWS) {
         __syncthreads();
-        for (int row = tid; row < p.max_rows; row += kPlanThreads) {
+        for (int row = tid; row < p.max_rows; row += THREADS) {
             if (row >= start) {
                 p.slots[row] = -1;
                 p.positions[row] = 0;
                 continue;
             }
-            int low = 0, high = p.n_seqs - 1;                // the first sequence that ends behind the row
-            while (low < high) {
-                const int mid = (low + high) >> 1;
-                if (granted_upto[mid] > row) high = mid;
-                else low = mid + 1;
-            }
-            fill_row(p, row, low, low ? granted_upto[low - 1] : 0, lens[low], before_of[low], counts[low], had);
+            const int s = part_of(parts, 0, p.n_seqs - 1, row);
+            const int4 part = parts[s];
+            fill_row(p, row, s, part.x, part.y, part.z, part.w, had);
         }
     }
 }
 
-constexpr int kRowsABlock = 1024;
-
 __global__ __launch_bounds__(256) void rows_kernel(AllotParams p) {
-    const int64_t row0 = ((int64_t)p.first_block + blockIdx.x) * kRowsABlock;
+    __shared__ int4 parts[kRowsABlock];
+    const int64_t block = (int64_t)p.first_block + blockIdx.x, row0 = block * kRowsABlock;
     const int total = p.starts[p.n_seqs], had = *p.had;
-    int low0 = 0, high0 = 0;
+    int low = 0, high = 0;
+    bool staged = false;
     if (row0 < total) {
-        low0 = find_above(p.starts + 1, p.n_seqs, (int)row0);
-        high0 = find_above(p.starts + 1, p.n_seqs, (int)min(row0 + kRowsABlock, (int64_t)total) - 1);
+        low = p.hints[block];
+        high = row0 + kRowsABlock < total ? p.hints[block + 1] : p.n_seqs - 1;
+        staged = high - low < kRowsABlock;
+        if (staged)
+            for (int i = (int)threadIdx.x; i <= high - low; i += 256) parts[i] = p.parts[low + i];
+        __syncthreads();
     }
 #pragma unroll
     for (int i = 0; i < kRowsABlock / 256; ++i) {
@@ -181,23 +230,26 @@ __global__ __launch_bounds__(256) void rows_kernel(AllotParams p) {
             p.positions[row] = 0;
             continue;
         }
-        int low = low0, high = high0;
-        while (low < high) {
-            const int mid = (low + high) >> 1;
-            if (p.starts[mid + 1] > row) high = mid;
-            else low = mid + 1;
+        int s;
+        int4 part;
+        if (staged) {
+            s = part_of(parts, 0, high - low, (int)row);
+            part = parts[s];
+            s += low;
+        } else {
+            s = part_of(p.parts, low, high, (int)row);
+            part = p.parts[s];
         }
-        const int grant = p.granted[low];
-        const int len = p.out_lens[low] - grant;             // lengths and counts may have been updated in place
-        const int count = p.out_counts ? p.out_counts[low] - grant : len;
-        fill_row(p, row, low, p.starts[low], len, p.before[low], count, had);
+        fill_row(p, row, s, part.x, part.y, part.z, part.w, had);
     }
 }
 
 // ---- pages given back -------------------------------------------------------------
 // Entries that are pages, in columns that a sequence's tokens do not reach, in the
 // order of sequences and columns onto the end of the stack.  The first kernel counts
-// them by pieces of rows, the second adds up what lies before its piece.
+// them by pieces of rows, the second adds up what lies before its piece; a thread has
+// all its entries of a piece on their way at once.  512 sequences of up to 4,098 columns,
+// a quarter ended (17 MB): 6.5 and 7.5 us (6 and 14 with 256 columns at a time).
 
 constexpr int kPiece = 4096;        // columns
 
@@ -237,8 +289,16 @@ __global__ __launch_bounds__(256) void release_count_kernel(ReleaseParams p) {
     const int s = (int)(unit / p.pieces), piece = (int)(unit % p.pieces);
     const int32_t* row = p.table + s * p.table_stride;
     const int end = (int)min((int64_t)(piece + 1) * kPiece, (int64_t)p.max_pages);
+    const int spare = first_spare(p, s);
+    int32_t id[kPiece / 256];
+#pragma unroll
+    for (int j = 0; j < kPiece / 256; ++j) {
+        const int i = piece * kPiece + j * 256 + (int)threadIdx.x;
+        id[j] = i < end && i >= spare ? row[i] : -1;
+    }
     int64_t n = 0;
-    for (int i = max(piece * kPiece, first_spare(p, s)) + (int)threadIdx.x; i < end; i += 256) n += row[i] >= 0;
+#pragma unroll
+    for (int j = 0; j < kPiece / 256; ++j) n += id[j] >= 0;
     n = block_sum(n, lds);
     if (threadIdx.x == 0) {
         p.counts[1 + unit] = n;
@@ -248,7 +308,8 @@ __global__ __launch_bounds__(256) void release_count_kernel(ReleaseParams p) {
 
 __global__ __launch_bounds__(256) void release_kernel(ReleaseParams p) {
     __shared__ int64_t lds[4];
-    __shared__ int scan[2][4];
+    __shared__ int scan[64];
+    static_assert(kPiece / 256 * 4 == 64, "a lane for each wave's part");
     const int64_t unit = (int64_t)p.first_block + blockIdx.x;
     const int s = (int)(unit / p.pieces), piece = (int)(unit % p.pieces);
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -267,23 +328,35 @@ __global__ __launch_bounds__(256) void release_kernel(ReleaseParams p) {
     if (unit == last && tid == 0) *p.out_n_free = (int32_t)min(at + p.counts[1 + unit], p.capacity);
     const int begin = piece * kPiece, end = (int)min((int64_t)begin + kPiece, (int64_t)p.max_pages), spare = first_spare(p, s);
     const bool moved = out != row;
-    for (int base = moved ? begin : max(begin, spare / 256 * 256), turn = 0; base < end; base += 256, turn ^= 1) {
-        const int i = base + tid;
-        const int32_t id = i < end ? row[i] : -1;
-        const bool goes = i >= spare && id >= 0;
-        const uint64_t all = __ballot(goes);
-        if (lane == 0) scan[turn][wave] = __popcll(all);
-        __syncthreads();
-        int64_t to = at + __popcll(all & ((1ull << lane) - 1));
+    if (!moved && p.counts[1 + unit] == 0) return;
+    constexpr int kOwn = kPiece / 256;
+    int32_t id[kOwn];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const int n = scan[turn][w];
-            if (w < wave) to += n;
-            at += n;
-        }
+    for (int j = 0; j < kOwn; ++j) {
+        const int i = begin + j * 256 + tid;
+        id[j] = i < end && (moved || i >= spare) ? row[i] : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+        const uint64_t all = __ballot(begin + j * 256 + tid >= spare && id[j] >= 0);
+        if (lane == 0) scan[4 * j + wave] = __popcll(all);
+    }
+    __syncthreads();
+    int upto = scan[lane];                                    // of 256 columns' four waves' counts, in their order
+    const int mine = upto;
+    for (int m = 1; m < 64; m <<= 1) {
+        const int y = __shfl_up(upto, m);
+        upto += lane >= m ? y : 0;
+    }
+    upto -= mine;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+        const int i = begin + j * 256 + tid;
+        const bool goes = i >= spare && id[j] >= 0;
+        const int64_t to = at + __shfl(upto, 4 * j + wave) + __popcll(__ballot(goes) & ((1ull << lane) - 1));
         const bool fits = goes && to < p.capacity;
-        if (fits) p.free_pages[to] = id;
-        if (i < end && (moved || fits)) out[i] = fits ? -1 : id;
+        if (fits) p.free_pages[to] = id[j];
+        if (i < end && (moved || fits)) out[i] = fits ? -1 : id[j];
     }
 }
 
@@ -311,8 +384,11 @@ int64_t release_pieces(int64_t max_pages) { return (max_pages + kPiece - 1) / kP
 
 }  // namespace
 
-extern "C" size_t ztcp_allot_pages_workspace(int64_t n_seqs) {
-    return n_seqs < 0 || n_seqs >= (int64_t)1 << 24 ? (size_t)-1 : (size_t)(n_seqs + 1) * sizeof(int32_t);
+extern "C" size_t ztcp_allot_pages_workspace(int64_t n_seqs, int64_t max_rows) {
+    if (n_seqs < 0 || n_seqs >= (int64_t)1 << 24 || max_rows < 0 || max_rows >= ((int64_t)1 << 31) - 1024) return (size_t)-1;
+    if (n_seqs <= kOneLaunchSeqs && max_rows <= kOneLaunchRows) return 0;
+    const int64_t blocks = (max_rows + kRowsABlock - 1) / kRowsABlock;
+    return (size_t)(n_seqs * (int64_t)sizeof(int4) + 4 * (blocks + 1));
 }
 
 extern "C" int ztcp_allot_pages(int32_t* page_table, int64_t table_stride, int64_t max_pages, const int32_t* kv_lens,
@@ -331,14 +407,14 @@ extern "C" int ztcp_allot_pages(int32_t* page_table, int64_t table_stride, int64
     if (!n_free || !out_n_free || !q_starts || (capacity > 0 && !free_pages) || (max_rows > 0 && (!slots || !positions)) ||
         (n_seqs > 0 && (!kv_lens || !q_lens || !out_lens || !granted)))
         return arg_result(ZTCP_EINVAL, "no array may be NULL");
-    const size_t need = ztcp_allot_pages_workspace(n_seqs);
-    if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 3u) != 0)
-        return arg_result(ZTCP_EINVAL, "workspace must hold ztcp_allot_pages_workspace bytes, 4-byte aligned");
+    const size_t need = ztcp_allot_pages_workspace(n_seqs, max_rows);
+    if (need > 0 && (!workspace || workspace_bytes < need || !hot_aligned(workspace)))
+        return arg_result(ZTCP_EINVAL, "workspace must hold ztcp_allot_pages_workspace bytes, 16-byte aligned");
     const int64_t seqs = 4 * n_seqs;
     const Span in[5] = {flat(kv_lens, seqs), flat(n_free, 4), flat(next_positions, seqs), flat(q_lens, seqs), flat(free_pages, 4 * capacity)};
     const Span out[9] = {flat(out_lens, seqs), flat(out_n_free, 4), flat(out_next_positions, seqs), flat(q_starts, seqs + 4),
                          flat(granted, seqs), flat(slots, 8 * max_rows), flat(positions, 4 * max_rows),
-                         flat(workspace, (int64_t)need), Span{page_table, n_seqs, 4 * max_pages, 4 * table_stride}};
+                         flat(need ? workspace : nullptr, (int64_t)need), Span{page_table, n_seqs, 4 * max_pages, 4 * table_stride}};
     for (int o = 0; o < 9; ++o) {
         for (int i = 0; i < 5; ++i)
             if (!(o == i && o < 3 && out[o].p == in[i].p) && meet(out[o], in[i]))
@@ -367,12 +443,14 @@ extern "C" int ztcp_allot_pages(int32_t* page_table, int64_t table_stride, int64
     p.slots = slots;
     p.positions = positions;
     p.granted = granted;
-    p.before = (int32_t*)workspace;
-    p.had = (int32_t*)workspace + n_seqs;
-    if (n_seqs <= kPlanThreads && max_rows <= kOneLaunchRows) {
-        hipLaunchKernelGGL((plan_kernel<true>), dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, p);
+    if (need == 0) {
+        if (max_rows <= 1024) hipLaunchKernelGGL((plan_kernel<256, true>), dim3(1), dim3(256), 0, (hipStream_t)stream, p);
+        else hipLaunchKernelGGL((plan_kernel<1024, true>), dim3(1), dim3(1024), 0, (hipStream_t)stream, p);
     } else {
-        hipLaunchKernelGGL((plan_kernel<false>), dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, p);
+        p.parts = (int4*)workspace;
+        p.had = (int32_t*)(p.parts + n_seqs);
+        p.hints = p.had + 1;
+        hipLaunchKernelGGL((plan_kernel<1024, false>), dim3(1), dim3(1024), 0, (hipStream_t)stream, p);
         launch_blocks(rows_kernel, (uint64_t)((max_rows + kRowsABlock - 1) / kRowsABlock), 256, 0, (hipStream_t)stream, p);
     }
     return hipGetLastError() == hipSuccess ? ZTCP_OK : ZTCP_EHIP;
