@@ -121,6 +121,9 @@ void selected_kernel(SelectedParams p) {
         for (int i = 0; i < DP / 16; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
         uint4 kf[2][kSteps], vf[kVLoads];                     // (K in LDS: loads by whole rows as V's, in order)
         uint32_t valid = 0;                                   // keys of the loaded tile that are there
+        // few rows read each page once, and leave no trace of it in the caches (32 sequences' 128 pages of 16 tokens, 269 MB:
+        // 56 us with ordinary loads, 49 so); many share pages
+        auto get = [](const uint8_t* src) { return WAVES > 1 ? ldg16_once(src) : ldg16(src); };
         auto load = [&](const Place& at) {
             const bool has = at.page >= 0;
             valid = (uint32_t)__ballot(has);
@@ -144,9 +147,9 @@ void selected_kernel(SelectedParams p) {
                 const int64_t pg = __shfl(page, from), rw = __shfl(in, from);
                 const int64_t in_page = (rw * p.kv_heads + head) * p.head_dim;
                 if constexpr (kKInLds)
-                    kf[i / kSteps][i % kSteps] = v_has ? ldg16(p.k_pool + 2 * (pg * p.k_page + in_page) + 16 * v_chunk)
+                    kf[i / kSteps][i % kSteps] = v_has ? get(p.k_pool + 2 * (pg * p.k_page + in_page) + 16 * v_chunk)
                                                        : make_uint4(0, 0, 0, 0);
-                vf[i] = v_has ? ldg16(p.v_pool + 2 * (pg * p.v_page + in_page) + 16 * v_chunk) : make_uint4(0, 0, 0, 0);
+                vf[i] = v_has ? get(p.v_pool + 2 * (pg * p.v_page + in_page) + 16 * v_chunk) : make_uint4(0, 0, 0, 0);
             }
         };
         Place at{-1, 0};                                      // of key (lane % 32) of the tile to be loaded
@@ -355,7 +358,7 @@ __global__ __launch_bounds__(256) void join_selected_kernel(SelectedParams p) {
 // wait for those that have.
 //
 // Two chunks of 1,024 tokens, 16 pages of 64 picked at random for each of 8 KV heads of
-// 128, 4 query heads each: 440 us, 2 us a tile: the time that a wave with work
+// 128, 4 query heads each: 350 us, 1.6 us a tile: the time that a wave with work
 // needs for it; 657 by rows, each of which brings its 512 KiB from the caches, 478 by
 // four waves of 32 rows.  Rows that pick alike share pages, which random ones hardly do.
 
@@ -624,14 +627,21 @@ void block_kernel(SelectedParams p) {
             }
             at = next;
             if (!__any(listed != 0)) continue;
+            // Waves that have work go first, the others' loads and looks at the list wait (352 us where it takes 372 without).
+            // LDS reads by fours in front of their products: the compiler, short of registers, would put each read right
+            // before its product (442).
+            __builtin_amdgcn_s_setprio(1);
             const uint8_t *kt = tiles[buffer][0], *vt = tiles[buffer][1];
             f32x4 sc[kSub];
 #pragma unroll
-            for (int u = 0; u < kSub; ++u) {
-                sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < kSteps; ++i) {
+                uint4 kf[kSub];
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i)
-                    sc[u] = mfma16<DT>(*reinterpret_cast<const uint4*>(kt + (16 * u + col) * kRowBytes + k_swizzle(col, 4 * i + quad) * 16), qf[i], sc[u]);
+                for (int u = 0; u < kSub; ++u)
+                    kf[u] = *reinterpret_cast<const uint4*>(kt + (16 * u + col) * kRowBytes + k_swizzle(col, 4 * i + quad) * 16);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < kSub; ++u) sc[u] = mfma16<DT>(kf[u], qf[i], i == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[u]);
             }
             const uint64_t mine = listed >> (4 * quad);       // keys 16 u + i of this lane
             float top = -INFINITY;
@@ -644,7 +654,8 @@ void block_kernel(SelectedParams p) {
                     top = fmaxf(top, sc[u][i]);
                 }
             top = max_halves(top);
-            top = fmaxf(top, __shfl_xor(top, 16));
+            const u32x2 rows_of_16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = fmaxf(__uint_as_float(rows_of_16.x), __uint_as_float(rows_of_16.y));   // (the lane's and that 16 further on)
             // the reference of the exponentials follows the maximum only when that has grown by 2^8: weights up to 256 lose
             // nothing in fp32 sums and 16-bit operands
             if (__any(top > m + 8.f)) {
@@ -669,17 +680,22 @@ void block_kernel(SelectedParams p) {
                 pf[h] = make_uint4(pack_hot<DT>(x[0], x[1]), pack_hot<DT>(x[2], x[3]), pack_hot<DT>(x[4], x[5]), pack_hot<DT>(x[6], x[7]));
             }
 #pragma unroll
-            for (int n = 0; n < DP / 16; ++n)
+            for (int h = 0; h < kSub / 2; ++h)
 #pragma unroll
-                for (int h = 0; h < kSub / 2; ++h) {
-                    uint2 v[2];
+                for (int n0 = 0; n0 < DP / 16; n0 += 4) {
+                    uint4 vf[4];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int row = 32 * h + 16 * u + 4 * quad + col / 4, chunk = 2 * n + (col & 3) / 2;
-                        v[u] = lds_read_transposed(vt + row * kRowBytes + v_swizzle(row, chunk) * 16 + (col & 1) * 8);
+                    for (int n = 0; n < 4; ++n) {
+                        const int row = 4 * quad + col / 4;
+                        const uint8_t* src = vt + row * kRowBytes + v_swizzle(row, 2 * (n0 + n) + (col & 3) / 2) * 16 + (col & 1) * 8 + 32 * h * kRowBytes;
+                        const uint2 x = lds_read_transposed(src), y = lds_read_transposed(src + 16 * kRowBytes);
+                        vf[n] = make_uint4(x.x, x.y, y.x, y.y);
                     }
-                    o[n] = mfma16<DT>(make_uint4(v[0].x, v[0].y, v[1].x, v[1].y), pf[h], o[n]);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) o[n0 + n] = mfma16<DT>(vf[n], pf[h], o[n0 + n]);
                 }
+            __builtin_amdgcn_s_setprio(0);
         }
         bool odd = false;
 #pragma unroll
