@@ -150,6 +150,18 @@ def test_select(A, lens, kv, group, d, t, dtype):
         _check_select(A, c, budget, sink, recent, (lens[:3], seed), max_q_len=None if seed % 2 else 1)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("lens,kv,group,d,t", [
+    ([(600, 900), (20, 300), (0, 40)], 8, 4, 128, 16), ([(260, 300)], 64, 1, 16, 16), ([(530, 700)], 4, 8, 64, 13),
+    ([(850, 1000)], 5, 3, 96, 32), ([(515, 520)], 16, 2, 256, 16), ([(270, 300)], 8, 8, 128, 16), ([(260, 500)], 8, 4, 240, 16), ([(530, 1500)], 8, 4, 64, 1)])
+def test_select_chunks(A, lens, kv, group, d, t, dtype):
+    """Rows enough for blocks of tokens over pieces of the pages."""
+    _say("select, chunks", lens, kv, group, d, t, dtype)
+    kind = ("random", "near", "few values")[(kv + d // 16) % 3]
+    c = _select_case(lens, kv, group, d, t, dtype, seed=d, missing=0.1, kind=kind)
+    _check_select(A, c, 9, 1, 2, (lens, kind))
+
+
 @pytest.mark.parametrize("kind", ["same pages", "zeros", "near", "few values"])
 def test_select_where_many_scores_are_equal(A, kind):
     """More pages at the border than are ranked at once (256); tables in and beyond what the local memory holds."""
@@ -157,6 +169,8 @@ def test_select_where_many_scores_are_equal(A, kind):
     c = _select_case([(1, 1500), (2, 700)], 2, 2, 64, 1, BF, kind=kind)
     for budget, sink, recent in ((100, 0, 1), (600, 1, 1), (1400, 10, 50), (2, 1, 1)):
         _check_select(A, c, budget, sink, recent, (kind, budget))
+    c = _select_case([(300, 320)], 32, 1, 16, 2, BF, kind=kind, missing=0.05)
+    _check_select(A, c, 30, 1, 1, (kind, "chunk"))
     c = _select_case([(1, 13000)], 1, 1, 16, 1, FP, kind=kind, missing=0.05)
     _check_select(A, c, 400, 2, 3, (kind, "long"))
 

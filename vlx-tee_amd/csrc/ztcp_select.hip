@@ -165,6 +165,30 @@ __device__ __forceinline__ float row_max(float x, int log) {
 }
 
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+
+// Two numbers, those with the sign bit (NaN too) as they are, 0 for the others.
+__device__ __forceinline__ uint32_t negatives(uint32_t w) { return w & __builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, w) >> (int16_t)15); }
+
+// The greatest magnitude among a wave's bounds of 16 pages from page0 on, written down; `counts`: the lane's (lane % 16)
+// page is there.  Numbers of one sign are ordered as their bits are; NaN is above infinity.
+template <int DT, int N>
+__device__ __forceinline__ void top_of(const SelectParams& p, const uint4 (&lo)[N], const uint4 (&hi)[N], int s, int head, int page0,
+                                       bool counts) {
+    const int lane = (int)threadIdx.x & 63;
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t w[8] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w, hi[i].x, hi[i].y, hi[i].z, hi[i].w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[j] & 0x7FFF7FFFu));
+    }
+    float top = __int_as_float(counts ? (int)max((uint32_t)most.x, (uint32_t)most.y) << 8 : 0);
+    top = row_max(top, 4);
+    const int all = max(max(__builtin_amdgcn_readlane(__float_as_int(top), 0), __builtin_amdgcn_readlane(__float_as_int(top), 16)),
+                        max(__builtin_amdgcn_readlane(__float_as_int(top), 32), __builtin_amdgcn_readlane(__float_as_int(top), 48)));
+    if (lane == 0) p.top[((int64_t)s * p.kv_heads + head) * p.tops + page0 / 16] = hot_lo<DT>((uint32_t)all >> 8);
+}
 
 template <int DT, int DP>
 __global__ __launch_bounds__(256) void score_kernel(SelectParams p) {
@@ -278,7 +302,7 @@ __global__ __launch_bounds__(256) void score_kernel(SelectParams p) {
                 const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
                 uint32_t n[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) n[j] = w[j] & ((w[j] >> 15 & 0x00010001u) * 0xFFFFu);
+                for (int j = 0; j < 4; ++j) n[j] = negatives(w[j]);
                 neg[i] = make_uint4(n[0], n[1], n[2], n[3]);
                 pos[i] = make_uint4(w[0] ^ n[0], w[1] ^ n[1], w[2] ^ n[2], w[3] ^ n[3]);
             }
@@ -299,21 +323,7 @@ __global__ __launch_bounds__(256) void score_kernel(SelectParams p) {
             lo[i] = *reinterpret_cast<const uint4*>(mine + col * DP * 2 + swizzle(col, 4 * i + quad) * 16);
             hi[i] = *reinterpret_cast<const uint4*>(mine + (16 + col) * DP * 2 + swizzle(col, 4 * i + quad) * 16);
         }
-        if (last_block) {                     // it sees every page
-            u16x2 most = {0, 0};
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                const uint32_t w[8] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w, hi[i].x, hi[i].y, hi[i].z, hi[i].w};
-#pragma unroll
-                for (int j = 0; j < 8; ++j) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[j] & 0x7FFF7FFFu));
-            }
-            // numbers of one sign are ordered as their bits are; NaN is above infinity
-            float top = __int_as_float((int)max((uint32_t)most.x, (uint32_t)most.y) << 8);
-            top = row_max(top, 4);
-            const int all = max(max(__builtin_amdgcn_readlane(__float_as_int(top), 0), __builtin_amdgcn_readlane(__float_as_int(top), 16)),
-                                max(__builtin_amdgcn_readlane(__float_as_int(top), 32), __builtin_amdgcn_readlane(__float_as_int(top), 48)));
-            if (lane == 0) p.top[((int64_t)s * p.kv_heads + head) * p.tops + page0 / 16] = hot_lo<DT>((uint32_t)all >> 8);
-        }
+        if (last_block) top_of<DT>(p, lo, hi, s, head, page0, true);   // it sees every page (what is not there is 0)
         for (int t0 = 0; t0 < tokens; t0 += token_step) {
             float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             for (int h0 = 0; h0 < p.group; h0 += heads) {
@@ -346,10 +356,133 @@ __global__ __launch_bounds__(256) void score_kernel(SelectParams p) {
     }
 }
 
+// Chunks: a workgroup keeps a block of tokens' columns in LDS, up to eight products of 16 tokens and one head each, their
+// negative and their positive numbers apart, and goes over up to 1,024 pages with them, 16 a wave and turn, whose bounds
+// come as the products want them, from the caches most of the time, a turn ahead.
+//
+// 2 x 2,000 tokens, 3 query heads to each of 5 KV heads of 96, over 525 pages: 42 us (52 with signs
+// looked at for every product), 12 of them before the first product; 57 by the kernel above,
+// whose waves wait for the columns of each product.
+constexpr int kPieceTiles = 16;
+// Tokens of a block: as many as make six products (48 KiB at 128 elements, three workgroups a compute unit), or 16 with up
+// to eight; half as many for wider vectors; 0: too many heads.
+__host__ __device__ inline int chunk_tokens(int group, int width) {
+    const int fit = width <= 128 ? 6 : 3, most = width <= 128 ? 8 : 4;
+    return group <= fit ? fit / group * 16 : group <= most ? 16 : 0;
+}
+
+template <int DT, int DP>
+__global__ __launch_bounds__(256) void score_chunk_kernel(SelectParams p) {
+    constexpr int kSteps = DP / 32, kChunks = DP / 8, kLoadRows = 64 / kChunks, kRowBytes = DP * 2;
+    extern __shared__ __attribute__((aligned(16))) uint8_t columns[];   // [negative, positive][product][16][DP]
+    const int lane = (int)threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+    const int col = lane & 15, quad = lane >> 4;
+    const uint32_t unit = p.first_block + blockIdx.x;
+    const int head = (int)(unit % (uint32_t)p.kv_heads), block_size = chunk_tokens(p.group, DP);
+    int at = (int)(unit / (uint32_t)p.kv_heads);
+    auto tiles_of = [&](const Seq& q) { return (pages_seen(p, q, q.n_new) + kTilePages - 1) / kTilePages; };
+    auto pieces_of = [&](const Seq& q) { return (tiles_of(q) + kPieceTiles - 1) / kPieceTiles; };
+    auto units_of = [&](const Seq& q) { return q.n_new > 0 ? ((q.n_new - 1) / block_size + 1) * pieces_of(q) : 0; };
+    const int s = uniform(find_tile(p.batch, at, units_of));
+    if (s >= p.batch.n_seqs) return;
+    const Seq seq = uniform(seq_of(p.batch, s));
+    const int pieces = uniform(pieces_of(seq));
+    if (at < 0 || at >= units_of(seq)) return;                // (starts that do not ascend)
+    at = uniform(at);
+    const int block = at / pieces, piece = at - block * pieces;
+    const int token0 = block * block_size, tokens = min(seq.n_new - token0, block_size);
+    const bool last_block = token0 + tokens == seq.n_new;
+    const int all_pages = pages_seen(p, seq, seq.n_new), pages = min(pages_seen(p, seq, token0 + tokens), (piece + 1) * kPieceTiles * kTilePages);
+    const int products = (tokens + 15) / 16 * p.group, block_bytes = block_size * p.group * kRowBytes;
+    auto swizzle = [](int row, int chunk) { return chunk ^ (row & (kChunks < 16 ? kChunks - 1 : 15)); };
+    int page0 = piece * kPieceTiles * kTilePages + wave * 16;
+    // bounds of page lane % 16, at the products' depths
+    uint4 bound[2][kSteps];
+    int id = -1;
+    auto fetch = [&](int page) { return page + col < all_pages ? seq.entry(page + col) : -1; };
+    bool there = false;                                       // this lane's page, which is loaded
+    auto load = [&](int of) {
+        there = (uint32_t)of < (uint32_t)p.batch.n_pages;
+        const uint8_t* src = p.bounds + 2 * ((int64_t)(there ? of : 0) * p.bounds_page + (int64_t)head * p.head_dim);
+        const int64_t upper = 2 * (int64_t)p.kv_heads * p.head_dim;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const int d = 32 * i + 8 * quad < p.head_dim ? 32 * i + 8 * quad : 0;   // (columns behind head_dim meet zeros)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) bound[u][i] = ldg16(src + u * upper + 2 * d);
+        }
+    };
+    load(fetch(page0));
+    id = fetch(page0 + kTilePages);
+    {
+        const int load_row = lane / kChunks, load_chunk = lane % kChunks;
+        for (int r0 = wave * kLoadRows; r0 < products * 16; r0 += 4 * kLoadRows) {
+            const int r = r0 + load_row, group16 = r / 16 / p.group, h = r / 16 - group16 * p.group;
+            const int token = token0 + min(group16 * 16 + (r & 15), tokens - 1);
+            const uint8_t* src = p.q + 2 * ((int64_t)(seq.row0 + token) * p.q_stride + ((int64_t)head * p.group + h) * p.head_dim);
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (load_chunk * 8 < p.head_dim) x = ldg16(src + 16 * load_chunk);
+            const uint4 n = make_uint4(negatives(x.x), negatives(x.y), negatives(x.z), negatives(x.w));
+            uint8_t* dst = columns + r * kRowBytes + swizzle(r, load_chunk) * 16;
+            *reinterpret_cast<uint4*>(dst) = n;
+            *reinterpret_cast<uint4*>(dst + block_bytes) = make_uint4(x.x ^ n.x, x.y ^ n.y, x.z ^ n.z, x.w ^ n.w);
+        }
+    }
+    __syncthreads();
+    for (; page0 < pages; page0 += kTilePages) {
+        uint4 lo[kSteps], hi[kSteps];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) lo[i] = bound[0][i], hi[i] = bound[1][i];
+        if (last_block) top_of<DT>(p, lo, hi, s, head, page0, there);
+        if (page0 + kTilePages < pages) {
+            load(id);
+            id = fetch(page0 + 2 * kTilePages);
+        }
+        float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        int t0 = 0, h = 0;
+        uint4 neg[kSteps], pos[kSteps];
+        const uint8_t* mine = columns + col * kRowBytes;
+        auto read = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const uint8_t* src = mine + 16 * j * kRowBytes + swizzle(col, 4 * i + quad) * 16;
+                neg[i] = *reinterpret_cast<const uint4*>(src);
+                pos[i] = *reinterpret_cast<const uint4*>(src + block_bytes);
+            }
+        };
+        read(0);
+        for (int j = 0; j < products; ++j) {
+            f32x4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                sum[0] = mfma16<DT>(lo[i], neg[i], sum[0]);
+                sum[1] = mfma16<DT>(hi[i], pos[i], sum[1]);
+            }
+            if (j + 1 < products) read(j + 1);
+            const f32x4 sc = sum[0] + sum[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) best[e] = fmaxf(best[e], fabsf(sc[e]) < INFINITY ? sc[e] : INFINITY);
+            if (++h < p.group) continue;
+            const int to = page0 + 4 * quad;
+            if (t0 + col < tokens && to < p.score_stride) {
+                float* dst = p.scores + ((int64_t)(seq.row0 + token0 + t0 + col) * p.kv_heads + head) * p.score_stride + to;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) best[e] = best[e] < INFINITY ? best[e] : NAN;
+                *reinterpret_cast<float4*>(dst) = make_float4(best[0], best[1], best[2], best[3]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) best[e] = -INFINITY;
+            h = 0;
+            t0 += 16;
+        }
+    }
+}
+
 // ---- selection --------------------------------------------------------------------
 // Which pages have the highest scores must not depend on how fp32 sums were rounded.
-// A score of n = 2 head_dim products, each exact in fp32, is off by at most
-//     E = n (2^-23 |q|_1 B + 2^-125 (1 + |q|_1 + B)),
+// A score is a sum of head_dim products other than 0 (of a column's two one is), each
+// exact in fp32, in two parts at most: it is off by at most
+//     E = (head_dim + 2) (2^-23 |q|_1 B + 2^-125 (1 + |q|_1 + B)),
 // B being the greatest bound (every addition rounds or cuts by 2^-23 of what it holds,
 // a number too small for fp32 loses 2^-126 times its partner): if T is the k-th highest
 // fp32 score, pages above T + 2 E are among the k highest and those below T - 2 E are
@@ -501,7 +634,7 @@ __device__ __forceinline__ void close_in(Shared& sh, Visit&& visit, Key& low, Ke
 // The keys from low to high are those that fp32 sums cannot tell from the k-th highest.
 __device__ __forceinline__ void border(const SelectParams& p, float sum, float top, uint32_t kth_key, uint32_t& low, uint32_t& high) {
     // (a hundredth more than E for the rounding of the sum, of E itself and of the borders)
-    const float err = 2.02f * (float)p.head_dim * (0x1p-23f * sum * top + 0x1p-125f * (1.f + sum + top));
+    const float err = 1.01f * (float)(p.head_dim + 2) * (0x1p-23f * sum * top + 0x1p-125f * (1.f + sum + top));
     const float kth = number_of(kth_key), reach = 2.f * err + 0x1p-22f * fabsf(kth);
     if (!(reach < INFINITY)) return;
     const float a = kth - reach, b = kth + reach;
@@ -718,10 +851,33 @@ __global__ __launch_bounds__(THREADS) void pick_kernel(SelectParams p) {
     for (int i = total + tid; i < p.budget; i += THREADS) out[i] = -1;
 }
 
+// f over a wave's 64 numbers, in every lane, without LDS.
+template <class F>
+__device__ __forceinline__ uint32_t over_wave(uint32_t x, F&& f, int width = 64) {
+    x = f(x, __float_as_uint(partner<0xB1>(__uint_as_float(x))));
+    x = f(x, __float_as_uint(partner<0x4E>(__uint_as_float(x))));
+    x = f(x, __float_as_uint(partner<0x141>(__uint_as_float(x))));
+    x = f(x, __float_as_uint(partner<0x140>(__uint_as_float(x))));
+    if (width > 16) {
+        const u32x2 r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        x = f(r.x, r.y);
+    }
+    if (width > 32) {
+        const u32x2 r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        x = f(r.x, r.y);
+    }
+    return x;
+}
+__device__ __forceinline__ float wave_max(float x) {           // NaN if there is one
+    const bool nan = __any(x != x);
+    x = __uint_as_float(over_wave(__float_as_uint(x), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+    return nan ? NAN : x;
+}
+
 // The same for rows of at most 1,024 pages: one wave for a row and KV head, its keys in registers, which pages are taken
 // in the bits of a word of each lane, and the k-th highest key found bit by bit.
 //
-// 4,000 rows of 5 KV heads over 525 pages: 205 us by workgroups, 57 so.
+// 4,000 rows of 5 KV heads over 525 pages: 205 us by workgroups, 50 so.
 constexpr int kFewPages = 1024;
 
 template <int DT, int OWN>
@@ -742,31 +898,29 @@ __global__ __launch_bounds__(256) void pick_few_kernel(SelectParams p) {
     const uint8_t* q = p.q + 2 * ((int64_t)row * p.q_stride + (int64_t)head * p.group * p.head_dim);
     int32_t* out = p.out + unit * p.budget;
 
-    // |q|_1, of four heads at once, and the greatest bound
-    float sum = 0.f, top = lane < (n + 15) / 16 ? p.top[((int64_t)s * p.kv_heads + head) * p.tops + lane] : 0.f;
-    for (int h0 = 0; h0 < p.group; h0 += 4) {
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int d = 2 * lane; d < p.head_dim; d += 128)
+    // |q|_1, of four heads at once (two of vectors of more than 128 elements), and the greatest bound
+    float sum = 0.f;
+    const float top = wave_max(lane < (n + 15) / 16 ? p.top[((int64_t)s * p.kv_heads + head) * p.tops + lane] : 0.f);
+    {
+        const int width = p.head_dim <= 128 ? 16 : 32, chunk = lane % width;
+        for (int h0 = 0; h0 < p.group; h0 += 64 / width) {
+            const int h = min(h0 + lane / width, p.group - 1);
+            const uint4 x = 8 * chunk < p.head_dim ? ldg16(q + 2 * ((int64_t)h * p.head_dim + 8 * chunk)) : make_uint4(0, 0, 0, 0);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            float part = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(q + 2 * ((int64_t)min(h0 + e, p.group - 1) * p.head_dim + d));
-                x[e] += fabsf(hot_lo<DT>(w)) + fabsf(hot_hi<DT>(w));
-            }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            x[e] = xor_sum(x[e], 64);
-            sum = x[e] > sum || x[e] != x[e] ? x[e] : sum;
+            for (int e = 0; e < 4; ++e) part += fabsf(hot_lo<DT>(w[e])) + fabsf(hot_hi<DT>(w[e]));
+            part = __uint_as_float(over_wave(__float_as_uint(part),
+                                             [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }, width));
+            part = wave_max(part);
+            sum = part > sum || part != part ? part : sum;
         }
-    }
-    for (int m = 1; m < 64; m <<= 1) {
-        const float x = __shfl_xor(top, m);
-        top = x > top || x != x ? x : top;
     }
     uint32_t key[kOwn], taken = 0, nears = 0;                 // key 0: not open; bit c: of page 64 c + lane
     int forced = 0, open = 0, unknown = 0;
+    int id[kOwn];
     {
         float x[kOwn];
-        int id[kOwn];
 #pragma unroll
         for (int c = 0; c < kOwn; ++c) {
             const int i = min(64 * c + lane, n - 1);
@@ -806,11 +960,9 @@ __global__ __launch_bounds__(256) void pick_few_kernel(SelectParams p) {
                 least = key[c] != 0 ? min(least, key[c]) : least;
                 most = max(most, key[c]);
             }
-            for (int m = 1; m < 64; m <<= 1) {
-                least = min(least, (uint32_t)__shfl_xor((int)least, m));
-                most = max(most, (uint32_t)__shfl_xor((int)most, m));
-            }
-            least = (uint32_t)uniform((int)least), most = (uint32_t)uniform((int)most);
+            auto lower = [](uint32_t a, uint32_t b) { return min(a, b); };
+            least = (uint32_t)uniform((int)over_wave(least, lower));
+            most = (uint32_t)uniform((int)over_wave(most, [](uint32_t a, uint32_t b) { return max(a, b); }));
             while (least < most) {
                 const uint32_t t = least + (most - least + 1) / 2;
                 const int reach = count([&](int c) { return key[c] >= t; });
@@ -820,8 +972,7 @@ __global__ __launch_bounds__(256) void pick_few_kernel(SelectParams p) {
                 most = kChosen;                               // the least of these
 #pragma unroll
                 for (int c = 0; c < kOwn; ++c) most = key[c] >= t ? min(most, key[c]) : most;
-                for (int m = 1; m < 64; m <<= 1) most = min(most, (uint32_t)__shfl_xor((int)most, m));
-                least = most;
+                least = most = (uint32_t)uniform((int)over_wave(most, lower));
             }
             const uint32_t kth_key = least;
             border(p, sum, top, kth_key, low, high);
@@ -847,7 +998,7 @@ __global__ __launch_bounds__(256) void pick_few_kernel(SelectParams p) {
                 if (64 * c >= n) continue;
                 for (uint64_t todo = __ballot(nears >> c & 1); todo; todo &= todo - 1) {
                     const int from = __ffsll((unsigned long long)todo) - 1;
-                    const uint64_t x = exact_key<DT>(p, q, seq.entry(64 * c + from), head);
+                    const uint64_t x = exact_key<DT>(p, q, __builtin_amdgcn_readlane(id[c], from), head);
                     if (lane == from) exact[c] = x;
                 }
             }
@@ -1007,24 +1158,43 @@ extern "C" int ztcp_select_pages(const void* q, int64_t q_stride, int64_t q_head
     // as many as the card holds at once, and no more than units
     const int64_t resident = (int64_t)cus * (d <= 64 ? 5 : d <= 128 ? 3 : 1), each = (resident + g->num_heads - 1) / g->num_heads;
     p.score_groups = (int32_t)(each < plan.units ? each : plan.units);
+    // chunks: sequences of more than 16 new tokens on average, as many workgroups as half the compute units at least
+    const int64_t block = chunk_tokens(p.group, d <= 128 ? 128 : 256);
+    const size_t chunk_lds = (size_t)(block * p.group) * (d <= 64 ? 64 : d <= 128 ? 128 : 256) * 4;
+    int64_t chunk_units = 0;
+    if (block > 0 && batch->n_rows > 16 * batch->n_seqs) {
+        const int64_t pieces = (batch->max_pages + kPieceTiles * kTilePages - 1) / (kPieceTiles * kTilePages);
+        chunk_units = (batch->n_rows / block + batch->n_seqs) * pieces * g->num_heads;
+        if (batch->n_rows / block * g->num_heads < cus / 2 || chunk_units >= (int64_t)1 << 31) chunk_units = 0;
+    }
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        const dim3 grid((uint32_t)(g->num_heads * p.score_groups));
-        hipLaunchKernelGGL((d <= 64 ? score_kernel<DT, 64> : d <= 128 ? score_kernel<DT, 128> : score_kernel<DT, 256>), grid, dim3(256), 0,
-                           (hipStream_t)stream, p);
+        if (chunk_units > 0) {
+            auto kernel = d <= 64 ? score_chunk_kernel<DT, 64> : d <= 128 ? score_chunk_kernel<DT, 128> : score_chunk_kernel<DT, 256>;
+            // over 64 KiB of dynamic LDS has to be asked for
+            if (chunk_lds > (size_t)48 * 1024 &&
+                hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024) != hipSuccess)
+                return false;
+            launch_blocks(kernel, (uint64_t)chunk_units, 256, chunk_lds, (hipStream_t)stream, p);
+        } else {
+            const dim3 grid((uint32_t)(g->num_heads * p.score_groups));
+            hipLaunchKernelGGL((d <= 64 ? score_kernel<DT, 64> : d <= 128 ? score_kernel<DT, 128> : score_kernel<DT, 256>), grid, dim3(256),
+                               0, (hipStream_t)stream, p);
+        }
         const uint64_t picks = (uint64_t)batch->n_rows * (uint64_t)g->num_heads;
         const bool many = picks > 2 * (uint64_t)cus;          // rows: a wave each if their pages are few
         if (batch->max_pages <= kFewPages || many)
             launch_blocks(batch->max_pages <= 256 ? pick_few_kernel<DT, 4> : batch->max_pages <= 576 ? pick_few_kernel<DT, 9> : pick_few_kernel<DT, 16>,
                           (picks + 3) / 4, 256, 0, (hipStream_t)stream, p);
-        if (batch->max_pages <= kFewPages) return;
+        if (batch->max_pages <= kFewPages) return true;
         p.few_pages = many ? kFewPages : 0;
         const bool in_lds = batch->max_pages <= kKeysInLds;
         const size_t lds = in_lds ? (size_t)batch->max_pages * 4 : 0;
         if (many) launch_blocks(in_lds ? pick_kernel<DT, 256, true> : pick_kernel<DT, 256, false>, picks, 256, lds, (hipStream_t)stream, p);
         else launch_blocks(in_lds ? pick_kernel<DT, 1024, true> : pick_kernel<DT, 1024, false>, picks, 1024, lds, (hipStream_t)stream, p);
+        return true;
     };
-    if (g->hot_dtype == ZTCP_HOT_BF16) go(std::integral_constant<int, kHotBf16>{});
-    else go(std::integral_constant<int, kHotFp16>{});
+    if (!(g->hot_dtype == ZTCP_HOT_BF16 ? go(std::integral_constant<int, kHotBf16>{}) : go(std::integral_constant<int, kHotFp16>{})))
+        return ZTCP_EHIP;
     return hipGetLastError() == hipSuccess ? ZTCP_OK : ZTCP_EHIP;
 }
