@@ -213,6 +213,13 @@ def test_select_wrong_numbers_and_nothing(A):
     assert A.select_pages(c["q"], c["b"], c["table"], c["lens"], _i32([0, 0, 0]), page_tokens=16, budget=4).shape == (0, 2, 4)
 
 
+def test_select_rows_that_see_no_page(A):
+    """Beside long contexts, few rows and many: their lists are all -1."""
+    _say("select, rows without pages")
+    for lens in ([(1, 0), (1, 20000), (3, 2)], [(40, 0), (200, 20000), (30, 17)]):
+        _check_select(A, _select_case(lens, 4, 2, 64, 16, BF), 9, 1, 2, lens)
+
+
 # ---- attention over selected pages ---------------------------------------------------
 
 def _attend_case(lens, kv, group, d, t, dtype, listed, *, seed=0, missing=0.0):

@@ -28,7 +28,8 @@ BUDGET = {
     "11plan_kernelILi256E": (128, 0), "11plan_kernelILi1024E": (128, 0), "11rows_kernel": (128, 0),
     "20release_count_kernel": (128, 0), "14release_kernel": (128, 0),
     "13bounds_kernel": (128, 0), "12score_kernelILi1ELi64E": (128, 0), "12score_kernelILi1ELi128E": (168, 0),
-    "12score_kernelILi1ELi256E": (512, 0), "15pick_few_kernel": (128, 0), "11pick_kernelILi1ELi1024E": (128, 0),
+    "12score_kernelILi1ELi256E": (512, 0), "18score_chunk_kernelILi1ELi64E": (128, 0), "18score_chunk_kernelILi1ELi128E": (168, 0),
+    "18score_chunk_kernelILi1ELi256E": (512, 0), "15pick_few_kernel": (128, 0), "11pick_kernelILi1ELi1024E": (128, 0),
     "11pick_kernelILi1ELi256E": (128, 0),
     "10few_kernelILi1ELi128ELi1ELb1E": (256, 0), "10few_kernelILi1ELi256ELi1ELb1E": (512, 0),
     "11many_kernelILi1ELi64ELb1ELb1E": (256, 0), "11many_kernelILi1ELi128ELb1ELb1E": (256, 160),

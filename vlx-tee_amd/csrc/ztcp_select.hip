@@ -139,7 +139,7 @@ struct SelectParams {
     int32_t score_stride, tops;      // floats of a row's scores (a multiple of 4), of a sequence's tops for a head
     float* scores;                   // [rows, kv_heads, score_stride]; NaN: no finite number
     int32_t score_groups;            // score kernel: workgroups of a KV head
-    int32_t few_pages;               // pick kernel: rows of at most so many pages are another kernel's
+    int32_t few_pages;               // pick kernel: rows of at most so many pages (-1: none) are another kernel's
     float* top;                      // [n_seqs, kv_heads, tops]: the greatest bound of 16 pages, by magnitude
     int32_t* out;
     uint32_t first_block;
@@ -695,10 +695,10 @@ __global__ __launch_bounds__(THREADS) void pick_kernel(SelectParams p) {
     if (row < seq.row0 || row >= seq.row0 + seq.n_new) return;
     const int n = pages_seen(p, seq, row - seq.row0 + 1);
     if (n <= p.few_pages) return;
-    float* scores = p.scores + unit * p.score_stride;
+    uint32_t* scores = reinterpret_cast<uint32_t*>(p.scores + unit * p.score_stride);   // (as words, since keys may take their place)
     uint32_t* keys;
     if constexpr (IN_LDS) keys = lds_keys;
-    else keys = reinterpret_cast<uint32_t*>(scores);
+    else keys = scores;
     const uint8_t* q = p.q + 2 * ((int64_t)row * p.q_stride + (int64_t)head * p.group * p.head_dim);
     int32_t* out = p.out + unit * p.budget;
 
@@ -722,7 +722,7 @@ __global__ __launch_bounds__(THREADS) void pick_kernel(SelectParams p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int i = base + j * THREADS + tid;
-            x[j] = i < n ? scores[i] : 0.f;
+            x[j] = i < n ? __uint_as_float(scores[i]) : 0.f;
             id[j] = i < n ? seq.entry(i) : -1;
         }
 #pragma unroll
@@ -1187,7 +1187,7 @@ extern "C" int ztcp_select_pages(const void* q, int64_t q_stride, int64_t q_head
             launch_blocks(batch->max_pages <= 256 ? pick_few_kernel<DT, 4> : batch->max_pages <= 576 ? pick_few_kernel<DT, 9> : pick_few_kernel<DT, 16>,
                           (picks + 3) / 4, 256, 0, (hipStream_t)stream, p);
         if (batch->max_pages <= kFewPages) return true;
-        p.few_pages = many ? kFewPages : 0;
+        p.few_pages = many ? kFewPages : -1;
         const bool in_lds = batch->max_pages <= kKeysInLds;
         const size_t lds = in_lds ? (size_t)batch->max_pages * 4 : 0;
         if (many) launch_blocks(in_lds ? pick_kernel<DT, 256, true> : pick_kernel<DT, 256, false>, picks, 256, lds, (hipStream_t)stream, p);
