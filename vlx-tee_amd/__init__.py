@@ -9,7 +9,8 @@ Modules:
                     (research/baseline_codec/fused_quant_crypto.py:99-659), native state
   pages             descriptor-based batch API for paged, multi-layer KV pools
   attention         operators on hot pages: append with norms and rotation, paged
-                    attention, the weight each page received, eviction
+                    attention, the weight each page received, eviction; page tables,
+                    attention of drafted trees and over selected pages
   serving           PoisonShield hit bitmap from per-page verdicts, pinned host ring
                     for the egress wire step
   spec              wire constants, AAD record and payload sizing (cold_page_spec.py mirror)

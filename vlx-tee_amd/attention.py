@@ -8,6 +8,13 @@ pages than its budget gives up those with the least weight (``evict_pages``);
 their ids select the descriptors that ``pages.egress`` takes to the cold tier,
 and pages that ``pages.ingress`` brought back are read like any other.
 
+Where the page tables live on the GPU, ``allot_pages`` gives the new tokens
+their pages, slots and positions, and ``release_pages`` takes back what ended or
+was drafted in vain; drafts that form a tree attend with ``tree_attention``.
+For long contexts ``page_bounds`` keeps bounds of every page's keys,
+``select_pages`` finds the pages that may matter most to each query, and
+``selected_attention`` attends over these alone.
+
 ``append_tokens`` and ``evict_pages`` take single-buffer (latent) pages too;
 ``paged_attention`` is for pages with K and V, and it and ``attention_mass`` for a
 head_dim of at most 256.
@@ -112,7 +119,8 @@ def page_bounds(k_pages: torch.Tensor, bounds: torch.Tensor, page_table: torch.T
                 q_starts: torch.Tensor, *, max_q_len: int | None = None) -> torch.Tensor:
     """Brings ``bounds`` [n_pages, 2, kv_heads, d] (the pages' dtype) up to date for the pages that hold the step's new
     tokens: the least and the greatest number of each column of a page's keys, over all of its tokens; NaN where a key's
-    is.  Other pages' bounds are left.  Returns ``bounds``."""
+    is.  Other pages' bounds are left: for pages whose keys were written otherwise (brought back by ``pages.ingress``,
+    moved), call it with ``q_starts`` that count all of a sequence's tokens as new.  Returns ``bounds``."""
     return _call().page_bounds(k_pages, bounds, page_table, kv_lens, q_starts, max_q_len)
 
 
@@ -219,7 +227,7 @@ def release_pages(page_table: torch.Tensor, kv_lens: torch.Tensor, free_pages: t
                   page_tokens: int, in_place: bool = False) -> Release:
     """Puts the pages that ``kv_lens`` tokens do not reach back onto the stack ``free_pages``, ``n_free`` (written in
     either case): those of a sequence that has ended (``kv_lens`` 0), or of drafted tokens that were not accepted.  Pages
-    go in the order of sequences and columns; negative entries are no pages; what the stack has no room for stays in the
+    go in the order of sequences and columns; negative entries are no pages, all others are; what the stack has no room for stays in the
     table.  The ids that ``evict_pages`` lists are given back, once they have been written out, by
     ``release_pages(cold.evicted, torch.zeros_like(kv_lens), ...)``.  ``in_place`` updates ``page_table`` and ``n_free``."""
     return Release._make(_call().release_pages(page_table, kv_lens, free_pages, n_free, page_tokens, in_place))
