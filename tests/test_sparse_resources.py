@@ -36,7 +36,7 @@ BUDGET = {
     "11many_kernelILi1ELi256ELb1ELb1E": (512, 256),
     "15selected_kernelILi1ELi64E": (168, 0), "15selected_kernelILi1ELi128E": (256, 0), "15selected_kernelILi1ELi256E": (512, 0),
     "12block_kernelILi1ELi64ELb1ELi1E": (128, 0), "12block_kernelILi1ELi128E": (128, 160), "12block_kernelILi1ELi256E": (256, 0),
-    "20join_selected_kernel": (128, 0),
+    "20join_selected_kernel": (128, 0), "16join_tree_kernel": (128, 0),
 }
 
 

@@ -485,8 +485,9 @@ __device__ __forceinline__ Cut cut_of(const AttendParams& p) {
 // A tree's rows are few blocks over contexts of any length, and a workgroup for each of these would leave the longest
 // one to itself: pieces of equal work instead, as many in all as the card holds at once beside one for each block, of
 // 128 tokens at least, laid out sequence behind sequence.  Drafts of 24 to 64 tokens of 32 sequences of 500 to 8,192
-// tokens: 257 us with a workgroup for each block, 174 now (half as many pieces 192 us, twice as many 182); a draft of 37
-// over 1,501: 32 us in pieces of 512 tokens, 22 now.
+// tokens: 257 us with a workgroup for each block, 174 so (half as many pieces 192 us, twice as many 182; pieces of a
+// context all alike 5 more), 154 now with a join of its own and without launches for sequences of few rows; a draft of
+// 37 over 1,501: 32 us in pieces of 512 tokens, 22 now.
 constexpr int kTreePiece = 128;
 __device__ __forceinline__ int blocks_of(const AttendParams& p, const Seq& q) {
     const int rows = q.n_new * p.group;
@@ -920,7 +921,7 @@ __global__ __launch_bounds__(256) void join_few_kernel(AttendParams p, int most_
 // took 60 us where their attention had taken 40.
 constexpr int kJoinRows = 8;
 
-template <int DT, bool TREE>
+template <int DT>
 __global__ __launch_bounds__(256) void join_many_kernel(AttendParams p) {
     const int wave = (int)threadIdx.x >> 6;
     const uint32_t unit = p.first_block + blockIdx.x;
@@ -931,13 +932,63 @@ __global__ __launch_bounds__(256) void join_many_kernel(AttendParams p) {
     if (cut.n == 1 || !find_unit(p, (int)(rest / (kManyRows / kJoinRows)), s, block)) return;
     const Seq seq = seq_of(p.batch, s);
     const int rows = seq.n_new * p.group, n = pieces_of(seq.len, cut.tokens);
-    if (TREE && n == 1) return;
     const int r0 = block * kManyRows + (int)(rest % (kManyRows / kJoinRows)) * kJoinRows;
     for (int r = r0 + wave; r < min(rows, r0 + kJoinRows); r += 4) {
         const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
         join_row<DT>(p, many_partial(p, seq.row0 + token, q_head, 0), p.head_dim + 2, n,
                      (int64_t)(seq.row0 + token) * p.kv_heads * p.group + q_head);
     }
+}
+
+// A tree's rows have few pieces and are few: a wave takes a new token's query heads two by two, half a wave each, and
+// finds its sequence by the rows' starts (45,000 rows and heads of 2.5 pieces: 14 us, 25 by the kernel above).
+template <int DT>
+__global__ __launch_bounds__(256) void join_tree_kernel(AttendParams p) {
+    const int lane = (int)threadIdx.x & 63, half = lane >> 5, q_heads = p.kv_heads * p.group, pairs = (q_heads + 1) / 2;
+    const int64_t unit = ((int64_t)p.first_block + blockIdx.x) * 4 + uniform((int)threadIdx.x >> 6), wide_row = unit / pairs;
+    if (wide_row >= p.batch.n_rows) return;
+    const int row = (int)wide_row, q_head = 2 * (int)(unit - wide_row * pairs) + half;
+    const int s = uniform(find_above(p.batch.starts + 1, p.batch.n_seqs, row));
+    if (s >= p.batch.n_seqs) return;
+    const Seq seq = uniform(seq_of(p.batch, s));
+    if (row < seq.row0 || row >= seq.row0 + seq.n_new || blocks_of(p, seq) == 0) return;
+    const int n = min(pieces_of(seq.len, p.cut[1]), p.splits), d0 = 4 * (lane & 31);
+    if (n == 1 || q_head >= q_heads) return;
+    const float* src = many_partial(p, row, q_head, 0);
+    const int64_t step = p.head_dim + 2, row_head = (int64_t)row * q_heads + q_head;
+    float2 of[2] = {{-INFINITY, 0.f}, {-INFINITY, 0.f}};     // of pieces lane % 32 and 32 further on: there are 64 at most
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int i = (lane & 31) + 32 * j;
+        if (i < n) of[j] = *reinterpret_cast<const float2*>(src + i * step + p.head_dim);
+    }
+    float top = fmaxf(of[0].x, of[1].x);
+    for (int k = 1; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
+    const float base = top == -INFINITY ? 0.f : top;
+    const float w[2] = {__builtin_amdgcn_exp2f(of[0].x - base), __builtin_amdgcn_exp2f(of[1].x - base)};
+    const float total = xor_sum(w[0] * of[0].y + w[1] * of[1].y, 32);
+    float y[2][4] = {};
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+        const float wi = __shfl(i < 32 ? w[0] : w[1], (i & 31) + (lane & 32));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int d = d0 + 128 * j;
+            if (d >= p.head_dim) continue;
+            const float2 a = *reinterpret_cast<const float2*>(src + i * step + d), b = *reinterpret_cast<const float2*>(src + i * step + d + 2);
+            y[j][0] = __builtin_fmaf(wi, a.x, y[j][0]);
+            y[j][1] = __builtin_fmaf(wi, a.y, y[j][1]);
+            y[j][2] = __builtin_fmaf(wi, b.x, y[j][2]);
+            y[j][3] = __builtin_fmaf(wi, b.y, y[j][3]);
+        }
+    }
+    const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        if (d0 + 128 * j < p.head_dim)
+            *reinterpret_cast<uint2*>(p.out + 2 * (row_head * p.head_dim + d0 + 128 * j)) =
+                make_uint2(pack_hot<DT>(y[j][0] * inv, y[j][1] * inv), pack_hot<DT>(y[j][2] * inv, y[j][3] * inv));
+    if ((lane & 31) == 0 && p.lse) p.lse[row_head] = total == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
 // ---- host -------------------------------------------------------------------------
@@ -967,6 +1018,8 @@ Plan plan_call(const ztcp_paged_batch* b, const ztcp_geometry* g, int64_t q_head
         plan.few_rows = 0x7FFFFFFF;
     } else {
         plan.nt = b->n_seqs > 1 && group <= 16 * most_nt ? (group <= 16 ? 1 : 2) : 0;
+        // drafts of many rows on average: two launches for those of few would mostly have none
+        if (tree && b->n_rows * group >= 64 * b->n_seqs) plan.nt = 0;
         plan.few_rows = 16 * plan.nt;
         plan.many = true;
         plan.many_units = (b->n_rows * group + kManyRows - 1) / kManyRows + b->n_seqs;
@@ -1031,8 +1084,10 @@ void launch(const AttendParams& base, const Plan& plan, float* workspace, hipStr
         const bool even = p.batch.page_tokens % (many_tile(DP) / 4) == 0 && p.head_dim == DP;
         launch_blocks(even ? many_kernel<DT, DP, true, TREE> : many_kernel<DT, DP, false, TREE>, (uint64_t)plan.many_groups, 256, 0,
                       stream, p);
-        if (p.splits > 1)
-            launch_blocks(join_many_kernel<DT, TREE>, (uint64_t)units * (kManyRows / kJoinRows), 256, 0, stream, p);
+        if (p.splits > 1 && TREE)
+            launch_blocks(join_tree_kernel<DT>, ((uint64_t)p.batch.n_rows * ((heads * (uint32_t)p.group + 1) / 2) + 3) / 4, 256, 0, stream, p);
+        else if (p.splits > 1)
+            launch_blocks(join_many_kernel<DT>, (uint64_t)units * (kManyRows / kJoinRows), 256, 0, stream, p);
     }
 }
 
