@@ -430,3 +430,91 @@ def test_a_serving_loop(A):
         for a, b in zip((got[2], *got[3], *state), want):
             assert torch.equal(a, b)
         check(*got)
+
+
+def test_tensors_that_are_written_have_a_new_version(A):
+    _say("versions")
+    c = _attend_case([(2, 40)], 2, 2, 64, 16, BF, 2)
+    bounds, out, picked = torch.zeros((c["k"].shape[0], 2, 2, 64), dtype=BF, device="cuda"), torch.empty_like(c["q"]).contiguous(), c["picked"]
+    table, free, n_free, lens = c["table"].clone(), _i32([1, 2, 3]), _i32([3]), c["lens"].clone()
+    batch, mask = (c["table"], c["lens"], c["starts"]), torch.ones((2, 1), dtype=torch.int64, device="cuda")
+    for written, call in (((bounds,), lambda: A.page_bounds(c["k"], bounds, *batch)),
+                          ((picked,), lambda: A.select_pages(c["q"], bounds, *batch, page_tokens=16, budget=2, out=picked)),
+                          ((out,), lambda: A.selected_attention(c["q"], c["k"], c["v"], *batch, picked, out=out)),
+                          ((out,), lambda: A.tree_attention(c["q"], c["k"], c["v"], *batch, mask, out=out)),
+                          ((table,), lambda: A.allot_pages(table, lens, _i32([1]), free, n_free, page_tokens=16, max_rows=2)),
+                          ((free,), lambda: A.release_pages(table, _i32([0]), free, n_free, page_tokens=16)),
+                          ((table, lens, n_free), lambda: A.allot_pages(table, lens, _i32([1]), free, n_free, page_tokens=16, max_rows=2, in_place=True)),
+                          ((table, free, n_free), lambda: A.release_pages(table, _i32([0]), free, n_free, page_tokens=16, in_place=True))):
+        before = [t._version for t in written]
+        call()
+        assert all(t._version > x for t, x in zip(written, before))
+
+
+@pytest.mark.parametrize("lens", [[(1, 700), (3, 400)], [(400, 900)]])
+def test_pages_behind_four_gigabytes(A, lens):
+    """Of a pool whose pages lie far apart: byte and element offsets pass 32 bits.  The same pages side by side give the
+    same bits."""
+    _say("far pages", lens)
+    c = _attend_case(lens, 8, 4, 64, 16, BF, 5, seed=1)
+    near, apart = c["k"].shape[0], 1 << 26                                # pages 128 MiB apart: 5 to 9 GiB
+    n = min(near, 40)
+    c["table"] = torch.where(c["table"] >= 0, c["table"] % n, c["table"])
+    batch, d, t, kv = (c["table"], c["lens"], c["starts"]), 64, 16, 8
+
+    def far(x, step):
+        room = torch.empty((n - 1) * step + x[0].numel(), dtype=BF, device="cuda")
+        y = room.as_strided((n, *x.shape[1:]), (step, *x[0].stride()))
+        y.copy_(x[:n])
+        return y
+
+    def run(k, v, bounds):
+        A.page_bounds(k, bounds, *batch)
+        picked = A.select_pages(c["q"], bounds, *batch, page_tokens=t, budget=5)
+        rows = c["q"].shape[0]
+        mask = torch.full((rows, -(-rows // 64)), -1, dtype=torch.int64, device="cuda")
+        return (bounds.contiguous(), picked, *A.selected_attention(c["q"], k, v, *batch, picked, return_lse=True),
+                *A.tree_attention(c["q"], k, v, *batch, mask, return_lse=True))
+
+    k, v = c["k"][:n].contiguous(), c["v"][:n].contiguous()
+    b = torch.randn((n, 2, kv, d), generator=torch.Generator().manual_seed(4)).to(BF).cuda()
+    want = run(k, v, b.clone())
+    got = run(far(k, apart), far(v, apart), far(b, apart))
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+    torch.cuda.empty_cache()
+
+
+def test_chunks_in_a_graph_and_on_two_streams(A):
+    """Chunks' kernels replayed from a graph, and two calls under way at once, against calls one by one."""
+    _say("chunks, graph and streams")
+    cases = [_attend_case([(600, 900), (20, 300)], 8, 4, 128, 16, BF, 9, seed=s) for s in (1, 2)]
+    for c in cases:
+        c["b"] = torch.randn((c["k"].shape[0], 2, 8, 128), device="cuda").to(BF)
+
+    def run(c):
+        batch = (c["table"], c["lens"], c["starts"])
+        picked = A.select_pages(c["q"], c["b"], *batch, page_tokens=16, budget=9, sink=1, recent=2)
+        return picked, *A.selected_attention(c["q"], c["k"], c["v"], *batch, picked, return_lse=True)
+
+    want = [run(c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = []
+    for c, stream in zip(cases, streams):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            got.append([run(c) for _ in range(3)][-1])
+    torch.cuda.synchronize()
+    for x, y in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(x, y))
+    graph, c = torch.cuda.CUDAGraph(), cases[0]
+    with torch.cuda.graph(graph):
+        result = run(c)
+    for i in range(4):
+        c["q"].copy_(torch.randn(c["q"].shape, device="cuda"))
+        want = run(c)
+        for x in result:
+            x.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(result, want)), i

@@ -158,3 +158,27 @@ def test_python_checks(N):
         a.update(kw)
         with pytest.raises(ValueError, match=why):
             A.select_pages(**a)
+
+
+def test_gradients_and_tangents_are_refused(N):
+    """The operators have no derivatives: a tensor that carries one would lose it without a word."""
+    import torch.autograd.forward_ad as fwAD
+    import vlx_tee_amd.attention as A
+
+    x, pages = torch.zeros((2, 4, 64), dtype=torch.bfloat16), torch.zeros((3, 16, 2, 64), dtype=torch.bfloat16)
+    i32 = torch.zeros(2, dtype=torch.int32)
+    at, mask, b = (i32[None], i32[:1], i32), i32.long()[:, None], pages[:, :2].clone()
+    for name, t, call in (("q", x, lambda t: A.tree_attention(t, pages, pages, *at, mask)),
+                          ("v_pages", pages, lambda t: A.tree_attention(x, pages, t, *at, mask)),
+                          ("q", x, lambda t: A.selected_attention(t, pages, pages, *at, i32[:, None, None])),
+                          ("k_pages", pages, lambda t: A.selected_attention(x, t, pages, *at, i32[:, None, None])),
+                          ("q", x, lambda t: A.select_pages(t, b, *at, page_tokens=16, budget=2)),
+                          ("bounds", b, lambda t: A.select_pages(x, t, *at, page_tokens=16, budget=2)),
+                          ("k_pages", pages, lambda t: A.page_bounds(t, b, *at)), ("bounds", b, lambda t: A.page_bounds(pages, t, *at))):
+        with fwAD.dual_level(), torch.no_grad(), pytest.raises(ValueError, match=f"{name} carries a tangent"):
+            call(fwAD.make_dual(t, torch.ones_like(t)))
+        leaf = t.clone().requires_grad_()
+        with pytest.raises(ValueError, match=f"{name} requires a gradient"):
+            call(leaf)
+        with torch.no_grad(), pytest.raises(ValueError, match="HIP"):
+            call(leaf)
