@@ -149,6 +149,28 @@ def test_release(A, seqs, cols, page, max_len, capacity, in_place):
         assert bool((wide[:, cols:] == 99).all())
 
 
+@pytest.mark.parametrize("seqs,cols", [(5000, 7), (1400, 9000), (60000, 1)])
+def test_release_from_thousands(A, seqs, cols):
+    """Counts that one workgroup adds up."""
+    _say("release, thousands", seqs, cols)
+    gen = torch.Generator(device="cuda").manual_seed(seqs)
+    table = torch.randint(-9, 1 << 20, (seqs, cols), generator=gen, device="cuda").int()
+    lens = torch.randint(0, 16 * cols, (seqs,), generator=gen, device="cuda").int()
+    at = torch.arange(cols, device="cuda")[None]
+    goes = (table >= 0) & (at >= ((lens + 15) // 16)[:, None])
+    ids, all_of = table[goes], goes.sum(1).int()
+    for capacity in (3 + ids.numel(), 3 + ids.numel() // 3):
+        free = torch.full((capacity,), 77, dtype=torch.int32, device="cuda")
+        given = table.clone()
+        got = A.release_pages(given, lens, free, _i32([3]), page_tokens=16, in_place=True)
+        fits = goes & ((goes.flatten().cumsum(0).reshape(seqs, cols) + 3) <= capacity)
+        assert torch.equal(got.n_free, _i32([min(capacity, 3 + ids.numel())]))
+        assert torch.equal(free[3:], ids[:capacity - 3]) and bool((free[:3] == 77).all())
+        assert torch.equal(given, torch.where(fits, -1, table)) and torch.equal(got.n_released, fits.sum(1).int())
+    assert torch.equal(A.release_pages(table, lens, torch.empty(4 + ids.numel(), dtype=torch.int32, device="cuda"), _i32([0]),
+                                       page_tokens=16).n_released, all_of)
+
+
 def test_release_nothing(A):
     empty = torch.zeros((0, 4), dtype=torch.int32, device="cuda")
     for n, want in ((2, 2), (9, 3), (-5, 0)):

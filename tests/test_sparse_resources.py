@@ -26,7 +26,7 @@ LDS_LOADS = ("ztcp_tree", "ztcp_selected")
 # kernel name fragment -> registers a wave may use (512 / waves per SIMD), bytes of scratch
 BUDGET = {
     "11plan_kernelILi256E": (128, 0), "11plan_kernelILi1024E": (128, 0), "11rows_kernel": (128, 0),
-    "20release_count_kernel": (128, 0), "14release_kernel": (128, 0),
+    "20release_count_kernel": (128, 0), "14release_kernel": (128, 0), "18release_sum_kernel": (128, 0),
     "13bounds_kernel": (128, 0), "12score_kernelILi1ELi64E": (128, 0), "12score_kernelILi1ELi128E": (168, 0),
     "12score_kernelILi1ELi256E": (512, 0), "18score_chunk_kernelILi1ELi64E": (128, 0), "18score_chunk_kernelILi1ELi128E": (168, 0),
     "18score_chunk_kernelILi1ELi256E": (512, 0), "15pick_few_kernel": (128, 0), "11pick_kernelILi1ELi1024E": (128, 0),

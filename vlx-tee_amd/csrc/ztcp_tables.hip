@@ -248,7 +248,8 @@ __global__ __launch_bounds__(256) void rows_kernel(AllotParams p) {
 // Entries that are pages, in columns that a sequence's tokens do not reach, in the
 // order of sequences and columns onto the end of the stack.  The first kernel counts
 // them by pieces of rows, the second adds up what lies before its piece; a thread has
-// all its entries of a piece on their way at once.  512 sequences of up to 4,098 columns,
+// all its entries of a piece on their way at once.  Of many thousand pieces, where adding up would be
+// the work, one workgroup turns the counts into sums in between.  512 sequences of up to 4,098 columns,
 // a quarter ended (17 MB): 6.5 and 7.5 us (6 and 14 with 256 columns at a time).
 
 constexpr int kPiece = 4096;        // columns
@@ -265,9 +266,11 @@ struct ReleaseParams {
     int64_t out_table_stride;
     int32_t* out_n_free;
     int32_t* released;
-    int64_t* counts;                 // [1 + n_seqs * pieces]: free pages there were, entries of each piece
+    int64_t* counts;                 // [2 + n_seqs * pieces]: free pages there were, entries of each piece
+    bool summed;                     // counts[1 + i] are those in front of piece i
     uint32_t first_block;
 };
+constexpr int64_t kMostCounted = 4096;   // pieces whose counts every workgroup adds up itself
 
 __device__ __forceinline__ int first_spare(const ReleaseParams& p, int s) {
     const int64_t n = ((int64_t)max(p.lens[s], 0) + p.page_tokens - 1) / p.page_tokens;
@@ -306,6 +309,44 @@ __global__ __launch_bounds__(256) void release_count_kernel(ReleaseParams p) {
     }
 }
 
+// Counts into what lies in front of each, and all behind the last.
+__global__ __launch_bounds__(1024) void release_sum_kernel(ReleaseParams p) {
+    constexpr int kOwn = 4;
+    __shared__ int64_t lds[16];
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t units = (int64_t)p.n_seqs * p.pieces;
+    int64_t before = 0;
+    for (int64_t first = 0; first < units; first += 1024 * kOwn) {
+        int64_t n[kOwn], own = 0;
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) {
+            const int64_t i = first + tid * kOwn + j;
+            own += n[j] = i < units ? p.counts[1 + i] : 0;
+        }
+        int64_t upto = own;
+        for (int m = 1; m < 64; m <<= 1) {
+            const int64_t y = (int64_t)__shfl_up((long long)upto, m);
+            upto += lane >= m ? y : 0;
+        }
+        __syncthreads();                                     // the sums of the turn before have been read
+        if (lane == 63) lds[wave] = upto;
+        __syncthreads();
+        int64_t at = before + upto - own;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            at += w < wave ? lds[w] : 0;
+            before += lds[w];
+        }
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) {
+            const int64_t i = first + tid * kOwn + j;
+            if (i < units) p.counts[1 + i] = at;
+            at += n[j];
+        }
+    }
+    if (tid == 0) p.counts[1 + units] = before;
+}
+
 __global__ __launch_bounds__(256) void release_kernel(ReleaseParams p) {
     __shared__ int64_t lds[4];
     __shared__ int scan[64];
@@ -316,19 +357,24 @@ __global__ __launch_bounds__(256) void release_kernel(ReleaseParams p) {
     const int32_t* row = p.table + s * p.table_stride;
     int32_t* out = p.out_table + s * p.out_table_stride;
     int64_t at = 0;
-    for (int64_t i = tid; i < unit; i += 256) at += p.counts[1 + i];
-    const int64_t had = p.counts[0];
-    at = had + block_sum(at, lds);
-    const int64_t last = (int64_t)p.n_seqs * p.pieces - 1;
+    if (p.summed) {
+        at = p.counts[1 + unit];
+    } else {
+        for (int64_t i = tid; i < unit; i += 256) at += p.counts[1 + i];
+        at = block_sum(at, lds);
+    }
+    at += p.counts[0];
+    auto count = [&](int64_t of) { return p.summed ? p.counts[2 + of] - p.counts[1 + of] : p.counts[1 + of]; };
+    const int64_t last = (int64_t)p.n_seqs * p.pieces - 1, here = count(unit);
     if (piece == 0 && tid == 0) {
         int64_t n = 0;
-        for (int i = 0; i < p.pieces; ++i) n += p.counts[1 + unit + i];
+        for (int i = 0; i < p.pieces; ++i) n += count(unit + i);
         p.released[s] = (int32_t)(min(at + n, p.capacity) - min(at, p.capacity));
     }
-    if (unit == last && tid == 0) *p.out_n_free = (int32_t)min(at + p.counts[1 + unit], p.capacity);
+    if (unit == last && tid == 0) *p.out_n_free = (int32_t)min(at + here, p.capacity);
     const int begin = piece * kPiece, end = (int)min((int64_t)begin + kPiece, (int64_t)p.max_pages), spare = first_spare(p, s);
     const bool moved = out != row;
-    if (!moved && p.counts[1 + unit] == 0) return;
+    if (!moved && here == 0) return;
     constexpr int kOwn = kPiece / 256;
     int32_t id[kOwn];
 #pragma unroll
@@ -458,7 +504,7 @@ extern "C" int ztcp_allot_pages(int32_t* page_table, int64_t table_stride, int64
 
 extern "C" size_t ztcp_release_pages_workspace(int64_t n_seqs, int64_t max_pages) {
     if (n_seqs < 0 || n_seqs >= (int64_t)1 << 24 || max_pages < 1 || max_pages >= (int64_t)1 << 31) return (size_t)-1;
-    return (size_t)(1 + n_seqs * release_pieces(max_pages)) * sizeof(int64_t);
+    return (size_t)(2 + n_seqs * release_pieces(max_pages)) * sizeof(int64_t);
 }
 
 extern "C" int ztcp_release_pages(const int32_t* page_table, int64_t table_stride, int64_t max_pages, const int32_t* kv_lens,
@@ -507,7 +553,9 @@ extern "C" int ztcp_release_pages(const int32_t* page_table, int64_t table_strid
         return hipGetLastError() == hipSuccess ? ZTCP_OK : ZTCP_EHIP;
     }
     const uint64_t units = (uint64_t)n_seqs * (uint64_t)p.pieces;
+    p.summed = units > kMostCounted;
     launch_blocks(release_count_kernel, units, 256, 0, (hipStream_t)stream, p);
+    if (p.summed) hipLaunchKernelGGL(release_sum_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, p);
     launch_blocks(release_kernel, units, 256, 0, (hipStream_t)stream, p);
     return hipGetLastError() == hipSuccess ? ZTCP_OK : ZTCP_EHIP;
 }
