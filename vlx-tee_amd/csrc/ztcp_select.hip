@@ -371,9 +371,10 @@ __host__ __device__ inline int chunk_tokens(int group, int width) {
     return group <= fit ? fit / group * 16 : group <= most ? 16 : 0;
 }
 
-template <int DT, int DP>
+// STEPS: products of depth 32 that hold head_dim.
+template <int DT, int DP, int STEPS>
 __global__ __launch_bounds__(256) void score_chunk_kernel(SelectParams p) {
-    constexpr int kSteps = DP / 32, kChunks = DP / 8, kLoadRows = 64 / kChunks, kRowBytes = DP * 2;
+    constexpr int kSteps = STEPS, kChunks = DP / 8, kLoadRows = 64 / kChunks, kRowBytes = DP * 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t columns[];   // [negative, positive][product][16][DP]
     const int lane = (int)threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, quad = lane >> 4;
@@ -932,11 +933,13 @@ __global__ __launch_bounds__(256) void pick_few_kernel(SelectParams p) {
             key[c] = 0;
             if (64 * c >= n) continue;
             const int i = 64 * c + lane;
-            const bool there = i < n && id[c] >= 0 && id[c] < p.batch.n_pages, always = there && (i < p.sink || i >= n - p.recent);
-            const bool known = x[c] == x[c];
-            if (there && !always) key[c] = known ? order_of(x[c]) : 1u;
-            taken |= always ? 1u << c : 0u;
-            forced += __popcll(__ballot(always));
+            const bool there = i < n && (uint32_t)id[c] < (uint32_t)p.batch.n_pages, known = x[c] == x[c];
+            if (there) key[c] = known ? order_of(x[c]) : 1u;
+            if (64 * c < p.sink || 64 * c + 64 > n - p.recent) {   // some that are always taken
+                const bool always = there && (i < p.sink || i >= n - p.recent);
+                if (always) key[c] = 0, taken |= 1u << c;
+                forced += __popcll(__ballot(always));
+            }
             open += __popcll(__ballot(key[c] != 0));
             unknown += __popcll(__ballot(key[c] == 1u));
         }
@@ -1170,7 +1173,8 @@ extern "C" int ztcp_select_pages(const void* q, int64_t q_stride, int64_t q_head
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         if (chunk_units > 0) {
-            auto kernel = d <= 64 ? score_chunk_kernel<DT, 64> : d <= 128 ? score_chunk_kernel<DT, 128> : score_chunk_kernel<DT, 256>;
+            auto kernel = d <= 64 ? score_chunk_kernel<DT, 64, 2> : d <= 96 ? score_chunk_kernel<DT, 128, 3> : d <= 128 ? score_chunk_kernel<DT, 128, 4>
+                        : d <= 192 ? score_chunk_kernel<DT, 256, 6> : score_chunk_kernel<DT, 256, 8>;
             // over 64 KiB of dynamic LDS has to be asked for
             if (chunk_lds > (size_t)48 * 1024 &&
                 hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024) != hipSuccess)
