@@ -360,9 +360,10 @@ __global__ __launch_bounds__(256) void score_kernel(SelectParams p) {
 // negative and their positive numbers apart, and goes over up to 1,024 pages with them, 16 a wave and turn, whose bounds
 // come as the products want them, from the caches most of the time, a turn ahead.
 //
-// 2 x 2,000 tokens, 3 query heads to each of 5 KV heads of 96, over 525 pages: 42 us (52 with signs
-// looked at for every product), 12 of them before the first product; 57 by the kernel above,
-// whose waves wait for the columns of each product.
+// 2 x 2,000 tokens, 3 query heads to each of 5 KV heads of 96, over 525 pages: 36 us (52 with signs looked at for every
+// product, 42 with products as deep as 128; 32 pages a wave and turn, which read the columns half as often, take the
+// registers of a third wave a SIMD: 47), 12 of them before the first product; 57 by the kernel above, whose waves wait
+// for the columns of each product.
 constexpr int kPieceTiles = 16;
 // Tokens of a block: as many as make six products (48 KiB at 128 elements, three workgroups a compute unit), or 16 with up
 // to eight; half as many for wider vectors; 0: too many heads.
