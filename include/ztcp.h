@@ -503,7 +503,8 @@ ZTCP_API int ztcp_selected_attention(const void* q, int64_t q_stride, void* out,
  *   q_starts [n_seqs + 1]: sums of granted [n_seqs], which is q or 0;
  *   slots, positions [max_rows]: of sequence s's i-th new token, which is token L + i,
  *   page * num_tokens + token in page (-1 where its entry is negative), and
- *   next_positions[s] + i (NULL: L + i); -1 and 0 behind the last row;
+ *   next_positions[s] + i (NULL: L + i), which are a line's positions (tokens of a tree stand
+ *   at their depths: the caller's to count); -1 and 0 behind the last row;
  *   out_next_positions [n_seqs] = next_positions + granted (may be next_positions).
  * workspace: ztcp_allot_pages_workspace(...) bytes (may be 0; (size_t)-1 for numbers that
  * the call refuses), 16-byte aligned, needed until the call's work is done, by one call

@@ -110,7 +110,10 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     """``paged_attention`` of drafted tokens that form a tree: each of a sequence's n new tokens sees all tokens in
     front of the new ones and, of these, the j-th if bit ``j % 64`` of word ``j // 64`` of its row of ``tree_mask``
     [rows, words] (int64) is set: itself and its ancestors.  Bits from n on are not looked at; new tokens behind the last
-    word are not seen; a token whose own bit is not set does not see itself."""
+    word are not seen; a token whose own bit is not set does not see itself.
+
+    The tokens of a tree are to be appended at the positions of their depths, the length in front of the draft plus the
+    number of a token's ancestors, which are not those that ``allot_pages`` lays out."""
     return _call().tree_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts, tree_mask, scale, max_q_len, return_lse,
                                   out)
 
@@ -207,8 +210,9 @@ def allot_pages(page_table: torch.Tensor, kv_lens: torch.Tensor, q_lens: torch.T
     its end and written into ``page_table``.  A sequence gets all or nothing: it waits (``granted`` 0) if the rows that
     it and the sequences in front ask for exceed ``max_rows``, if it needs a page and the pages that they ask for exceed
     ``n_free``, or if its table row has no column left.  Positions go on from ``next_positions`` (after an eviction a
-    sequence's own count is more than its length), from ``kv_lens`` if there are none.  A new token whose page is not
-    there (its last page is cold) has slot -1.
+    sequence's own count is more than its length), from ``kv_lens`` if there are none, one further for each row: a line's,
+    not a drafted tree's, whose tokens stand at their depths.  A new token whose page is not there (its last page is cold)
+    has slot -1.
 
     ``page_table`` is written in either case; ``in_place`` updates ``kv_lens``, ``n_free`` and ``next_positions`` too."""
     return Allotment._make(_call().allot_pages(page_table, kv_lens, q_lens, free_pages, n_free, page_tokens, max_rows,
