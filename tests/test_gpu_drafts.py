@@ -110,3 +110,25 @@ def test_an_accepted_line_is_what_plain_decoding_leaves(A, dtype, counted):
         assert torch.equal(a, b)
     if counted:
         assert torch.equal(tree.next, plain.next)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_bounds_of_pages_that_moved_keys_fill(A, dtype):
+    """The line ends with its page, which no later token enters: only a renewal brings the moved keys into the page's bounds."""
+    e = Engine(A, dtype, False)
+    e.append([29, 13, 61], _rand(29 + 13 + 61, 3, dtype))
+    held = e.lens.clone()
+    plan, _ = e.append([len(PARENTS)] * SEQS, _rand(len(PARENTS) * SEQS, 4, dtype), DEPTH)
+    e.accept(plan, held, LINE)
+    assert bool((e.lens % T == 0).all())
+    A.release_pages(e.table, e.lens, e.free, e.n_free, page_tokens=T, in_place=True)
+    want = R.bounds(e.k, torch.zeros_like(e.bounds), e.table, e.lens, torch.cat([e.lens.new_zeros(1), e.lens.cumsum(0)]).int())
+    ids = torch.cat([e.table[s, :int(e.lens[s]) // T] for s in range(SEQS)]).long()
+
+    def covers():
+        return bool((e.bounds[ids, 0] <= want.cuda()[ids, 0]).all() and (e.bounds[ids, 1] >= want.cuda()[ids, 1]).all())
+
+    assert not covers()   # what the draft left does not hold of the moved keys
+    starts = torch.arange(SEQS + 1, dtype=torch.int32, device="cuda") * len(LINE)
+    A.page_bounds(e.k, e.bounds, e.table, e.lens, starts)
+    assert torch.equal(e.bounds[ids].cpu(), want[ids.cpu()])

@@ -122,8 +122,9 @@ def page_bounds(k_pages: torch.Tensor, bounds: torch.Tensor, page_table: torch.T
                 q_starts: torch.Tensor, *, max_q_len: int | None = None) -> torch.Tensor:
     """Brings ``bounds`` [n_pages, 2, kv_heads, d] (the pages' dtype) up to date for the pages that hold the step's new
     tokens: the least and the greatest number of each column of a page's keys, over all of its tokens; NaN where a key's
-    is.  Other pages' bounds are left: for pages whose keys were written otherwise (brought back by ``pages.ingress``,
-    moved), call it with ``q_starts`` that count all of a sequence's tokens as new.  Returns ``bounds``."""
+    is.  Other pages' bounds are left: for keys that were written otherwise call it with ``q_starts`` that count these as
+    new, the accepted tokens of a draft that have been moved, or all tokens of a sequence whose pages ``pages.ingress``
+    brought back.  Returns ``bounds``."""
     return _call().page_bounds(k_pages, bounds, page_table, kv_lens, q_starts, max_q_len)
 
 
