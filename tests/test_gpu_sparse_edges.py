@@ -1,0 +1,55 @@
+"""GPU tests of page selection and attention over selected pages at the ends of what one form of a kernel takes."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import sparse_reference as R
+from test_gpu_sparse import BF, FP, A, _attend, _attend_case, _check_select, _i32, _reference, _say, _select_case  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def _nan_as(c, what):
+    """A row's log-sum-exp, and with it all of its result, is NaN exactly where the formula's is; other numbers as they are."""
+    out, lse = _attend(A_, c)
+    want = _reference(c)
+    bad = torch.isnan(want[1])
+    assert torch.equal(torch.isnan(lse.cpu()), bad), what
+    assert torch.equal(torch.isnan(out.cpu()), torch.isnan(want[0])), what
+    return bad
+
+
+@pytest.fixture(autouse=True)
+def _module(A):
+    global A_
+    A_ = A
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("lens,kv,group,d,t,listed", [
+    ([(4, 100), (1, 60)], 2, 2, 64, 16, 4), ([(3, 900), (1, 500)], 2, 40, 128, 16, 20), ([(2, 700)], 1, 3, 256, 13, 9),
+    ([(1200, 1300)], 1, 1, 64, 16, 3), ([(300, 700), (260, 500)], 8, 4, 128, 16, 6), ([(300, 700), (260, 500)], 8, 4, 96, 13, 6)])
+def test_a_key_of_nan_makes_its_rows_nan(lens, kv, group, d, t, listed, dtype):
+    """Few rows, rows one by one and blocks: a maximum that passes NaN over must not lose it."""
+    _say("selected, keys of NaN", lens, kv, group, d, t)
+    bad = []
+    for seed in (1, 2):
+        c = _attend_case(lens, kv, group, d, t, dtype, listed, seed=seed)
+        for s, (_, n) in enumerate(lens):
+            pages = -(-n // t)
+            for page in (0, pages // 2, pages - 1):
+                if page * t < n:
+                    c["k"][int(c["table"][s, page]), 0, page % kv, 3] = math.nan
+        bad.append(_nan_as(c, (lens, seed)))
+    assert bool(torch.stack(bad).any()) and not bool(torch.stack(bad).all())
+
+
+@pytest.mark.parametrize("columns", [11788, 11789, 12287, 12288, 12289])
+def test_select_of_tables_at_the_local_memory_s_end(columns):
+    _say("select, columns", columns)
+    for lens in ([(1, columns)], [(257, columns)]) if columns in (12288, 12289) else ([(1, columns)],):   # a row a workgroup of 1,024, of 256
+        c = _select_case(lens, 2, 1, 16, 1, BF, missing=0.02, seed=columns)
+        _check_select(A_, c, 50, 1, 2, (columns, lens))
