@@ -61,3 +61,16 @@ def test_registers_and_scratch_fit(metadata, frag):
     for name, m in hits.items():
         assert m["private_segment_fixed_size"] <= scratch, (name, m)
         assert m["vgpr_count"] <= registers, (name, m)   # both kinds of registers
+
+
+# registers that the chunk kernels spill: kernel<dtype, head_dim, whole tiles, drafted trees>
+SPILLS = {"11many_kernelILi%dELi64ELb0ELb0E": 0, "11many_kernelILi%dELi64ELb1ELb0E": 0, "11many_kernelILi%dELi128ELb0ELb0E": 30,
+          "11many_kernelILi%dELi128ELb1ELb0E": 19, "11many_kernelILi%dELi256ELb0ELb0E": 70, "11many_kernelILi%dELi256ELb1ELb0E": 40}
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("frag", sorted(SPILLS))
+def test_chunk_kernels_spill_no_more(metadata, frag, dtype):
+    """Scratch that spills share does not tell their number: reads of it in a chunk's loop are time."""
+    hits = [m for n, m in metadata.items() if frag % dtype in n]
+    assert len(hits) == 1 and hits[0]["vgpr_spill_count"] <= SPILLS[frag], hits

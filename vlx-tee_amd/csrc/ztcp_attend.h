@@ -558,9 +558,20 @@ void many_kernel(AttendParams p) {
     const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
     const int limit = r < rows ? max(0, seq.len - seq.n_new + (TREE ? 0 : token + 1)) : 0;   // (TREE: keys in front of the new ones)
     const int tree_row = r < rows ? seq.row0 + token : seq.row0;                         // row of this lane's mask
-    auto sees = [&](int row) { return max(0, seq.len - seq.n_new + (TREE ? 0 : row / p.group + 1)); };
-    const int stop = TREE ? key1 : min(key1, sees(min(rows, (block + 1) * kManyRows) - 1));                  // of the workgroup
-    const int wave_stop = r0 >= rows ? 0 : TREE ? key1 : min(key1, sees(min(rows, r0 + 32) - 1));            // of this wave
+    // (A chunk's in expressions of its own: written as one with the tree's, the compiler spills 120 registers more at 256
+    // elements.)
+    int stop, wave_stop;                                      // of the workgroup, of this wave
+    auto sees = [&](int row) {
+        if constexpr (TREE) return max(0, seq.len - seq.n_new);
+        else return max(0, seq.len - seq.n_new + row / p.group + 1);
+    };
+    if constexpr (TREE) {
+        stop = key1;
+        wave_stop = r0 >= rows ? 0 : key1;
+    } else {
+        stop = min(key1, sees(min(rows, (block + 1) * kManyRows) - 1));
+        wave_stop = r0 < rows ? min(key1, sees(min(rows, r0 + 32) - 1)) : 0;
+    }
     const int first_sees = sees(block * kManyRows);                                      // the row that sees least
     const int wave_full = r0 + 32 <= rows ? sees(r0) : 0;                                // keys that all its rows see
     // 16-byte pieces are permuted within a row so that the rows of one read lie in different banks

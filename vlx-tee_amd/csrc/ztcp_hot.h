@@ -231,7 +231,7 @@ __device__ __forceinline__ Place place_of(const PagedView& v, const Seq& q, int 
     Place p{-1, 0};
     if (key < stop) {
         const int at = div_page(key, v.page_div);
-        const int id = q.entry(at);
+        const int id = q.table[at];
         if (id >= 0 && id < v.n_pages) p.page = id;
         p.row = key - at * v.page_tokens;
     }
