@@ -493,6 +493,13 @@ __device__ __forceinline__ int blocks_of(const AttendParams& p, const Seq& q) {
     const int rows = q.n_new * p.group;
     return rows > p.few_rows ? (rows + kManyRows - 1) / kManyRows : 0;
 }
+// Tokens of a piece, of `work` tokens of all blocks and KV heads: at least 1 / splits of the longest context, and no more
+// than hold that whole (a share of much work has more bits than a length).
+constexpr __host__ __device__ int tree_piece_tokens(int64_t work, int resident, int longest, int splits) {
+    const int64_t share = work * 2 / (3 * (int64_t)resident), least = ((int64_t)longest + splits - 1) / splits;
+    const int64_t wanted = share > least ? share : least, tokens = wanted < longest ? wanted : longest;
+    return (int)((tokens + kTreePiece - 1) / kTreePiece * kTreePiece);
+}
 __device__ __forceinline__ Cut tree_cut(const AttendParams& p) {
     if (p.splits == 1) return Cut{1, p.batch.max_tokens};
     const int lane = (int)threadIdx.x & 63;
@@ -509,9 +516,7 @@ __device__ __forceinline__ Cut tree_cut(const AttendParams& p) {
         work += (int64_t)__shfl_xor((long long)work, m);
         longest = max(longest, __shfl_xor(longest, m));
     }
-    const int64_t share = work * p.kv_heads * 2 / (3 * (int64_t)p.resident), least = ((int64_t)longest + p.splits - 1) / p.splits;
-    const int64_t tokens = max(max(share, least), (int64_t)1);
-    return Cut{p.splits, uniform((int)((tokens + kTreePiece - 1) / kTreePiece * kTreePiece))};
+    return Cut{p.splits, uniform(tree_piece_tokens(work * p.kv_heads, p.resident, longest, p.splits))};
 }
 
 // Zeros that the tile loads read in the place of tokens that are not there: a row of 256 elements.
