@@ -1,0 +1,39 @@
+"""What the operators on hot pages keep between their kernels does not grow with the call beyond a gigabyte (and what grows with
+the batch's tables alone): larger calls are done in parts."""
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+import torch
+
+import sparse_reference as R
+from test_gpu_sparse import BF, FP, _select_case
+from test_hot_refusals import N, _batch, _geo, _pool  # noqa: F401  (N: the module's fixture)
+
+MOST = 1 << 30
+
+
+@pytest.mark.parametrize("rows,pages,kv,group", [(65536, 4096, 8, 4), (65536, 8192, 8, 8), (100000, 500, 1, 1), (3, 1 << 20, 8, 4), (1, 1 << 22, 64, 1)])
+def test_selection(N, rows, pages, kv, group):
+    batch, geo = _batch(N, n_rows=rows, max_pages=pages, table_stride=pages, n_seqs=4), _geo(N, h=kv)
+    need = N.lib().ztcp_select_pages_workspace(C.byref(batch), 1 << 20, C.byref(geo), kv * group)
+    assert 4 * kv * pages <= need <= max(MOST, 4 * kv * pages) + 4 * (4 * kv * (-(-pages // 16)) + 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,group,d", [(BF, 2, 16), (FP, 9, 16), (BF, 4, 96), (FP, 1, 256)])
+def test_selection_in_parts(hip, dtype, group, d):
+    """Tables of 8,192 columns and 39,855 rows: three parts of 13,285 rows, with sequences across both borders.  Most rows see
+    no page, which costs the reference nothing."""
+    import vlx_tee_amd.attention as A
+
+    lens = [(13270, 0), (40, 1200), (13090, 0), (300, 400), (13154, 0), (1, 1200)]
+    print("case", dtype, group, d, flush=True)
+    c = _select_case(lens, 2, group, d, 1, dtype, seed=d, missing=0.1)
+    wide = torch.full((len(lens), 8192), -1, dtype=torch.int32, device="cuda")
+    wide[:, :c["table"].shape[1]] = c["table"]
+    out = torch.full((c["q"].shape[0], 2, 9), -7, dtype=torch.int32, device="cuda")
+    want = R.select(c["q"], c["b"], wide, c["lens"], c["starts"], 1, 9, 1, 2, out)
+    got = A.select_pages(c["q"], c["b"], wide, c["lens"], c["starts"], page_tokens=1, budget=9, sink=1, recent=2, out=out)
+    assert torch.equal(got.cpu(), want), int((got.cpu() != want).sum())

@@ -66,6 +66,10 @@ inline void launch_blocks(void (*kernel)(Params, More...), uint64_t blocks, uint
     }
 }
 
+// Bytes that a call which could do with less keeps between its kernels at most: beyond, it works in parts that use the same
+// memory again.
+constexpr int64_t kMostBetween = (int64_t)1 << 30;
+
 // Compute units of the current device.
 inline int cu_count(int& cus) {
     int dev = 0;

@@ -136,14 +136,27 @@ struct SelectParams {
     int64_t bounds_page;             // elements between pages
     int32_t kv_heads, group, head_dim;
     int32_t budget, sink, recent;
+    int32_t row0, row1;              // rows that these launches take
     int32_t score_stride, tops;      // floats of a row's scores (a multiple of 4), of a sequence's tops for a head
-    float* scores;                   // [rows, kv_heads, score_stride]; NaN: no finite number
+    float* scores;                   // [row1 - row0, kv_heads, score_stride]; NaN: no finite number
     int32_t score_groups;            // score kernel: workgroups of a KV head
     int32_t few_pages;               // pick kernel: rows of at most so many pages (-1: none) are another kernel's
     float* top;                      // [n_seqs, kv_heads, tops]: the greatest bound of 16 pages, by magnitude
     int32_t* out;
     uint32_t first_block;
 };
+
+// What a sequence has in rows row0 .. row1: these as its new tokens, of a length that its last one there sees.
+__device__ __forceinline__ Seq part_of(const SelectParams& p, Seq q) {
+    const int first = max(q.row0, p.row0), behind = q.row0 + q.n_new, end = min(behind, p.row1);
+    q.len -= behind - end;
+    q.row0 = first;
+    q.n_new = max(end - first, 0);
+    return q;
+}
+__device__ __forceinline__ float* scores_of(const SelectParams& p, int row, int head) {
+    return p.scores + ((int64_t)(row - p.row0) * p.kv_heads + head) * p.score_stride;
+}
 
 // Pages that a sequence's first `tokens` new tokens see.
 __device__ __forceinline__ int pages_seen(const SelectParams& p, const Seq& q, int tokens) {
@@ -200,7 +213,10 @@ __global__ __launch_bounds__(256) void score_kernel(SelectParams p) {
     const int head = (int)(blockIdx.x % (uint32_t)p.kv_heads), group = (int)(blockIdx.x / (uint32_t)p.kv_heads);
     auto tiles_of = [&](const Seq& q) { return (pages_seen(p, q, q.n_new) + kTilePages - 1) / kTilePages; };
     auto blocks_of = [&](const Seq& q) { return q.n_new > 0 ? (q.n_new - 1) / kBlockTokens + 1 : 0; };
-    auto units_of = [&](const Seq& q) { return tiles_of(q) * blocks_of(q); };
+    auto units_of = [&](const Seq& whole) {
+        const Seq q = part_of(p, whole);
+        return tiles_of(q) * blocks_of(q);
+    };
     struct Unit {
         int s, tile, block, tiles, pages;
         Seq seq;
@@ -213,7 +229,7 @@ __global__ __launch_bounds__(256) void score_kernel(SelectParams p) {
     int left = min(quota, total - first);
     auto open = [&](Unit& u) {       // u.s's sequence, or the next one that has units
         for (; u.s < p.batch.n_seqs; ++u.s) {
-            u.seq = uniform(seq_of(p.batch, u.s));
+            u.seq = uniform(part_of(p, seq_of(p.batch, u.s)));
             u.pages = uniform(pages_seen(p, u.seq, u.seq.n_new));
             u.tiles = (u.pages + kTilePages - 1) / kTilePages;
             if (u.seq.n_new > 0 && u.tiles > 0) return;
@@ -347,7 +363,7 @@ __global__ __launch_bounds__(256) void score_kernel(SelectParams p) {
             const int at = page0 + 4 * quad;
             if (col_head == 0 && t0 + col_token < tokens && at < p.score_stride) {
                 const int token = token0 + t0 + col_token;
-                float* dst = p.scores + ((int64_t)(seq.row0 + token) * p.kv_heads + head) * p.score_stride + at;
+                float* dst = scores_of(p, seq.row0 + token, head) + at;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) best[e] = best[e] < INFINITY ? best[e] : NAN;
                 *reinterpret_cast<float4*>(dst) = make_float4(best[0], best[1], best[2], best[3]);
@@ -384,12 +400,15 @@ __global__ __launch_bounds__(256) void score_chunk_kernel(SelectParams p) {
     int at = (int)(unit / (uint32_t)p.kv_heads);
     auto tiles_of = [&](const Seq& q) { return (pages_seen(p, q, q.n_new) + kTilePages - 1) / kTilePages; };
     auto pieces_of = [&](const Seq& q) { return (tiles_of(q) + kPieceTiles - 1) / kPieceTiles; };
-    auto units_of = [&](const Seq& q) { return q.n_new > 0 ? ((q.n_new - 1) / block_size + 1) * pieces_of(q) : 0; };
+    auto units_of = [&](const Seq& whole) {
+        const Seq q = part_of(p, whole);
+        return q.n_new > 0 ? ((q.n_new - 1) / block_size + 1) * pieces_of(q) : 0;
+    };
     const int s = uniform(find_tile(p.batch, at, units_of));
     if (s >= p.batch.n_seqs) return;
-    const Seq seq = uniform(seq_of(p.batch, s));
+    const Seq whole = seq_of(p.batch, s), seq = uniform(part_of(p, whole));
     const int pieces = uniform(pieces_of(seq));
-    if (at < 0 || at >= units_of(seq)) return;                // (starts that do not ascend)
+    if (at < 0 || at >= units_of(whole)) return;              // (starts that do not ascend)
     at = uniform(at);
     const int block = at / pieces, piece = at - block * pieces;
     const int token0 = block * block_size, tokens = min(seq.n_new - token0, block_size);
@@ -467,7 +486,7 @@ __global__ __launch_bounds__(256) void score_chunk_kernel(SelectParams p) {
             if (++h < p.group) continue;
             const int to = page0 + 4 * quad;
             if (t0 + col < tokens && to < p.score_stride) {
-                float* dst = p.scores + ((int64_t)(seq.row0 + token0 + t0 + col) * p.kv_heads + head) * p.score_stride + to;
+                float* dst = scores_of(p, seq.row0 + token0 + t0 + col, head) + to;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) best[e] = best[e] < INFINITY ? best[e] : NAN;
                 *reinterpret_cast<float4*>(dst) = make_float4(best[0], best[1], best[2], best[3]);
@@ -690,19 +709,19 @@ __global__ __launch_bounds__(THREADS) void pick_kernel(SelectParams p) {
     __shared__ PickShared<THREADS> sh;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int64_t unit = (int64_t)p.first_block + blockIdx.x;
-    const int row = (int)(unit / p.kv_heads), head = (int)(unit % p.kv_heads);
+    const int row = p.row0 + (int)(unit / p.kv_heads), head = (int)(unit % p.kv_heads);
     int s = find_above(p.batch.starts + 1, p.batch.n_seqs, row);
     if (s >= p.batch.n_seqs) return;
     const Seq seq = uniform(seq_of(p.batch, s));
     if (row < seq.row0 || row >= seq.row0 + seq.n_new) return;
     const int n = pages_seen(p, seq, row - seq.row0 + 1);
     if (n <= p.few_pages) return;
-    uint32_t* scores = reinterpret_cast<uint32_t*>(p.scores + unit * p.score_stride);   // (as words, since keys may take their place)
+    uint32_t* scores = reinterpret_cast<uint32_t*>(scores_of(p, row, head));   // (as words, since keys may take their place)
     uint32_t* keys;
     if constexpr (IN_LDS) keys = lds_keys;
     else keys = scores;
     const uint8_t* q = p.q + 2 * ((int64_t)row * p.q_stride + (int64_t)head * p.group * p.head_dim);
-    int32_t* out = p.out + unit * p.budget;
+    int32_t* out = p.out + ((int64_t)row * p.kv_heads + head) * p.budget;
 
     for (int i = tid; i < kBins; i += THREADS) sh.bins[i] = 0;
     if (tid == 0) sh.n_few = sh.n_near = 0;
@@ -887,8 +906,8 @@ __global__ __launch_bounds__(256) void pick_few_kernel(SelectParams p) {
     constexpr int kOwn = OWN;                                 // pages of a lane: 64 OWN are enough for every row
     const int lane = (int)threadIdx.x & 63;
     const int64_t unit = ((int64_t)p.first_block + blockIdx.x) * 4 + uniform((int)threadIdx.x >> 6);
-    const int64_t wide_row = unit / p.kv_heads;
-    if (wide_row >= p.batch.n_rows) return;
+    const int64_t wide_row = p.row0 + unit / p.kv_heads;
+    if (wide_row >= p.row1) return;
     const int row = (int)wide_row, head = (int)(unit % p.kv_heads);
     const int s = uniform(find_above(p.batch.starts + 1, p.batch.n_seqs, row));
     if (s >= p.batch.n_seqs) return;
@@ -896,9 +915,9 @@ __global__ __launch_bounds__(256) void pick_few_kernel(SelectParams p) {
     if (row < seq.row0 || row >= seq.row0 + seq.n_new) return;
     const int n = uniform(pages_seen(p, seq, row - seq.row0 + 1));
     if (n > 64 * OWN) return;                                 // (another kernel's)
-    const float* scores = p.scores + unit * p.score_stride;
+    const float* scores = scores_of(p, row, head);
     const uint8_t* q = p.q + 2 * ((int64_t)row * p.q_stride + (int64_t)head * p.group * p.head_dim);
-    int32_t* out = p.out + unit * p.budget;
+    int32_t* out = p.out + ((int64_t)row * p.kv_heads + head) * p.budget;
 
     // |q|_1, of four heads at once (two of vectors of more than 128 elements), and the greatest bound
     float sum = 0.f;
@@ -1049,14 +1068,19 @@ const char* check_bounds(const void* bounds, int64_t stride, const ztcp_geometry
 }
 
 struct SelectPlan {
-    int64_t stride, tops, units, floats;   // units: 64 pages and a block of tokens each, at most
+    int64_t stride, tops, units;     // units: 64 pages and a block of tokens each, at most
+    int64_t scores, rows, floats;    // scores of the call; rows that are scored and chosen for at a time; the workspace
 };
 SelectPlan plan_select(const ztcp_paged_batch* b, const ztcp_geometry* g) {
     SelectPlan plan;
     plan.stride = (b->max_pages + 3) / 4 * 4;
     plan.tops = (b->max_pages + 15) / 16;
     plan.units = (b->n_rows / kBlockTokens + b->n_seqs) * ((b->max_pages + kTilePages - 1) / kTilePages);
-    plan.floats = b->n_rows * g->num_heads * plan.stride + (b->n_seqs * g->num_heads * plan.tops + 3) / 4 * 4;
+    const int64_t row = g->num_heads * plan.stride, most = kMostBetween / (row * (int64_t)sizeof(float));
+    plan.scores = b->n_rows * row;
+    const int64_t parts = b->n_rows > 0 ? (b->n_rows - 1) / (most > 0 ? most : 1) + 1 : 1;
+    plan.rows = (b->n_rows + parts - 1) / parts;             // alike
+    plan.floats = plan.rows * row + (b->n_seqs * g->num_heads * plan.tops + 3) / 4 * 4;
     return plan;
 }
 
@@ -1075,7 +1099,7 @@ const char* check_select(const ztcp_paged_batch* batch, const void* bounds, int6
     pool.k_stride = 0;
     if (const char* why = check_batch(batch, &pool, g, q_heads, view)) return why;
     const SelectPlan plan = plan_select(batch, g);
-    if (plan.stride >= (int64_t)1 << 31 || plan.units * g->num_heads >= (int64_t)1 << 31 || plan.floats >= (int64_t)1 << 40)
+    if (plan.stride >= (int64_t)1 << 31 || plan.units * g->num_heads >= (int64_t)1 << 31 || plan.scores >= (int64_t)1 << 40)
         return "too many rows and pages in one call";
     return nullptr;
 }
@@ -1165,14 +1189,15 @@ extern "C" int ztcp_select_pages(const void* q, int64_t q_stride, int64_t q_head
     // chunks: sequences of more than 16 new tokens on average, as many workgroups as half the compute units at least
     const int64_t block = chunk_tokens(p.group, d <= 128 ? 128 : 256);
     const size_t chunk_lds = (size_t)(block * p.group) * (d <= 64 ? 64 : d <= 128 ? 128 : 256) * 4;
-    int64_t chunk_units = 0;
-    if (block > 0 && batch->n_rows > 16 * batch->n_seqs) {
-        const int64_t pieces = (batch->max_pages + kPieceTiles * kTilePages - 1) / (kPieceTiles * kTilePages);
-        chunk_units = (batch->n_rows / block + batch->n_seqs) * pieces * g->num_heads;
-        if (batch->n_rows / block * g->num_heads < cus / 2 || chunk_units >= (int64_t)1 << 31) chunk_units = 0;
-    }
+    const int64_t pieces = (batch->max_pages + kPieceTiles * kTilePages - 1) / (kPieceTiles * kTilePages);
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
+        const int64_t rows = p.row1 - p.row0;
+        int64_t chunk_units = 0;
+        if (block > 0 && batch->n_rows > 16 * batch->n_seqs) {
+            chunk_units = (rows / block + batch->n_seqs) * pieces * g->num_heads;
+            if (rows / block * g->num_heads < cus / 2 || chunk_units >= (int64_t)1 << 31) chunk_units = 0;
+        }
         if (chunk_units > 0) {
             auto kernel = d <= 64 ? score_chunk_kernel<DT, 64, 2> : d <= 96 ? score_chunk_kernel<DT, 128, 3> : d <= 128 ? score_chunk_kernel<DT, 128, 4>
                         : d <= 192 ? score_chunk_kernel<DT, 256, 6> : score_chunk_kernel<DT, 256, 8>;
@@ -1186,7 +1211,7 @@ extern "C" int ztcp_select_pages(const void* q, int64_t q_stride, int64_t q_head
             hipLaunchKernelGGL((d <= 64 ? score_kernel<DT, 64> : d <= 128 ? score_kernel<DT, 128> : score_kernel<DT, 256>), grid, dim3(256),
                                0, (hipStream_t)stream, p);
         }
-        const uint64_t picks = (uint64_t)batch->n_rows * (uint64_t)g->num_heads;
+        const uint64_t picks = (uint64_t)rows * (uint64_t)g->num_heads;
         const bool many = picks > 2 * (uint64_t)cus;          // rows: a wave each if their pages are few
         if (batch->max_pages <= kFewPages || many)
             launch_blocks(batch->max_pages <= 256 ? pick_few_kernel<DT, 4> : batch->max_pages <= 576 ? pick_few_kernel<DT, 9> : pick_few_kernel<DT, 16>,
@@ -1199,7 +1224,12 @@ extern "C" int ztcp_select_pages(const void* q, int64_t q_stride, int64_t q_head
         else launch_blocks(in_lds ? pick_kernel<DT, 1024, true> : pick_kernel<DT, 1024, false>, picks, 1024, lds, (hipStream_t)stream, p);
         return true;
     };
-    if (!(g->hot_dtype == ZTCP_HOT_BF16 ? go(std::integral_constant<int, kHotBf16>{}) : go(std::integral_constant<int, kHotFp16>{})))
-        return ZTCP_EHIP;
+    // rows of as many scores as the workspace holds, and then those behind them in the same place
+    for (int64_t row0 = 0; row0 < batch->n_rows; row0 += plan.rows) {
+        p.row0 = (int32_t)row0;
+        p.row1 = (int32_t)(batch->n_rows - row0 < plan.rows ? batch->n_rows : row0 + plan.rows);
+        if (!(g->hot_dtype == ZTCP_HOT_BF16 ? go(std::integral_constant<int, kHotBf16>{}) : go(std::integral_constant<int, kHotFp16>{})))
+            return ZTCP_EHIP;
+    }
     return hipGetLastError() == hipSuccess ? ZTCP_OK : ZTCP_EHIP;
 }
