@@ -37,3 +37,34 @@ def test_selection_in_parts(hip, dtype, group, d):
     want = R.select(c["q"], c["b"], wide, c["lens"], c["starts"], 1, 9, 1, 2, out)
     got = A.select_pages(c["q"], c["b"], wide, c["lens"], c["starts"], page_tokens=1, budget=9, sink=1, recent=2, out=out)
     assert torch.equal(got.cpu(), want), int((got.cpu() != want).sum())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,kv,group,d", [(16384, 8, 4, 128), (65536, 8, 8, 256), (8192, 32, 1, 64), (40, 1, 8, 128)])
+def test_pieces_of_trees(hip, N, rows, kv, group, d):
+    for pages in (3, 300, 9000):
+        batch, geo = _batch(N, n_rows=rows, max_pages=pages, table_stride=pages, n_seqs=4), _geo(N, h=kv, d=d)
+        pool = _pool(N, k_stride=16 * kv * d, v_stride=16 * kv * d)
+        need = N.lib().ztcp_tree_attention_workspace(C.byref(batch), C.byref(pool), C.byref(geo), kv * group)
+        assert need <= MOST + 16, (pages, need)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,group,d", [(8400, 4, 128), (2600, 25, 64)])
+def test_trees_among_many_rows(hip, rows, group, d):
+    """Of arrays for many rows, whose pieces' results would pass a gigabyte: most rows are no sequence's."""
+    import vlx_tee_amd.attention as A
+    from test_gpu_tree import _case, _close
+
+    print("case", rows, group, d, flush=True)
+    c = _case([(40, 1700), (64, 2500), (3, 900)], 8, group, d, 16, BF, words=2)
+    real = c["q"].shape[0]
+    q = torch.zeros((rows, *c["q"].shape[1:]), dtype=BF, device="cuda")
+    mask = torch.zeros((rows, c["mask"].shape[1]), dtype=torch.int64, device="cuda")
+    q[:real], mask[:real] = c["q"], c["mask"]
+    out = torch.full_like(q, 7.0)
+    got, lse = A.tree_attention(q, c["k"], c["v"], c["table"], c["lens"], c["starts"], mask, return_lse=True, out=out)
+    want = R.tree(c["q"], c["k"], c["v"], c["table"], c["lens"], c["starts"], c["mask"], d ** -0.5)
+    _close(got[:real], want[0], want[2], "out")
+    _close(lse[:real], want[1], want[3], "lse")
+    assert bool((got[real:] == 7).all())

@@ -1060,6 +1060,9 @@ Plan plan_call(const ztcp_paged_batch* b, const ztcp_geometry* g, int64_t q_head
             n = 2 * plan.resident / blocks;
             n = n > 8 ? n : 8;
             n = n < (max_tokens + kTreePiece - 1) / kTreePiece ? n : (max_tokens + kTreePiece - 1) / kTreePiece;
+            // rows enough that these results would pass that are blocks enough to end nearly together as they are
+            const int64_t hold = kMostBetween / (b->n_rows * q_heads * piece * (int64_t)sizeof(float));
+            n = n < hold ? n : hold;
         }
         n = n < 64 ? n : 64;
         plan.splits = (int)(n > 1 ? n : 1);
