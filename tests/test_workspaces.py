@@ -68,3 +68,42 @@ def test_trees_among_many_rows(hip, rows, group, d):
     _close(got[:real], want[0], want[2], "out")
     _close(lse[:real], want[1], want[3], "lse")
     assert bool((got[real:] == 7).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,kv,group,listed,pages", [(65536, 32, 1, 128, 8192), (65536, 8, 4, 128, 8192), (1 << 18, 8, 8, 512, 1 << 17)])
+def test_lists_of_blocks(hip, N, rows, kv, group, listed, pages):
+    batch, geo = _batch(N, n_rows=rows, max_pages=pages, table_stride=pages, n_seqs=4), _geo(N, h=kv)
+    pool = _pool(N, k_stride=16 * kv * 128, v_stride=16 * kv * 128)
+    need = N.lib().ztcp_selected_attention_workspace(C.byref(batch), C.byref(pool), C.byref(geo), kv * group, listed)
+    assert MOST // 4 < need <= MOST + 256, need
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,t", [(BF, 16), (FP, 13)])
+def test_lists_in_parts(hip, dtype, t):
+    """92,560 rows over tables of 8,192 columns: lists of 196 KiB a workgroup, two launches of 2,900 workgroups of 8 heads.
+    The sequences between those that are looked at have no tokens."""
+    import vlx_tee_amd.attention as A
+    from test_gpu_sparse import _attend_case, _close
+
+    print("case", dtype, t, flush=True)
+    c = _attend_case([(300, 700), (260, 500)], 8, 1, 32, t, dtype, 64, seed=4)
+    lens = [(46000, 0), (300, 700), (46000, 0), (260, 500)]
+    table = torch.full((4, 8192), -1, dtype=torch.int32, device="cuda")
+    table[1::2, :c["table"].shape[1]] = c["table"]
+    starts = torch.tensor([0] + [n for n, _ in lens], device="cuda").cumsum(0).int()
+    rows = int(starts[-1])
+    at = torch.cat([torch.arange(46000, 46300), torch.arange(92300, 92560)]).cuda()
+    q = torch.zeros((rows, *c["q"].shape[1:]), dtype=dtype, device="cuda")
+    picked = torch.full((rows, *c["picked"].shape[1:]), -1, dtype=torch.int32, device="cuda")
+    q[at], picked[at] = c["q"], c["picked"]
+    kv_lens = torch.tensor([n for _, n in lens], dtype=torch.int32, device="cuda")
+    out, lse = A.selected_attention(q, c["k"], c["v"], table, kv_lens, starts, picked, return_lse=True)
+    c["table"] = table[1::2]   # (which columns there are tells what a list's entry is)
+    want = R.selected(*(c[x] for x in ("q", "k", "v", "table", "lens", "starts", "picked")), 32 ** -0.5)
+    _close(out[at], want[0], want[2], "out")
+    _close(lse[at], want[1], want[3], "lse")
+    rest = torch.ones(rows, dtype=torch.bool, device="cuda")
+    rest[at] = False
+    assert bool((out[rest] == 0).all()) and bool((lse[rest] == -float("inf")).all())

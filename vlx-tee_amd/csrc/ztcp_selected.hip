@@ -35,7 +35,7 @@ struct SelectedParams {
     float scale_log2;                // scale * log2(e): exponentials are powers of two
     int32_t splits, piece;           // pieces of a unit's keys, and their keys
     float* partial;                  // results of pieces: sums [head_dim], maximum, total
-    int2* lists;                     // blocks: for each workgroup list_stride columns and pages that its rows list
+    int2* lists;                     // blocks: for each workgroup of a launch list_stride columns and pages that its rows list
     uint32_t* masks;                 // and for each of these the tokens that list it
     int64_t list_stride;
     uint32_t first_block;            // of this launch
@@ -475,8 +475,8 @@ void block_kernel(SelectedParams p) {
     const Seq seq = uniform(seq_of(p.batch, s));
     const int rows = seq.n_new * p.group;
     const int mask_words = block_words(p.group);
-    int2* list = p.lists + (int64_t)unit * p.list_stride;
-    uint32_t* masks = p.masks + (int64_t)unit * p.list_stride * mask_words;
+    int2* list = p.lists + (int64_t)blockIdx.x * p.list_stride;
+    uint32_t* masks = p.masks + (int64_t)blockIdx.x * p.list_stride * mask_words;
     const int stop = uniform(list_pages(p, seq, head, block, reinterpret_cast<uint32_t*>(&tiles[0][0][0]), list, masks)) * p.batch.page_tokens;
     const int r = block * kBlockRows + wave * 16 + col;
     const int token = r / p.group, q_head = head * p.group + (r - token * p.group);
@@ -749,19 +749,22 @@ void block_kernel(SelectedParams p) {
 struct SelectedPlan {
     int waves, splits;               // rows: waves of a workgroup, pieces of a unit
     int64_t piece;
-    int64_t units, list;             // blocks: workgroups (0: by rows), columns of a workgroup's list
+    int64_t units, part, list;       // blocks: workgroups (0: by rows), those of a launch, columns of a workgroup's list
     int64_t bytes;                   // of the workspace
 };
 
 SelectedPlan plan_selected(const ztcp_paged_batch* b, const ztcp_geometry* g, int64_t q_heads, int64_t listed, int cus) {
-    SelectedPlan plan{1, 1, listed * g->num_tokens, 0, 0, 0};
+    SelectedPlan plan{1, 1, listed * g->num_tokens, 0, 0, 0, 0};
     const int64_t heads = g->num_heads, group = q_heads / heads, rows = b->n_rows * group;
     // by blocks if these keep half of the compute units busy and are not mostly empty: a sequence's last one may be
     if (rows / kBlockRows * heads >= cus / 2 && rows >= 64 * b->n_seqs && b->max_pages <= kMostColumns) {
         const int64_t most = block_tokens((int)group) * listed;
         plan.units = ((rows + kBlockRows - 1) / kBlockRows + b->n_seqs) * heads;
         plan.list = ((most < b->max_pages ? most : b->max_pages) + 31) / 32 * 32;   // whole lines: none is two workgroups'
-        plan.bytes = plan.units * plan.list * ((int64_t)sizeof(int2) + 4 * block_words((int)group));
+        const int64_t each = plan.list * ((int64_t)sizeof(int2) + 4 * block_words((int)group)), hold = kMostBetween / each;
+        const int64_t parts = (plan.units - 1) / hold + 1;
+        plan.part = (plan.units + parts - 1) / parts;        // alike
+        plan.bytes = plan.part * each;
         return plan;
     }
     const int64_t units = b->n_rows * heads, keys = listed * g->num_tokens;
@@ -856,7 +859,7 @@ extern "C" int ztcp_selected_attention(const void* q, int64_t q_stride, void* ou
     p.piece = (int32_t)plan.piece;
     p.partial = (float*)workspace;
     p.lists = (int2*)workspace;
-    p.masks = (uint32_t*)((int2*)workspace + plan.units * plan.list);
+    p.masks = (uint32_t*)(p.lists + plan.part * plan.list);
     p.list_stride = plan.list;
     if (plan.units >= (int64_t)1 << 31) return arg_result(ZTCP_EINVAL, "too many rows and heads in one call");
     auto go = [&](auto dt, auto dp) {
@@ -864,9 +867,14 @@ extern "C" int ztcp_selected_attention(const void* q, int64_t q_stride, void* ou
         if (plan.units > 0) {
             const bool even = g->num_tokens % (block_tile(DP) / kBlockWaves) == 0 && d == DP;
             const bool one = block_words(p.group) == 1;
-            launch_blocks(one ? even ? block_kernel<DT, DP, true, 1> : block_kernel<DT, DP, false, 1>
-                              : even ? block_kernel<DT, DP, true, 4> : block_kernel<DT, DP, false, 4>,
-                          (uint64_t)plan.units, kBlockThreads, 0, (hipStream_t)stream, p);
+            auto kernel = one ? even ? block_kernel<DT, DP, true, 1> : block_kernel<DT, DP, false, 1>
+                              : even ? block_kernel<DT, DP, true, 4> : block_kernel<DT, DP, false, 4>;
+            // launches whose lists lie in the same place, one after the other
+            for (int64_t first = 0; first < plan.units; first += plan.part) {
+                p.first_block = (uint32_t)first;
+                const int64_t n = plan.units - first < plan.part ? plan.units - first : plan.part;
+                hipLaunchKernelGGL(kernel, dim3((uint32_t)n), dim3(kBlockThreads), 0, (hipStream_t)stream, p);
+            }
             return;
         }
         const uint64_t units = (uint64_t)batch->n_rows * (uint64_t)g->num_heads * (uint64_t)plan.splits;
