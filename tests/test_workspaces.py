@@ -107,3 +107,38 @@ def test_lists_in_parts(hip, dtype, t):
     rest = torch.ones(rows, dtype=torch.bool, device="cuda")
     rest[at] = False
     assert bool((out[rest] == 0).all()) and bool((lse[rest] == -float("inf")).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,group", [([(300, 700), (260, 500)], 4), ([(1, 900), (2, 300)], 4)])
+@pytest.mark.parametrize("off", [0, 16, 48, 112])
+def test_a_workspace_anywhere(hip, N, lens, group, off):
+    """Any 16-byte aligned workspace of the size that is asked for: lists lie in lines of their own within it, and nothing
+    around it is written."""
+    import vlx_tee_amd.attention as A
+    from test_gpu_sparse import _attend_case
+
+    print("case", lens, off, flush=True)
+    c = _attend_case(lens, 8, group, 64, 16, BF, 40, seed=2)
+    q, k, v, table = c["q"].contiguous(), c["k"], c["v"], c["table"]
+    want = A.selected_attention(q, k, v, table, c["lens"], c["starts"], c["picked"], return_lse=True)
+    rows, heads, d = q.shape
+    geo = N.geometry(16, 8, d, 0, 1, False)
+    step = k.stride(0)
+    pool = N.PagePool(k=k.data_ptr(), v=v.data_ptr(), n_pages=k.shape[0], k_stride=step, v_stride=step)
+    batch = N.PagedBatch(page_table=table.data_ptr(), table_stride=table.stride(0), max_pages=table.shape[1],
+                         kv_lens=c["lens"].data_ptr(), q_starts=c["starts"].data_ptr(), n_seqs=len(lens), n_rows=rows, max_q_len=0)
+    L = N.lib()
+    need = L.ztcp_selected_attention_workspace(C.byref(batch), C.byref(pool), C.byref(geo), heads, 40)
+    room = torch.full((need + 512,), 0x5A, dtype=torch.uint8, device="cuda")
+    base = -room.data_ptr() % 128 + off
+    out, lse = torch.empty_like(q), torch.empty((rows, heads), device="cuda")
+    for size, rc in ((need - 1, N.EINVAL), (need, N.OK)):
+        if need:
+            assert L.ztcp_selected_attention(q.data_ptr(), heads * d, out.data_ptr(), lse.data_ptr(), heads, C.byref(pool), C.byref(batch),
+                                             C.byref(geo), c["picked"].data_ptr(), 40, d ** -0.5, room.data_ptr() + base, size,
+                                             torch.cuda.current_stream().cuda_stream) == rc
+    assert need and torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    assert bool((room[:base] == 0x5A).all()) and bool((room[base + need:] == 0x5A).all())
+    if lens[0][0] > 1:   # blocks
+        assert bool((room[base:base + -(room.data_ptr() + base) % 128] == 0x5A).all())

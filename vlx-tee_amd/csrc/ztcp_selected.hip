@@ -746,6 +746,8 @@ void block_kernel(SelectedParams p) {
 
 // ---- host -------------------------------------------------------------------------
 
+constexpr int64_t kLine = 128;       // bytes
+
 struct SelectedPlan {
     int waves, splits;               // rows: waves of a workgroup, pieces of a unit
     int64_t piece;
@@ -760,11 +762,11 @@ SelectedPlan plan_selected(const ztcp_paged_batch* b, const ztcp_geometry* g, in
     if (rows / kBlockRows * heads >= cus / 2 && rows >= 64 * b->n_seqs && b->max_pages <= kMostColumns) {
         const int64_t most = block_tokens((int)group) * listed;
         plan.units = ((rows + kBlockRows - 1) / kBlockRows + b->n_seqs) * heads;
-        plan.list = ((most < b->max_pages ? most : b->max_pages) + 31) / 32 * 32;   // whole lines: none is two workgroups'
+        plan.list = ((most < b->max_pages ? most : b->max_pages) + 31) / 32 * 32;   // whole lines, as the first starts with one: none is two workgroups'
         const int64_t each = plan.list * ((int64_t)sizeof(int2) + 4 * block_words((int)group)), hold = kMostBetween / each;
         const int64_t parts = (plan.units - 1) / hold + 1;
         plan.part = (plan.units + parts - 1) / parts;        // alike
-        plan.bytes = plan.part * each;
+        plan.bytes = plan.part * each + kLine - 16;
         return plan;
     }
     const int64_t units = b->n_rows * heads, keys = listed * g->num_tokens;
@@ -858,7 +860,7 @@ extern "C" int ztcp_selected_attention(const void* q, int64_t q_stride, void* ou
     p.splits = plan.splits;
     p.piece = (int32_t)plan.piece;
     p.partial = (float*)workspace;
-    p.lists = (int2*)workspace;
+    p.lists = (int2*)(((uintptr_t)workspace + kLine - 1) / kLine * kLine);
     p.masks = (uint32_t*)(p.lists + plan.part * plan.list);
     p.list_stride = plan.list;
     if (plan.units >= (int64_t)1 << 31) return arg_result(ZTCP_EINVAL, "too many rows and heads in one call");
