@@ -277,7 +277,7 @@ __global__ __launch_bounds__(256) void score_kernel(SelectParams p) {
     open(unit);
     unit.block = uniform(first) / unit.tiles;
     unit.tile = uniform(first) - unit.block * unit.tiles;
-    if (unit.s >= p.batch.n_seqs || unit.block >= blocks_of(unit.seq)) return;   // (starts that do not ascend)
+    if (first < 0 || unit.s >= p.batch.n_seqs || unit.block >= blocks_of(unit.seq)) return;   // (starts that do not ascend)
     load(ids(unit), unit.seq.n_new <= kBlockTokens);
     Unit next = unit;
     advance(next);
