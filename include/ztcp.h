@@ -450,8 +450,10 @@ ZTCP_API int ztcp_evict_pages(const float* mass, const int32_t* page_table, int6
  * the least and the greatest number of the page's keys.  Written for the pages that hold
  * new tokens of the batch, over all of a page's tokens up to kv_lens[s]; a page with a
  * NaN in a column has NaN as both its bounds.  The pool's v is not read and may be NULL;
- * head_dim at most 1024.  A page that two sequences list has the bounds that one of them
- * gives it. */
+ * head_dim at most 1024; n_rows is any bound on the new tokens up to 2^31 - 1.  A page that
+ * several sequences list and that holds new tokens of more than one of them has, column by
+ * column, the bounds that one of these gives it: the same where their lengths are in the
+ * page or behind it alike. */
 ZTCP_API int ztcp_page_bounds(const ztcp_page_pool* pool, const ztcp_paged_batch* batch, const ztcp_geometry* g,
                      void* bounds, int64_t bounds_stride, void* stream);
 

@@ -53,3 +53,15 @@ def test_select_of_tables_at_the_local_memory_s_end(columns):
     for lens in ([(1, columns)], [(257, columns)]) if columns in (12288, 12289) else ([(1, columns)],):   # a row a workgroup of 1,024, of 256
         c = _select_case(lens, 2, 1, 16, 1, BF, missing=0.02, seed=columns)
         _check_select(A_, c, 50, 1, 2, (columns, lens))
+
+
+def test_bounds_of_more_rows_than_a_call_with_queries_takes():
+    """Of 64 heads: sequences behind 2^31 / 64 rows of others have their pages' bounds too."""
+    _say("bounds, many rows")
+    gen = torch.Generator().manual_seed(1)
+    k = torch.randn((9, 16, 64, 16), generator=gen).to(BF).cuda()
+    table = torch.arange(9, dtype=torch.int32, device="cuda").repeat(2, 1).contiguous()
+    bounds = torch.full((9, 2, 64, 16), 9.0, dtype=BF, device="cuda")
+    lens, starts = _i32([0, 100]), _i32([0, 40_000_000, 40_000_100])
+    want = R.bounds(k, bounds, table, lens, starts, 2 ** 31 - 1)
+    assert torch.equal(A_.page_bounds(k, bounds, table, lens, starts).cpu(), want)

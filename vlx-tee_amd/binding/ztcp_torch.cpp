@@ -299,7 +299,7 @@ PyObject* page_bounds(PyObject* const* a) {
              bounds->size(2) == k_pages->size(2) && bounds->size(3) == k_pages->size(3),
          "bounds must match the pages in number, heads, head_dim, dtype and device");
     // how many rows there are, the device knows
-    const ztcp_paged_batch batch = p.batch(*table, *lens, *starts, (((int64_t)1 << 31) - 1024) / p.g.num_heads, a[5]);
+    const ztcp_paged_batch batch = p.batch(*table, *lens, *starts, ((int64_t)1 << 31) - 1, a[5]);
     const c10::DeviceGuard guard(d);
     done(ztcp_page_bounds(&p.pool, &batch, &p.g, bounds->data_ptr(), step, stream_of(d)), "page_bounds");
     written(bounds);

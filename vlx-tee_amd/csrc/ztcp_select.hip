@@ -1111,7 +1111,12 @@ extern "C" int ztcp_page_bounds(const ztcp_page_pool* pool, const ztcp_paged_bat
     arg_result(ZTCP_OK, "");
     BoundsParams p{};
     if (const char* why = check_pool(pool, g, 1024)) return arg_result(ZTCP_EINVAL, why);
-    if (const char* why = check_batch(batch, pool, g, g->num_heads, p.batch)) return arg_result(ZTCP_EINVAL, why);
+    if (!batch) return arg_result(ZTCP_EINVAL, "batch must not be NULL");
+    if (batch->n_rows < 0 || batch->n_rows >= (int64_t)1 << 31) return arg_result(ZTCP_EINVAL, "n_rows must be 0 .. 2^31 - 1");
+    ztcp_paged_batch rest = *batch;                           // there is no q, whose rows times heads are bounded
+    rest.n_rows = 0;
+    if (const char* why = check_batch(&rest, pool, g, g->num_heads, p.batch)) return arg_result(ZTCP_EINVAL, why);
+    p.batch.n_rows = (int32_t)batch->n_rows;
     if (const char* why = check_bounds(bounds, bounds_stride, g, pool->n_pages)) return arg_result(ZTCP_EINVAL, why);
     const int64_t row = g->num_heads * g->head_dim;
     if (rows_overlap(bounds, pool->n_pages, 4 * row, 2 * bounds_stride, pool->k, pool->n_pages, 2 * g->num_tokens * row, 2 * pool->k_stride))
