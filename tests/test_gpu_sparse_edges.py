@@ -65,3 +65,16 @@ def test_bounds_of_more_rows_than_a_call_with_queries_takes():
     lens, starts = _i32([0, 100]), _i32([0, 40_000_000, 40_000_100])
     want = R.bounds(k, bounds, table, lens, starts, 2 ** 31 - 1)
     assert torch.equal(A_.page_bounds(k, bounds, table, lens, starts).cpu(), want)
+
+
+@pytest.mark.parametrize("kw", [dict(budget=1 << 31), dict(budget=1 << 62), dict(budget=0), dict(budget=(1 << 31) - 1, sink=1 << 31),
+                                dict(budget=(1 << 31) - 1, recent=1 << 31), dict(budget=(1 << 31) - 1, sink=-1),
+                                dict(budget=(1 << 31) - 1, sink=2 ** 63 - 1, recent=2 ** 63 - 1)])
+def test_budgets_are_looked_at_before_anything_is_allocated(kw):
+    _say("select, budgets", kw)
+    c = _select_case([(300, 400)], 8, 1, 64, 16, BF)
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    with pytest.raises(ValueError, match="budget"):
+        A_.select_pages(c["q"], c["b"], c["table"], c["lens"], c["starts"], page_tokens=16, **kw)
+    assert torch.cuda.max_memory_allocated() == held

@@ -326,7 +326,9 @@ PyObject* select_pages(PyObject* const* a) {
     const ztcp_paged_batch batch{(const int32_t*)table->data_ptr(), stride, table->size(1),
                                  (const int32_t*)Pool::plain(*lens, "kv_lens", at::kInt, {s}, d),
                                  (const int32_t*)Pool::plain(*starts, "q_starts", at::kInt, {s + 1}, d), s, n, most};
-    need(budget > 0, "budget must be positive");
+    need(budget > 0 && budget < (int64_t)1 << 31, "budget must be 1 .. 2^31 - 1");   // (before an output of that size is allocated)
+    need(sink >= 0 && sink <= budget && recent >= 1 && recent <= budget - sink,
+         "sink must not be negative, recent at least 1, budget at least sink + recent");
     const int64_t shape[3] = {n, kv, budget};
     if (given) Pool::plain(*given, "out", at::kInt, shape, d);
     const c10::DeviceGuard guard(d);
