@@ -78,3 +78,12 @@ def test_budgets_are_looked_at_before_anything_is_allocated(kw):
     with pytest.raises(ValueError, match="budget"):
         A_.select_pages(c["q"], c["b"], c["table"], c["lens"], c["starts"], page_tokens=16, **kw)
     assert torch.cuda.max_memory_allocated() == held
+
+
+@pytest.mark.parametrize("pages", [1, 63, 64, 65, 256, 257, 320, 321, 385, 449, 512, 513, 576, 577, 640, 641, 705, 769, 833, 897, 961, 1023, 1024, 1025])
+def test_select_of_tables_around_the_registers(pages):
+    """Keys in as many registers as the table's columns need."""
+    _say("select, pages", pages)
+    c = _select_case([(3, 16 * pages), (2, 5 * pages)], 2, 3, 32, 16, FP, seed=pages, missing=0.05, kind=("random", "near", "few values")[pages % 3])
+    for budget in (2, 40, 700):
+        _check_select(A_, c, budget, 1, 1, (pages, budget))

@@ -1058,6 +1058,16 @@ __global__ __launch_bounds__(256) void pick_few_kernel(SelectParams p) {
     for (int i = at + lane; i < p.budget; i += 64) out[i] = -1;
 }
 
+// The kernel with as many registers of keys as a table's columns need: every turn of the search compares and counts all of
+// them (selections of 2 x 2,000 rows of 5 KV heads over 520 pages: 83 us with 9 registers, 91 with 12; over 600: 90 with 10,
+// 93 with 12, 107 with 16).
+template <int DT, int OWN>
+auto pick_few(int64_t max_pages) -> void (*)(SelectParams) {
+    if constexpr (OWN > 1)
+        if (max_pages <= 64 * (OWN - 1)) return pick_few<DT, OWN - 1>(max_pages);
+    return pick_few_kernel<DT, OWN>;
+}
+
 constexpr int kKeysInLds = 12288;   // 48 KiB
 
 // What is wrong with bounds [n_pages, 2, num_heads, head_dim], pages `stride` elements apart, or nullptr.
@@ -1219,8 +1229,7 @@ extern "C" int ztcp_select_pages(const void* q, int64_t q_stride, int64_t q_head
         const uint64_t picks = (uint64_t)rows * (uint64_t)g->num_heads;
         const bool many = picks > 2 * (uint64_t)cus;          // rows: a wave each if their pages are few
         if (batch->max_pages <= kFewPages || many)
-            launch_blocks(batch->max_pages <= 256 ? pick_few_kernel<DT, 4> : batch->max_pages <= 576 ? pick_few_kernel<DT, 9> : pick_few_kernel<DT, 16>,
-                          (picks + 3) / 4, 256, 0, (hipStream_t)stream, p);
+            launch_blocks(pick_few<DT, kFewPages / 64>(batch->max_pages), (picks + 3) / 4, 256, 0, (hipStream_t)stream, p);
         if (batch->max_pages <= kFewPages) return true;
         p.few_pages = many ? kFewPages : -1;
         const bool in_lds = batch->max_pages <= kKeysInLds;
