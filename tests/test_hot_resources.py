@@ -74,3 +74,8 @@ def test_chunk_kernels_spill_no_more(metadata, frag, dtype):
     """Scratch that spills share does not tell their number: reads of it in a chunk's loop are time."""
     hits = [m for n, m in metadata.items() if frag % dtype in n]
     assert len(hits) == 1 and hits[0]["vgpr_spill_count"] <= SPILLS[frag], hits
+
+
+def test_only_kernels_that_are_launched(metadata):
+    """Contexts' pieces of drafted trees have a join of their own."""
+    assert not any("join_tree_kernel" in n for n in metadata)

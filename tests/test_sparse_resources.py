@@ -76,3 +76,8 @@ def test_loads_to_lds_wait_for_their_address_and_base(listings, name):
         assert lines[i - 2].startswith("s_mov_b32 m0,") and re.match(r"s_nop|s_mov_b64", lines[i - 1]), lines[i - 3:i + 1]
         base = re.match(r"global_load_lds\S*\s+v\S+,\s*(s\[\S+\])", lines[i])
         assert not base or re.match(r"s_mov_b64 " + re.escape(base[1]) + ",", lines[i - 1]), lines[i - 2:i + 1]
+
+
+def test_only_kernels_that_are_launched(listings):
+    """Chunks' pieces of paged attention have a join of their own."""
+    assert not any("join_many_kernel" in n for n in _kernels(listings["ztcp_tree"]))

@@ -984,7 +984,6 @@ __global__ __launch_bounds__(256) void join_tree_kernel(AttendParams p) {
     const float w[2] = {__builtin_amdgcn_exp2f(of[0].x - base), __builtin_amdgcn_exp2f(of[1].x - base)};
     const float total = xor_sum(w[0] * of[0].y + w[1] * of[1].y, 32);
     float y[2][4] = {};
-#pragma unroll 8
     for (int i = 0; i < n; ++i) {
         const float wi = __shfl(i < 32 ? w[0] : w[1], (i & 31) + (lane & 32));
 #pragma unroll
@@ -1099,14 +1098,14 @@ void launch(const AttendParams& base, const Plan& plan, float* workspace, hipStr
             p.cut = (int32_t*)workspace;
             p.partial = workspace + kCutFloats;
         }
-        const uint32_t units = (uint32_t)plan.many_units * heads;
         const bool even = p.batch.page_tokens % (many_tile(DP) / 4) == 0 && p.head_dim == DP;
         launch_blocks(even ? many_kernel<DT, DP, true, TREE> : many_kernel<DT, DP, false, TREE>, (uint64_t)plan.many_groups, 256, 0,
                       stream, p);
-        if (p.splits > 1 && TREE)
+        if (p.splits == 1) return;
+        if constexpr (TREE)
             launch_blocks(join_tree_kernel<DT>, ((uint64_t)p.batch.n_rows * ((heads * (uint32_t)p.group + 1) / 2) + 3) / 4, 256, 0, stream, p);
-        else if (p.splits > 1)
-            launch_blocks(join_many_kernel<DT>, (uint64_t)units * (kManyRows / kJoinRows), 256, 0, stream, p);
+        else
+            launch_blocks(join_many_kernel<DT>, (uint64_t)plan.many_units * heads * (kManyRows / kJoinRows), 256, 0, stream, p);
     }
 }
 
