@@ -25,9 +25,6 @@ using namespace ztcp;
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
 struct AttendParams {
     PagedView batch;
     const uint8_t* q;
@@ -74,23 +71,7 @@ __device__ __forceinline__ int pieces_of(int len, int tokens) { return len > 0 ?
 // added afterwards to the rows that see them.  An infinity or a NaN needs no
 // weight for that.  Keys in front of first_sees every row sees: they stay in
 // the product.
-template <int DT>
-__device__ __forceinline__ bool not_finite16(uint32_t h) {
-    constexpr uint32_t e = DT == kHotBf16 ? 0x7F80u : 0x7C00u;
-    return (h & e) == e;
-}
-template <int DT>
-__device__ __forceinline__ bool drop_not_finite(uint4& x) {
-    uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (not_finite16<DT>(w[i])) w[i] &= 0xFFFF0000u, any = true;
-        if (not_finite16<DT>(w[i] >> 16)) w[i] &= 0x0000FFFFu, any = true;
-    }
-    if (any) x = make_uint4(w[0], w[1], w[2], w[3]);
-    return any;
-}
+
 // Four numbers of a V row from column d on: those that are not finite, 0 for the others.
 template <int DT>
 __device__ __forceinline__ f32x4 only_not_finite(const AttendParams& p, const Place& at, int head, int d) {

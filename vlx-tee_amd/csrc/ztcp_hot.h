@@ -138,6 +138,9 @@ inline const char* check_batch(const ztcp_paged_batch* b, const ztcp_page_pool* 
 
 // ---- device ----------------------------------------------------------------
 
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
 // A value that every lane of the wave has, in a scalar register.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 template <class T>
@@ -292,6 +295,25 @@ __device__ __forceinline__ f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+template <int DT>
+__device__ __forceinline__ bool not_finite16(uint32_t h) {
+    constexpr uint32_t e = DT == kHotBf16 ? 0x7F80u : 0x7C00u;
+    return (h & e) == e;
+}
+// Sets those of eight numbers to 0 that are no finite numbers; whether there was one.
+template <int DT>
+__device__ __forceinline__ bool drop_not_finite(uint4& x) {
+    uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (not_finite16<DT>(w[i])) w[i] &= 0xFFFF0000u, any = true;
+        if (not_finite16<DT>(w[i] >> 16)) w[i] &= 0x0000FFFFu, any = true;
+    }
+    if (any) x = make_uint4(w[0], w[1], w[2], w[3]);
+    return any;
 }
 
 // Transposing LDS read of 16-bit numbers: the 16 lanes of a group give the

@@ -10,7 +10,6 @@ using namespace ztcp;
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kFewKeys = 128, kManyKeys = 64;   // keys that a workgroup of either kernel has in registers, 32 a wave
 
 struct MassParams {

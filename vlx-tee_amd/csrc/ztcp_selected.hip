@@ -17,9 +17,6 @@ using namespace ztcp;
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
 struct SelectedParams {
     PagedView batch;
     const uint8_t* q;
@@ -365,12 +362,6 @@ __global__ __launch_bounds__(256) void join_selected_kernel(SelectedParams p) {
 constexpr int kBlockWaves = 8, kBlockRows = 16 * kBlockWaves, kBlockThreads = 64 * kBlockWaves;
 constexpr int block_tile(int dp) { return dp <= 128 ? 64 : 32; }
 
-template <int DT>
-__device__ __forceinline__ bool not_finite16(uint32_t h) {
-    constexpr uint32_t e = DT == kHotBf16 ? 0x7F80u : 0x7C00u;
-    return (h & e) == e;
-}
-
 // Tokens that a block's rows can belong to, and words of a bit for each.
 __host__ __device__ inline int block_tokens(int group) { return kBlockRows % group == 0 ? kBlockRows / group : (kBlockRows - 1) / group + 2; }
 __host__ __device__ inline int block_words(int group) { return (block_tokens(group) + 31) / 32; }
@@ -610,17 +601,12 @@ void block_kernel(SelectedParams p) {
                 bool dropped = false;
                 for (int i = (int)threadIdx.x; i < kTileBytes / 16; i += kBlockThreads) {
                     uint4* piece = reinterpret_cast<uint4*>(tiles[buffer][1]) + i;
-                    const uint4 x = *piece;
-                    uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                    uint4 x = *piece;
                     if (!((at.here >> (i / kChunks)) & 1u)) {
                         *piece = make_uint4(0, 0, 0, 0);
-                    } else if (careful) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if (not_finite16<DT>(w[e])) w[e] &= 0xFFFF0000u, dropped = true;
-                            if (not_finite16<DT>(w[e] >> 16)) w[e] &= 0x0000FFFFu, dropped = true;
-                        }
-                        *piece = make_uint4(w[0], w[1], w[2], w[3]);
+                    } else if (careful && drop_not_finite<DT>(x)) {
+                        *piece = x;
+                        dropped = true;
                     }
                 }
                 apart |= __syncthreads_or(dropped) != 0;
