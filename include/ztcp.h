@@ -470,8 +470,9 @@ ZTCP_API int ztcp_page_bounds(const ztcp_page_pool* pool, const ztcp_paged_batch
  * sink + recent <= budget.  Rows that no sequence has are left.  workspace:
  * ztcp_select_pages_workspace bytes ((size_t)-1 for arguments that the call refuses),
  * needed until the call's work is done, by one call at a time: 4 bytes for each row, head
- * and column of the table, up to 2^30 (rows beyond these, or beyond one, are done in parts
- * that use them again), and 4 for each sequence, head and 16 columns. */
+ * and column of the table (8 where it has more than 12,288), up to 2^30 (rows beyond these,
+ * or beyond one, are done in parts that use them again), and 4 for each sequence, head and
+ * 16 columns. */
 ZTCP_API size_t ztcp_select_pages_workspace(const ztcp_paged_batch* batch, int64_t n_pages, const ztcp_geometry* g,
                                    int64_t q_heads);
 ZTCP_API int ztcp_select_pages(const void* q, int64_t q_stride, int64_t q_heads, const void* bounds,

@@ -87,3 +87,26 @@ def test_select_of_tables_around_the_registers(pages):
     c = _select_case([(3, 16 * pages), (2, 5 * pages)], 2, 3, 32, 16, FP, seed=pages, missing=0.05, kind=("random", "near", "few values")[pages % 3])
     for budget in (2, 40, 700):
         _check_select(A_, c, budget, 1, 1, (pages, budget))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("lens,group", [([(1, 3000), (2, 1100)], 2), ([(2, 900), (3, 300)], 3), ([(1, 13000)], 1), ([(130, 1030)], 2)])
+@pytest.mark.parametrize("kind", ["random", "near", "few values"])
+def test_select_where_some_scores_are_no_numbers(lens, group, dtype, kind):
+    """Fewer of these than are wanted, as many, and more, among scores that are finite, apart and equal: infinities of either
+    sign in either bound, NaN, infinities that meet a query's 0, and sums that pass fp32 while all numbers are finite."""
+    _say("select, some no numbers", lens, group, dtype, kind)
+    for seed, bad in enumerate((1, 5, 40, 300) if lens[0][0] < 100 else (5, 300)):
+        kv = 2 if len(lens) > 1 or lens[0][0] == 1 else 4
+        c = _select_case(lens, kv, group, 32, 1, dtype, seed=seed, missing=0.03, kind=kind)
+        gen = torch.Generator().manual_seed(seed)
+        at = torch.randperm(c["b"].shape[0], generator=gen)[:bad * len(lens)].cuda()
+        for j, (side, column, x) in enumerate([(1, 3, math.inf), (0, 4, -math.inf), (0, 5, math.nan), (1, 6, -math.inf), (0, 7, math.inf)]):
+            c["b"][at[j::6], side, j % kv, column] = x
+        if dtype == BF:
+            c["b"][at[5::6], :, :, :] = 3e38
+            c["q"][0, :, :8] = 2.0
+        c["q"][-1, 0, 3] = 0.0
+        many = sum(n for n, _ in lens) > 100   # (the reference takes its time)
+        for budget in (7, 42) if many else (2, 7, 42, 320):
+            _check_select(A_, c, budget, 1, 1, (lens, kind, bad, budget))

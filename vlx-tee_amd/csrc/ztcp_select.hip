@@ -137,11 +137,11 @@ struct SelectParams {
     int32_t kv_heads, group, head_dim;
     int32_t budget, sink, recent;
     int32_t row0, row1;              // rows that these launches take
-    int32_t score_stride, tops;      // floats of a row's scores (a multiple of 4), of a sequence's tops for a head
+    int32_t score_stride, tops;      // words of a row's scores and keys (a multiple of 4), of a sequence's tops for a head
     float* scores;                   // [row1 - row0, kv_heads, score_stride]; NaN: no finite number
     int32_t score_groups;            // score kernel: workgroups of a KV head
     int32_t few_pages;               // pick kernel: rows of at most so many pages (-1: none) are another kernel's
-    float* top;                      // [n_seqs, kv_heads, tops]: the greatest bound of 16 pages, by magnitude
+    float* top;                      // [n_seqs, kv_heads, tops]: the greatest finite bound of 16 pages, by magnitude
     int32_t* out;
     uint32_t first_block;
 };
@@ -184,7 +184,8 @@ typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t negatives(uint32_t w) { return w & __builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, w) >> (int16_t)15); }
 
 // The greatest magnitude among a wave's bounds of 16 pages from page0 on, written down; `counts`: the lane's (lane % 16)
-// page is there.  Numbers of one sign are ordered as their bits are; NaN is above infinity.
+// page is there.  Numbers of one sign are ordered as their bits are, infinity and NaN above all others: where there is one,
+// the greatest of the others is looked for.  (A page that has one has no finite score.)
 template <int DT, int N>
 __device__ __forceinline__ void top_of(const SelectParams& p, const uint4 (&lo)[N], const uint4 (&hi)[N], int s, int head, int page0,
                                        bool counts) {
@@ -196,11 +197,26 @@ __device__ __forceinline__ void top_of(const SelectParams& p, const uint4 (&lo)[
 #pragma unroll
         for (int j = 0; j < 8; ++j) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[j] & 0x7FFF7FFFu));
     }
-    float top = __int_as_float(counts ? (int)max((uint32_t)most.x, (uint32_t)most.y) << 8 : 0);
-    top = row_max(top, 4);
-    const int all = max(max(__builtin_amdgcn_readlane(__float_as_int(top), 0), __builtin_amdgcn_readlane(__float_as_int(top), 16)),
-                        max(__builtin_amdgcn_readlane(__float_as_int(top), 32), __builtin_amdgcn_readlane(__float_as_int(top), 48)));
-    if (lane == 0) p.top[((int64_t)s * p.kv_heads + head) * p.tops + page0 / 16] = hot_lo<DT>((uint32_t)all >> 8);
+    auto of_all = [&](uint32_t x) {
+        const float top = row_max(__int_as_float(counts ? (int)x << 8 : 0), 4);
+        return (uint32_t)max(max(__builtin_amdgcn_readlane(__float_as_int(top), 0), __builtin_amdgcn_readlane(__float_as_int(top), 16)),
+                             max(__builtin_amdgcn_readlane(__float_as_int(top), 32), __builtin_amdgcn_readlane(__float_as_int(top), 48))) >> 8;
+    };
+    uint32_t all = of_all(max((uint32_t)most.x, (uint32_t)most.y));
+    if (not_finite16<DT>(all)) {
+        uint32_t rest = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t w[8] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w, hi[i].x, hi[i].y, hi[i].z, hi[i].w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                rest = max(rest, not_finite16<DT>(w[j]) ? 0u : w[j] & 0x7FFFu);
+                rest = max(rest, not_finite16<DT>(w[j] >> 16) ? 0u : w[j] >> 16 & 0x7FFFu);
+            }
+        }
+        all = of_all(rest);
+    }
+    if (lane == 0) p.top[((int64_t)s * p.kv_heads + head) * p.tops + page0 / 16] = hot_lo<DT>(all);
 }
 
 template <int DT, int DP>
@@ -504,30 +520,34 @@ __global__ __launch_bounds__(256) void score_chunk_kernel(SelectParams p) {
 // A score is a sum of head_dim products other than 0 (of a column's two one is), each
 // exact in fp32, in two parts at most: it is off by at most
 //     E = (head_dim + 2) (2^-23 |q|_1 B + 2^-125 (1 + |q|_1 + B)),
-// B being the greatest bound (every addition rounds or cuts by 2^-23 of what it holds,
-// a number too small for fp32 loses 2^-126 times its partner): if T is the k-th highest
-// fp32 score, pages above T + 2 E are among the k highest and those below T - 2 E are
-// not.  Those between, hardly ever more than a few, are scored again in fp64 and ranked;
-// equal ones by their place.  A score that is no finite number tells nothing: then E is
-// infinite.  NaN counts as more than every number.
+// B being the greatest finite bound (every addition rounds or cuts by 2^-23 of what it
+// holds, a number too small for fp32 loses 2^-126 times its partner).  Of k pages that
+// are wanted, u have a score that is no finite number, which tells nothing of its rank
+// (their sums pass fp32, or infinity or NaN is in them): each may be before or behind
+// every other.  If T is the k-th highest of the finite fp32 scores and S the (k - u)-th,
+// pages above S + 2 E are among the k highest and those below T - 2 E are not.  Those
+// between, hardly ever more than a few, and the u are scored in fp64 and ranked; equal
+// ones by their place.  NaN counts as more than every number.
 
 constexpr int kBins = 2048;
 constexpr int kFew = 256;
 constexpr uint32_t kChosen = 0xFFFFFFFFu;   // in the place of a page's key: it is taken; 0: it is not
+constexpr uint32_t kUnknown = 1;            // its score is no finite number
 
 __device__ __forceinline__ uint32_t order_of(float x) {       // of finite numbers: neither 0 nor kChosen; -0 as 0
     const uint32_t b = __float_as_uint(x + 0.f);
     return b >> 31 ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float number_of(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7FFFFFFFu : ~k); }
+// (Neither word that is upper in the place of a number is 0 or kChosen.)
 __device__ __forceinline__ uint64_t order_of(double x) {
-    if (x != x) return ~0ull;
+    if (x != x) return 0xFFFFFFFE00000000ull;
     const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
     return b >> 63 ? ~b : b | 1ull << 63;
 }
 
 struct PickSums {
-    uint32_t least, most;            // keys of open pages
+    uint32_t least, most;            // keys of open pages whose scores are finite
     int forced, open, unknown;       // pages
     float sum, top;                  // |q|_1, the greatest bound
 };
@@ -701,7 +721,7 @@ __device__ __forceinline__ uint64_t exact_key(const SelectParams& p, const uint8
     return best;
 }
 
-// One workgroup for a row and KV head.  Keys are in LDS, or (IN_LDS false) in the place of the scores.
+// One workgroup for a row and KV head.  Keys are in LDS, or (IN_LDS false) behind the scores.
 template <int DT, int THREADS, bool IN_LDS>
 __global__ __launch_bounds__(THREADS) void pick_kernel(SelectParams p) {
     extern __shared__ uint32_t lds_keys[];
@@ -716,10 +736,10 @@ __global__ __launch_bounds__(THREADS) void pick_kernel(SelectParams p) {
     if (row < seq.row0 || row >= seq.row0 + seq.n_new) return;
     const int n = pages_seen(p, seq, row - seq.row0 + 1);
     if (n <= p.few_pages) return;
-    uint32_t* scores = reinterpret_cast<uint32_t*>(scores_of(p, row, head));   // (as words, since keys may take their place)
+    uint32_t* scores = reinterpret_cast<uint32_t*>(scores_of(p, row, head));   // (as words, since keys' lower ones may take their place)
     uint32_t* keys;
     if constexpr (IN_LDS) keys = lds_keys;
-    else keys = scores;
+    else keys = scores + p.score_stride / 2;
     const uint8_t* q = p.q + 2 * ((int64_t)row * p.q_stride + (int64_t)head * p.group * p.head_dim);
     int32_t* out = p.out + ((int64_t)row * p.kv_heads + head) * p.budget;
 
@@ -751,9 +771,9 @@ __global__ __launch_bounds__(THREADS) void pick_kernel(SelectParams p) {
             const int i = base + j * THREADS + tid;
             const bool there = id[j] >= 0 && id[j] < p.batch.n_pages, always = there && (i < p.sink || i >= n - p.recent);
             const bool may = there && !always, known = x[j] == x[j];
-            const uint32_t k = always ? kChosen : may ? (known ? order_of(x[j]) : 1u) : 0u;
+            const uint32_t k = always ? kChosen : may ? (known ? order_of(x[j]) : kUnknown) : 0u;
             if (i < n) keys[i] = k;
-            if (may) all.least = min(all.least, k), all.most = max(all.most, k);
+            if (may && known) all.least = min(all.least, k), all.most = max(all.most, k);
             all.forced += __popcll(__ballot(always)), all.open += __popcll(__ballot(may)), all.unknown += __popcll(__ballot(may && !known));
         }
     }
@@ -777,9 +797,22 @@ __global__ __launch_bounds__(THREADS) void pick_kernel(SelectParams p) {
     const int wanted = p.budget - all.forced;
     bool every = all.open <= wanted;                          // what is neither 0 nor kChosen by the end is taken
     if (!every && wanted > 0) {
-        uint32_t low = 1, high = kChosen - 1;                 // keys of pages that may or may not be taken
-        // the fp32 scores' k-th highest, and how far from it fp32 sums cannot tell
-        if (all.unknown == 0) border(p, all.sum, all.top, kth_key(sh, keys, n, all.least, all.most, wanted), low, high);
+        // keys of pages that may or may not be taken, beside kUnknown: from what fp32 sums cannot tell from the k-th highest
+        // to what they cannot tell from the (k - u)-th
+        uint32_t low = kUnknown + 1, high = kChosen - 1;
+        for (int nth = wanted;; nth = wanted - all.unknown) {
+            if (nth > 0 && nth <= all.open - all.unknown) {
+                uint32_t from = low, to = high;
+                border(p, all.sum, all.top, kth_key(sh, keys, n, all.least, all.most, nth), from, to);
+                if (nth == wanted) low = from;
+                if (nth == wanted - all.unknown) high = to;
+            }
+            if (nth == wanted - all.unknown) break;
+            __syncthreads();                                  // the first key has been read
+            for (int i = tid; i < kBins; i += THREADS) sh.bins[i] = 0;
+            if (tid == 0) sh.n_few = 0;
+            __syncthreads();
+        }
         int above = 0;
         for (int base = 0; base < n; base += THREADS) {
             const int i = base + tid;
@@ -787,7 +820,7 @@ __global__ __launch_bounds__(THREADS) void pick_kernel(SelectParams p) {
             const bool over = k > high && k != kChosen;
             above += __popcll(__ballot(over));
             if (over) keys[i] = kChosen;
-            if (k >= low && k <= high) {
+            if (k == kUnknown || (k >= low && k <= high)) {
                 const int at = atomicAdd(&sh.n_near, 1);
                 if (at < kFew) sh.few_page[at] = i;
             }
@@ -799,7 +832,7 @@ __global__ __launch_bounds__(THREADS) void pick_kernel(SelectParams p) {
         for (int w = 0; w < kWaves; ++w) above += sh.scan[w];
         const int left = wanted - above, near = sh.n_near;
         if (near <= left) {                                   // all that are near, and of the others none
-            for (int i = tid; i < n; i += THREADS) keys[i] = keys[i] >= low ? kChosen : 0u;
+            for (int i = tid; i < n; i += THREADS) keys[i] = keys[i] >= low || keys[i] == kUnknown ? kChosen : 0u;
         } else if (near <= kFew) {
             for (int j = wave; j < near; j += kWaves) {
                 const uint64_t x = exact_key<DT>(p, q, seq.entry(sh.few_page[j]), head);
@@ -814,26 +847,26 @@ __global__ __launch_bounds__(THREADS) void pick_kernel(SelectParams p) {
                 if (rank < left) keys[page] = kChosen;
             }
         } else {
-            uint64_t exact_low = 1, exact_high = ~0ull;       // (a score's place is never 0)
-            int ties = left;
-            auto chunk = [&](int base) {                      // of THREADS pages: the scores of those near the border, 0 for the others
-                __syncthreads();
-                for (int j = wave; j < THREADS; j += kWaves) {
-                    const int i = base + j;
-                    const uint32_t k = i < n ? keys[i] : 0u;
-                    const bool is = k >= low && k <= high;
-                    const uint64_t x = is ? exact_key<DT>(p, q, seq.entry(i), head) : 0ull;
-                    if (lane == 0) sh.few[j] = x;
-                }
-                __syncthreads();
-                return sh.few[tid];
+            // each once: their upper words in the place of the keys, the lower ones in that of the scores
+            for (int i = wave; i < n; i += kWaves) {
+                const uint32_t k = keys[i];
+                if (k == kChosen) continue;
+                const bool is = k == kUnknown || k >= low;    // (above high they are taken)
+                const uint64_t x = is ? exact_key<DT>(p, q, seq.entry(i), head) : 0ull;
+                if (lane == 0) keys[i] = (uint32_t)(x >> 32), scores[i] = (uint32_t)x;
+            }
+            __syncthreads();
+            auto exact = [&](int i) {                         // 0: it is taken, or is not near
+                const uint32_t k = i < n ? keys[i] : 0u;
+                return k == 0 || k == kChosen ? 0ull : (uint64_t)k << 32 | scores[i];
             };
-            close_in(sh, [&](auto&& f) { for (int base = 0; base < n; base += THREADS) f(chunk(base)); }, exact_low, exact_high, ties);
+            uint64_t exact_low = 1, exact_high = ~0ull;
+            int ties = left;
+            close_in(sh, [&](auto&& f) { for (int i = tid; i < n; i += THREADS) f(exact(i)); }, exact_low, exact_high, ties);
             int tied = 0;
             for (int base = 0; base < n; base += THREADS) {
                 const int i = base + tid;
-                const uint32_t k = i < n ? keys[i] : 0u;
-                const uint64_t x = chunk(base);               // 0 for pages that are not near
+                const uint64_t x = exact(i);
                 const bool tie = x >= exact_low && x <= exact_high;
                 const uint64_t all_ties = __ballot(tie);
                 __syncthreads();
@@ -844,7 +877,7 @@ __global__ __launch_bounds__(THREADS) void pick_kernel(SelectParams p) {
                     rank += w < wave ? sh.scan[w] : 0;
                     tied += sh.scan[w];
                 }
-                if (i < n && k != kChosen) keys[i] = x > exact_high || (tie && rank < ties) ? kChosen : 0u;
+                if (x != 0) keys[i] = x > exact_high || (tie && rank < ties) ? kChosen : 0u;
             }
         }
     }
@@ -954,14 +987,14 @@ __global__ __launch_bounds__(256) void pick_few_kernel(SelectParams p) {
             if (64 * c >= n) continue;
             const int i = 64 * c + lane;
             const bool there = i < n && (uint32_t)id[c] < (uint32_t)p.batch.n_pages, known = x[c] == x[c];
-            if (there) key[c] = known ? order_of(x[c]) : 1u;
+            if (there) key[c] = known ? order_of(x[c]) : kUnknown;
             if (64 * c < p.sink || 64 * c + 64 > n - p.recent) {   // some that are always taken
                 const bool always = there && (i < p.sink || i >= n - p.recent);
                 if (always) key[c] = 0, taken |= 1u << c;
                 forced += __popcll(__ballot(always));
             }
             open += __popcll(__ballot(key[c] != 0));
-            unknown += __popcll(__ballot(key[c] == 1u));
+            unknown += __popcll(__ballot(key[c] == kUnknown));
         }
     }
     auto count = [&](auto&& is) {
@@ -975,36 +1008,41 @@ __global__ __launch_bounds__(256) void pick_few_kernel(SelectParams p) {
 #pragma unroll
         for (int c = 0; c < kOwn; ++c) taken |= key[c] != 0 ? 1u << c : 0u;
     } else if (wanted > 0) {
-        uint32_t low = 1, high = kChosen - 1;
-        if (unknown == 0) {
-            uint32_t least = kChosen, most = 0;               // the k-th highest is one of these and those between
+        uint32_t low = kUnknown + 1, high = kChosen - 1;      // as in pick_kernel
+        for (int nth = wanted;; nth = wanted - unknown) {
+            if (nth > 0 && nth <= open - unknown) {
+                uint32_t least = kChosen, most = 0;           // the nth highest is one of these and those between
 #pragma unroll
-            for (int c = 0; c < kOwn; ++c) {
-                least = key[c] != 0 ? min(least, key[c]) : least;
-                most = max(most, key[c]);
-            }
-            auto lower = [](uint32_t a, uint32_t b) { return min(a, b); };
-            least = (uint32_t)uniform((int)over_wave(least, lower));
-            most = (uint32_t)uniform((int)over_wave(most, [](uint32_t a, uint32_t b) { return max(a, b); }));
-            while (least < most) {
-                const uint32_t t = least + (most - least + 1) / 2;
-                const int reach = count([&](int c) { return key[c] >= t; });
-                if (reach >= wanted) least = t;
-                else most = t - 1;
-                if (reach != wanted) continue;
-                most = kChosen;                               // the least of these
+                for (int c = 0; c < kOwn; ++c) {
+                    least = key[c] > kUnknown ? min(least, key[c]) : least;
+                    most = max(most, key[c]);
+                }
+                auto lower = [](uint32_t a, uint32_t b) { return min(a, b); };
+                least = (uint32_t)uniform((int)over_wave(least, lower));
+                most = (uint32_t)uniform((int)over_wave(most, [](uint32_t a, uint32_t b) { return max(a, b); }));
+                while (least < most) {
+                    const uint32_t t = least + (most - least + 1) / 2;
+                    const int reach = count([&](int c) { return key[c] >= t; });
+                    if (reach >= nth) least = t;
+                    else most = t - 1;
+                    if (reach != nth) continue;
+                    most = kChosen;                           // the least of these
 #pragma unroll
-                for (int c = 0; c < kOwn; ++c) most = key[c] >= t ? min(most, key[c]) : most;
-                least = most = (uint32_t)uniform((int)over_wave(most, lower));
+                    for (int c = 0; c < kOwn; ++c) most = key[c] >= t ? min(most, key[c]) : most;
+                    least = most = (uint32_t)uniform((int)over_wave(most, lower));
+                }
+                uint32_t from = low, to = high;
+                border(p, sum, top, least, from, to);
+                if (nth == wanted) low = from;
+                if (nth == wanted - unknown) high = to;
             }
-            const uint32_t kth_key = least;
-            border(p, sum, top, kth_key, low, high);
+            if (nth == wanted - unknown) break;
         }
         int above = 0, near = 0;
 #pragma unroll
         for (int c = 0; c < kOwn; ++c) {
             if (64 * c >= n) continue;
-            const bool over = key[c] > high, is = key[c] >= low && key[c] <= high;
+            const bool over = key[c] > high, is = key[c] == kUnknown || (key[c] >= low && key[c] <= high);
             above += __popcll(__ballot(over));
             near += __popcll(__ballot(is));
             taken |= over ? 1u << c : 0u;
@@ -1078,12 +1116,12 @@ const char* check_bounds(const void* bounds, int64_t stride, const ztcp_geometry
 }
 
 struct SelectPlan {
-    int64_t stride, tops, units;     // units: 64 pages and a block of tokens each, at most
+    int64_t stride, tops, units;     // words of a row's scores, and of its keys where these are not in LDS; units: 64 pages and a block of tokens each, at most
     int64_t scores, rows, floats;    // scores of the call; rows that are scored and chosen for at a time; the workspace
 };
 SelectPlan plan_select(const ztcp_paged_batch* b, const ztcp_geometry* g) {
     SelectPlan plan;
-    plan.stride = (b->max_pages + 3) / 4 * 4;
+    plan.stride = (b->max_pages + 3) / 4 * 4 * (b->max_pages > kKeysInLds ? 2 : 1);
     plan.tops = (b->max_pages + 15) / 16;
     plan.units = (b->n_rows / kBlockTokens + b->n_seqs) * ((b->max_pages + kTilePages - 1) / kTilePages);
     const int64_t row = g->num_heads * plan.stride, most = kMostBetween / (row * (int64_t)sizeof(float));
