@@ -467,7 +467,8 @@ ZTCP_API int ztcp_page_bounds(const ztcp_page_pool* pool, const ztcp_paged_batch
  * more than every number, of equal ones the first is taken.
  *   q as in ztcp_paged_attention; bounds as ztcp_page_bounds writes them, of n_pages pages;
  *   out [n_rows, num_heads, budget]: columns of the page table, ascending, -1 behind them.
- * sink + recent <= budget.  Rows that no sequence has are left.  workspace:
+ * sink + recent <= budget.  Rows that no sequence has are left.  max_q_len is not used.
+ * workspace:
  * ztcp_select_pages_workspace bytes ((size_t)-1 for arguments that the call refuses),
  * needed until the call's work is done, by one call at a time: 4 bytes for each row, head
  * and column of the table (8 where it has more than 12,288), up to 2^30 (rows beyond these,
@@ -485,7 +486,8 @@ ZTCP_API int ztcp_select_pages(const void* q, int64_t q_stride, int64_t q_heads,
  * columns selected[row, h, 0 .. listed - 1] of its sequence's table row, which ascend:
  * entries outside the table's columns list nothing, and neither does one that is not
  * above all columns in front of it.
- * selected [n_rows, num_heads, listed]; listed * num_tokens at most 2^31 - 4096. */
+ * selected [n_rows, num_heads, listed]; listed * num_tokens at most 2^31 - 4096.
+ * max_q_len is not used. */
 ZTCP_API size_t ztcp_selected_attention_workspace(const ztcp_paged_batch* batch, const ztcp_page_pool* pool,
                                          const ztcp_geometry* g, int64_t q_heads, int64_t listed);
 ZTCP_API int ztcp_selected_attention(const void* q, int64_t q_stride, void* out, float* lse, int64_t q_heads,

@@ -136,7 +136,8 @@ def select_pages(q: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor
     taken, and of the others those with the highest scores: for a query head the most that ``q . k`` can be within the
     page's ``bounds``, the sum of ``max(q, 0) * hi + min(q, 0) * lo``, for a KV head the greatest of its query heads'.
     Scores count in 64 bits, NaN as more than every number; of equal ones the first page is taken.  Pages that are not
-    there are not taken.  Rows of no sequence keep what ``out`` holds (in one allocated here, anything)."""
+    there are not taken.  Rows of no sequence keep what ``out`` holds (in one allocated here, anything).  ``max_q_len`` is
+    not made use of."""
     return _call().select_pages(q, bounds, page_table, kv_lens, q_starts, page_tokens, budget, sink, recent, max_q_len, out)
 
 
@@ -146,7 +147,7 @@ def selected_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     """``paged_attention`` over a part of the pages: a row's query heads of KV head h see, of the tokens that they would
     see, those of the pages in columns ``selected[row, h]`` ([rows, kv_heads, any number] int32, ascending as
     ``select_pages`` gives them).  Entries outside the table's columns (-1) list nothing, and neither does one that is not
-    above all columns in front of it.  The log-sum-exp is over what the row sees here."""
+    above all columns in front of it.  The log-sum-exp is over what the row sees here.  ``max_q_len`` is not made use of."""
     return _call().selected_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts, selected, scale, max_q_len,
                                       return_lse, out)
 
@@ -230,9 +231,11 @@ class Release(NamedTuple):
 
 def release_pages(page_table: torch.Tensor, kv_lens: torch.Tensor, free_pages: torch.Tensor, n_free: torch.Tensor, *,
                   page_tokens: int, in_place: bool = False) -> Release:
-    """Puts the pages that ``kv_lens`` tokens do not reach back onto the stack ``free_pages``, ``n_free`` (written in
-    either case): those of a sequence that has ended (``kv_lens`` 0), or of drafted tokens that were not accepted.  Pages
-    go in the order of sequences and columns; negative entries are no pages, all others are; what the stack has no room for stays in the
-    table.  The ids that ``evict_pages`` lists are given back, once they have been written out, by
-    ``release_pages(cold.evicted, torch.zeros_like(kv_lens), ...)``.  ``in_place`` updates ``page_table`` and ``n_free``."""
+    """Puts the pages that ``kv_lens`` tokens do not reach back onto the stack ``free_pages``, of which the first ``n_free``
+    are there: those of a sequence that has ended (``kv_lens`` 0), or of drafted tokens that were not accepted.  Pages go in
+    the order of sequences and columns; negative entries are no pages, all others are, and one that occurs twice is given
+    back twice; what the stack has no room for stays in the table.  The ids that ``evict_pages`` lists are given back, once
+    they have been written out, by ``release_pages(cold.evicted, torch.zeros_like(kv_lens), ...)``.
+
+    ``free_pages`` is written in either case; ``in_place`` updates ``page_table`` and ``n_free`` too."""
     return Release._make(_call().release_pages(page_table, kv_lens, free_pages, n_free, page_tokens, in_place))
